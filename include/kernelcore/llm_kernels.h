@@ -286,6 +286,143 @@ typedef struct kcFlashDecodeArgs {
     float scale;
 } kcFlashDecodeArgs;
 
+/* ---- operators over a key/value cache (no reference counterpart) ----------------------------------
+ * A cache is K and V rows by position and KV head, each D values: fp16 (names ending in _f16) or ggml's
+ * Q4_0 blocks (names ending in _q4_0): 32 values in 18 bytes, an fp16 scale d, then 16 bytes of which
+ * byte e holds the code of value e in its low four bits and of value e + 16 in its high ones; code c
+ * stands for d (c - 8). Row and head strides of caches are in bytes and may be any (multiples of 4 for
+ * fp16, of 2 for Q4_0; base pointers likewise), offsets are 64-bit.
+ *
+ * set_rows_q4_0: dst row idx[r] (int64) = the blocks of src row r (n values, n % 32 == 0). Of the value xm
+ * of largest magnitude in a block (the first of several) d = xm / -8, and value x gets the code
+ * floor(x / d + 8.5), at most 15 (8 where d is 0), decided without rounding; d is then stored as fp16. A
+ * block that holds an infinity or NaN reads back as NaN. An index outside [0, dst_rows) stores nothing;
+ * of rows with the same index the last one is stored. The rest of dst stays as it is. */
+typedef struct kcSetRowsQ40Args {
+    const float* src;
+    const int* idx; /* rows int64 values */
+    void* dst;
+    int n;
+    int rows;
+    int src_row;  /* floats between src rows */
+    int dst_rows; /* rows dst holds */
+    long long dst_row; /* bytes between dst rows */
+} kcSetRowsQ40Args;
+/* get_rows_q4_0: y[r][0..n) = the values of src row idx[r] (int64); zeros for an index outside [0, src_rows). */
+typedef struct kcGetRowsQ40Args {
+    const void* src;
+    const int* idx;
+    float* y;
+    int n;
+    int rows;
+    int src_rows;
+    long long src_row; /* bytes between src rows */
+} kcGetRowsQ40Args;
+
+/* Sizes and rules of flash_ext_* and attn_weights_*: N query tokens of H heads over T cached positions of
+ * H_kv heads (query head h reads KV head h / (H / H_kv)), D = 64, 128 or 256 values a head.
+ *   score(i, h, j) = scale q_ih . k_j; softcap > 0: softcap tanh(score / softcap);
+ *                    - slopes[h] |qpos_i - kpos_j| where slopes is given; + mask[i][j] where mask is given
+ * and key j is seen by query i when
+ *   kpos_j >= 0 (a negative position marks an empty slot), and
+ *   causal == 0, or kpos_j <= qpos_i, or kpos_j < prefix, and
+ *   qdoc_i == kdoc_j where document numbers are given (both or neither).
+ * qpos may be null: token i is at pos0 + i; kpos may be null: row j is position j. kpos and kdoc hold T
+ * values, for each KV head its own (key_row ints apart) or one list for all (key_row 0). Positions are
+ * below 2^31 - 1. mask: ggml's f16 mask, rows m_row 32-bit words apart, of which (T + 1) / 2 are read. What a
+ * key holds that a query does not see (NaN and infinities too) does not reach that query's result. */
+typedef struct kcFlashExtDims {
+    int H;
+    int H_kv;
+    int D;
+    int N;
+    int T;
+    int q_tok;  /* floats between tokens of q */
+    int q_head; /* floats between heads of q */
+    int m_row;
+    int key_row;
+    int pos0;
+    int causal;
+    int prefix;
+    long long k_row, k_head, v_row, v_head; /* bytes */
+} kcFlashExtDims;
+/* flash_ext_f16 / flash_ext_q4_0: out[N][H][D] = sum_j softmax_j(score) v_j over the seen keys, for single
+ * tokens and for prompts; a query that sees none gets zeros. lse (may be null): [N][H], the natural
+ * logarithm of the sum of exp(score), -infinity for such a query. part: kcFlashExtPartBytes bytes of
+ * workspace, which calls that may overlap must not share; null where that is 0. */
+typedef struct kcFlashExtArgs {
+    const float* q;
+    const void* k;
+    const void* v;
+    const int* mask;
+    const int* qpos;
+    const int* kpos;
+    const int* qdoc;
+    const int* kdoc;
+    const float* slopes;
+    float* out;
+    float* lse;
+    float* part;
+    kcFlashExtDims d;
+    float scale;
+    float softcap;
+} kcFlashExtArgs;
+KC_API kcError_t kcFlashExtPartBytes(const kcFlashExtDims* dims, size_t* bytes) KC_NOEXCEPT;
+/* attn_weights_f16 / attn_weights_q4_0: what the queries gave each cached position,
+ *   w[g][j] = decay w_in[g][j] + sum over tokens i and the query heads h of KV head g of exp(score(i, h, j) - lse[i][h])
+ * over the seen keys, lse as flash_ext_* wrote it (-infinity: the query adds nothing). w_in may be null (0)
+ * or w itself; rows of w and w_in are w_row floats apart. */
+typedef struct kcAttnWeightsArgs {
+    const float* q;
+    const void* k;
+    const int* mask;
+    const int* qpos;
+    const int* kpos;
+    const int* qdoc;
+    const int* kdoc;
+    const float* slopes;
+    const float* lse;
+    const float* w_in;
+    float* w;
+    kcFlashExtDims d;
+    int w_row;
+    float decay;
+    float scale;
+    float softcap;
+} kcAttnWeightsArgs;
+/* kv_keep: for each of `heads` rows of T weights (w_row floats apart) the n_keep positions to keep, ascending:
+ * the first `first`, the last `recent` and the largest of the others (equal weights: the lowest position;
+ * -0 equals 0, NaN comes after every number). keep rows are keep_row ints apart. first + recent <= n_keep <= T. */
+typedef struct kcKvKeepArgs {
+    const float* w;
+    int* keep;
+    int heads;
+    int T;
+    int w_row;
+    int n_keep;
+    int keep_row;
+    int first;
+    int recent;
+} kcKvKeepArgs;
+/* kv_gather: dst row r of head g = src row keep[g][r] of head g, r < n_keep, for 1 to 4 planes (K, V, weights,
+ * positions) in one launch; rows are `bytes` bytes, strides in bytes (all multiples of 2). Planes' sources and
+ * destinations must not overlap. An index outside [0, T) leaves its dst row as it is. */
+typedef struct kcKvPlane {
+    const void* src;
+    void* dst;
+    long long src_row, src_head, dst_row, dst_head;
+    int bytes;
+} kcKvPlane;
+typedef struct kcKvGatherArgs {
+    kcKvPlane planes[4];
+    int n_planes;
+    const int* keep;
+    int heads;
+    int n_keep;
+    int keep_row;
+    int T;
+} kcKvGatherArgs;
+
 /* ---- K-quant weight streams (this device's layout; no reference counterpart beyond
  * llm::ref::repackQ4K/Q6K and the ggml backend's unpack_stream, ggml-kernelcore.cpp:124-154) ----
  * Rows are grouped in tiles of 16 and super-blocks in groups of 4 (padding rows and super-blocks
@@ -384,6 +521,14 @@ typedef ::kcGetRowsKquantArgs GetRowsKquantArgs;
 typedef ::kcQuantizeKquantArgs QuantizeKquantArgs;
 typedef ::kcFillNormalArgs FillNormalArgs;
 typedef ::kcFlashAttnArgs FlashAttnArgs;
+typedef ::kcSetRowsQ40Args SetRowsQ40Args;
+typedef ::kcGetRowsQ40Args GetRowsQ40Args;
+typedef ::kcFlashExtDims FlashExtDims;
+typedef ::kcFlashExtArgs FlashExtArgs;
+typedef ::kcAttnWeightsArgs AttnWeightsArgs;
+typedef ::kcKvKeepArgs KvKeepArgs;
+typedef ::kcKvPlane KvPlane;
+typedef ::kcKvGatherArgs KvGatherArgs;
 inline int scratchInts(int nb) { return nb * 11; }
 inline float* scratchScales(int* q, int nb) { return reinterpret_cast<float*>(q + nb * 8); }
 inline int scratchKInts(int nsb) { return nsb * 85; }

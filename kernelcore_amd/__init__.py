@@ -86,6 +86,26 @@ FlashAttnArgs = _struct("FlashAttnArgs", [("q", _p), ("k", _p), ("v", _p), ("mas
                                           ("d", FaDims), ("scale", _f)])
 FlashDecodeArgs = _struct("FlashDecodeArgs", [("q", _p), ("k", _p), ("v", _p), ("mask", _p), ("out", _p),
                                              ("part", _p), ("dims", _p), ("d", FaDims), ("scale", _f)])
+_l = C.c_longlong
+SetRowsQ40Args = _struct("SetRowsQ40Args", [("src", _p), ("idx", _p), ("dst", _p), ("n", _i), ("rows", _i), ("src_row", _i),
+                                            ("dst_rows", _i), ("dst_row", _l)])
+GetRowsQ40Args = _struct("GetRowsQ40Args", [("src", _p), ("idx", _p), ("y", _p), ("n", _i), ("rows", _i), ("src_rows", _i),
+                                            ("src_row", _l)])
+FlashExtDims = _struct("FlashExtDims", [(n, _i) for n in ("H", "H_kv", "D", "N", "T", "q_tok", "q_head", "m_row", "key_row",
+                                                          "pos0", "causal", "prefix")] +
+                       [(n, _l) for n in ("k_row", "k_head", "v_row", "v_head")])
+FlashExtArgs = _struct("FlashExtArgs", [(n, _p) for n in ("q", "k", "v", "mask", "qpos", "kpos", "qdoc", "kdoc", "slopes",
+                                                          "out", "lse", "part")] +
+                       [("d", FlashExtDims), ("scale", _f), ("softcap", _f)])
+AttnWeightsArgs = _struct("AttnWeightsArgs", [(n, _p) for n in ("q", "k", "mask", "qpos", "kpos", "qdoc", "kdoc", "slopes",
+                                                                "lse", "w_in", "w")] +
+                          [("d", FlashExtDims), ("w_row", _i), ("decay", _f), ("scale", _f), ("softcap", _f)])
+KvKeepArgs = _struct("KvKeepArgs", [("w", _p), ("keep", _p)] + [(n, _i) for n in ("heads", "T", "w_row", "n_keep", "keep_row",
+                                                                                  "first", "recent")])
+KvPlane = _struct("KvPlane", [("src", _p), ("dst", _p), ("src_row", _l), ("src_head", _l), ("dst_row", _l), ("dst_head", _l),
+                              ("bytes", _i)])
+KvGatherArgs = _struct("KvGatherArgs", [("planes", KvPlane * 4), ("n_planes", _i), ("keep", _p), ("heads", _i), ("n_keep", _i),
+                                        ("keep_row", _i), ("T", _i)])
 GetRowsKquantArgs = _struct("GetRowsKquantArgs", [("qw", _p), ("ids", _p), ("y", _p), ("qtype", _i), ("rows", _i),
                                                   ("k", _i), ("n", _i)])
 QuantizeKquantArgs = _struct("QuantizeKquantArgs", [("x", _p), ("blocks", _p), ("qtype", _i), ("rows", _i), ("k", _i)])
@@ -142,6 +162,7 @@ def lib():
         L.kcLaunchKernel.argtypes = [C.c_char_p, _p, _p]
         L.kcLaunchKernelChunked.argtypes = [C.c_char_p, _p, C.c_uint, C.c_int64, _p]
         L.kcKquantStreamBytes.argtypes = [_i, _i, _i, C.POINTER(C.c_size_t)]
+        L.kcFlashExtPartBytes.argtypes = [C.POINTER(FlashExtDims), C.POINTER(C.c_size_t)]
         L.kcEventElapsedTime.argtypes = [C.POINTER(_f), _p, _p]
         for n in ("kcEventRecord", "kcStreamWaitEvent"):
             getattr(L, n).argtypes = [_p, _p]
@@ -218,6 +239,13 @@ def status(fn, *args):
 def stream_bytes(qtype, rows, k):
     n = C.c_size_t()
     call("kcKquantStreamBytes", QTYPE[qtype], rows, k, C.byref(n))
+    return n.value
+
+
+def flash_ext_part_bytes(dims):
+    """kcFlashExtPartBytes (host only): the workspace flash_ext_f16 / flash_ext_q4_0 need for these FlashExtDims."""
+    n = C.c_size_t()
+    call("kcFlashExtPartBytes", C.byref(dims), C.byref(n))
     return n.value
 
 

@@ -1,0 +1,89 @@
+// kflash_ext.hpp -- parameters and launchers of the attention kernels over a key/value cache (kflash_ext.hip: flash_ext_f16 /
+// flash_ext_q4_0; kattn_weights.hip: attn_weights_f16 / attn_weights_q4_0).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <kernelcore/llm_kernels.h>
+
+#include <algorithm>
+#include <cstdint>
+
+namespace kcamd {
+
+struct FxParams {
+    const float* q;
+    const char* k;
+    const char* v;
+    const unsigned short* mask;
+    const int *qpos, *kpos, *qdoc, *kdoc;
+    const float* slopes;
+    float* out;
+    float* lse;
+    float* part;
+    const float* w_in;  // attn_weights
+    float* w;
+    long long k_row, k_head, v_row, v_head;
+    int H, H_kv, G, N, T, q_tok, q_head, m_row2, key_row, pos0, causal, prefix, rows;
+    int splits, per;  // key ranges, units of 64 keys in each
+    int w_row;
+    float scale, softcap, decay;
+};
+
+// How flash_ext splits a call: up to 32 rows (16 of 256 values, beyond which the few-rows kernel runs out of registers) run on
+// the few-rows kernel, the keys in `splits` ranges of `per` units of 64 keys.
+struct FxPlan {
+    bool few;
+    int splits, per;
+    int64_t partFloats;
+};
+inline FxPlan fxPlan(const kcFlashExtDims& d) {
+    const int64_t rows = int64_t(d.N) * (d.H / d.H_kv), units = (int64_t(d.T) + 63) / 64;
+    FxPlan p{rows <= (d.D == 256 ? 16 : 32), 1, 1, 0};
+    const int64_t base = int64_t(d.H_kv) * (p.few ? 1 : (rows + 127) / 128);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, base), (units + 3) / 4));
+    if (!p.few) splits = std::min<int64_t>(splits, 32);
+    p.per = int(std::max<int64_t>(1, (units + splits - 1) / splits));
+    p.splits = int(std::max<int64_t>(1, (units + p.per - 1) / p.per));
+    p.partFloats = p.splits > 1 ? int64_t(p.splits) * d.H_kv * rows * (d.D + 2) : 0;
+    return p;
+}
+
+int launchFlashExt(bool q4, const kcFlashExtArgs& a, hipStream_t s);
+int launchAttnWeights(bool q4, const kcAttnWeightsArgs& a, hipStream_t s);
+
+// The kernels' parameters of checked arguments.
+inline FxParams fxParams(const kcFlashExtDims& d, const float* q, const void* k, const int* mask, const int* qpos,
+                         const int* kpos, const int* qdoc, const int* kdoc, const float* slopes, float scale,
+                         float softcap) {
+    FxParams p{};
+    p.q = q;
+    p.k = static_cast<const char*>(k);
+    p.mask = reinterpret_cast<const unsigned short*>(mask);
+    p.qpos = qpos;
+    p.kpos = kpos;
+    p.qdoc = qdoc;
+    p.kdoc = kdoc;
+    p.slopes = slopes;
+    p.k_row = d.k_row;
+    p.k_head = d.k_head;
+    p.v_row = d.v_row;
+    p.v_head = d.v_head;
+    p.H = d.H;
+    p.H_kv = d.H_kv;
+    p.G = d.H / d.H_kv;
+    p.N = d.N;
+    p.T = d.T;
+    p.q_tok = d.q_tok;
+    p.q_head = d.q_head;
+    p.m_row2 = 2 * d.m_row;
+    p.key_row = d.key_row;
+    p.pos0 = d.pos0;
+    p.causal = d.causal;
+    p.prefix = d.prefix;
+    p.rows = d.N * p.G;
+    p.scale = scale;
+    p.softcap = softcap;
+    return p;
+}
+
+}  // namespace kcamd

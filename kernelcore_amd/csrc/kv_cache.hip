@@ -1,0 +1,333 @@
+// kv_cache.hip -- rows of a cache: set_rows_q4_0 / get_rows_q4_0 (4-bit blocks), kv_keep (which positions to keep by their
+// accumulated weight) and kv_gather (the kept rows into other memory).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "internal.hpp"
+#include "kv_cache.hpp"
+
+namespace kcamd {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f4a4 __attribute__((aligned(4)));
+typedef uint32_t u32a2 __attribute__((aligned(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ long long index64(const int* idx, long long i) {
+    return (long long)(((unsigned long long)(unsigned)idx[2 * i + 1] << 32) | (unsigned)idx[2 * i]);
+}
+
+// ---------------------------------------------------------------------------------------------- 4-bit rows
+// Eight lanes per block of 32 values, four values each; R rows per workgroup. Bound by reading the f32 rows.
+// Code of x: floor(x / d + 8.5), d = xm / -8. With a = |d| and y = x sign(d) that is the largest c with (c - 8.5) a <= y:
+// the product c' a of a half-integer and an f32 is rounded by the fma only after y is subtracted, so the sign of
+// y - c' a is exact and settles a guess from the rounded quotient.
+__device__ __forceinline__ int code4(float y, float a, float inv) {
+    float c = fminf(fmaxf(floorf(y * inv + 8.5f), 0.0f), 15.0f);
+    if (fmaf(8.5f - c, a, y) < 0.0f) c -= 1.0f;
+    else if (fmaf(7.5f - c, a, y) >= 0.0f) c += 1.0f;
+    return (int)fminf(fmaxf(c, 0.0f), 15.0f);
+}
+
+template <int R>
+__global__ __launch_bounds__(256) void set_rows_q4_0_kernel(const float* __restrict__ src, const int* __restrict__ idx,
+                                                            char* __restrict__ dst, int nb, int rows, int src_row,
+                                                            int dst_rows, long long dst_row) {
+    __shared__ unsigned later;
+    const int r0 = blockIdx.y * R, tid = threadIdx.x;
+    const int b = blockIdx.x * 32 + (tid >> 3), l = tid & 7;
+    const bool live = b < nb;
+    f32x4 x[R];
+    long long at[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int r = min(r0 + k, rows - 1);
+        at[k] = index64(idx, r);
+        x[k] = *reinterpret_cast<const f4a4*>(src + (size_t)r * src_row + 32 * min(b, nb - 1) + 4 * l);
+    }
+    // rows whose index a later row repeats are left to that row
+    if (tid == 0) later = 0;
+    __syncthreads();
+    unsigned mine = 0;
+    for (int i = r0 + 1 + tid; i < rows; i += 256) {
+        const long long other = index64(idx, i);
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (i > r0 + k && other == at[k]) mine |= 1u << k;
+    }
+    if (mine) atomicOr(&later, mine);
+    __syncthreads();
+    const unsigned skip = later;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        if (r0 + k >= rows || (skip >> k & 1u) || at[k] < 0 || at[k] >= dst_rows) continue;  // (the same for the workgroup)
+        // the value of largest magnitude, the first of several
+        float m = 0.0f;
+        int first = 32;
+        bool wild = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = x[k][e];
+            wild |= !(fabsf(v) < INFINITY);
+            if (fabsf(v) > fabsf(m)) {
+                m = v;
+                first = 4 * l + e;
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) {
+            const float m2 = __shfl_xor(m, o);
+            const int f2 = __shfl_xor(first, o);
+            wild |= __shfl_xor((int)wild, o) != 0;
+            if (fabsf(m2) > fabsf(m) || (fabsf(m2) == fabsf(m) && f2 < first)) {
+                m = m2;
+                first = f2;
+            }
+        }
+        const float d = m * -0.125f, up = fabsf(d) < 0x1p-100f ? 0x1p64f : 1.0f;  // (subnormal steps scaled: exact)
+        const float a = fabsf(d) * up, inv = 1.0f / a;
+        uint32_t w = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = wild || a == 0.0f ? 8 : code4((d < 0.0f ? -x[k][e] : x[k][e]) * up, a, inv);
+            w |= (uint32_t)c << (8 * e);
+        }
+        w |= (uint32_t)__shfl_xor((int)w, 4) << 4;  // (lanes 0 .. 3: the codes of values 16 on in the high bits)
+        if (live) {
+            char* p = dst + (size_t)at[k] * dst_row + 18 * (size_t)b;
+            if (l < 4) *reinterpret_cast<u32a2*>(p + 2 + 4 * l) = w;
+            if (l == 4) *reinterpret_cast<unsigned short*>(p) = wild ? (unsigned short)0x7E00 : __builtin_bit_cast(unsigned short, (_Float16)d);
+        }
+    }
+}
+
+// Eight lanes per block, four values (16 bytes of y) each. Bound by writing y.
+__global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restrict__ src, const int* __restrict__ idx,
+                                                            float* __restrict__ y, int nb, int rows, int src_rows,
+                                                            long long src_row) {
+    const int b = blockIdx.x * 32 + (threadIdx.x >> 3), l = threadIdx.x & 7;
+    if (b >= nb) return;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        const long long at = index64(idx, r);
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0 && at < src_rows) {
+            const char* p = src + (size_t)at * src_row + 18 * (size_t)b;
+            const float d = (float)__builtin_bit_cast(_Float16, *reinterpret_cast<const unsigned short*>(p));
+            const uint32_t w = *reinterpret_cast<const u32a2*>(p + 2 + 4 * (l & 3)) >> (l & 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = d * (float)((int)(w >> (8 * e) & 15u) - 8);
+        }
+        *reinterpret_cast<f4a4*>(y + (size_t)r * nb * 32 + 32 * b + 4 * l) = v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- positions to keep
+// One workgroup per head. The weight of rank `want` among the free positions by a radix search from the top (four
+// digits of eight bits over order-preserving codes), then the positions above it and the first of those equal to it, written
+// in ascending order: each wavefront owns a contiguous piece of the row, so that ballots and one prefix over the
+// wavefronts give every position its place.
+constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
+
+__device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first
+    const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.0f ? 0.0f : w);
+    return w != w ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+}
+
+__global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __restrict__ w, int* __restrict__ keep, int T,
+                                                               int w_row, int n_keep, int keep_row, int first, int recent) {
+    __shared__ unsigned hist[256];
+    __shared__ unsigned found[2];
+    __shared__ int above[kKeepWaves], equal[kKeepWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float* wr = w + (size_t)blockIdx.x * w_row;
+    int* out = keep + (size_t)blockIdx.x * keep_row;
+    const int lo = first, hi = T - recent;      // the free positions
+    unsigned want = n_keep - first - recent;    // how many of them stay
+    for (int i = tid; i < first; i += kKeepThreads) out[i] = i;
+    for (int i = tid; i < recent; i += kKeepThreads) out[n_keep - recent + i] = T - recent + i;
+    if (want == 0) return;
+    const int piece = ((hi - lo + kKeepWaves - 1) / kKeepWaves + 63) / 64 * 64;
+    const int p0 = (int)min((long long)hi, lo + (long long)wave * piece), p1 = min(hi, p0 + piece);
+
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = p0 + lane; i < p1; i += 64) {
+            const uint32_t u = rankCode(wr[i]);
+            if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[u >> shift & 255u], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {  // the digit at which the count from the top reaches `want`
+            unsigned c[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += c[e] = hist[255 - (4 * lane + e)];
+            unsigned upto = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const unsigned x = __shfl_up(upto, o);
+                if (lane >= o) upto += x;
+            }
+            unsigned before = upto - sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (before < want && before + c[e] >= want) {
+                    found[0] = 255 - (4 * lane + e);
+                    found[1] = want - before;
+                }
+                before += c[e];
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | found[0];
+        want = found[1];
+    }
+    // prefix: the code of the last weight that stays; want: how many equal to it stay
+    int gt = 0, eq = 0;
+#pragma unroll 4
+    for (int i = p0 + lane; i < p1; i += 64) {
+        const uint32_t u = rankCode(wr[i]);
+        gt += u > prefix;
+        eq += u == prefix;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        gt += __shfl_xor(gt, o);
+        eq += __shfl_xor(eq, o);
+    }
+    if (lane == 0) {
+        above[wave] = gt;
+        equal[wave] = eq;
+    }
+    __syncthreads();
+    int at = first, ties = 0;  // of the pieces before this one
+    for (int x = 0; x < wave; ++x) {
+        at += above[x];
+        ties += equal[x];
+    }
+    at += min(ties, (int)want);
+    for (int i0 = p0; i0 < p1; i0 += 64) {
+        const int i = i0 + lane;
+        const uint32_t u = i < p1 ? rankCode(wr[i]) : 0u;
+        const unsigned long long below = (1ull << lane) - 1;
+        const unsigned long long e = __ballot(i < p1 && u == prefix);
+        const bool stays = i < p1 && (u > prefix || (u == prefix && ties + (int)__popcll(e & below) < (int)want));
+        const unsigned long long s = __ballot(stays);
+        if (stays) out[at + __popcll(s & below)] = i;
+        at += __popcll(s);
+        ties += __popcll(e);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- kept rows
+// One grid over planes, heads and the rows' units (the widest of 16, 4 and 2 bytes that all addresses of a plane
+// allow); eight units per thread in flight. Bound by memory.
+struct GatherPlane {
+    const char* src;
+    char* dst;
+    long long src_row, src_head, dst_row, dst_head;
+    int units, unit;  // of a row
+};
+struct GatherArgs {
+    GatherPlane p[4];
+    const int* keep;
+    int n_keep, keep_row, T;
+};
+constexpr int kGather = 8;
+
+template <class U>
+__device__ __forceinline__ void gatherRows(const GatherPlane& p, const int* keep, int n_keep, int T, long long i0, int g) {
+    const long long total = (long long)n_keep * p.units;
+    U x[kGather];
+    int from[kGather];
+#pragma unroll
+    for (int k = 0; k < kGather; ++k) {
+        const long long i = i0 + 256 * k;
+        from[k] = -1;
+        if (i < total) {
+            const int s = keep[i / p.units];
+            from[k] = s < T ? s : -1;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kGather; ++k) {
+        const long long i = i0 + 256 * k;
+        if (from[k] >= 0)
+            x[k] = *reinterpret_cast<const U*>(p.src + (long long)from[k] * p.src_row + g * p.src_head + (i % p.units) * (long long)sizeof(U));
+    }
+#pragma unroll
+    for (int k = 0; k < kGather; ++k) {
+        const long long i = i0 + 256 * k;
+        if (from[k] >= 0)
+            *reinterpret_cast<U*>(p.dst + (i / p.units) * p.dst_row + g * p.dst_head + (i % p.units) * (long long)sizeof(U)) = x[k];
+    }
+}
+
+__global__ __launch_bounds__(256) void kv_gather_kernel(GatherArgs a) {
+    const GatherPlane& p = a.p[blockIdx.z];
+    const int g = blockIdx.y;
+    const long long i0 = (long long)blockIdx.x * 256 * kGather + threadIdx.x;
+    const int* keep = a.keep + (size_t)g * a.keep_row;
+    if (p.unit == 16) gatherRows<u4>(p, keep, a.n_keep, a.T, i0, g);
+    else if (p.unit == 4) gatherRows<uint32_t>(p, keep, a.n_keep, a.T, i0, g);
+    else gatherRows<unsigned short>(p, keep, a.n_keep, a.T, i0, g);
+}
+
+}  // namespace
+
+int launchSetRowsQ40(const kcSetRowsQ40Args& a, hipStream_t s) {
+    if (a.rows == 0) return 0;
+    const int nb = a.n / 32;
+    char* dst = static_cast<char*>(a.dst);
+    // few rows: a workgroup each; more: eight per workgroup, which then share the search for repeated indices
+    if (a.rows <= 64)
+        hipLaunchKernelGGL(set_rows_q4_0_kernel<1>, dim3((nb + 31) / 32, a.rows), dim3(256), 0, s, a.src, a.idx, dst, nb, a.rows,
+                           a.src_row, a.dst_rows, a.dst_row);
+    else
+        hipLaunchKernelGGL(set_rows_q4_0_kernel<8>, dim3((nb + 31) / 32, (a.rows + 7) / 8), dim3(256), 0, s, a.src, a.idx, dst, nb,
+                           a.rows, a.src_row, a.dst_rows, a.dst_row);
+    return fromHip(hipGetLastError(), "set_rows_q4_0");
+}
+
+int launchGetRowsQ40(const kcGetRowsQ40Args& a, hipStream_t s) {
+    if (a.rows == 0) return 0;
+    const int nb = a.n / 32;
+    hipLaunchKernelGGL(get_rows_q4_0_kernel, dim3((nb + 31) / 32, std::min(a.rows, 4096)), dim3(256), 0, s,
+                       static_cast<const char*>(a.src), a.idx, a.y, nb, a.rows, a.src_rows, a.src_row);
+    return fromHip(hipGetLastError(), "get_rows_q4_0");
+}
+
+int launchKvKeep(const kcKvKeepArgs& a, hipStream_t s) {
+    if (a.n_keep == 0) return 0;
+    hipLaunchKernelGGL(kv_keep_kernel, dim3(a.heads), dim3(kKeepThreads), 0, s, a.w, a.keep, a.T, a.w_row, a.n_keep, a.keep_row,
+                       a.first, a.recent);
+    return fromHip(hipGetLastError(), "kv_keep");
+}
+
+int launchKvGather(const kcKvGatherArgs& a, hipStream_t s) {
+    if (a.n_keep == 0) return 0;
+    GatherArgs g{};
+    long long blocks = 1;
+    for (int i = 0; i < a.n_planes; ++i) {
+        const kcKvPlane& p = a.planes[i];
+        const auto all = reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.dst) | uintptr_t(p.src_row) |
+                         uintptr_t(p.src_head) | uintptr_t(p.dst_row) | uintptr_t(p.dst_head) | uintptr_t(p.bytes);
+        const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
+        g.p[i] = GatherPlane{static_cast<const char*>(p.src), static_cast<char*>(p.dst), p.src_row, p.src_head, p.dst_row,
+                             p.dst_head, p.bytes / unit, unit};
+        blocks = std::max(blocks, ((long long)a.n_keep * (p.bytes / unit) + 256 * kGather - 1) / (256 * kGather));
+    }
+    g.keep = a.keep;
+    g.n_keep = a.n_keep;
+    g.keep_row = a.keep_row;
+    g.T = a.T;
+    hipLaunchKernelGGL(kv_gather_kernel, dim3((unsigned)blocks, a.heads, a.n_planes), dim3(256), 0, s, g);
+    return fromHip(hipGetLastError(), "kv_gather");
+}
+
+}  // namespace kcamd

@@ -12,10 +12,12 @@
 #include <cstdint>
 
 #include "internal.hpp"
+#include "kflash_ext.hpp"
 #include "kquant.hpp"
 #include "launch.hpp"
 #include "kquantize.hpp"
 #include "kdecode.hpp"
+#include "kv_cache.hpp"
 #include "model_kernels.hpp"
 
 namespace {
@@ -450,6 +452,167 @@ int getRowsLaunch(const void* p, void* s) {
     return kcamd::launchGetRows(a.qtype == KC_QTYPE_Q6_K, a.qw, a.ids, a.y, a.n, a.k, a.rows, hs(s));
 }
 
+// ---- operators over a key/value cache: set_rows_q4_0, get_rows_q4_0, flash_ext_*, attn_weights_*, kv_keep, kv_gather
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// Bytes from the first of n rows `row` bytes apart to the end of the last one's `bytes`; false past 2^62.
+bool extent(int64_t n, int64_t row, int64_t bytes, int64_t* out) {
+    if (n <= 0) {
+        *out = 0;
+        return true;
+    }
+    int64_t x;
+    if (row < 0 || __builtin_mul_overflow(n - 1, row, &x) || __builtin_add_overflow(x, bytes, &x) || x > (int64_t(1) << 62)) return false;
+    *out = x;
+    return true;
+}
+
+int setRowsQ40Validate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcSetRowsQ40Args*>(p);
+    int64_t src, dst;
+    if (a.n <= 0 || a.n % 32 || a.rows < 0 || a.rows > 65535 * 8 || a.src_row < a.n || a.dst_rows < 0 || a.dst_row < a.n / 32 * 18 ||
+        a.dst_row % 2 || !extent(a.rows, a.src_row, a.n, &src) || !extent(a.dst_rows, a.dst_row, a.n / 32 * 18, &dst))
+        return invalid("set_rows_q4_0: n a positive multiple of 32, rows of at least n values, dst_row even");
+    if (!aligned(a.src, 4) || !aligned(a.idx, 4) || !aligned(a.dst, 2)) return invalid("set_rows_q4_0: src and idx 4-byte, dst 2-byte aligned");
+    KC_TRY(checkRange(a.src, size_t(src) * 4, "src"));
+    KC_TRY(checkRange(a.idx, size_t(a.rows) * 8, "idx"));
+    return checkRange(a.dst, size_t(dst), "dst");
+}
+int setRowsQ40Launch(const void* p, void* s) { return kcamd::launchSetRowsQ40(*static_cast<const kcSetRowsQ40Args*>(p), hs(s)); }
+
+int getRowsQ40Validate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcGetRowsQ40Args*>(p);
+    int64_t src;
+    if (a.n <= 0 || a.n % 32 || a.rows < 0 || a.src_rows < 0 || a.src_row < a.n / 32 * 18 || a.src_row % 2 ||
+        !extent(a.src_rows, a.src_row, a.n / 32 * 18, &src))
+        return invalid("get_rows_q4_0: n a positive multiple of 32, rows of at least n values, src_row even");
+    if (!aligned(a.src, 2) || !aligned(a.idx, 4) || !aligned(a.y, 4)) return invalid("get_rows_q4_0: idx and y 4-byte, src 2-byte aligned");
+    KC_TRY(checkRange(a.src, size_t(src), "src"));
+    KC_TRY(checkRange(a.idx, size_t(a.rows) * 8, "idx"));
+    return checkRange(a.y, size_t(a.rows) * size_t(a.n) * 4, "y");
+}
+int getRowsQ40Launch(const void* p, void* s) { return kcamd::launchGetRowsQ40(*static_cast<const kcGetRowsQ40Args*>(p), hs(s)); }
+
+// The sizes alone (no pointers): what kcFlashExtPartBytes accepts too.
+int fxShape(const kcFlashExtDims& d) {
+    if (d.H <= 0 || d.H_kv <= 0 || d.H % d.H_kv || d.H_kv > 65535 || (d.D != 64 && d.D != 128 && d.D != 256) || d.N < 0 || d.T < 0 ||
+        d.T > INT32_MAX - 64)
+        return invalid("flash_ext: H a positive multiple of H_kv, D 64, 128 or 256, N and T not negative");
+    if (d.q_tok < 0 || d.q_head < 0 || d.m_row < 0 || d.key_row < 0 || d.k_row < 0 || d.k_head < 0 || d.v_row < 0 || d.v_head < 0)
+        return invalid("flash_ext: negative strides");
+    if ((d.causal != 0 && d.causal != 1) || d.prefix < 0) return invalid("flash_ext: causal 0 or 1, prefix not negative");
+    if (d.pos0 < 0 || int64_t(d.pos0) + d.N >= INT32_MAX) return invalid("flash_ext: positions from 0 to 2^31 - 2");
+    const int64_t rows = int64_t(d.N) * (d.H / d.H_kv);
+    if (rows * d.H_kv * d.D > INT32_MAX || (rows + 127) / 128 > 65535) return invalid("flash_ext: too many query rows");
+    return 0;
+}
+int fxCache(const kcFlashExtDims& d, bool q4, const void* p, int64_t row, int64_t head, const char* what) {
+    const int64_t bytes = q4 ? d.D / 32 * 18 : d.D * 2, unit = q4 ? 2 : 4;
+    int64_t a, b;
+    if (row % unit || head % unit || !aligned(p, size_t(unit)))
+        return invalid(q4 ? "flash_ext: Q4_0 rows, heads and base at multiples of 2 bytes" : "flash_ext: fp16 rows, heads and base at multiples of 4 bytes");
+    if (!extent(d.H_kv, head, bytes, &a) || !extent(d.T, row, a, &b)) return invalid("flash_ext: strides too large");
+    return checkRange(p, size_t(b), what);
+}
+int fxInputs(const kcFlashExtDims& d, bool q4, const float* q, const void* k, const int* mask, const int* qpos, const int* kpos,
+             const int* qdoc, const int* kdoc, const float* slopes, float scale, float softcap) {
+    KC_TRY(fxShape(d));
+    if (!(scale == scale) || scale - scale != 0.0f || !(softcap >= 0.0f) || softcap - softcap != 0.0f)
+        return invalid("flash_ext: scale finite, softcap finite and not negative");
+    if ((qdoc != nullptr) != (kdoc != nullptr)) return invalid("flash_ext: qdoc and kdoc are both given or both null");
+    if (d.key_row && d.key_row < d.T && d.H_kv > 1) return invalid("flash_ext: key_row is 0 or at least T");
+    if (!aligned(q, 4) || !aligned(mask, 4) || !aligned(qpos, 4) || !aligned(kpos, 4) || !aligned(qdoc, 4) || !aligned(kdoc, 4) ||
+        !aligned(slopes, 4))
+        return invalid("flash_ext: 4-byte aligned arrays");
+    int64_t x, y;
+    if (!extent(d.H, d.q_head, d.D, &x) || !extent(d.N, d.q_tok, x, &y)) return invalid("flash_ext: q strides too large");
+    KC_TRY(checkRange(q, size_t(y) * 4, "q"));
+    KC_TRY(fxCache(d, q4, k, d.k_row, d.k_head, "k"));
+    if (mask && d.N && d.T) {
+        if (d.m_row < (int64_t(d.T) + 1) / 2) return invalid("flash_ext: mask rows hold T values");
+        KC_TRY(checkRange(mask, (size_t(d.N - 1) * size_t(d.m_row) + (size_t(d.T) + 1) / 2) * 4, "mask"));
+    }
+    const size_t keys = d.T ? (size_t(d.H_kv - 1) * size_t(d.key_row) + size_t(d.T)) * 4 : 0;
+    if (qpos) KC_TRY(checkRange(qpos, size_t(d.N) * 4, "qpos"));
+    if (qdoc) KC_TRY(checkRange(qdoc, size_t(d.N) * 4, "qdoc"));
+    if (kpos) KC_TRY(checkRange(kpos, keys, "kpos"));
+    if (kdoc) KC_TRY(checkRange(kdoc, keys, "kdoc"));
+    if (slopes) KC_TRY(checkRange(slopes, size_t(d.H) * 4, "slopes"));
+    return 0;
+}
+
+template <bool Q4>
+int flashExtValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcFlashExtArgs*>(p);
+    KC_TRY(fxInputs(a.d, Q4, a.q, a.k, a.mask, a.qpos, a.kpos, a.qdoc, a.kdoc, a.slopes, a.scale, a.softcap));
+    KC_TRY(fxCache(a.d, Q4, a.v, a.d.v_row, a.d.v_head, "v"));
+    if (!aligned(a.out, 4) || !aligned(a.lse, 4) || !aligned(a.part, 4)) return invalid("flash_ext: 4-byte aligned arrays");
+    KC_TRY(checkRange(a.out, f32Bytes(int64_t(a.d.N) * a.d.H * a.d.D), "out"));
+    if (a.lse) KC_TRY(checkRange(a.lse, f32Bytes(int64_t(a.d.N) * a.d.H), "lse"));
+    return checkRange(a.part, f32Bytes(kcamd::fxPlan(a.d).partFloats), "part");
+}
+template <bool Q4>
+int flashExtLaunch(const void* p, void* s) {
+    return kcamd::launchFlashExt(Q4, *static_cast<const kcFlashExtArgs*>(p), hs(s));
+}
+
+template <bool Q4>
+int attnWeightsValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcAttnWeightsArgs*>(p);
+    KC_TRY(fxInputs(a.d, Q4, a.q, a.k, a.mask, a.qpos, a.kpos, a.qdoc, a.kdoc, a.slopes, a.scale, a.softcap));
+    if (a.w_row < a.d.T) return invalid("attn_weights: w_row holds T values");
+    if (!(a.decay == a.decay)) return invalid("attn_weights: decay is a number");
+    if (!aligned(a.lse, 4) || !aligned(a.w, 4) || !aligned(a.w_in, 4)) return invalid("attn_weights: 4-byte aligned arrays");
+    const size_t w = a.d.T ? (size_t(a.d.H_kv - 1) * size_t(a.w_row) + size_t(a.d.T)) * 4 : 0;
+    KC_TRY(checkRange(a.lse, f32Bytes(int64_t(a.d.N) * a.d.H), "lse"));
+    if (a.w_in) KC_TRY(checkRange(a.w_in, w, "w_in"));
+    return checkRange(a.w, w, "w");
+}
+template <bool Q4>
+int attnWeightsLaunch(const void* p, void* s) {
+    return kcamd::launchAttnWeights(Q4, *static_cast<const kcAttnWeightsArgs*>(p), hs(s));
+}
+
+int kvKeepValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcKvKeepArgs*>(p);
+    if (a.heads <= 0 || a.T < 0 || a.T > INT32_MAX - 2048 || a.w_row < a.T || a.first < 0 || a.recent < 0 || a.n_keep > a.T ||
+        int64_t(a.first) + a.recent > a.n_keep || a.keep_row < a.n_keep)
+        return invalid("kv_keep: heads positive, first + recent <= n_keep <= T, rows that hold T weights and n_keep positions");
+    if (!aligned(a.w, 4) || !aligned(a.keep, 4)) return invalid("kv_keep: 4-byte aligned arrays");
+    if (a.T) KC_TRY(checkRange(a.w, (size_t(a.heads - 1) * size_t(a.w_row) + size_t(a.T)) * 4, "w"));
+    return checkRange(a.keep, a.n_keep ? (size_t(a.heads - 1) * size_t(a.keep_row) + size_t(a.n_keep)) * 4 : 0, "keep");
+}
+int kvKeepLaunch(const void* p, void* s) { return kcamd::launchKvKeep(*static_cast<const kcKvKeepArgs*>(p), hs(s)); }
+
+int kvGatherValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcKvGatherArgs*>(p);
+    if (a.n_planes < 1 || a.n_planes > 4 || a.heads <= 0 || a.heads > 65535 || a.n_keep < 0 || a.T < 0 || a.keep_row < a.n_keep)
+        return invalid("kv_gather: 1 to 4 planes, heads positive, keep_row at least n_keep");
+    if (!aligned(a.keep, 4)) return invalid("kv_gather: 4-byte aligned keep");
+    if (a.n_keep == 0) return 0;
+    KC_TRY(checkRange(a.keep, (size_t(a.heads - 1) * size_t(a.keep_row) + size_t(a.n_keep)) * 4, "keep"));
+    int64_t src[4], dst[4];
+    for (int i = 0; i < a.n_planes; ++i) {
+        const kcKvPlane& q = a.planes[i];
+        int64_t s, d;
+        if (q.bytes <= 0 || q.bytes % 2 || q.src_row % 2 || q.src_head % 2 || q.dst_row % 2 || q.dst_head % 2 || !aligned(q.src, 2) ||
+            !aligned(q.dst, 2) || q.src_row < q.bytes || q.dst_row < q.bytes || q.src_head < 0 || q.dst_head < 0 ||
+            (a.heads > 1 && q.dst_head < q.bytes) ||
+            !extent(a.heads, q.src_head, q.bytes, &s) || !extent(a.T, q.src_row, s, &src[i]) || !extent(a.heads, q.dst_head, q.bytes, &d) ||
+            !extent(a.n_keep, q.dst_row, d, &dst[i]))
+            return invalid("kv_gather: bytes and strides even, rows of at least `bytes` bytes");
+        KC_TRY(checkRange(q.src, size_t(src[i]), "src"));
+        KC_TRY(checkRange(q.dst, size_t(dst[i]), "dst"));
+    }
+    for (int i = 0; i < a.n_planes; ++i)
+        for (int j = 0; j < a.n_planes; ++j) {
+            const auto s = reinterpret_cast<uintptr_t>(a.planes[i].src), d = reinterpret_cast<uintptr_t>(a.planes[j].dst);
+            if (s < d + uintptr_t(dst[j]) && d < s + uintptr_t(src[i])) return invalid("kv_gather: a destination overlaps a source");
+        }
+    return 0;
+}
+int kvGatherLaunch(const void* p, void* s) { return kcamd::launchKvGather(*static_cast<const kcKvGatherArgs*>(p), hs(s)); }
+
 // ---- quantize_kquant / fill_normal_f32 (synthetic weights; no reference kernel)
 
 int quantKquantValidate(const void* p, const kcLaunchContext*) {
@@ -510,6 +673,14 @@ const kcKernelEntry kTable[] = {
     {"fa_values", faValuesValidate, faValuesLaunch, 1},
     {"flash_attn_f16", flashValidate, flashLaunch, 0},
     {"flash_decode_f16", flashDecodeValidate, flashDecodeLaunch, 0},
+    {"set_rows_q4_0", setRowsQ40Validate, setRowsQ40Launch, 0},
+    {"get_rows_q4_0", getRowsQ40Validate, getRowsQ40Launch, 0},
+    {"flash_ext_f16", flashExtValidate<false>, flashExtLaunch<false>, 0},
+    {"flash_ext_q4_0", flashExtValidate<true>, flashExtLaunch<true>, 0},
+    {"attn_weights_f16", attnWeightsValidate<false>, attnWeightsLaunch<false>, 0},
+    {"attn_weights_q4_0", attnWeightsValidate<true>, attnWeightsLaunch<true>, 0},
+    {"kv_keep", kvKeepValidate, kvKeepLaunch, 0},
+    {"kv_gather", kvGatherValidate, kvGatherLaunch, 0},
     {"repack_kquant", repackValidate<false>, repackLaunch<false>, 0},
     {"unpack_kquant", repackValidate<true>, repackLaunch<true>, 0},
     {"get_rows_kquant", getRowsValidate, getRowsLaunch, 0},
@@ -528,5 +699,11 @@ kcError_t kcKquantStreamBytes(int qtype, int rows, int k, size_t* bytes) noexcep
     if (!bytes || (qtype != KC_QTYPE_Q4_K && qtype != KC_QTYPE_Q6_K) || rows < 0 || k <= 0 || k % 256 != 0)
         return kc::Error::InvalidValue;
     *bytes = kcamd::streamBytes(qtype == KC_QTYPE_Q6_K, rows, k);
+    return kc::Error::Success;
+}
+
+kcError_t kcFlashExtPartBytes(const kcFlashExtDims* dims, size_t* bytes) noexcept {
+    if (!dims || !bytes || fxShape(*dims)) return kc::Error::InvalidValue;
+    *bytes = f32Bytes(kcamd::fxPlan(*dims).partFloats);
     return kc::Error::Success;
 }

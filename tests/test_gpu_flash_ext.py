@@ -1,0 +1,347 @@
+"""flash_ext_f16 / flash_ext_q4_0 and attn_weights_f16 / attn_weights_q4_0 against the definition in 64 bits (tests/kvcache.py
+derives the bounds), at the sizes, layouts and masks where they can go wrong."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kernelcore_amd as kc
+from tests.kvcache import Case, pack_q4
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def runtime():
+    kc.init()
+    yield
+    kc.synchronize()
+
+
+CACHES = pytest.mark.parametrize("q4", [False, True], ids=["f16", "q4_0"])
+# few rows, one range: a key, a part of a tile, tiles' edges; several ranges; the second column tile; many rows, one range and several
+SIZES = [(8, 8, 64, 1, 1), (4, 1, 64, 1, 31), (6, 2, 64, 2, 33), (8, 2, 128, 1, 63), (8, 2, 128, 1, 64), (8, 2, 128, 1, 65),
+         (6, 2, 128, 5, 300), (16, 1, 128, 1, 257), (16, 1, 128, 2, 515), (10, 2, 64, 6, 1111), (8, 2, 128, 7, 1023), (4, 4, 256, 1, 77),
+         (16, 2, 256, 2, 640), (16, 2, 256, 3, 129), (33, 1, 64, 1, 100), (8, 2, 64, 33, 33), (6, 2, 128, 40, 97), (8, 2, 128, 129, 641),
+         (4, 4, 128, 70, 64), (4, 2, 256, 65, 130), (2, 1, 256, 257, 400), (5, 1, 64, 200, 1001)]
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", SIZES)
+def test_causal(q4, H, K, D, N, T):
+    print(f"flash_ext q4={q4} H={H}/{K} D={D} N={N} T={T}", flush=True)
+    Case(q4, H, K, D, N, T).check()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 333), (6, 2, 64, 4, 95), (8, 2, 128, 50, 333), (4, 2, 256, 40, 77), (24, 8, 128, 9, 513)])
+@pytest.mark.parametrize("shape", ["cap", "bias", "prefix", "docs", "open", "all"])
+def test_shaped(q4, H, K, D, N, T, shape):
+    print(f"flash_ext q4={q4} H={H}/{K} D={D} N={N} T={T} {shape}", flush=True)
+    kw = dict(cap=dict(cap=5.0, spread=3.0), bias=dict(bias=True), prefix=dict(prefix=T // 2 + 3, pos0=T // 3), docs=dict(docs=5), open=dict(causal=0),
+              all=dict(cap=20.0, bias=True, prefix=7, docs=3, spread=2.0))[shape]
+    Case(q4, H, K, D, N, T, **kw).check()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 70), (8, 2, 64, 3, 129), (6, 2, 128, 45, 131), (4, 4, 256, 34, 65)])
+def test_mask(q4, H, K, D, N, T):
+    """ggml's mask: biases, -infinity, the type's lowest value, a row that leaves nothing, rows longer than T."""
+    r = np.random.default_rng(T)
+    m = r.standard_normal((N, (T + 1) // 2 * 2 + 6)).astype(np.float16)
+    m[r.random(m.shape) < 0.4] = -np.inf
+    m[:, T // 2] = -65504  # (its weight is 0 in 32 bits and in 64)
+    m[0, :] = -np.inf
+    if N > 2:
+        m[1, :] = -np.inf
+        m[1, T - 1] = 0
+    c = Case(q4, H, K, D, N, T, causal=0, mask=m)
+    out, sums = c.check()
+    assert (out[0] == 0).all() and np.isneginf(sums[0]).all()
+    Case(q4, H, K, D, N, T, causal=1, mask=m, cap=9.0).check()
+
+
+@CACHES
+@pytest.mark.parametrize("N", [1, 3, 37])
+def test_positions(q4, N):
+    """A thinned cache: each head its own positions, empty slots, queries at positions of their own."""
+    H, K, D, T = 8, 2, 128, 201
+    r = np.random.default_rng(N)
+    kpos = np.sort(r.choice(1000, (K, T), replace=True), axis=1).astype(np.int32)
+    kpos[r.random((K, T)) < 0.2] = -1
+    qpos = r.integers(0, 1000, N).astype(np.int32)
+    Case(q4, H, K, D, N, T, kpos=kpos, qpos=qpos, bias=True, pos0=0).check()
+    kpos[:] = -1  # nothing in the cache
+    out, sums = Case(q4, H, K, D, N, T, kpos=kpos, qpos=qpos, pos0=0).check()
+    assert (out == 0).all() and np.isneginf(sums).all()
+    shared = np.arange(T, dtype=np.int32)[None] * 3
+    Case(q4, H, K, D, N, T, kpos=shared, qpos=qpos, prefix=100, pos0=0).check()
+
+
+@CACHES
+def test_no_keys_and_no_queries(q4):
+    for N in (1, 40):
+        c = Case(q4, 4, 2, 64, N, 0, pos0=0)
+        out, sums = c.attend()
+        assert (out == 0).all() and np.isneginf(sums).all()
+    Case(q4, 4, 2, 64, 0, 17, pos0=17).attend()
+
+
+@CACHES
+@pytest.mark.parametrize("N,T", [(1, 150), (5, 200), (70, 200), (140, 260)])
+def test_what_is_not_seen_does_not_reach_the_result(q4, N, T):
+    """NaN and infinities in keys and values that some queries do not see: those queries' results stay as they were; the
+    others' become what the definition says."""
+    H, K, D = 8, 2, 128
+    c = Case(q4, H, K, D, N, T)
+    clean, _ = c.attend()
+    first = T - N  # rows from here on are seen by the later queries alone
+    r = np.random.default_rng(1)
+    at = sorted({first + N // 2, T - 1} - {first if N == 1 else -1})
+    if N == 1:  # one query: hidden by its mask
+        at = [3, 77, 149]
+        m = np.zeros((1, T + T % 2), np.float16)
+        m[0, at] = -np.inf
+        c.mask, c.causal = m, 1
+        clean, _ = c.attend()
+    for x, bad in zip(at, (np.nan, np.inf, -np.inf)):
+        for name in ("k", "v"):
+            a = getattr(c, name)
+            if q4:  # the scale of one block
+                a.reshape(T, K, -1, 18)[x, 1, 2, :2] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
+            else:
+                a[x, 1, 40 + x % 7] = bad
+    got, _ = c.attend()
+    if N == 1:
+        assert np.array_equal(got, clean)
+        return
+    hidden = np.arange(N) + first < at[0]
+    assert np.array_equal(got[hidden], clean[hidden])
+    assert np.array_equal(got[:, : H // K], clean[:, : H // K])  # (the other KV head)
+    assert not np.isfinite(got[N - 1, H // K:]).all()
+    # a value's infinity alone: just its own column, for the queries that see it
+    c = Case(q4, H, K, D, N, T)
+    clean, _ = c.attend()
+    if q4:
+        c.v.reshape(T, K, -1, 18)[at[0], 1, 2, :2] = np.frombuffer(np.float16(np.inf).tobytes(), np.uint8)
+        cols = np.arange(64, 96)
+    else:
+        c.v[at[0], 1, 45] = np.inf
+        cols = np.array([45])
+    got, _ = c.attend()
+    others = np.setdiff1d(np.arange(D), cols)
+    assert np.array_equal(got[hidden], clean[hidden])
+    assert np.isfinite(got[..., others]).all()
+    assert not np.isfinite(got[~hidden][:, H // K:][..., cols]).any()
+
+
+def test_large_scales_of_4_bit_values():
+    """Scales whose values leave fp16's range (d up to 65504: values up to 524032) stay exact."""
+    for N in (1, 40):
+        c = Case(True, 4, 2, 64, N, 100)
+        b = c.v.reshape(100, 2, -1, 18)
+        for j, d in ((0, 8188.0), (1, 8192.0), (50, 65504.0), (60, -30000.0)):
+            b[j, :, 0, :2] = np.frombuffer(np.float16(d).tobytes(), np.uint8)
+        c.check()
+
+
+@CACHES
+def test_query_magnitudes(q4):
+    """q far above and below fp16's range, a negative scale, zeros."""
+    for N in (2, 40):
+        for spread, scale in ((1e6, 1e-7), (1e-9, 1e8), (1e30, 1e-31), (1.0, -0.1)):
+            Case(q4, 4, 2, 64, N, 90, spread=spread, scale=scale).check()
+        c = Case(q4, 4, 2, 64, N, 90)
+        c.q[0] = 0
+        c.check()
+        Case(q4, 4, 2, 64, N, 90, scale=0.0).check()
+
+
+@CACHES
+@pytest.mark.parametrize("N", [1, 60])
+def test_strides(q4, N):
+    """Head-major caches at odd offsets, q heads and tokens apart, against the packed layout's bits."""
+    H, K, D, T = 8, 2, 128, 150
+    c = Case(q4, H, K, D, N, T)
+    want, _ = c.attend()
+    hb = c.head_bytes()
+    row, base = hb + (2 if q4 else 4), 2 if q4 else 4
+    raw = np.zeros((2, base + K * T * row), np.uint8)
+    for which, a in ((0, c.k), (1, c.v)):
+        raw[which, base:].reshape(K, T, row)[..., :hb] = np.ascontiguousarray(a).view(np.uint8).reshape(T, K, hb).transpose(1, 0, 2)
+    q = np.full(1 + N * (H * (D + 3) + 5), 7.0, np.float32)
+    for i in range(N):
+        for h in range(H):
+            at = 1 + i * (H * (D + 3) + 5) + h * (D + 3)
+            q[at:at + D] = c.q[i, h]
+    bk, bv, bq = kc.Buffer.of(raw[0]), kc.Buffer.of(raw[1]), kc.Buffer.of(q)
+    d = c.dims(k_row=row, k_head=T * row, v_row=row, v_head=T * row, q_tok=H * (D + 3) + 5, q_head=D + 3)
+    out, part = kc.Buffer(4 * N * H * D), kc.Buffer(kc.flash_ext_part_bytes(d))
+    kc.launch(c.name("flash_ext"), kc.FlashExtArgs(q=bq.ptr + 4, k=bk.ptr + base, v=bv.ptr + base, out=out.ptr, part=part.ptr, d=d,
+                                                   scale=c.scale, softcap=0.0))
+    assert np.array_equal(out.download(np.float32).reshape(N, H, D), want)
+    for b in (bk, bv, bq, out, part):
+        b.free()
+
+
+@CACHES
+def test_offsets_past_32_bits(q4):
+    """Rows 1.5 GiB apart: the last ones lie past 4 GiB."""
+    H, K, D, T = 4, 2, 64, 4
+    for N in (1, 40):
+        c = Case(q4, H, K, D, N, T, causal=0, pos0=0)
+        want, _ = c.attend()
+        step = 3 << 29
+        big = kc.Buffer(step * (T - 1) + 2 * K * c.head_bytes())
+        hb = K * c.head_bytes()
+        for j in range(T):
+            big.upload(np.ascontiguousarray(c.k[j]).view(np.uint8).ravel(), j * step)
+            big.upload(np.ascontiguousarray(c.v[j]).view(np.uint8).ravel(), j * step + hb)
+        b = c.upload()
+        d = c.dims(k_row=step, v_row=step)
+        out, part = kc.Buffer(4 * N * H * D), kc.Buffer(kc.flash_ext_part_bytes(d))
+        kc.launch(c.name("flash_ext"), kc.FlashExtArgs(q=b["q"].ptr, k=big.ptr, v=big.ptr + hb, out=out.ptr, part=part.ptr, d=d, scale=c.scale))
+        assert np.array_equal(out.download(np.float32).reshape(N, H, D), want)
+        for x in (big, out, part, *b.values()):
+            x.free()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 1), (8, 2, 128, 1, 333), (8, 8, 64, 3, 130), (6, 2, 128, 20, 97), (8, 2, 64, 16, 200), (4, 2, 256, 70, 130),
+                                       (4, 1, 128, 100, 65)])
+@pytest.mark.parametrize("shape", ["plain", "cap_bias", "docs", "mask", "kept"])
+def test_weights(q4, H, K, D, N, T, shape):
+    print(f"attn_weights q4={q4} H={H}/{K} D={D} N={N} T={T} {shape}", flush=True)
+    r = np.random.default_rng(T)
+    kw = {}
+    if shape == "cap_bias":
+        kw = dict(cap=10.0, bias=True, prefix=T // 3)
+    if shape == "docs":
+        kw = dict(docs=3)
+    if shape == "mask":
+        m = r.standard_normal((N, (T + 1) // 2 * 2)).astype(np.float16)
+        m[r.random(m.shape) < 0.4] = -np.inf
+        m[0] = -np.inf
+        kw = dict(mask=m, causal=0)
+    if shape == "kept":
+        kpos = np.sort(r.choice(3 * T + 1, (K, T)), axis=1).astype(np.int32)
+        kpos[r.random((K, T)) < 0.2] = -1
+        kw = dict(kpos=kpos, pos0=2 * T, bias=True)
+    c = Case(q4, H, K, D, N, T, **kw)
+    lse = c.expected()[2].astype(np.float32)
+    w_in = r.random((K, T)).astype(np.float32)
+    for w0, decay in ((None, 0.0), (w_in, 0.75)):
+        got = c.weights(lse, w0, decay)
+        want, bound = c.expected_weights(lse, w0, decay)
+        assert (np.abs(got - want) <= bound).all()
+
+
+def test_weights_in_place_and_no_queries():
+    c = Case(True, 4, 2, 64, 2, 40)
+    lse = c.expected()[2].astype(np.float32)
+    w0 = np.random.default_rng(0).random((2, 40)).astype(np.float32)
+    b, d = c.upload(), c.dims()
+    bl, w = kc.Buffer.of(lse), kc.Buffer.of(w0)
+    kc.launch("attn_weights_q4_0", kc.AttnWeightsArgs(lse=bl.ptr, w_in=w.ptr, w=w.ptr, w_row=40, decay=0.5, **c.shape_args(b, d)))
+    want, bound = c.expected_weights(lse, w0, 0.5)
+    got = w.download(np.float32).reshape(2, 40)
+    assert (np.abs(got - want) <= bound).all()
+    d0 = c.dims(N=0)
+    kc.launch("attn_weights_q4_0", kc.AttnWeightsArgs(lse=bl.ptr, w_in=w.ptr, w=w.ptr, w_row=40, decay=0.5, **c.shape_args(b, d0)))
+    assert np.array_equal(w.download(np.float32).reshape(2, 40), got * np.float32(0.5))
+    for x in (bl, w, *b.values()):
+        x.free()
+
+
+def test_a_weight_row_past_nothing_seen_is_zero():
+    """NaN in hidden keys adds nothing to any position; a hidden position gets 0."""
+    c = Case(False, 4, 2, 64, 3, 50)
+    lse = c.expected()[2].astype(np.float32)
+    clean = c.weights(lse)
+    c.k[49] = np.nan  # seen by the last query alone
+    c2 = c.weights(lse)
+    assert np.array_equal(c2[:, :49], clean[:, :49]) and np.isnan(c2[:, 49]).all()
+
+
+@CACHES
+def test_graph_replays(q4):
+    """Two captured graphs with workspaces of their own, replayed in turn over changing inputs, eager calls between."""
+    c = Case(q4, 8, 2, 128, 2, 700)
+    s = C.c_void_p()
+    kc.call("kcStreamCreate", C.byref(s))
+    made = []
+    for _ in range(2):
+        b, d = c.upload(), c.dims()
+        out, part = kc.Buffer(4 * 2 * 8 * 128), kc.Buffer(kc.flash_ext_part_bytes(d))
+        args = kc.FlashExtArgs(v=b["v"].ptr, out=out.ptr, part=part.ptr, **c.shape_args(b, d))
+        kc.call("kcStreamBeginCapture", s)
+        kc.launch(c.name("flash_ext"), args, s)
+        g = C.c_void_p()
+        kc.call("kcStreamEndCapture", s, C.byref(g))
+        made.append((b, out, part, g, args))
+    r = np.random.default_rng(3)
+    for _ in range(3):
+        want = []
+        for b, *_ in made:
+            c.q = r.standard_normal(c.q.shape).astype(np.float32)
+            b["q"].upload(c.q)
+            want.append(c.attend()[0])
+        for b, out, part, g, _ in made:
+            kc.call("kcGraphLaunch", g, s)
+        kc.call("kcStreamSynchronize", s)
+        for (b, out, *_), w in zip(made, want):
+            assert np.array_equal(out.download(np.float32).reshape(w.shape), w)
+    for b, out, part, g, _ in made:
+        kc.call("kcGraphDestroy", g)
+        for x in (out, part, *b.values()):
+            x.free()
+    kc.call("kcStreamDestroy", s)
+
+
+def test_one_result_for_every_run():
+    """The same call gives the same bits, whatever ran before (no atomics in the sums)."""
+    for N, T in ((1, 3000), (90, 900)):
+        c = Case(True, 8, 2, 128, N, T)
+        a, b = c.attend(), c.attend()
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_cache_filled_step_by_step():
+    """A prompt stored into a 4-bit cache in two chunks, attended to, thinned by its weights, then a token decoded over what is
+    left: every step against the definition over the same bytes."""
+    H, K, D, T = 8, 2, 128, 90
+    r = np.random.default_rng(5)
+    kv = [r.standard_normal((T, K * D)).astype(np.float32) for _ in range(2)]
+    n = K * D
+    row = n // 32 * 18
+    cache = [kc.Buffer(T * row) for _ in range(2)]
+    for lo, hi in ((0, 61), (61, T)):
+        for buf, x in zip(cache, kv):
+            bx, bi = kc.Buffer.of(x[lo:hi]), kc.Buffer.of(np.arange(lo, hi, dtype=np.int64))
+            kc.launch("set_rows_q4_0", kc.SetRowsQ40Args(bx.ptr, bi.ptr, buf.ptr, n, hi - lo, n, T, row))
+            kc.synchronize()
+            bx.free(), bi.free()
+    c = Case(True, H, K, D, 29, T)
+    c.k, c.v = (pack_q4(x.reshape(T, K, D)) for x in kv)
+    for buf, a in zip(cache, (c.k, c.v)):
+        assert np.array_equal(buf.download(np.uint8), a.ravel())
+    out, lse = c.check()
+    w = c.weights(lse)
+    keep_n = 40
+    bw, bk = kc.Buffer.of(w), kc.Buffer(4 * K * keep_n)
+    kc.launch("kv_keep", kc.KvKeepArgs(bw.ptr, bk.ptr, K, T, T, keep_n, keep_n, 2, 8))
+    thin = [kc.Buffer(keep_n * row) for _ in range(2)]
+    pos, tpos = kc.Buffer.of(np.tile(np.arange(T, dtype=np.int32), (K, 1))), kc.Buffer(4 * K * keep_n)
+    hb = row // K
+    planes = (kc.KvPlane * 4)(*[kc.KvPlane(a.ptr, b.ptr, row, hb, row, hb, hb) for a, b in zip(cache, thin)],
+                              kc.KvPlane(pos.ptr, tpos.ptr, 4, 4 * T, 4, 4 * keep_n, 4))
+    kc.launch("kv_gather", kc.KvGatherArgs(planes, 3, bk.ptr, K, keep_n, keep_n, T))
+    keep = bk.download(np.int32).reshape(K, keep_n)
+    one = Case(True, H, K, D, 1, keep_n, kpos=tpos.download(np.int32).reshape(K, keep_n), pos0=T, bias=True)
+    assert np.array_equal(one.kpos, keep)
+    one.k, one.v = (np.stack([a.reshape(T, K, hb)[keep[g], g] for g in range(K)], 1) for a in (c.k, c.v))
+    for buf, a in zip(thin, (one.k, one.v)):
+        assert np.array_equal(buf.download(np.uint8), a.ravel())
+    one.check()
+    for b in (*cache, bw, bk, *thin, pos, tpos):
+        b.free()
