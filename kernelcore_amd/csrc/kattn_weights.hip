@@ -1,9 +1,10 @@
 // kattn_weights.hip -- attn_weights_f16 / attn_weights_q4_0 (gfx950): what the query rows gave each cached position,
-//   w_gj = decay w_in_gj + sum over rows r of KV head g of exp(x_rj - lse_r)
-// with x as flash_ext computes it (kflash_ext.hpp). Tiles of 32 keys x 32 rows on the matrix cores, S^T = K Q^T; a wavefront
-// keeps its key tile and walks over the rows, each lane adding up its own row's weights for its 16 keys, so that the sum over
-// the lanes is taken once, at the end, in one order. Four wavefronts share a tile's rows, or take tiles of their own where
-// there are few rows: a single token's call reads K once and is bound by that.
+//   w_gj = decay w_in_gj + sum over rows r of KV head g of exp(y_rj - lse_r),
+// with the scores y of flash_ext (kflash_ext_device.hpp). Tiles of 32 rows x 32 keys on the matrix cores, S = Q K^T (A = q rows, B =
+// keys): lane (j, h) holds rows 8 (v / 4) + 4 h + v % 4 of key j, so a key's sum over the rows is a sum of registers and
+// nothing crosses lanes until the end. A workgroup stages its key tiles once; then its wavefronts share the rows (RW of them
+// to a tile) and walk over the row tiles without a barrier, q read once for all of the tiles. Sums in one order, no atomics.
+// A single token's call reads K once and is bound by that.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,117 +24,189 @@ struct WGeo {
     static constexpr int oS = 32 * kKeyRow<D>, oMeta = oS + (Q4 ? NB * 128 : 0), Tile = oMeta + 256;
 };
 
-// RW wavefronts per key tile (1, 2 or 4), 4 / RW tiles per workgroup.
-template <int D, bool Q4, int RW>
+// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup.
+template <int D, bool Q4, int RW, int TP>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxParams a) {
     using G = WGeo<D, Q4>;
-    constexpr int NB = G::NB, KT = 4 / RW, GT = 64 * RW;
+    constexpr int NB = G::NB, KW = 4 / RW, KT = KW * TP, PR = Q4 ? NB : D / 8, KS = D / 16;
     extern __shared__ int4 lds4[];
-    __shared__ float part[4][32];
+    __shared__ float part[4][TP][32];
+    __shared__ float4 rows4[4][32];  // factor, lse (base 2), slope, -
+    __shared__ int4 rows4i[4][32];   // limit, position, document, token
+    char* lds = reinterpret_cast<char*>(lds4);
     const int kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, h = lane >> 5;
-    const int kt = wave / RW, rw = wave % RW, gt = tid % GT;
-    const int t = blockIdx.x * KT + kt;
-    char* tile = reinterpret_cast<char*>(lds4) + kt * G::Tile;
+    const int kw = wave / RW, rw = wave % RW;
+    const int t0 = blockIdx.x * KT;
     const char* kb = a.k + (size_t)kvh * a.k_head;
     const int* kpos = a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
     const int* kdoc = a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
-    const bool meta = kpos || kdoc;
-    const bool have = (long long)t * 32 < a.T;
-    if (have) {
-        if constexpr (Q4) {
-            for (int i = gt; i < 32 * NB; i += GT) {
-                const int key = i / NB, b = i % NB;
-                const char* p = kb + (size_t)min(t * 32 + key, a.T - 1) * a.k_row + 18 * b;
-                const u4 raw = *reinterpret_cast<const u4a2*>(p + 2);
-                h8 code[4];
-                blockCodes(raw, code);
-                h8* dst = reinterpret_cast<h8*>(tile + key * kKeyRow<D> + 64 * b);
+    constexpr int IT = KT * 32 * PR, NL = (IT + 255) / 256;
+    u4 raw[NL];
+    uint32_t sc[Q4 ? NL : 1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) dst[e] = code[e];
-                reinterpret_cast<float*>(tile + G::oS)[b * 32 + key] = halfBits(loadHalf(p));
-            }
+    for (int n = 0; n < NL; ++n) {
+        const int i = tid + 256 * n;
+        if (i >= IT) break;
+        const char* p = kb + (size_t)min((long long)t0 * 32 + i / PR, (long long)a.T - 1) * a.k_row + (Q4 ? 18 : 16) * (i % PR);
+        if constexpr (Q4) {
+            raw[n] = *reinterpret_cast<const u4a2*>(p + 2);
+            sc[n] = loadHalf(p);
         } else {
-            for (int i = gt; i < 32 * (D / 8); i += GT) {
-                const int key = i / (D / 8), ch = i % (D / 8);
-                *reinterpret_cast<u4*>(tile + key * kKeyRow<D> + 16 * ch) =
-                    *reinterpret_cast<const u4a4*>(kb + (size_t)min(t * 32 + key, a.T - 1) * a.k_row + 16 * ch);
-            }
-        }
-        if (meta && gt < 64) {
-            const int key = t * 32 + (gt & 31);
-            int x;
-            if (gt < 32) {
-                x = key < a.T ? (kpos ? kpos[key] : key) : kNoKey;
-                if (x < 0) x = kNoKey;
-            } else {
-                x = kdoc && key < a.T ? kdoc[key] : 0;
-            }
-            reinterpret_cast<int*>(tile + G::oMeta)[gt] = x;
+            raw[n] = *reinterpret_cast<const u4a4*>(p);
         }
     }
-    __syncthreads();
-    float acc[16];
+    // this lane's keys: key j of each of the wavefront's tiles
+    int pos[TP], doc[TP];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) acc[v] = 0.0f;
+    for (int p = 0; p < TP; ++p) {
+        const long long key = (long long)(t0 + kw * TP + p) * 32 + j;
+        pos[p] = key < a.T ? (kpos ? kpos[key] : (int)key) : kNoKey;
+        if (pos[p] < 0) pos[p] = kNoKey;
+        doc[p] = kdoc && key < a.T ? kdoc[key] : 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+        const int i = tid + 256 * n, key = i / PR, b = i % PR;
+        if (i >= IT) break;
+        char* tile = lds + (key >> 5) * G::Tile;
+        if constexpr (Q4) {
+            h8 code[4];
+            blockCodes(raw[n], code);
+            h8* dst = reinterpret_cast<h8*>(tile + (key & 31) * kKeyRow<D> + 64 * b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = code[e];
+            reinterpret_cast<float*>(tile + G::oS)[b * 32 + (key & 31)] = halfBits(sc[n]);
+        } else {
+            *reinterpret_cast<u4*>(tile + (key & 31) * kKeyRow<D> + 16 * b) = raw[n];
+        }
+    }
     const Shape shape = shapeOf(a);
-    for (int r0 = 32 * rw; have && r0 < a.rows; r0 += 32 * RW) {
+    __syncthreads();
+    f32x16 zero;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) zero[v] = 0.0f;
+    float acc[TP];
+#pragma unroll
+    for (int p = 0; p < TP; ++p) acc[p] = 0.0f;
+    const int key0 = (t0 + kw * TP) * 32;
+    for (int r0 = 32 * rw; r0 < a.rows; r0 += 32 * RW) {
         const Row row = rowOf(a, kvh, r0 + j);
-        const int wmax = waveMax(row.live ? row.limit : -1);
-        if (!kpos && t * 32 > wmax) continue;
-        h8 qh[D / 16], ql[D / 16];
+        const int wmax = waveMax(row.live ? row.limit : -1), wmin = waveMin(row.live ? row.limit : INT_MAX);
+        if (!kpos && key0 > wmax) continue;
+        h8 qh[KS], ql[KS];
         const float c = loadRow32<D>(a, row, h, qh, ql);
         const float lse = row.live ? a.lse[(size_t)row.token * a.H + row.head] : -INFINITY;
-        const unsigned short* mrow = a.mask ? a.mask + (size_t)row.token * a.m_row2 : nullptr;
-        MaskWords mk;
-        if (mrow) mk.load(mrow, t, h, a.T);
-        float x[16];
-        keyScores<D, Q4>(tile, tile + G::oS, j, h, qh, ql, x);
-        shapeScores(x, c, shape, row, meta ? reinterpret_cast<const int*>(tile + G::oMeta) : nullptr, mrow ? &mk : nullptr, t, h);
-        const int last = meta ? INT_MAX : min(row.limit, a.T - 1) - t * 32 - 4 * h;
-        const float l2 = lse * kLog2e;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const float p = 8 * (v >> 2) + (v & 3) <= last && x[v] != -INFINITY ? ex2(x[v] - l2) : 0.0f;
-            acc[v] += lse == -INFINITY ? 0.0f : p;
+        if (h == 0) {  // (a row that saw nothing gives nothing: its factor's place holds the mark)
+            rows4[wave][j] = make_float4(c, lse == -INFINITY ? INFINITY : lse * kLog2e, row.slope, 0.0f);
+            rows4i[wave][j] = make_int4(lse == -INFINITY ? -1 : row.limit, row.pos, row.doc, row.token);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const bool easy = !kpos && !kdoc && !a.mask && !__any(row.live ? lse == -INFINITY : r0 + j < a.rows);
+#pragma unroll
+        for (int p = 0; p < TP; ++p) {
+            const int k0 = key0 + 32 * p;
+            if (!kpos && k0 > wmax) continue;
+            const char* tile = lds + (kw * TP + p) * G::Tile;
+            const char* kr = tile + j * kKeyRow<D> + 16 * h;
+            float x[16];
+            if constexpr (Q4) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const h8 ka = *reinterpret_cast<const h8*>(kr + 64 * b), kc = *reinterpret_cast<const h8*>(kr + 64 * b + 32);
+                    f32x16 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[2 * b], ka, zero, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[2 * b + 1], kc, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[2 * b], ka, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[2 * b + 1], kc, s, 0, 0, 0);
+                    const float d = reinterpret_cast<const float*>(tile + G::oS)[b * 32 + j];
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) x[v] = b ? fmaf(d, s[v], x[v]) : d * s[v];
+                }
+            } else {
+                f32x16 s = zero;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const h8 ka = *reinterpret_cast<const h8*>(kr + 32 * k);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[k], ka, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[k], ka, s, 0, 0, 0);
+                }
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] = s[v];
+            }
+            const bool full = easy && r0 + 32 <= a.rows && k0 + 31 <= wmin && k0 + 31 < a.T;
+            if (full && shape.inv_cap == 0.0f && !shape.bias) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const float2 cl = *reinterpret_cast<const float2*>(&rows4[wave][8 * (v >> 2) + 4 * h + (v & 3)]);
+                    acc[p] += ex2(fmaf(x[v], factor2(cl.x), -cl.y));
+                }
+                continue;
+            }
+            float4 rf[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) rf[v] = rows4[wave][8 * (v >> 2) + 4 * h + (v & 3)];
+            if (shape.inv_cap > 0.0f) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] *= rf[v].x;
+                capScores<16>(x, shape.inv_cap, shape);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] *= factor2(rf[v].x);
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int4 ri = rows4i[wave][8 * (v >> 2) + 4 * h + (v & 3)];
+                if (shape.bias) x[v] = fmaf(-rf[v].z * kLog2e, fabsf((float)(ri.y - pos[p])), x[v]);
+                bool seen = pos[p] <= ri.x && doc[p] == ri.z;
+                if (a.mask && seen) {
+                    const uint32_t mv = a.mask[(size_t)ri.w * a.m_row2 + k0 + j];
+                    seen = mv != 0xFC00u;
+                    x[v] = addMask(x[v], mv);
+                }
+                acc[p] += seen ? ex2(x[v] - rf[v].y) : 0.0f;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) acc[v] += __shfl_xor(acc[v], o);
-        if (j == 0) part[wave][8 * (v >> 2) + 4 * h + (v & 3)] = acc[v];
+    for (int p = 0; p < TP; ++p) {
+        acc[p] += __shfl_xor(acc[p], 32);
+        if (h == 0) part[wave][p][j] = acc[p];
     }
     __syncthreads();
     if (tid < 32 * KT) {
-        const int g = tid >> 5, key = (blockIdx.x * KT + g) * 32 + (tid & 31);
+        const int g = tid >> 5, w0 = g / TP * RW;
+        const long long key = (long long)(t0 + g) * 32 + (tid & 31);
         if (key < a.T) {
-            float s = part[g * RW][tid & 31];
+            float s = part[w0][g % TP][tid & 31];
 #pragma unroll
-            for (int x = 1; x < RW; ++x) s += part[g * RW + x][tid & 31];
+            for (int x = 1; x < RW; ++x) s += part[w0 + x][g % TP][tid & 31];
             const size_t at = (size_t)kvh * a.w_row + key;
             a.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], s) : s;
         }
     }
 }
 
-template <int D, bool Q4, int RW>
+template <int D, bool Q4, int RW, int TP>
 int run(const FxParams& p, hipStream_t s) {
-    constexpr int lds = WGeo<D, Q4>::Tile * (4 / RW);
-    static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_weights_kernel<D, Q4, RW>),
+    constexpr int kt = 4 / RW * TP, lds = WGeo<D, Q4>::Tile * kt;
+    static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_weights_kernel<D, Q4, RW, TP>),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds), "attn_weights: LDS size");
     if (ok) return ok;
-    const int tiles = p.T / 32 + (p.T % 32 != 0), kt = 4 / RW;
-    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW>), dim3((tiles + kt - 1) / kt, p.H_kv), dim3(256), lds, s, p);
+    const int tiles = p.T / 32 + (p.T % 32 != 0);
+    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP>), dim3((tiles + kt - 1) / kt, p.H_kv), dim3(256), lds, s, p);
     return fromHip(hipGetLastError(), "attn_weights");
 }
 
 template <int D, bool Q4>
 int runRows(const FxParams& p, hipStream_t s) {
-    if (p.rows <= 32) return run<D, Q4, 1>(p, s);
-    if (p.rows <= 64) return run<D, Q4, 2>(p, s);
-    return run<D, Q4, 4>(p, s);
+    if (p.rows <= 32) return run<D, Q4, 1, 1>(p, s);
+    if (p.rows <= 64) return run<D, Q4, 2, 1>(p, s);
+    // four tiles to a wavefront, q read a quarter as often, where that leaves a workgroup for every compute unit
+    return (long long)p.T * p.H_kv >= 128 * 256 ? run<D, Q4, 4, 4>(p, s) : run<D, Q4, 4, 1>(p, s);
 }
 
 }  // namespace

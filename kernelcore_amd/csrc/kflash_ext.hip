@@ -1,8 +1,8 @@
 // kflash_ext.hip -- flash_ext_f16 / flash_ext_q4_0 (gfx950): attention of N query tokens over T cached positions of an
-// fp16 or a 4-bit cache with shaped scores: for query row i of a KV head (kflash_ext.hpp packs tokens and the
+// fp16 or a 4-bit cache with shaped scores: for query row i of a KV head (kflash_ext_device.hpp packs tokens and the
 // group's heads into rows)
-//   x_ij = cap tanh(scale q_i.k_j / cap) - slope_i |pos_i - pos_j| + mask_ij,   o_i = sum_j 2^(y_ij - m_i) v_j / l_i,
-//   y = x log2 e, m_i = max_j y_ij, l_i = sum_j 2^(y_ij - m_i)
+//   x_ij = log2 e (cap tanh(scale q_i.k_j / cap) - slope_i |pos_i - pos_j| + mask_ij),   o_i = sum_j 2^(x_ij - m_i) v_j / l_i,
+//   m_i = max_j x_ij, l_i = sum_j 2^(x_ij - m_i)
 // over the keys that i sees, in one pass over the keys with running m and l.
 //
 // Three kernels: few rows (up to 32: single and drafted tokens), many rows (prompts), and the join of key ranges where
@@ -20,16 +20,10 @@ namespace {
 
 using namespace fx;
 
-// p in [0, 1] is split into fp16 parts at this scale, so that what the parts cannot hold is below 2^-40
-constexpr float kP = 32768.0f;
+// p in [0, 1] is split into fp16 parts at the scale 2^15, so that what the parts cannot hold is below 2^-40 (p = 2^(x - m + 15); l
+// and o carry the factor until the end)
+constexpr float kPBits = 15.0f, kPInv = 1.0f / 32768.0f;
 
-template <int N>
-__device__ __forceinline__ float pick(const float* p, int i) {
-    float r = p[0];
-#pragma unroll
-    for (int e = 1; e < N; ++e) r = i == e ? p[e] : r;
-    return r;
-}
 // The value at dd of a V row that the matrix products left out (0 where they took it).
 template <bool Q4>
 __device__ float wildValue(const char* row, int dd) {
@@ -44,88 +38,125 @@ __device__ float wildValue(const char* row, int dd) {
         return (x & 0x7C00u) == 0x7C00u ? halfBits(x) : 0.0f;
     }
 }
+// A word's infinities and NaNs as zeros.
+__device__ __forceinline__ uint32_t tameHalves(uint32_t w) {
+    const uint32_t z = wildHalves(w);
+    return w & ~((z >> 15 & 1u) * 0xFFFFu | (z >> 31) * 0xFFFF0000u);
+}
 
 // ---------------------------------------------------------------------------------------------- many rows
-// Workgroup: 128 rows of a KV head (four wavefronts of 32) over one range of keys, 32 keys at a time, which all four
-// read from LDS; two buffers, the next keys' global loads in flight in registers while the present ones are
-// computed. Matrix form (v_mfma_f32_32x32x16_f16, lane (j, h) = row j, lane half h):
+// Workgroup: 128 rows of a KV head (four wavefronts of 32 rows) over one range of keys. A step takes KS tiles of 32 keys; with
+// KS = 2 two sets of wavefronts take a tile each (two wavefronts per SIMD whose vector and matrix phases overlap, and half
+// the steps on the longest rows), joined through LDS at the end. The step's keys and values lie in LDS, two buffers, the next
+// step's global loads in flight in registers while the present one is computed. Matrix form (v_mfma_f32_32x32x16_f16, lane
+// (j, h) = row j, lane half h):
 //   S^T = K Q^T: A = key rows (LDS), B = q hi / lo (registers). Lane (j, h) holds keys 8 (v / 4) + 4 h + v % 4 of row j.
 //   O^T += V^T P^T: A = V^T through transposed LDS reads, B = p hi / lo, the score registers as they are (the products'
 //   index runs over the keys in the order those registers hold).
 // 4-bit keys and values are unpacked once per workgroup, on the way to LDS.
 template <int D, bool Q4>
 struct Geo {
+    static constexpr int KS = D == 256 ? 1 : 2;  // (256 values: one wavefront's registers fill a SIMD)
+    static constexpr int Threads = 256 * KS, TK = 32 * KS;
     static constexpr int NB = D / 32;
     static constexpr int KRow = kKeyRow<D>;
-    static constexpr int VRow = 2 * D + 32;  // two, for the transposed reads
-    static constexpr int oV = 32 * KRow, oVl = oV + 32 * VRow, oS = oV + 32 * VRow * (Q4 ? 2 : 1);
-    static constexpr int oMeta = oS + (Q4 ? NB * 128 : 0);
-    static constexpr int Buf = oMeta + 256;  // 32 positions, 32 document numbers
-    static constexpr int MapWords = 1024;    // key tiles of a range, a bit each
-    static constexpr int Lds = 2 * Buf + MapWords * 4 + 64;
+    static constexpr int VRow = 2 * D + 32;  // two pad chunks, for the transposed reads
+    static constexpr int oV = TK * KRow, oVl = oV + TK * VRow, oS = oV + TK * VRow * (Q4 ? 2 : 1);
+    static constexpr int oMeta = oS + (Q4 ? NB * TK * 4 : 0);
+    static constexpr int Buf = oMeta + TK * 8;  // positions, document numbers
+    static constexpr int MapWords = 1024;       // a range's steps, a bit each
+    static constexpr int ORow = D / 2 + 4;      // the join of the two sets: floats per lane
+    static constexpr int Main = 2 * Buf > 256 * ORow * 4 * (KS - 1) ? 2 * Buf : 256 * ORow * 4;
+    static constexpr int Lds = Main + 2 * MapWords * 4 + 64;
 };
 
 template <int D, bool Q4, bool SHAPED>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void flash_ext_kernel(FxParams a) {
+__global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void flash_ext_kernel(FxParams a) {
     using G = Geo<D, Q4>;
-    constexpr int KS = D / 16, DB = D / 32, NB = G::NB;
+    constexpr int DB = D / 32, NB = G::NB, TK = G::TK, NT = G::Threads;
     extern __shared__ int4 lds4[];
     char* lds = reinterpret_cast<char*>(lds4);
-    uint32_t* map = reinterpret_cast<uint32_t*>(lds + 2 * G::Buf);
-    int* misc = reinterpret_cast<int*>(map + G::MapWords);  // 0: largest limit, 1 / 2: least / largest document, 4 + i: wild keys
-    const int kvh = blockIdx.x, rb = (int)gridDim.y - 1 - (int)blockIdx.y, sp = blockIdx.z;
+    uint32_t* map = reinterpret_cast<uint32_t*>(lds + G::Main);  // steps with a key that some row may see
+    uint32_t* whole = map + G::MapWords;                         // steps whose keys every row sees
+    int* misc = reinterpret_cast<int*>(whole + G::MapWords);     // 0 / 1: least / largest limit, 2 / 3: document, 4 + i: wild keys
+    const int kvh = blockIdx.x, rb = (int)gridDim.y - 1 - (int)blockIdx.y, sp = blockIdx.z;  // (longest rows first)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int j = lane & 31, h = lane >> 5;
-    const Row row = rowOf(a, kvh, rb * 128 + wave * 32 + j);
+    const int j = lane & 31, h = lane >> 5, rw = wave & 3, ks = wave >> 2;
+    const int r = rb * 128 + rw * 32 + j;
+    const Row row = rowOf(a, kvh, r);
     const int wmin = waveMin(row.live ? row.limit : INT_MAX), wmax = waveMax(row.live ? row.limit : -1);
 
     if (tid == 0) {
-        misc[0] = -1;
-        misc[1] = INT_MAX;
-        misc[2] = INT_MIN;
+        misc[0] = INT_MAX;
+        misc[1] = -1;
+        misc[2] = INT_MAX;
+        misc[3] = INT_MIN;
     }
-    if (tid >= 4 && tid < 8) misc[tid] = 0;
+    if (tid >= 4 && tid < 10) misc[tid] = 0;
     __syncthreads();
-    if (lane == 0) atomicMax(&misc[0], wmax);
-    if (SHAPED && a.qdoc && row.live) {
-        atomicMin(&misc[1], row.doc);
-        atomicMax(&misc[2], row.doc);
+    if (lane == 0 && ks == 0) {
+        atomicMin(&misc[0], wmin);
+        atomicMax(&misc[1], wmax);
+    }
+    if (SHAPED && a.qdoc && row.live && ks == 0) {
+        atomicMin(&misc[2], row.doc);
+        atomicMax(&misc[3], row.doc);
     }
     __syncthreads();
-    const int bmax = __builtin_amdgcn_readfirstlane(misc[0]);
+    const int bmax = __builtin_amdgcn_readfirstlane(misc[1]);
 
-    // this range's key tiles
+    // this range's steps
     const bool meta = SHAPED && (a.kpos || a.kdoc);
-    const int t0 = sp * a.per * 2;
-    int t1 = (int)min((long long)t0 + 2LL * a.per, ((long long)a.T + 31) / 32);
-    if (!(SHAPED && a.kpos)) t1 = bmax < 0 ? t0 : min(t1, bmax / 32 + 1);
     const int* kpos = SHAPED && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
     const int* kdoc = SHAPED && a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
+    const int t0 = sp * a.per * (64 / TK);
+    int t1 = (int)min((long long)t0 + (long long)a.per * (64 / TK), ((long long)a.T + TK - 1) / TK);
+    if (!kpos) t1 = bmax < 0 ? t0 : min(t1, bmax / TK + 1);
     const bool mapped = meta && t1 - t0 <= 32 * G::MapWords;
     if constexpr (SHAPED) {
-        if (mapped) {  // the tiles that hold a position some row may see, in a document between the rows' least and largest
-            const int dmin = misc[1], dmax = misc[2];
-            for (int i = tid; i * 32 < t1 - t0; i += 256) map[i] = 0;
+        if (mapped) {  // four keys a lane, all loads issued before the ballots
+            const int bmin = misc[0], dmin = misc[2], dmax = misc[3];
+            for (int i = tid; i * 32 < t1 - t0; i += NT) map[i] = whole[i] = 0;
             __syncthreads();
-            for (int t = t0 + 2 * wave; t < t1; t += 8) {
-                const int key = t * 32 + lane;
-                bool ok = key < a.T;
-                if (ok && kpos) {
-                    const int p = kpos[key];
-                    ok = p >= 0 && p <= bmax;
+            constexpr int LPT = TK / 4;  // lanes to a step
+            const int key1 = min(a.T, t1 * TK);
+            for (int key = t0 * TK + 4 * tid; key - 4 * lane < key1; key += 4 * NT) {
+                bool some = false, all = true;
+                int4 p = {key, key + 1, key + 2, key + 3}, x = {dmin, dmin, dmin, dmin};
+                if (key + 3 < key1) {
+                    if (kpos) p = *reinterpret_cast<const int4a4*>(kpos + key);
+                    if (kdoc) x = *reinterpret_cast<const int4a4*>(kdoc + key);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (key + e < key1) {
+                            if (kpos) (&p.x)[e] = kpos[key + e];
+                            if (kdoc) (&x.x)[e] = kdoc[key + e];
+                        } else {
+                            (&p.x)[e] = -1;
+                        }
+                    }
                 }
-                if (ok && kdoc) {
-                    const int x = kdoc[key];
-                    ok = x >= dmin && x <= dmax;
+                const bool docs = kdoc != nullptr;
+                const int pp[4] = {p.x, p.y, p.z, p.w}, xx[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool in = pp[e] >= 0 && pp[e] <= bmax && (!docs || (xx[e] >= dmin && xx[e] <= dmax));
+                    some |= in;
+                    all &= in && pp[e] <= bmin && (!docs || dmin == dmax);
                 }
-                const unsigned long long b = __ballot(ok);
-                const uint32_t bits = ((uint32_t)b ? 1u : 0u) | ((uint32_t)(b >> 32) ? 2u : 0u);
-                if (lane == 0 && bits) atomicOr(&map[(t - t0) >> 5], bits << ((t - t0) & 31));
+                const unsigned long long group = ((1ull << LPT) - 1) << (lane / LPT * LPT);
+                const unsigned long long s = __ballot(some) & group, w = __ballot(all) & group;
+                const int at = (key - t0 * TK) / TK;
+                if (lane % LPT == 0 && s) {
+                    atomicOr(&map[at >> 5], 1u << (at & 31));
+                    if (w == group) atomicOr(&whole[at >> 5], 1u << (at & 31));
+                }
             }
             __syncthreads();
         }
     }
-    auto next = [&](int t) -> int {  // the first tile from t on that is to be computed; t1 if none
+    auto next = [&](int t) -> int {  // the first step from t on that is to be computed; t1 if none
         if (!mapped) return min(t, t1);
         while (t < t1) {
             const uint32_t w = __builtin_amdgcn_readfirstlane(map[(t - t0) >> 5]) >> ((t - t0) & 31);
@@ -135,46 +166,40 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void flash_ext_kernel(FxPara
         return t1;
     };
 
-    h8 qh[KS], ql[KS];
-    const float c = loadRow32<D>(a, row, h, qh, ql);
-    const Shape shape = shapeOf(a);
-    const unsigned short* mrow = SHAPED && a.mask ? a.mask + (size_t)row.token * a.m_row2 : nullptr;
-
-    // ---- staging: 16-byte chunks (fp16) or whole blocks (4-bit) of the tile's K and V rows, through registers
-    constexpr int NL = Q4 ? (64 * NB + 255) / 256 : D / 32;  // chunks or blocks per thread
+    // ---- staging: 16-byte chunks (fp16) or whole blocks (4-bit) of the step's K and V rows, through registers
+    constexpr int PR = Q4 ? NB : D / 8, IT = TK * PR;       // of a row, of the step's K (and V)
+    constexpr bool Once = 2 * IT <= NT;                     // (4 bits: the first IT threads K, the next V)
+    constexpr int NL = Once ? 1 : 2 * IT / NT;
+    static_assert(Once || IT % NT == 0, "the step's rows over the threads");
     u4 raw[NL];
     uint32_t rsc[Q4 ? NL : 1];
     int rmeta = 0;
     const char* kb = a.k + (size_t)kvh * a.k_head;
     const char* vb = a.v + (size_t)kvh * a.v_head;
+    auto isV = [&](int n) { return Once ? tid >= IT : n >= NL / 2; };
+    auto item = [&](int n) { return Once ? tid % IT : tid + NT * (n >= NL / 2 ? n - NL / 2 : n); };
+    const bool idle = Once && tid >= 2 * IT;
     auto fetch = [&](int t) {
-        if constexpr (Q4) {
 #pragma unroll
-            for (int n = 0; n < NL; ++n) {
-                const int i = tid + 256 * n;
-                if (i < 64 * NB) {
-                    const bool isv = i >= 32 * NB;
-                    const int ii = isv ? i - 32 * NB : i, key = t * 32 + ii / NB, b = ii % NB;
-                    const size_t r = min(key, a.T - 1);
-                    const char* p = (isv ? vb + r * a.v_row : kb + r * a.k_row) + 18 * b;
-                    raw[n] = *reinterpret_cast<const u4a2*>(p + 2);
-                    rsc[n] = isv && key >= a.T ? 0u : loadHalf(p);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NL; ++n) {  // the first half of the chunks K, the second V
-                const bool isv = n >= NL / 2;
-                const int i = tid + 256 * (isv ? n - NL / 2 : n), key = t * 32 + i / (D / 8), ch = i % (D / 8);
-                const size_t r = min(key, a.T - 1);
-                raw[n] = *reinterpret_cast<const u4a4*>((isv ? vb + r * a.v_row : kb + r * a.k_row) + 16 * ch);
-                if (isv && key >= a.T) raw[n] = u4{0, 0, 0, 0};
+        for (int n = 0; n < NL; ++n) {
+            if (idle) break;
+            const bool v = isV(n);
+            const int i = item(n), key = t * TK + i / PR, part = i % PR;
+            const size_t at = min(key, a.T - 1);
+            const char* p = (v ? vb + at * a.v_row : kb + at * a.k_row) + (Q4 ? 18 : 16) * part;
+            if constexpr (Q4) {
+                raw[n] = *reinterpret_cast<const u4a2*>(p + 2);
+                rsc[n] = loadHalf(p);
+                if (v && key >= a.T) rsc[n] = 0;
+            } else {
+                raw[n] = *reinterpret_cast<const u4a4*>(p);
+                if (v && key >= a.T) raw[n] = u4{0, 0, 0, 0};
             }
         }
         if constexpr (SHAPED) {
-            if (meta && tid < 64) {
-                const int key = t * 32 + (tid & 31);
-                if (tid < 32) {
+            if (meta && tid < 2 * TK) {
+                const int key = t * TK + tid % TK;
+                if (tid < TK) {
                     const int p = key < a.T ? (kpos ? kpos[key] : key) : kNoKey;
                     rmeta = p < 0 ? kNoKey : p;
                 } else {
@@ -184,199 +209,212 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void flash_ext_kernel(FxPara
         }
     };
     auto store = [&](char* buf, int* wild) {
-        if constexpr (Q4) {
 #pragma unroll
-            for (int n = 0; n < NL; ++n) {
-                const int i = tid + 256 * n;
-                if (i < 64 * NB) {
-                    const bool isv = i >= 32 * NB;
-                    const int ii = isv ? i - 32 * NB : i, key = ii / NB, b = ii % NB;
-                    h8 code[4];
-                    blockCodes(raw[n], code);
-                    if (!isv) {
-                        h8* p = reinterpret_cast<h8*>(buf + key * G::KRow + 64 * b);
+        for (int n = 0; n < NL; ++n) {
+            if (idle) break;
+            const bool v = isV(n);
+            const int i = item(n), key = i / PR, part = i % PR;
+            if constexpr (Q4) {
+                h8 code[4];
+                blockCodes(raw[n], code);
+                if (!v) {
+                    h8* p = reinterpret_cast<h8*>(buf + key * G::KRow + 64 * part);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) p[e] = code[e];
-                        reinterpret_cast<float*>(buf + G::oS)[b * 32 + key] = halfBits(rsc[n]);
-                    } else {
-                        uint32_t s = rsc[n];
-                        if (wildScale(s)) {
-                            s = 0;
-                            atomicOr(wild, 1 << key);
-                        }
-                        const _Float16 d = __builtin_bit_cast(_Float16, (unsigned short)s);
-                        const _Float16 dh = __builtin_bit_cast(_Float16, (unsigned short)(s & 0xFFF0u));
-                        const _Float16 dl = d - dh;
-                        h8* p = reinterpret_cast<h8*>(buf + G::oV + key * G::VRow + 64 * b);
-                        h8* pl = reinterpret_cast<h8*>(buf + G::oVl + key * G::VRow + 64 * b);
+                    for (int e = 0; e < 4; ++e) p[e] = code[e];
+                    reinterpret_cast<float*>(buf + G::oS)[part * TK + key] = halfBits(rsc[n]);
+                } else {
+                    uint32_t s = rsc[n];
+                    if (wildScale(s)) {
+                        s = 0;
+                        atomicOr(wild + (key >> 5), 1 << (key & 31));
+                    }
+                    const _Float16 d1 = __builtin_bit_cast(_Float16, (unsigned short)s);
+                    const h8 d = {d1, d1, d1, d1, d1, d1, d1, d1};
+                    h8* p = reinterpret_cast<h8*>(buf + G::oV + key * G::VRow + 64 * part);
+                    h8* pl = reinterpret_cast<h8*>(buf + G::oVl + key * G::VRow + 64 * part);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            p[e] = code[e] * dh;
-                            pl[e] = code[e] * dl;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const h8 x = code[e] * d;
+                        p[e] = x;
+                        pl[e] = __builtin_elementwise_fma(code[e], d, -x);
                     }
                 }
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NL; ++n) {
-                const bool isv = n >= NL / 2;
-                const int i = tid + 256 * (isv ? n - NL / 2 : n), key = i / (D / 8), ch = i % (D / 8);
+            } else {
                 u4 x = raw[n];
-                if (isv) {
-                    const uint32_t any = wildHalves(x[0]) | wildHalves(x[1]) | wildHalves(x[2]) | wildHalves(x[3]);
-                    if (any) {
+                if (v && (wildHalves(x[0]) | wildHalves(x[1]) | wildHalves(x[2]) | wildHalves(x[3]))) {
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const uint32_t z = wildHalves(x[w]);
-                            x[w] &= ~((z >> 15 & 1u) * 0xFFFFu | (z >> 31) * 0xFFFF0000u);
-                        }
-                        atomicOr(wild, 1 << key);
-                    }
+                    for (int w = 0; w < 4; ++w) x[w] = tameHalves(x[w]);
+                    atomicOr(wild + (key >> 5), 1 << (key & 31));
                 }
-                *reinterpret_cast<u4*>(buf + (isv ? G::oV + key * G::VRow : key * G::KRow) + 16 * ch) = x;
+                *reinterpret_cast<u4*>(buf + (v ? G::oV + key * G::VRow : key * G::KRow) + 16 * part) = x;
             }
         }
         if constexpr (SHAPED)
-            if (meta && tid < 64) reinterpret_cast<int*>(buf + G::oMeta)[tid] = rmeta;
+            if (meta && tid < 2 * TK) reinterpret_cast<int*>(buf + G::oMeta)[tid] = rmeta;
     };
 
-    f32x16 zero;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) zero[v] = 0.0f;
+    int t = next(t0);
+    if (t < t1) fetch(t);
+    h8 qh[D / 16], ql[D / 16];
+    const float c = loadRow32<D>(a, row, h, qh, ql), c2 = factor2(c);
+    const Shape shape = SHAPED ? shapeOf(a) : Shape{};
+    const unsigned short* mrow = SHAPED && a.mask ? a.mask + (size_t)row.token * a.m_row2 : nullptr;
+
     f32x16 o[DB];
 #pragma unroll
-    for (int t = 0; t < DB; ++t) o[t] = zero;
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-
-    int t = next(t0);
-    int slot = 0;  // of the wild-key words: three in turn, the one two tiles on is cleared while none reads it
-    if (t < t1) {
-        fetch(t);
-        store(lds, &misc[4]);
-    }
+    int slot = 0;  // of the wild-key words: three pairs in turn, the one two steps on is cleared while none reads it
+    if (t < t1) store(lds, &misc[4]);
     __syncthreads();
-    const int vlane = (4 * (lane >> 5) + ((lane & 15) >> 2)) * (G::VRow / 2) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int vlane = ks * 32 * (G::VRow / 2) + (4 * (lane >> 5) + ((lane & 15) >> 2)) * (G::VRow / 2) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     for (int it = 0; t < t1; ++it) {
         const int tn = next(t + 1);
         char* cur = lds + (it & 1) * G::Buf;
         if (tn < t1) fetch(tn);
-        const bool full = !meta && !(SHAPED && mrow) && t * 32 + 31 <= wmin && t * 32 + 31 < a.T;
-        if (full || meta || t * 32 <= wmax) {
+        const int k0 = t * TK + 32 * ks;  // this wavefront's 32 keys
+        bool full = !(SHAPED && mrow) && k0 + 31 < a.T;
+        if (meta) full = full && mapped && (__builtin_amdgcn_readfirstlane(whole[(t - t0) >> 5]) >> ((t - t0) & 31) & 1);
+        else full = full && k0 + 31 <= wmin;
+        if (full || meta || k0 <= wmax) {
             MaskWords mk;
             if constexpr (SHAPED) {
-                if (mrow) mk.load(mrow, t, h, a.T);
+                if (mrow) mk.load(mrow, t * (TK / 32) + ks, h, a.T);
             }
             float x[16];
-            keyScores<D, Q4>(cur, cur + G::oS, j, h, qh, ql, x);
-            if constexpr (SHAPED) {
-                shapeScores(x, c, shape, row, meta ? reinterpret_cast<const int*>(cur + G::oMeta) : nullptr, mrow ? &mk : nullptr, t, h);
-            } else {
-                const float c2 = c * kLog2e;
+            keyScores<D, Q4, TK>(cur + ks * 32 * G::KRow, cur + G::oS + ks * 128, j, h, qh, ql, x);
+            const int* kp = reinterpret_cast<const int*>(cur + G::oMeta) + 32 * ks + 4 * h;
+            if constexpr (SHAPED) shapeScores(x, c, shape, row, meta ? kp : nullptr, k0 + 4 * h, mrow ? &mk : nullptr);
+            if (!full) {
+                if (meta) {
+                    hideKeys(x, row, kp, kp + TK);
+                } else {
+                    const int last = min(row.limit, a.T - 1) - k0 - 4 * h;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] *= c2;
-            }
-            if (!meta && !full) {
-                const int last = min(row.limit, a.T - 1) - t * 32 - 4 * h;
-#pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] = 8 * (v >> 2) + (v & 3) <= last ? x[v] : -INFINITY;
+                    for (int v = 0; v < 16; ++v) x[v] = 8 * (v >> 2) + (v & 3) <= last ? x[v] : -INFINITY;
+                }
             }
             float bm = x[0];
 #pragma unroll
             for (int v = 1; v < 16; ++v) bm = fmaxf(bm, x[v]);
-            bm = fmaxf(bm, __shfl_xor(bm, 32));
+            bm = swap32Max(bm);
+            if constexpr (!SHAPED) bm *= c2;
             const float mn = fmaxf(m, bm);
-            const float ms = mn == -INFINITY ? 0.0f : mn;  // (nothing seen yet: every p is 0)
+            const float off = kPBits - (mn == -INFINITY ? 0.0f : mn);  // (nothing seen yet: every p is 0)
             if (__any(mn > m)) {
-                const float alpha = ex2(m - ms);
+                const float alpha = ex2(m + off - kPBits);
                 l *= alpha;
 #pragma unroll
-                for (int t2 = 0; t2 < DB; ++t2)
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) o[t2][v] *= alpha;
+                    for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
                 m = mn;
             }
-            h8 ph[2], pl[2];
             float ls = 0.0f;
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                x[v] = ex2(x[v] - ms);
+                x[v] = ex2(SHAPED ? x[v] + off : fmaf(x[v], c2, off));
                 ls += x[v];
             }
             l += ls;
-            uint32_t wild = __builtin_amdgcn_readfirstlane(misc[4 + slot]);
+            uint32_t wild = __builtin_amdgcn_readfirstlane(misc[4 + 2 * slot + ks]);
             while (__builtin_expect(wild != 0, 0)) {  // values that are no matrix operands, for the rows that see them
                 const int key = __builtin_ctz(wild);
                 wild &= wild - 1;
-                const float p = __shfl(pick<16>(x, (key >> 3) * 4 + (key & 3)), j + 32 * ((key >> 2) & 1)) * kP;
-                const char* vr = vb + (size_t)(t * 32 + key) * a.v_row;
+                const float p = __shfl(pick<16>(x, (key >> 3) * 4 + (key & 3)), j + 32 * ((key >> 2) & 1));
+                if (!__any(p != 0.0f)) continue;
+                const char* vr = vb + (size_t)(k0 + key) * a.v_row;
 #pragma unroll
-                for (int t2 = 0; t2 < DB; ++t2)
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) {
-                        const float z = wildValue<Q4>(vr, 32 * t2 + 8 * (v >> 2) + 4 * h + (v & 3));
-                        if (p != 0.0f && z != 0.0f) o[t2][v] = fmaf(p, z, o[t2][v]);
+                        const float z = wildValue<Q4>(vr, 32 * d + 8 * (v >> 2) + 4 * h + (v & 3));
+                        if (p != 0.0f && z != 0.0f) o[d][v] = fmaf(p, z, o[d][v]);
                     }
             }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float ps = x[v] * kP;
-                const _Float16 hi = (_Float16)ps;
-                ph[v >> 3][v & 7] = hi;
-                pl[v >> 3][v & 7] = (_Float16)(ps - (float)hi);
-            }
+            h8 ph[2], pl[2];
+            splitParts<16>(x, ph, pl);
             const _Float16* vcol = reinterpret_cast<const _Float16*>(cur + G::oV) + vlane;
 #pragma unroll
             for (int mm = 0; mm < 2; ++mm)
 #pragma unroll
-                for (int t2 = 0; t2 < DB; ++t2) {
-                    const _Float16* vp = vcol + 16 * mm * (G::VRow / 2) + 32 * t2;
+                for (int d = 0; d < DB; ++d) {
+                    const _Float16* vp = vcol + 16 * mm * (G::VRow / 2) + 32 * d;
                     const s4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)vp);
                     const s4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(vp + 8 * (G::VRow / 2)));
                     const h8 va = __builtin_bit_cast(h8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[t2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[mm], o[t2], 0, 0, 0);
-                    o[t2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[mm], o[t2], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[mm], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[mm], o[d], 0, 0, 0);
                     if constexpr (Q4) {
                         const _Float16* vq = vp + (G::oVl - G::oV) / 2;
                         const s4 y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)vq);
                         const s4 y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(vq + 8 * (G::VRow / 2)));
                         const h8 vl = __builtin_bit_cast(h8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        o[t2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[mm], o[t2], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[mm], o[d], 0, 0, 0);
                     }
                 }
         }
-        // the next tile into the other buffer (read last two tiles ago, before the barrier below)
+        // the next step into the other buffer (last read before the barrier that ended the step before this one)
         const int sn = slot == 2 ? 0 : slot + 1, sc = sn == 2 ? 0 : sn + 1;
-        if (tn < t1) store(lds + ((it + 1) & 1) * G::Buf, &misc[4 + sn]);
-        if (tid == 0) misc[4 + sc] = 0;
+        if (tn < t1) store(lds + ((it + 1) & 1) * G::Buf, &misc[4 + 2 * sn]);
+        if (tid < 2) misc[4 + 2 * sc + tid] = 0;
         slot = sn;
         t = tn;
         __syncthreads();
     }
 
     l += __shfl_xor(l, 32);
+    if constexpr (G::KS == 2) {  // the second set's (o, m, l) to the first
+        float* mg = reinterpret_cast<float*>(lds) + (size_t)(rw * 64 + lane) * G::ORow;
+        if (ks == 1) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4*>(mg + 16 * d + 4 * g) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+            mg[D / 2] = m;
+            mg[D / 2 + 1] = l;
+        }
+        __syncthreads();
+        if (ks == 1) return;
+        const float m1 = mg[D / 2], l1 = mg[D / 2 + 1], M = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.0f : ex2(m - M), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - M);
+        l = l * f0 + l1 * f1;
+        m = M;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(mg + 16 * d + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d][4 * g + e] = o[d][4 * g + e] * f0 + y[e] * f1;
+            }
+    }
     if (!row.live) return;
-    const int r = rb * 128 + wave * 32 + j;
     float* dst;
     float f;
     if (a.splits == 1) {
         dst = a.out + ((size_t)row.token * a.H + row.head) * D;
-        f = l == 0.0f ? 0.0f : 1.0f / (l * kP);
-        if (a.lse && h == 0) a.lse[(size_t)row.token * a.H + row.head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l));
+        f = l == 0.0f ? 0.0f : 1.0f / l;
+        if (a.lse && h == 0) a.lse[(size_t)row.token * a.H + row.head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l * kPInv));
     } else {
-        dst = a.part + (((size_t)sp * a.H_kv + kvh) * a.rows + r) * (D + 2);
-        f = 1.0f / kP;
+        const size_t at = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
+        dst = a.part + at * D;
+        f = kPInv;
         if (h == 0) {
-            dst[D] = m;
-            dst[D + 1] = l;
+            float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * at;
+            ml[0] = m;
+            ml[1] = l * kPInv;
         }
     }
 #pragma unroll
-    for (int t2 = 0; t2 < DB; ++t2)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const f32x4 y = {o[t2][4 * g] * f, o[t2][4 * g + 1] * f, o[t2][4 * g + 2] * f, o[t2][4 * g + 3] * f};
-            *reinterpret_cast<f4a4*>(dst + 32 * t2 + 8 * g + 4 * h) = y;
+            const f32x4 y = {o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f};
+            *reinterpret_cast<f4a4*>(dst + 32 * d + 8 * g + 4 * h) = y;
         }
 }
 
@@ -395,7 +433,8 @@ struct FewGeo {
     static constexpr int Row = D / 2 + 16;   // LDS bytes of a key's codes
     static constexpr int VRow = 2 * D + 32;  // of an fp16 row
     static constexpr int oV = 64 * Row, oS = 2 * oV, oD = oS + NB * 256;  // 4-bit: codes of K, of V, K scales, V scales
-    static constexpr int Wave = Q4 ? oD + NB * 256 : 32 * VRow;
+    static constexpr int oMeta = Q4 ? oD + NB * 128 : 32 * VRow;  // positions, document numbers
+    static constexpr int Wave = oMeta + TK * 8;
     static constexpr int ORow = D + 4;       // join: floats per row
     static constexpr int Join = 4 * NR * 16 * (ORow + 2) * 4;
     static constexpr int Lds = 4 * Wave > Join ? 4 * Wave : Join;
@@ -418,6 +457,68 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int i = lane & 15, kg = lane >> 4;
     char* mine = lds + wave * G::Wave;
+    const char* kb = a.k + (size_t)kvh * a.k_head;
+    const char* vb = a.v + (size_t)kvh * a.v_head;
+    const int t0 = sp * a.per * (64 / TK);
+    int t1 = (int)min((long long)t0 + (long long)a.per * (64 / TK), ((long long)a.T + TK - 1) / TK);
+
+    const bool meta = SHAPED && (a.kpos || a.kdoc);
+    const int* kpos = SHAPED && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
+    const int* kdoc = SHAPED && a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
+
+    // a tile's loads. 4-bit: blocks lane + 64 n of the tile's 64 NB. fp16: K as the A operand [u][b], V chunks lane + 64 n.
+    // Addresses: the tile's first row (the same for the wavefront) + the lane's share; rows past the end reread the last one.
+    constexpr int NV = Q4 ? NB : 2 * NB, PR = Q4 ? NB : D / 8;  // V items per lane; items of a row
+    u4 kr[NV], vr[NV];
+    uint32_t kscale[Q4 ? NB : 1], vscale[Q4 ? NB : 1];
+    const long long klane = Q4 ? (long long)(lane / PR) * a.k_row + 18 * (lane % PR) : (long long)i * a.k_row + 16 * kg;
+    const long long vlane = (long long)(lane / PR) * a.v_row + (Q4 ? 18 : 16) * (lane % PR);
+    int rkp = 0, rkd = 0;
+    auto fetch = [&](int t) {
+        const long long row0 = (long long)t * TK;
+        if constexpr (SHAPED) {
+            if (meta && lane < TK) {
+                const int key = (int)row0 + lane;
+                rkp = key < a.T ? (kpos ? kpos[key] : key) : kNoKey;
+                rkd = kdoc && key < a.T ? kdoc[key] : 0;
+            }
+        }
+        if (row0 + TK <= a.T) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const char* vp = vb + (row0 + 64 / PR * n) * a.v_row + vlane;
+                if constexpr (Q4) {
+                    const char* kp = kb + (row0 + 64 / PR * n) * a.k_row + klane;
+                    kr[n] = *reinterpret_cast<const u4a2*>(kp + 2);
+                    kscale[n] = loadHalf(kp);
+                    vr[n] = *reinterpret_cast<const u4a2*>(vp + 2);
+                    vscale[n] = loadHalf(vp);
+                } else {
+                    kr[n] = *reinterpret_cast<const u4a4*>(kb + (row0 + 16 * (n / NB)) * a.k_row + 64 * (n % NB) + klane);
+                    vr[n] = *reinterpret_cast<const u4a4*>(vp);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int vkey = (int)row0 + (lane + 64 * n) / PR, part = (lane + 64 * n) % PR;
+                const char* vp = vb + (size_t)min(vkey, a.T - 1) * a.v_row + (Q4 ? 18 : 16) * part;
+                if constexpr (Q4) {
+                    const char* kp = kb + (size_t)min(vkey, a.T - 1) * a.k_row + 18 * part;
+                    kr[n] = *reinterpret_cast<const u4a2*>(kp + 2);
+                    kscale[n] = loadHalf(kp);
+                    vr[n] = *reinterpret_cast<const u4a2*>(vp + 2);
+                    vscale[n] = vkey < a.T ? loadHalf(vp) : 0u;
+                } else {
+                    const int kkey = min((int)row0 + 16 * (n / NB) + i, a.T - 1);
+                    kr[n] = *reinterpret_cast<const u4a4*>(kb + (size_t)kkey * a.k_row + 64 * (n % NB) + 16 * kg);
+                    vr[n] = *reinterpret_cast<const u4a4*>(vp);
+                    if (vkey >= a.T) vr[n] = u4{0, 0, 0, 0};
+                }
+            }
+        }
+    };
+
     Row row[NR];
     int wmin = INT_MAX, wmax = -1;
 #pragma unroll
@@ -430,12 +531,9 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     }
     wmin = waveMin(wmin);
     wmax = waveMax(wmax);
-    const bool meta = SHAPED && (a.kpos || a.kdoc);
-    const int* kpos = SHAPED && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
-    const int* kdoc = SHAPED && a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
-    const int t0 = sp * a.per * (64 / TK);
-    int t1 = (int)min((long long)t0 + (long long)a.per * (64 / TK), ((long long)a.T + TK - 1) / TK);
     if (!kpos) t1 = wmax < 0 ? t0 : min(t1, wmax / TK + 1);
+    int t = t0 + wave;
+    if (t < t1) fetch(t);
 
     // q as the B operand of step b (32 values): fp16 keys: values 32 b + 8 kg + e; 4-bit keys: the order nibbles() gives
     h8 qh[NR][NB], ql[NR][NB];
@@ -454,8 +552,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 top = fmaxf(top, fabsf(x[b][e]));
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = swap32Max(swap16Max(top));
         const QScale qs = qScale(top, a.scale);
         c[n] = qs.c;
 #pragma unroll
@@ -468,50 +565,16 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 ql[n][b][e] = lo;
             }
     }
-    const Shape shape = shapeOf(a);
-    const char* kb = a.k + (size_t)kvh * a.k_head;
-    const char* vb = a.v + (size_t)kvh * a.v_head;
+    const Shape shape = SHAPED ? shapeOf(a) : Shape{};
+    const NibbleMagic magic = nibbleMagic();
 
-    // a tile's loads. 4-bit: blocks lane + 64 n of the tile's 64 NB. fp16: K as the A operand [u][b], V chunks lane + 64 n.
-    u4 kr[Q4 ? NB : 2 * NB], vr[Q4 ? NB : 2 * NB];
-    uint32_t ks[Q4 ? NB : 1], vs[Q4 ? NB : 1];
-    auto fetch = [&](int t) {
-        if constexpr (Q4) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const int ii = lane + 64 * n, key = t * 64 + ii / NB, b = ii % NB;
-                const size_t r = min(key, a.T - 1);
-                const char *kp = kb + r * a.k_row + 18 * b, *vp = vb + r * a.v_row + 18 * b;
-                kr[n] = *reinterpret_cast<const u4a2*>(kp + 2);
-                ks[n] = loadHalf(kp);
-                vr[n] = *reinterpret_cast<const u4a2*>(vp + 2);
-                vs[n] = key < a.T ? loadHalf(vp) : 0u;
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const size_t r = min(t * 32 + 16 * u + i, a.T - 1);
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    kr[u * NB + b] = *reinterpret_cast<const u4a4*>(kb + r * a.k_row + 64 * b + 16 * kg);
-            }
-#pragma unroll
-            for (int n = 0; n < 2 * NB; ++n) {
-                const int ii = lane + 64 * n, key = t * 32 + ii / (D / 8), ch = ii % (D / 8);
-                const size_t r = min(key, a.T - 1);
-                vr[n] = *reinterpret_cast<const u4a4*>(vb + r * a.v_row + 16 * ch);
-                if (key >= a.T) vr[n] = u4{0, 0, 0, 0};
-            }
-        }
-    };
-
-    f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 o[NR][DT];
     float m[NR], l[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[n][t] = zero;
+        for (int d = 0; d < DT; ++d) o[n][d] = zero;
         m[n] = -INFINITY;
         l[n] = 0.0f;
     }
@@ -520,72 +583,67 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     const int xn = i & 7, en = 2 * (xn & 3) + (xn >> 2);
     const int trow = 32 * (i >> 3) + 16 * (en >> 2) + 4 * kg + (en & 3);
 
-    int t = t0 + wave;
-    if (t < t1) fetch(t);
     for (; t < t1; t += 4) {
         bool wild = false;
         h8 ka[Q4 ? 1 : 2 * NB];
-        if constexpr (Q4) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const int ii = lane + 64 * n, key = ii / NB, b = ii % NB;
-                *reinterpret_cast<u4*>(mine + key * G::Row + 16 * b) = kr[n];
-                *reinterpret_cast<u4*>(mine + G::oV + key * G::Row + 16 * b) = vr[n];
-                reinterpret_cast<float*>(mine + G::oS)[b * 64 + key] = halfBits(ks[n]);
-                uint32_t s = vs[n];
+        for (int n = 0; n < NV; ++n) {
+            const int key = (lane + 64 * n) / PR, part = (lane + 64 * n) % PR;
+            if constexpr (Q4) {
+                *reinterpret_cast<u4*>(mine + key * G::Row + 16 * part) = kr[n];
+                *reinterpret_cast<u4*>(mine + G::oV + key * G::Row + 16 * part) = vr[n];
+                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = halfBits(kscale[n]);
+                uint32_t s = vscale[n];
                 if (wildScale(s)) {
                     s = 0;
                     wild = true;
                 }
-                const uint32_t dh = s & 0xFFF0u;
-                const _Float16 dl = __builtin_bit_cast(_Float16, (unsigned short)s) - __builtin_bit_cast(_Float16, (unsigned short)dh);
                 // in the order of the products: [block][tile half][kg][16-key half, key % 4]
-                const int at = ((b * 2 + (key >> 5)) * 4 + ((key & 15) >> 2)) * 8 + 4 * ((key >> 4) & 1) + (key & 3);
-                unsigned short* vd = reinterpret_cast<unsigned short*>(mine + G::oD);
-                vd[at] = (unsigned short)dh;
-                vd[64 * NB + at] = __builtin_bit_cast(unsigned short, dl);
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < 2 * NB; ++n) {
-                const int ii = lane + 64 * n, key = ii / (D / 8), ch = ii % (D / 8);
+                const int at = ((part * 2 + (key >> 5)) * 4 + ((key & 15) >> 2)) * 8 + 4 * ((key >> 4) & 1) + (key & 3);
+                reinterpret_cast<unsigned short*>(mine + G::oD)[at] = (unsigned short)s;
+            } else {
                 u4 x = vr[n];
-                const uint32_t any = wildHalves(x[0]) | wildHalves(x[1]) | wildHalves(x[2]) | wildHalves(x[3]);
-                if (any) {
+                if (wildHalves(x[0]) | wildHalves(x[1]) | wildHalves(x[2]) | wildHalves(x[3])) {
                     wild = true;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t z = wildHalves(x[w]);
-                        x[w] &= ~((z >> 15 & 1u) * 0xFFFFu | (z >> 31) * 0xFFFF0000u);
-                    }
+                    for (int w = 0; w < 4; ++w) x[w] = tameHalves(x[w]);
                 }
-                *reinterpret_cast<u4*>(mine + key * G::VRow + 16 * ch) = x;
+                *reinterpret_cast<u4*>(mine + key * G::VRow + 16 * part) = x;
                 ka[n] = __builtin_bit_cast(h8, kr[n]);
             }
         }
-        const bool more = t + 4 < t1;
-        if (more) fetch(t + 4);
+        if constexpr (SHAPED) {
+            if (meta && lane < TK) {
+                int* mt = reinterpret_cast<int*>(mine + G::oMeta);
+                mt[lane] = rkp < 0 ? kNoKey : rkp;
+                mt[TK + lane] = rkd;
+            }
+        }
+        if (t + 4 < t1) fetch(t + 4);
         waveLds();
         float x[NR][U * 4];
         if constexpr (Q4) {
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int v = 0; v < U * 4; ++v) x[n][v] = 0.0f;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                f32x4 s[NR][NB];  // all blocks' products before their sums are taken: the matrix unit's latency overlaps
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const h8 kk = nibbles(*reinterpret_cast<const uint32_t*>(mine + (16 * u + i) * G::Row + 16 * b + 4 * kg));
-                    const f32x4 d = *reinterpret_cast<const f32x4*>(mine + G::oS + (b * 64 + 16 * u + 4 * kg) * 4);
+                    const h8 kk = nibbles(*reinterpret_cast<const uint32_t*>(mine + (16 * u + i) * G::Row + 16 * b + 4 * kg), magic);
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
-                        f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[n][b], zero, 0, 0, 0);
-                        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[n][b], s, 0, 0, 0);
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) x[n][4 * u + v] = fmaf(d[v], s[v], x[n][4 * u + v]);
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[n][b], zero, 0, 0, 0);
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[n][b], s[n][b], 0, 0, 0);
                     }
                 }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const f32x4 d = *reinterpret_cast<const f32x4*>(mine + G::oS + (b * 64 + 16 * u + 4 * kg) * 4);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) x[n][4 * u + v] = b ? fmaf(d[v], s[n][b][v], x[n][4 * u + v]) : d[v] * s[n][b][v];
+                }
+            }
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -605,59 +663,70 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         h8 ph[NR][TT], pl[NR][TT];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
+            const float c2 = factor2(c[n]);
             if constexpr (SHAPED) {
+                if (shape.inv_cap > 0.0f) {
+                    capScores<U * 4>(x[n], c[n] * shape.inv_cap, shape);
+                } else {
 #pragma unroll
-                for (int v = 0; v < U * 4; ++v) x[n][v] *= c[n];
-                if (shape.cap > 0.0f) {
-#pragma unroll
-                    for (int v = 0; v < U * 4; ++v) x[n][v] = shape.cap * tanhFit(x[n][v] * shape.inv_cap);
+                    for (int v = 0; v < U * 4; ++v) x[n][v] *= c2;
                 }
+                const float slope = -row[n].slope * kLog2e;
+                const int* mt = reinterpret_cast<const int*>(mine + G::oMeta) + 4 * kg;
 #pragma unroll
-                for (int v = 0; v < U * 4; ++v) {
-                    const int key = t * TK + 16 * (v >> 2) + 4 * kg + (v & 3);
-                    const bool in = key < a.T;
-                    int p = in ? key : kNoKey, dd = 0;
-                    if (in && kpos) {
-                        p = kpos[key];
-                        if (p < 0) p = kNoKey;
+                for (int u = 0; u < U; ++u) {
+                    const int key = t * TK + 16 * u + 4 * kg;
+                    int4 p4 = {key, key + 1, key + 2, key + 3}, d4 = {row[n].doc, row[n].doc, row[n].doc, row[n].doc};
+                    if (meta) {
+                        p4 = *reinterpret_cast<const int4*>(mt + 16 * u);
+                        d4 = *reinterpret_cast<const int4*>(mt + TK + 16 * u);
                     }
-                    if (in && kdoc) dd = kdoc[key];
-                    if (shape.bias) x[n][v] = fmaf(-row[n].slope, fabsf((float)(row[n].pos - p)), x[n][v]);
-                    if (a.mask && in) x[n][v] = addMask(x[n][v], a.mask[(size_t)row[n].token * a.m_row2 + key]);
-                    x[n][v] = p <= row[n].limit && dd == row[n].doc ? x[n][v] * kLog2e : -INFINITY;
-                }
-            } else {
-                const float c2 = c[n] * kLog2e;
+                    const int p[4] = {p4.x, p4.y, p4.z, p4.w}, dd[4] = {d4.x, d4.y, d4.z, d4.w};
+                    if (shape.bias) {
 #pragma unroll
-                for (int v = 0; v < U * 4; ++v) x[n][v] *= c2;
-                if (!full) {
-                    const int last = min(row[n].limit, a.T - 1) - t * TK - 4 * kg;
+                        for (int v = 0; v < 4; ++v) x[n][4 * u + v] = fmaf(slope, fabsf((float)(row[n].pos - p[v])), x[n][4 * u + v]);
+                    }
+                    if (a.mask) {
+                        const uint32_t* mr = reinterpret_cast<const uint32_t*>(a.mask + (size_t)row[n].token * a.m_row2) + key / 2;
+                        const uint32_t w0 = key < a.T ? mr[0] : 0xFC00FC00u, w1 = key + 2 < a.T ? mr[1] : 0xFC00FC00u;
+                        x[n][4 * u] = addMask(x[n][4 * u], w0 & 0xFFFFu);
+                        x[n][4 * u + 1] = addMask(x[n][4 * u + 1], w0 >> 16);
+                        x[n][4 * u + 2] = addMask(x[n][4 * u + 2], w1 & 0xFFFFu);
+                        x[n][4 * u + 3] = addMask(x[n][4 * u + 3], w1 >> 16);
+                    }
+                    if (!full) {
 #pragma unroll
-                    for (int v = 0; v < U * 4; ++v) x[n][v] = 16 * (v >> 2) + (v & 3) <= last ? x[n][v] : -INFINITY;
+                        for (int v = 0; v < 4; ++v)
+                            if (p[v] > row[n].limit || dd[v] != row[n].doc || key + v >= a.T) x[n][4 * u + v] = -INFINITY;
+                    }
                 }
+            } else if (!full) {
+                const int last = min(row[n].limit, a.T - 1) - t * TK - 4 * kg;
+#pragma unroll
+                for (int v = 0; v < U * 4; ++v) x[n][v] = 16 * (v >> 2) + (v & 3) <= last ? x[n][v] : -INFINITY;
             }
             float bm = x[n][0];
 #pragma unroll
             for (int v = 1; v < U * 4; ++v) bm = fmaxf(bm, x[n][v]);
-            bm = fmaxf(bm, __shfl_xor(bm, 16));
-            bm = fmaxf(bm, __shfl_xor(bm, 32));
-            const float mn = fmaxf(m[n], bm), ms = mn == -INFINITY ? 0.0f : mn;
+            bm = swap32Max(swap16Max(bm));
+            if constexpr (!SHAPED) bm *= c2;
+            const float mn = fmaxf(m[n], bm);
+            const float off = kPBits - (mn == -INFINITY ? 0.0f : mn);
             if (__any(mn > m[n])) {
-                const float alpha = ex2(m[n] - ms);
+                const float alpha = ex2(m[n] + off - kPBits);
                 l[n] *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[n][d] *= alpha;
                 m[n] = mn;
             }
+            float ls = 0.0f;
 #pragma unroll
             for (int v = 0; v < U * 4; ++v) {
-                x[n][v] = ex2(x[n][v] - ms);
-                l[n] += x[n][v];
-                const float ps = x[n][v] * kP;
-                const _Float16 hi = (_Float16)ps;
-                ph[n][v >> 3][v & 7] = hi;
-                pl[n][v >> 3][v & 7] = (_Float16)(ps - (float)hi);
+                x[n][v] = ex2(SHAPED ? x[n][v] + off : fmaf(x[n][v], c2, off));
+                ls += x[n][v];
             }
+            l[n] += ls;
+            splitParts<U * 4>(x[n], ph[n], pl[n]);
         }
         if (__builtin_expect(__any(wild), 0)) {  // values that are no matrix operands, for the rows that see them
 #pragma unroll 1
@@ -666,7 +735,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 const int xi = 4 * (key >> 4) + (key & 3), from = i + 16 * ((key >> 2) & 3);
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    const float p = __shfl(pick<U * 4>(x[n], xi), from) * kP;
+                    const float p = __shfl(pick<U * 4>(x[n], xi), from);
                     if (!__any(p != 0.0f)) continue;
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
@@ -683,20 +752,17 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             const unsigned short* vd = reinterpret_cast<const unsigned short*>(mine + G::oD);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                h8 dh[2], dl[2];
+                h8 dd[2];
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    dh[w] = *reinterpret_cast<const h8*>(vd + ((b * 2 + w) * 4 + kg) * 8);
-                    dl[w] = *reinterpret_cast<const h8*>(vd + 64 * NB + ((b * 2 + w) * 4 + kg) * 8);
-                }
+                for (int w = 0; w < 2; ++w) dd[w] = *reinterpret_cast<const h8*>(vd + ((b * 2 + w) * 4 + kg) * 8);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const int d = 2 * b + s;
                     const i2 w2 = __builtin_amdgcn_ds_read_tr4_b64_v2i32((LdsI2)(mine + G::oV + trow * G::Row + 8 * d));
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const h8 code = nibbles((uint32_t)w2[w]);
-                        const h8 vh = code * dh[w], vl = code * dl[w];
+                        const h8 code = nibbles((uint32_t)w2[w], magic);
+                        const h8 vh = code * dd[w], vl = __builtin_elementwise_fma(code, dd[w], -vh);
 #pragma unroll
                         for (int n = 0; n < NR; ++n) {
                             o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[n][w], o[n][d], 0, 0, 0);
@@ -756,66 +822,73 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         const int b = at >> 5, rr = at & 15, dd = Q4 ? 32 * b + 8 * ((at >> 4) & 1) + (rr >> 1) + 16 * (rr & 1) : at;
         if (a.splits == 1) {
             const int token = r / a.G, head = kvh * a.G + (r - token * a.G);
-            a.out[((size_t)token * a.H + head) * D + dd] = L == 0.0f ? 0.0f : y * (1.0f / (L * kP));
-            if (a.lse && at == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
+            a.out[((size_t)token * a.H + head) * D + dd] = L == 0.0f ? 0.0f : y * (1.0f / L);
+            if (a.lse && at == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L * kPInv));
         } else {
-            float* dst = a.part + (((size_t)sp * a.H_kv + kvh) * a.rows + r) * (D + 2);
-            dst[dd] = y * (1.0f / kP);
+            const size_t pr = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
+            a.part[pr * D + dd] = y * kPInv;
             if (at == 0) {
-                dst[D] = M;
-                dst[D + 1] = L;
+                float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * pr;
+                ml[0] = M;
+                ml[1] = L * kPInv;
             }
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------- joining key ranges
-// One workgroup per row: o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), the ranges dealt to four wavefronts whose sums are
-// added in order. What counts is the latency of two dependent loads.
-template <int D>
+// o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) for each row. A thread takes four of a row's values in every SG-th range,
+// its loads issued without waiting for the weights; the SG sums are added in order through LDS. What counts is the
+// latency of one round trip.
+template <int D, int SG>
 __global__ __launch_bounds__(256) void flash_ext_join_kernel(FxParams a) {
-    constexpr int V = D / 64;
-    __shared__ float sum[4][D];
-    const int r = blockIdx.x, kvh = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const size_t step = (size_t)a.H_kv * a.rows * (D + 2);
-    const float* base = a.part + ((size_t)kvh * a.rows + r) * (D + 2);
+    constexpr int LP = D / 4, RPB = 256 / LP / SG;  // lanes to a row, rows to a workgroup
+    __shared__ f32x4 sum[SG > 1 ? 256 : 1];
+    __shared__ float den[SG > 1 ? 256 / LP : 1];
+    const int tid = threadIdx.x, at = tid % LP, g = tid / LP % SG, x = tid / LP / SG;
+    const int total = a.H_kv * a.rows, n = blockIdx.x * RPB + x, nr = min(n, total - 1);  // row n / .. of KV head n / rows
+    const float* po = a.part + (size_t)nr * D + 4 * at;
+    const float* ml = a.part + (size_t)a.splits * total * D + 2 * (size_t)nr;
     float M = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, base[s * step + D]);
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) M = fmaxf(M, __shfl_xor(M, x));
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[(size_t)s * total * 2]);
     float L = 0.0f;
-    for (int s = lane; s < a.splits; s += 64) {
-        const float ms = base[s * step + D];
-        L += ms == -INFINITY ? 0.0f : ex2(ms - M) * base[s * step + D + 1];
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int s = g; s < a.splits; s += SG) {
+        const f32x4 z = *reinterpret_cast<const f4a4*>(po + (size_t)s * total * D);
+        const float ms = ml[(size_t)s * total * 2], f = ms == -INFINITY ? 0.0f : ex2(ms - M);
+        L = fmaf(f, ml[(size_t)s * total * 2 + 1], L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = f != 0.0f ? fmaf(f, z[e], y[e]) : y[e];
     }
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) L += __shfl_xor(L, x);
-    float y[V] = {};
-#pragma unroll 4
-    for (int s = wave; s < a.splits; s += 4) {
-        const float ms = base[s * step + D], f = ms == -INFINITY ? 0.0f : ex2(ms - M);
-#pragma unroll
-        for (int x = 0; x < V; ++x) {
-            const float z = base[s * step + lane + 64 * x];
-            y[x] = f != 0.0f ? fmaf(f, z, y[x]) : y[x];
+    if constexpr (SG > 1) {
+        sum[tid] = y;
+        if (at == 0) den[tid / LP] = L;
+        __syncthreads();
+        if (g) return;
+        for (int k = 1; k < SG; ++k) {
+            y += sum[tid + k * LP];
+            L += den[tid / LP + k];
         }
     }
-#pragma unroll
-    for (int x = 0; x < V; ++x) sum[wave][lane + 64 * x] = y[x];
-    __syncthreads();
-    const int token = r / a.G, head = kvh * a.G + (r - token * a.G);
-    for (int x = threadIdx.x; x < D; x += 256) {
-        const float z = sum[0][x] + sum[1][x] + sum[2][x] + sum[3][x];
-        a.out[((size_t)token * a.H + head) * D + x] = L == 0.0f ? 0.0f : z * (1.0f / L);
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
+    if (n >= total) return;
+    const int kvh = n / a.rows, r = n - kvh * a.rows, token = r / a.G, head = kvh * a.G + (r - token * a.G);
+    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<f4a4*>(a.out + ((size_t)token * a.H + head) * D + 4 * at) = f32x4{y[0] * f, y[1] * f, y[2] * f, y[3] * f};
+    if (a.lse && at == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
 }
 
 template <class F>
 int allow(F* kernel, int lds) {
     return fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
                    "flash_ext: LDS size");
+}
+
+template <int D, int SG>
+int join(const FxParams& p, hipStream_t s) {
+    constexpr int rows = 256 / (D / 4) / SG;
+    hipLaunchKernelGGL((flash_ext_join_kernel<D, SG>), dim3((p.H_kv * p.rows + rows - 1) / rows), dim3(256), 0, s, p);
+    return fromHip(hipGetLastError(), "flash_ext (join)");
 }
 
 template <int D, bool Q4, bool SHAPED>
@@ -835,17 +908,15 @@ int run(const FxParams& p, const FxPlan& plan, hipStream_t s) {
             hipLaunchKernelGGL((flash_ext_few_kernel<D, Q4, SHAPED, NR2>), grid, dim3(256), lds, s, p);
         }
     } else {
-        constexpr int lds = Geo<D, Q4>::Lds;
-        static const int ok = allow(flash_ext_kernel<D, Q4, SHAPED>, lds);
+        using G = Geo<D, Q4>;
+        static const int ok = allow(flash_ext_kernel<D, Q4, SHAPED>, G::Lds);
         if (ok) return ok;
-        hipLaunchKernelGGL((flash_ext_kernel<D, Q4, SHAPED>), dim3(p.H_kv, (p.rows + 127) / 128, p.splits), dim3(256), lds, s, p);
+        hipLaunchKernelGGL((flash_ext_kernel<D, Q4, SHAPED>), dim3(p.H_kv, (p.rows + 127) / 128, p.splits), dim3(G::Threads), G::Lds, s, p);
     }
     if (int e = fromHip(hipGetLastError(), "flash_ext")) return e;
-    if (p.splits > 1) {
-        hipLaunchKernelGGL(flash_ext_join_kernel<D>, dim3(p.rows, p.H_kv), dim3(256), 0, s, p);
-        return fromHip(hipGetLastError(), "flash_ext (join)");
-    }
-    return 0;
+    // two to four ranges: a thread adds them up; more: the row's threads share them
+    if (p.splits > 4) return join<D, D == 256 ? 4 : 8>(p, s);
+    return p.splits > 1 ? join<D, 1>(p, s) : 0;
 }
 
 template <int D>

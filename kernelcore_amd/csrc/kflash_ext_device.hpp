@@ -8,9 +8,8 @@
 // Precision. q and out are f32. q is scaled by a power of two so that its largest value is in [2^7, 2^8)
 // and split into fp16 parts hi = fp16(q), lo = fp16(q - hi): the products with fp16 keys are within about
 // 2^-22 of f32 ones. The softmax's p is split the same way. A 4-bit block's codes - 8 are exact fp16
-// integers; the scale d is applied to the f32 sums of each 32 keys' values (K), or split into d_hi (the seven
-// leading bits of its significand) and d_lo (the other four), whose products with a code are exact in fp16
-// (V): a third matrix chain instead of a rounded value.
+// integers; its scale d multiplies the f32 sum over the block's 32 values (K), or each value (V): d (c - 8) has 15
+// bits, so it is an fp16 value and an exact fp16 rest (a third matrix chain instead of a rounded value).
 #pragma once
 
 #include <climits>
@@ -31,6 +30,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef u4 u4a4 __attribute__((aligned(4)));
 typedef u4 u4a2 __attribute__((aligned(2)));
 typedef f32x4 f4a4 __attribute__((aligned(4)));
+struct __attribute__((packed, aligned(4))) int4a4 {
+    int x, y, z, w;
+    __device__ operator int4() const { return {x, y, z, w}; }
+};
 typedef __attribute__((address_space(3))) s4* LdsS4;
 typedef __attribute__((address_space(3))) i2* LdsI2;
 
@@ -38,20 +41,30 @@ constexpr float kLog2e = 1.44269504088896f;
 constexpr float kLn2 = 0.693147180559945f;
 constexpr int kNoKey = INT_MAX;  // the position of a row past the cache's end or in an empty slot
 
-// eight codes - 8 of a word as fp16, in the order of nibbles 0, 4, 1, 5, 2, 6, 3, 7: a nibble under the exponent of
-// 1024 reads 1024 + code, so 1032 is subtracted (exact)
-__device__ __forceinline__ h8 nibbles(uint32_t w) {
-    h8 r;
-    const h2 off = {(_Float16)1032.0f, (_Float16)1032.0f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const h2 x = __builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u) - off;
-        r[2 * i] = x[0];
-        r[2 * i + 1] = x[1];
-    }
-    return r;
+// Constants kept in registers, where one instruction can mask and merge a word with them.
+struct NibbleMagic {
+    uint32_t low, high, base;
+};
+__device__ __forceinline__ NibbleMagic nibbleMagic() {
+    NibbleMagic m{0x000F000Fu, 0x00F000F0u, 0x64006400u};
+    asm("" : "+s"(m.low));
+    asm("" : "+s"(m.high));
+    asm("" : "+v"(m.base));
+    return m;
 }
-// the codes - 8 of a word's low (or, of w >> 4, high) nibbles as fp16, in the order of its bytes
+// Eight codes - 8 of a word as fp16, in the order of nibbles 0, 4, 1, 5, 2, 6, 3, 7. A nibble at the foot of the significand of
+// 1024 reads 1024 + code, one four bits up 1024 + 16 code: less 1032, or / 16 less 72 (both exact).
+__device__ __forceinline__ h8 nibbles(uint32_t w, const NibbleMagic& k) {
+    const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const h2 by16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const uint32_t w8 = w >> 8;
+    const h2 a = __builtin_bit_cast(h2, (w & k.low) | k.base) + off;
+    const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & k.high) | k.base), by16, off16);
+    const h2 c = __builtin_bit_cast(h2, (w8 & k.low) | k.base) + off;
+    const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w8 & k.high) | k.base), by16, off16);
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The codes - 8 of a word's low (or, of w >> 4, high) nibbles as fp16, in the order of its bytes
 __device__ __forceinline__ void byteCodes(uint32_t w, h2& a, h2& b) {
     const h2 off = {(_Float16)1032.0f, (_Float16)1032.0f};
     const uint32_t m = w & 0x0F0F0F0Fu;
@@ -100,35 +113,121 @@ __device__ __forceinline__ Row rowOf(const FxParams& a, int kvh, int r) {
     return w;
 }
 
-// tanh(x) = x P(x^2) / Q(x^2), the relative minimax fit of these degrees on |x| <= 9 (2e-8; beyond, tanh is 1 within
-// 3e-8): a relative error of about 3e-7 over the whole range, where 1 - 2 / (exp(2x) + 1) would lose the small arguments
-__device__ __forceinline__ float tanhFit(float x) {
-    const float x0 = x;
-    x = __builtin_amdgcn_fmed3f(x, -9.0f, 9.0f);
-    const float u = x * x;
-    float p = fmaf(u, 1.335463029050743e-08f, 2.0609057173714973e-05f);
-    p = fmaf(u, p, 0.003495586570352316f);
-    p = fmaf(u, p, 0.13381023705005646f);
-    p = fmaf(u, p, 1.0f);
-    float q = fmaf(u, 7.776545203341811e-07f, 0.00032856324105523527f);
-    q = fmaf(u, q, 0.025876976549625397f);
-    q = fmaf(u, q, 0.46714338660240173f);
-    q = fmaf(u, q, 1.0f);
-    return x0 == x0 ? x * p * __builtin_amdgcn_rcpf(q) : x0;
-}
-
-// A shaped score from the sum of scaled products: cap and distance (the mask's value and what is not seen come after).
+// Scores in base 2: x = y log2 e. What shapes them, made once per workgroup.
 struct Shape {
-    float cap, inv_cap;
+    float inv_cap;   // 0: no cap
+    float p5[6];     // cap log2 e times the coefficients of tanh(y) / y in y^2, |y| <= 3/4
+    float p[5], q[4];  // of the quotient for |y| <= 9, P times cap log2 e
     bool bias;
 };
+__device__ __forceinline__ float uniform(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
 __device__ __forceinline__ Shape shapeOf(const FxParams& a) {
-    return {a.softcap, a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f, a.slopes != nullptr};
+    Shape s{};
+    s.bias = a.slopes != nullptr;
+    if (a.softcap > 0.0f) {
+        s.inv_cap = uniform(1.0f / a.softcap);
+        const float k = uniform(a.softcap * kLog2e);
+        const float p5[6] = {1.0f, -0.33332958817481995f, 0.1332540661096573f, -0.05334447696805f, 0.01958298869431019f, -0.0047163087874650955f};
+        const float p[5] = {1.0f, 0.13381023705005646f, 0.003495586570352316f, 2.0609057173714973e-05f, 1.335463029050743e-08f};
+        const float q[4] = {0.46714338660240173f, 0.025876976549625397f, 0.00032856324105523527f, 7.776545203341811e-07f};
+#pragma unroll
+        for (int i = 0; i < 6; ++i) s.p5[i] = uniform(k * p5[i]);
+#pragma unroll
+        for (int i = 0; i < 5; ++i) s.p[i] = uniform(k * p[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.q[i] = q[i];
+    }
+    return s;
+}
+// x[v] = cap log2 e tanh(x[v] k), k = score factor / cap. Two relative minimax fits of tanh(y) / y in y^2: a polynomial for |y| <= 3/4
+// (3e-8), taken where all of a wavefront's scores are that small (they mostly are: caps lie well above the scores), else a
+// quotient for |y| <= 9 (2e-8; beyond, tanh is 1 within 3e-8). A form through exp would lose the small arguments' last bits.
+// NaN stays NaN.
+template <int N>
+__device__ __forceinline__ void capScores(float (&x)[N], float k, const Shape& s) {
+    float top = 0.0f;
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+        x[v] *= k;
+        top = fmaxf(top, fabsf(x[v]));
+    }
+    if (!__any(top > 0.75f)) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const float u = x[v] * x[v];
+            float r = fmaf(u, s.p5[5], s.p5[4]);
+#pragma unroll
+            for (int i = 3; i >= 0; --i) r = fmaf(u, r, s.p5[i]);
+            x[v] *= r;
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const float y = __builtin_elementwise_maximum(__builtin_elementwise_minimum(x[v], 9.0f), -9.0f);
+            const float u = y * y;
+            float p = fmaf(u, s.p[4], s.p[3]), q = fmaf(u, s.q[3], s.q[2]);
+            p = fmaf(u, p, s.p[2]);
+            q = fmaf(u, q, s.q[1]);
+            p = fmaf(u, p, s.p[1]);
+            q = fmaf(u, q, s.q[0]);
+            p = fmaf(u, p, s.p[0]);
+            q = fmaf(u, q, 1.0f);
+            x[v] = y * p * __builtin_amdgcn_rcpf(q);
+        }
+    }
 }
 
 // exp2 on the transcendental unit: 0 below 2^-126, where the sums it joins do not see it
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The factor of a row's sums that makes them base-2 scores (never 0: a masked sum is -infinity, and stays it).
+__device__ __forceinline__ float factor2(float c) { return fmaxf(c * kLog2e, 1.17549435e-38f); }
+
+// Maxima over the lanes 32 (16) apart, without LDS: a swap of one register's upper half (odd rows of 16) with a copy's lower half
+// (even rows). The swap may read a register two wait states after its write; the two sides of the compiler's builtin
+// come out as one value here, hence the instruction itself.
+__device__ __forceinline__ float swap32Max(float x) {
+    float y = x;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+    return fmaxf(x, y);
+}
+__device__ __forceinline__ float swap16Max(float x) {
+    float y = x;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+    return fmaxf(x, y);
+}
+
+// N values (p 2^15) as fp16 parts hi + lo
+template <int N>
+__device__ __forceinline__ void splitParts(const float (&x)[N], h8 (&hi)[N / 8], h8 (&lo)[N / 8]) {
+#pragma unroll
+    for (int v = 0; v < N; v += 2) {
+        const h2 h = {(_Float16)x[v], (_Float16)x[v + 1]};
+        const uint32_t hb = __builtin_bit_cast(uint32_t, h);
+        float r0, r1;  // x - hi in one instruction each
+        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hb), "v"(x[v]));
+        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hb), "v"(x[v + 1]));
+        const h2 l = {(_Float16)r0, (_Float16)r1};
+        hi[v >> 3][v & 7] = h[0];
+        hi[v >> 3][(v & 7) + 1] = h[1];
+        lo[v >> 3][v & 7] = l[0];
+        lo[v >> 3][(v & 7) + 1] = l[1];
+    }
+}
+
+// x[i] of registers for a lane's own i
+template <int N>
+__device__ __forceinline__ float pick(const float (&x)[N], int i) {
+    float r = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) {
+        r = i == e ? x[e] : r;
+        asm("" : "+v"(r));  // (selects, not an indexed array, which would move x to memory)
+    }
+    return r;
+}
 
 __device__ __forceinline__ int waveMin(int x) {
 #pragma unroll
@@ -197,8 +296,8 @@ __device__ __forceinline__ void blockCodes(const u4& raw, h8 (&code)[4]) {
 }
 
 // Sums of scaled products of the lane's 16 keys, 8 (v / 4) + 4 h + v % 4, from key rows in LDS (fp16 values, or codes - 8
-// and f32 scales [block][key]).
-template <int D, bool Q4>
+// and f32 scales [block][key], SK keys to a block).
+template <int D, bool Q4, int SK = 32>
 __device__ __forceinline__ void keyScores(const char* keys, const char* scales, int j, int h, const h8 (&qh)[D / 16],
                                           const h8 (&ql)[D / 16], float (&x)[16]) {
     f32x16 zero;
@@ -215,7 +314,7 @@ __device__ __forceinline__ void keyScores(const char* keys, const char* scales, 
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[2 * b + 1], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[2 * b], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[2 * b + 1], s, 0, 0, 0);
-            const float* ks = reinterpret_cast<const float*>(scales) + 32 * b + 4 * h;
+            const float* ks = reinterpret_cast<const float*>(scales) + SK * b + 4 * h;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 d = *reinterpret_cast<const f32x4*>(ks + 8 * g);
@@ -224,19 +323,19 @@ __device__ __forceinline__ void keyScores(const char* keys, const char* scales, 
             }
         }
     } else {
-        f32x16 sh = zero, sl = zero;
+        f32x16 s = zero;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
             const h8 ka = *reinterpret_cast<const h8*>(kr + 32 * ks);
-            sh = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[ks], sh, 0, 0, 0);
-            sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[ks], sl, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[ks], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[ks], s, 0, 0, 0);
         }
 #pragma unroll
-        for (int v = 0; v < 16; ++v) x[v] = sh[v] + sl[v];
+        for (int v = 0; v < 16; ++v) x[v] = s[v];
     }
 }
 
-// The mask's values of the lane's 16 keys of tile t.
+// The mask's values of the lane's 16 keys of tile t (32 keys).
 struct MaskWords {
     uint32_t w[8];
     __device__ __forceinline__ void load(const unsigned short* mrow, int t, int h, int T) {
@@ -252,44 +351,47 @@ struct MaskWords {
 };
 
 // (a masked place is -infinity whatever its key holds)
-__device__ __forceinline__ float addMask(float x, uint32_t bits) { return bits == 0xFC00u ? -INFINITY : x + halfBits(bits); }
+__device__ __forceinline__ float addMask(float x, uint32_t bits) {
+    return bits == 0xFC00u ? -INFINITY : fmaf(halfBits(bits), kLog2e, x);
+}
 
-// Sums of products (times c) into shaped scores in base 2. meta (may be null): the tile's 32 positions and 32 document numbers
-// in LDS; with it, what the row does not see becomes -infinity.
-__device__ __forceinline__ void shapeScores(float (&x)[16], float c, const Shape& shape, const Row& row, const int* meta,
-                                            const MaskWords* mk, int t, int h) {
+// Sums of products into shaped scores in base 2. c: the factor of the row's scores; kp: the keys' positions where they are not the
+// tile's own (LDS, in groups of four at 8 g + 4 h), key0 the first of the lane's; mk the mask's values, null without.
+__device__ __forceinline__ void shapeScores(float (&x)[16], float c, const Shape& shape, const Row& row, const int* kp, int key0,
+                                            const MaskWords* mk) {
+    if (shape.inv_cap > 0.0f) {
+        capScores(x, c * shape.inv_cap, shape);
+    } else {
+        const float c2 = factor2(c);
 #pragma unroll
-    for (int v = 0; v < 16; ++v) x[v] *= c;
-    if (shape.cap > 0.0f) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) x[v] = shape.cap * tanhFit(x[v] * shape.inv_cap);
+        for (int v = 0; v < 16; ++v) x[v] *= c2;
     }
     if (shape.bias) {
+        const float slope = -row.slope * kLog2e;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            int4 kp = {};
-            if (meta) kp = *reinterpret_cast<const int4*>(meta + 8 * g + 4 * h);
-            const int p[4] = {kp.x, kp.y, kp.z, kp.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[4 * g + e] = fmaf(-row.slope, fabsf((float)(row.pos - (meta ? p[e] : t * 32 + 8 * g + 4 * h + e))), x[4 * g + e]);
+            int4 p = {key0 + 8 * g, key0 + 8 * g + 1, key0 + 8 * g + 2, key0 + 8 * g + 3};
+            if (kp) p = *reinterpret_cast<const int4*>(kp + 8 * g);
+            x[4 * g] = fmaf(slope, fabsf((float)(row.pos - p.x)), x[4 * g]);
+            x[4 * g + 1] = fmaf(slope, fabsf((float)(row.pos - p.y)), x[4 * g + 1]);
+            x[4 * g + 2] = fmaf(slope, fabsf((float)(row.pos - p.z)), x[4 * g + 2]);
+            x[4 * g + 3] = fmaf(slope, fabsf((float)(row.pos - p.w)), x[4 * g + 3]);
         }
     }
     if (mk) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[v] = addMask(x[v], (v & 1) ? mk->w[v >> 1] >> 16 : mk->w[v >> 1] & 0xFFFFu);
     }
+}
+
+// What the row does not see becomes -infinity: by the keys' positions and document numbers in LDS.
+__device__ __forceinline__ void hideKeys(float (&x)[16], const Row& row, const int* kp, const int* kd) {
 #pragma unroll
-    for (int v = 0; v < 16; ++v) x[v] *= kLog2e;
-    if (meta) {
+    for (int g = 0; g < 4; ++g) {
+        const int4 a = *reinterpret_cast<const int4*>(kp + 8 * g), b = *reinterpret_cast<const int4*>(kd + 8 * g);
+        const int p[4] = {a.x, a.y, a.z, a.w}, d[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int4 kp = *reinterpret_cast<const int4*>(meta + 8 * g + 4 * h);
-            const int4 kd = *reinterpret_cast<const int4*>(meta + 32 + 8 * g + 4 * h);
-            const int p[4] = {kp.x, kp.y, kp.z, kp.w}, dd[4] = {kd.x, kd.y, kd.z, kd.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * g + e] = p[e] <= row.limit && dd[e] == row.doc ? x[4 * g + e] : -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) x[4 * g + e] = p[e] <= row.limit && d[e] == row.doc ? x[4 * g + e] : -INFINITY;
     }
 }
 

@@ -198,7 +198,7 @@ class Case:
     def check(self):
         out, sums = self.attend()
         want, bound, lse, lse_bound = self.expected()
-        bad = np.abs(out - want) > bound
+        bad = ~(np.abs(out - want) <= bound)
         assert not bad.any(), (np.argwhere(bad)[:4].tolist(), float(np.abs(out - want)[bad].max()), float(bound[bad].min()))
         assert (np.isneginf(sums) == np.isneginf(lse)).all()
         fin = np.isfinite(lse)
