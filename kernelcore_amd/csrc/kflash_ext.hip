@@ -20,9 +20,10 @@ namespace {
 
 using namespace fx;
 
-// p in [0, 1] is split into fp16 parts at the scale 2^15, so that what the parts cannot hold is below 2^-40 (p = 2^(x - m + 15); l
-// and o carry the factor until the end)
-constexpr float kPBits = 15.0f, kPInv = 1.0f / 32768.0f;
+// A row's m may lag behind its maximum by up to kLag (p = 2^(x - m) up to 16), so that the sums are rescaled rarely; p is split
+// into fp16 parts at the scale 2^11 (up to 2^15 then), so that what the parts cannot hold is below 2^-36 of the largest p.
+// (x - m + 11 is what is exponentiated; l and o carry the factor until the end.)
+constexpr float kLag = 4.0f, kPBits = 11.0f, kPInv = 1.0f / 2048.0f;
 
 // The value at dd of a V row that the matrix products left out (0 where they took it).
 template <bool Q4>
@@ -44,16 +45,24 @@ __device__ __forceinline__ uint32_t tameHalves(uint32_t w) {
     return w & ~((z >> 15 & 1u) * 0xFFFFu | (z >> 31) * 0xFFFF0000u);
 }
 
+// The lanes' loads and stores of LDS before this are done before those after it (a wavefront's own LDS accesses run in
+// order: only the compiler has to keep them so).
+__device__ __forceinline__ void waveLds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---------------------------------------------------------------------------------------------- many rows
 // Workgroup: 128 rows of a KV head (four wavefronts of 32 rows) over one range of keys. A step takes KS tiles of 32 keys; with
-// KS = 2 two sets of wavefronts take a tile each (two wavefronts per SIMD whose vector and matrix phases overlap, and half
-// the steps on the longest rows), joined through LDS at the end. The step's keys and values lie in LDS, two buffers, the next
-// step's global loads in flight in registers while the present one is computed. Matrix form (v_mfma_f32_32x32x16_f16, lane
-// (j, h) = row j, lane half h):
+// KS = 2 two sets of four wavefronts take a tile each, joined through LDS at the end. Matrix form (v_mfma_f32_32x32x16_f16,
+// lane (j, h) = row j, lane half h):
 //   S^T = K Q^T: A = key rows (LDS), B = q hi / lo (registers). Lane (j, h) holds keys 8 (v / 4) + 4 h + v % 4 of row j.
 //   O^T += V^T P^T: A = V^T through transposed LDS reads, B = p hi / lo, the score registers as they are (the products'
 //   index runs over the keys in the order those registers hold).
-// 4-bit keys and values are unpacked once per workgroup, on the way to LDS.
+// 4-bit keys and values are unpacked once per workgroup, on the way to LDS; a step's keys and values lie in one of two
+// buffers, the next step's stored while the present one is computed and the loads of the one after in flight, one barrier a step. The
+// two wavefronts of a SIMD drift apart within a step, and one's softmax runs beside the other's products. (Keeping them half
+// a step apart by a second barrier, the values' products a step behind, was slower: 103 against 94 us for 2048 tokens.)
 template <int D, bool Q4>
 struct Geo {
     static constexpr int KS = D == 256 ? 1 : 2;  // (256 values: one wavefront's registers fill a SIMD)
@@ -61,97 +70,94 @@ struct Geo {
     static constexpr int NB = D / 32;
     static constexpr int KRow = kKeyRow<D>;
     static constexpr int VRow = 2 * D + 32;  // two pad chunks, for the transposed reads
-    static constexpr int oV = TK * KRow, oVl = oV + TK * VRow, oS = oV + TK * VRow * (Q4 ? 2 : 1);
-    static constexpr int oMeta = oS + (Q4 ? NB * TK * 4 : 0);
-    static constexpr int Buf = oMeta + TK * 8;  // positions, document numbers
-    static constexpr int MapWords = 1024;       // a range's steps, a bit each
-    static constexpr int ORow = D / 2 + 4;      // the join of the two sets: floats per lane
-    static constexpr int Main = 2 * Buf > 256 * ORow * 4 * (KS - 1) ? 2 * Buf : 256 * ORow * 4;
-    static constexpr int Lds = Main + 2 * MapWords * 4 + 64;
+    static constexpr int oScale = TK * KRow;                              // 4-bit: the keys' scales
+    static constexpr int oV = oScale + (Q4 ? NB * TK * 2 : 0), oLow = TK * VRow;  // values, 4-bit: their rests
+    static constexpr int oMeta = oV + TK * VRow * (Q4 ? 2 : 1);           // positions, document numbers
+    static constexpr int Buf = oMeta + TK * 8, oMap = 2 * Buf;
+    static constexpr int MapEntries = 2048;      // 256 keys each: the steps with a key that some row may see, those all rows see
+    static constexpr int oWild = oMap + 2 * MapEntries;  // 3 x the step's wild keys
+    static constexpr int oZ = oWild + 32;                // a wild key's values, for each wavefront
+    static constexpr int ORow = D / 2 + 4;       // the join of the two sets: floats per lane
+    static constexpr int Join = KS == 2 ? 256 * ORow * 4 : 0;
+    static constexpr int End = oZ + 4 * KS * D * 4;
+    static constexpr int Lds = End > Join ? End : Join;
 };
 
 template <int D, bool Q4, bool SHAPED>
 __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void flash_ext_kernel(FxParams a) {
     using G = Geo<D, Q4>;
-    constexpr int DB = D / 32, NB = G::NB, TK = G::TK, NT = G::Threads;
+    constexpr int DB = D / 32, NB = G::NB, TK = G::TK, NT = G::Threads, SPC = 256 / TK;
     extern __shared__ int4 lds4[];
     char* lds = reinterpret_cast<char*>(lds4);
-    uint32_t* map = reinterpret_cast<uint32_t*>(lds + G::Main);  // steps with a key that some row may see
-    uint32_t* whole = map + G::MapWords;                         // steps whose keys every row sees
-    int* misc = reinterpret_cast<int*>(whole + G::MapWords);     // 0 / 1: least / largest limit, 2 / 3: document, 4 + i: wild keys
+    unsigned short* map = reinterpret_cast<unsigned short*>(lds + G::oMap);
+    int* wildAt = reinterpret_cast<int*>(lds + G::oWild);
     const int kvh = blockIdx.x, rb = (int)gridDim.y - 1 - (int)blockIdx.y, sp = blockIdx.z;  // (longest rows first)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, h = lane >> 5, rw = wave & 3, ks = wave >> 2;
-    const int r = rb * 128 + rw * 32 + j;
+    const int r0 = rb * 128 + rw * 32, r = r0 + j;
     const Row row = rowOf(a, kvh, r);
-    const int wmin = waveMin(row.live ? row.limit : INT_MAX), wmax = waveMax(row.live ? row.limit : -1);
-
-    if (tid == 0) {
-        misc[0] = INT_MAX;
-        misc[1] = -1;
-        misc[2] = INT_MAX;
-        misc[3] = INT_MIN;
-    }
-    if (tid >= 4 && tid < 10) misc[tid] = 0;
-    __syncthreads();
-    if (lane == 0 && ks == 0) {
-        atomicMin(&misc[0], wmin);
-        atomicMax(&misc[1], wmax);
-    }
-    if (SHAPED && a.qdoc && row.live && ks == 0) {
-        atomicMin(&misc[2], row.doc);
-        atomicMax(&misc[3], row.doc);
-    }
-    __syncthreads();
-    const int bmax = __builtin_amdgcn_readfirstlane(misc[1]);
-
-    // this range's steps
+    h8 qh[D / 16], ql[D / 16];
+    const float c = loadRow32<D>(a, row, h, qh, ql), c2 = factor2(c);
+    const unsigned short* mrow = SHAPED && a.mask ? a.mask + (size_t)row.token * a.m_row2 : nullptr;
     const bool meta = SHAPED && (a.kpos || a.kdoc);
     const int* kpos = SHAPED && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
     const int* kdoc = SHAPED && a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
+
+    // the least and largest position limit of the wavefront's rows and of the workgroup's, and of their document numbers
+    int wmin, wmax, bmin, bmax, dmin = 0, dmax = 0;
+    const int b0 = rb * 128 / a.G, b1 = min(rb * 128 + 127, a.rows - 1) / a.G;  // the workgroup's tokens
+    if (!(SHAPED && a.qpos)) {  // (ascending with the rows)
+        wmin = r0 < a.rows ? limitOf(a, a.pos0 + r0 / a.G) : INT_MAX;
+        wmax = r0 < a.rows ? limitOf(a, a.pos0 + min(r0 + 31, a.rows - 1) / a.G) : -1;
+        bmin = limitOf(a, a.pos0 + b0);
+        bmax = limitOf(a, a.pos0 + b1);
+    } else {
+        wmin = waveMin(row.live ? row.limit : INT_MAX);
+        wmax = waveMax(row.live ? row.limit : -1);
+        const int l0 = limitOf(a, a.qpos[min(b0 + lane, b1)]), l1 = limitOf(a, a.qpos[min(b0 + 64 + lane, b1)]);
+        bmin = waveMin(min(l0, l1));
+        bmax = waveMax(max(l0, l1));
+    }
+
+    // this range's steps
     const int t0 = sp * a.per * (64 / TK);
     int t1 = (int)min((long long)t0 + (long long)a.per * (64 / TK), ((long long)a.T + TK - 1) / TK);
     if (!kpos) t1 = bmax < 0 ? t0 : min(t1, bmax / TK + 1);
-    const bool mapped = meta && t1 - t0 <= 32 * G::MapWords;
+    const bool mapped = meta && (t1 - t0 + SPC - 1) / SPC <= G::MapEntries;
     if constexpr (SHAPED) {
-        if (mapped) {  // four keys a lane, all loads issued before the ballots
-            const int bmin = misc[0], dmin = misc[2], dmax = misc[3];
-            for (int i = tid; i * 32 < t1 - t0; i += NT) map[i] = whole[i] = 0;
-            __syncthreads();
+        if (mapped) {  // a wavefront takes 256 keys, four a lane
+            if (a.qdoc) {
+                const int d0 = a.qdoc[min(b0 + lane, b1)], d1 = a.qdoc[min(b0 + 64 + lane, b1)];
+                dmin = waveMin(min(d0, d1));
+                dmax = waveMax(max(d0, d1));
+            }
             constexpr int LPT = TK / 4;  // lanes to a step
             const int key1 = min(a.T, t1 * TK);
-            for (int key = t0 * TK + 4 * tid; key - 4 * lane < key1; key += 4 * NT) {
-                bool some = false, all = true;
-                int4 p = {key, key + 1, key + 2, key + 3}, x = {dmin, dmin, dmin, dmin};
+            for (int at = wave; at * 256 < key1 - t0 * TK; at += NT / 64) {
+                const int key = t0 * TK + at * 256 + 4 * lane;
+                int p[4] = {key, key + 1, key + 2, key + 3}, x[4] = {dmin, dmin, dmin, dmin};
                 if (key + 3 < key1) {
-                    if (kpos) p = *reinterpret_cast<const int4a4*>(kpos + key);
-                    if (kdoc) x = *reinterpret_cast<const int4a4*>(kdoc + key);
+                    if (kpos) *reinterpret_cast<int4*>(p) = *reinterpret_cast<const int4a4*>(kpos + key);
+                    if (kdoc) *reinterpret_cast<int4*>(x) = *reinterpret_cast<const int4a4*>(kdoc + key);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if (key + e < key1) {
-                            if (kpos) (&p.x)[e] = kpos[key + e];
-                            if (kdoc) (&x.x)[e] = kdoc[key + e];
-                        } else {
-                            (&p.x)[e] = -1;
-                        }
+                        if (kpos && key + e < key1) p[e] = kpos[key + e];
+                        if (kdoc && key + e < key1) x[e] = kdoc[key + e];
+                        if (key + e >= key1) p[e] = -1;
                     }
                 }
-                const bool docs = kdoc != nullptr;
-                const int pp[4] = {p.x, p.y, p.z, p.w}, xx[4] = {x.x, x.y, x.z, x.w};
+                bool some = false, all = true;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool in = pp[e] >= 0 && pp[e] <= bmax && (!docs || (xx[e] >= dmin && xx[e] <= dmax));
+                    const bool in = p[e] >= 0 && p[e] <= bmax && x[e] >= dmin && x[e] <= dmax;
                     some |= in;
-                    all &= in && pp[e] <= bmin && (!docs || dmin == dmax);
+                    all &= in && p[e] <= bmin && dmin == dmax;
                 }
-                const unsigned long long group = ((1ull << LPT) - 1) << (lane / LPT * LPT);
-                const unsigned long long s = __ballot(some) & group, w = __ballot(all) & group;
-                const int at = (key - t0 * TK) / TK;
-                if (lane % LPT == 0 && s) {
-                    atomicOr(&map[at >> 5], 1u << (at & 31));
-                    if (w == group) atomicOr(&whole[at >> 5], 1u << (at & 31));
-                }
+                const unsigned long long s = __ballot(some), w = __ballot(all), group = (1ull << LPT) - 1;
+                const unsigned long long sb = __ballot(lane < SPC && (s >> (lane % SPC * LPT) & group)),
+                                         wb = __ballot(lane < SPC && (w >> (lane % SPC * LPT) & group) == group);
+                if (lane == 0) map[at] = (unsigned short)(sb | wb << 8);
             }
             __syncthreads();
         }
@@ -159,132 +165,146 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     auto next = [&](int t) -> int {  // the first step from t on that is to be computed; t1 if none
         if (!mapped) return min(t, t1);
         while (t < t1) {
-            const uint32_t w = __builtin_amdgcn_readfirstlane(map[(t - t0) >> 5]) >> ((t - t0) & 31);
+            const uint32_t w = (__builtin_amdgcn_readfirstlane(map[(t - t0) / SPC]) & 0xFFu) >> ((t - t0) % SPC);
             if (w) return min(t + __builtin_ctz(w), t1);
-            t = t0 + (((t - t0) >> 5) + 1) * 32;
+            t = t0 + ((t - t0) / SPC + 1) * SPC;
         }
         return t1;
     };
 
-    // ---- staging: 16-byte chunks (fp16) or whole blocks (4-bit) of the step's K and V rows, through registers
-    constexpr int PR = Q4 ? NB : D / 8, IT = TK * PR;       // of a row, of the step's K (and V)
-    constexpr bool Once = 2 * IT <= NT;                     // (4 bits: the first IT threads K, the next V)
-    constexpr int NL = Once ? 1 : 2 * IT / NT;
-    static_assert(Once || IT % NT == 0, "the step's rows over the threads");
-    u4 raw[NL];
-    uint32_t rsc[Q4 ? NL : 1];
+    // ---- staging, through registers: 16-byte chunks (fp16) or half blocks of 8 bytes (4-bit) of a step's K and V rows, of each NL
+    // per thread. Addresses: the step's first row, the same for the workgroup, + the thread's share.
+    constexpr int PR = Q4 ? 2 * NB : D / 8, IT = TK * PR, NL = (IT + NT - 1) / NT;
+    typedef __attribute__((ext_vector_type(Q4 ? 2 : 4))) uint32_t Item;
+    Item kraw[NL], vraw[NL];
+    uint32_t ksc[Q4 ? NL : 1], vsc[Q4 ? NL : 1];
     int rmeta = 0;
     const char* kb = a.k + (size_t)kvh * a.k_head;
     const char* vb = a.v + (size_t)kvh * a.v_head;
-    auto isV = [&](int n) { return Once ? tid >= IT : n >= NL / 2; };
-    auto item = [&](int n) { return Once ? tid % IT : tid + NT * (n >= NL / 2 ? n - NL / 2 : n); };
-    const bool idle = Once && tid >= 2 * IT;
+    const int part = tid % PR, key0 = tid / PR;                       // (NT is a multiple of PR)
+    const int pb = Q4 ? 18 * (part >> 1) : 16 * part;                 // the block, or the chunk
+    const bool idle = IT < NT && tid >= IT;
+    auto load = [&](const char* p, Item& x, uint32_t& sc) {
+        if constexpr (Q4) {
+            x = *reinterpret_cast<const __attribute__((aligned(2))) Item*>(p + 2 + 8 * (part & 1));
+            sc = *reinterpret_cast<const u32a2*>(p);
+        } else {
+            x = *reinterpret_cast<const __attribute__((aligned(4))) Item*>(p);
+        }
+    };
     auto fetch = [&](int t) {
+        if (!idle) {
 #pragma unroll
-        for (int n = 0; n < NL; ++n) {
-            if (idle) break;
-            const bool v = isV(n);
-            const int i = item(n), key = t * TK + i / PR, part = i % PR;
-            const size_t at = min(key, a.T - 1);
-            const char* p = (v ? vb + at * a.v_row : kb + at * a.k_row) + (Q4 ? 18 : 16) * part;
-            if constexpr (Q4) {
-                raw[n] = *reinterpret_cast<const u4a2*>(p + 2);
-                rsc[n] = loadHalf(p);
-                if (v && key >= a.T) rsc[n] = 0;
-            } else {
-                raw[n] = *reinterpret_cast<const u4a4*>(p);
-                if (v && key >= a.T) raw[n] = u4{0, 0, 0, 0};
+            for (int n = 0; n < NL; ++n) {
+                long long at = (long long)t * TK + NT / PR * n;
+                if (t * TK + TK > a.T) at = min(at, (long long)a.T - 1 - key0);  // (rows past the end reread the last one)
+                load(kb + at * a.k_row + (key0 * a.k_row + pb), kraw[n], ksc[Q4 ? n : 0]);
+                load(vb + at * a.v_row + (key0 * a.v_row + pb), vraw[n], vsc[Q4 ? n : 0]);
             }
         }
         if constexpr (SHAPED) {
             if (meta && tid < 2 * TK) {
-                const int key = t * TK + tid % TK;
-                if (tid < TK) {
-                    const int p = key < a.T ? (kpos ? kpos[key] : key) : kNoKey;
-                    rmeta = p < 0 ? kNoKey : p;
-                } else {
-                    rmeta = kdoc && key < a.T ? kdoc[key] : 0;
-                }
+                const int key = min(t * TK + tid % TK, a.T - 1);
+                const int* src = tid < TK ? kpos : kdoc;
+                rmeta = src ? src[key] : tid < TK ? key : 0;
             }
         }
     };
-    auto store = [&](char* buf, int* wild) {
+    // (whatever is done to a loaded value is done here: done in fetch, it would wait for the loads there)
+    auto store = [&](int t, char* buf, int* wild) {
+        if (t * TK + TK > a.T) {  // values past the end are 0
 #pragma unroll
-        for (int n = 0; n < NL; ++n) {
-            if (idle) break;
-            const bool v = isV(n);
-            const int i = item(n), key = i / PR, part = i % PR;
-            if constexpr (Q4) {
-                h8 code[4];
-                blockCodes(raw[n], code);
-                if (!v) {
-                    h8* p = reinterpret_cast<h8*>(buf + key * G::KRow + 64 * part);
+            for (int n = 0; n < NL; ++n)
+                if (t * TK + NT / PR * n + key0 >= a.T) {
+                    vsc[Q4 ? n : 0] = 0;
+                    if constexpr (!Q4) vraw[n] = Item{};
+                }
+        }
+        if (!idle) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] = code[e];
-                    reinterpret_cast<float*>(buf + G::oS)[part * TK + key] = halfBits(rsc[n]);
-                } else {
-                    uint32_t s = rsc[n];
+            for (int n = 0; n < NL; ++n) {
+                const int key = NT / PR * n + key0;
+                char* pk = buf + key * G::KRow + (Q4 ? 64 * (part >> 1) + 16 * (part & 1) : 16 * part);
+                char* pv = buf + G::oV + key * G::VRow + (Q4 ? 64 * (part >> 1) + 16 * (part & 1) : 16 * part);
+                if constexpr (Q4) {
+                    h8 lo, hi;  // values 8 (part % 2) .. + 8 of the block, and those 16 on
+                    byteCodes8(kraw[n], lo, hi);
+                    *reinterpret_cast<h8*>(pk) = lo;
+                    *reinterpret_cast<h8*>(pk + 32) = hi;
+                    if (!(part & 1))
+                        reinterpret_cast<unsigned short*>(buf + G::oScale)[(key >> 5) * NB * 32 + scaleAt(part >> 1, key & 31)] = (unsigned short)ksc[n];
+                    uint32_t s = vsc[n] & 0xFFFFu;
                     if (wildScale(s)) {
                         s = 0;
                         atomicOr(wild + (key >> 5), 1 << (key & 31));
                     }
                     const _Float16 d1 = __builtin_bit_cast(_Float16, (unsigned short)s);
                     const h8 d = {d1, d1, d1, d1, d1, d1, d1, d1};
-                    h8* p = reinterpret_cast<h8*>(buf + G::oV + key * G::VRow + 64 * part);
-                    h8* pl = reinterpret_cast<h8*>(buf + G::oVl + key * G::VRow + 64 * part);
+                    byteCodes8(vraw[n], lo, hi);
+                    const h8 x = lo * d, y = hi * d;
+                    *reinterpret_cast<h8*>(pv) = x;
+                    *reinterpret_cast<h8*>(pv + 32) = y;
+                    *reinterpret_cast<h8*>(pv + G::oLow) = __builtin_elementwise_fma(lo, d, -x);
+                    *reinterpret_cast<h8*>(pv + G::oLow + 32) = __builtin_elementwise_fma(hi, d, -y);
+                } else {
+                    *reinterpret_cast<Item*>(pk) = kraw[n];
+                    float squares = 0.0f;  // infinite or NaN where one of the values is
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const h8 x = code[e] * d;
-                        p[e] = x;
-                        pl[e] = __builtin_elementwise_fma(code[e], d, -x);
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t word = vraw[n][w];  // (a bit cast of the element itself takes the vector's first)
+                        const h2 x = __builtin_bit_cast(h2, word);
+                        squares = __builtin_amdgcn_fdot2(x, x, squares, false);
                     }
-                }
-            } else {
-                u4 x = raw[n];
-                if (v && (wildHalves(x[0]) | wildHalves(x[1]) | wildHalves(x[2]) | wildHalves(x[3]))) {
+                    if (!(squares < INFINITY)) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) x[w] = tameHalves(x[w]);
-                    atomicOr(wild + (key >> 5), 1 << (key & 31));
+                        for (int w = 0; w < 4; ++w) vraw[n][w] = tameHalves(vraw[n][w]);
+                        atomicOr(wild + (key >> 5), 1 << (key & 31));
+                    }
+                    *reinterpret_cast<Item*>(pv) = vraw[n];
                 }
-                *reinterpret_cast<u4*>(buf + (v ? G::oV + key * G::VRow : key * G::KRow) + 16 * part) = x;
             }
         }
         if constexpr (SHAPED)
-            if (meta && tid < 2 * TK) reinterpret_cast<int*>(buf + G::oMeta)[tid] = rmeta;
+            if (meta && tid < 2 * TK)
+                reinterpret_cast<int*>(buf + G::oMeta)[tid] = tid < TK && (rmeta < 0 || t * TK + tid >= a.T) ? kNoKey : rmeta;
     };
 
-    int t = next(t0);
-    if (t < t1) fetch(t);
-    h8 qh[D / 16], ql[D / 16];
-    const float c = loadRow32<D>(a, row, h, qh, ql), c2 = factor2(c);
     const Shape shape = SHAPED ? shapeOf(a) : Shape{};
-    const unsigned short* mrow = SHAPED && a.mask ? a.mask + (size_t)row.token * a.m_row2 : nullptr;
-
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    int slot = 0;  // of the wild-key words: three pairs in turn, the one two steps on is cleared while none reads it
-    if (t < t1) store(lds, &misc[4]);
+
+    int t = next(t0), tn = t < t1 ? next(t + 1) : t1;
+    if (tid < 8) wildAt[tid] = 0;
+    if (t < t1) fetch(t);
+    __syncthreads();
+    if (t < t1) store(t, lds, wildAt);
+    if (tn < t1) fetch(tn);
     __syncthreads();
     const int vlane = ks * 32 * (G::VRow / 2) + (4 * (lane >> 5) + ((lane & 15) >> 2)) * (G::VRow / 2) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    int slot = 0;  // of the wild-key words: three pairs in turn, the one two steps on is cleared while none reads it
     for (int it = 0; t < t1; ++it) {
-        const int tn = next(t + 1);
         char* cur = lds + (it & 1) * G::Buf;
-        if (tn < t1) fetch(tn);
+        const int sn = slot == 2 ? 0 : slot + 1, sc = sn == 2 ? 0 : sn + 1, tnn = tn < t1 ? next(tn + 1) : t1;
         const int k0 = t * TK + 32 * ks;  // this wavefront's 32 keys
         bool full = !(SHAPED && mrow) && k0 + 31 < a.T;
-        if (meta) full = full && mapped && (__builtin_amdgcn_readfirstlane(whole[(t - t0) >> 5]) >> ((t - t0) & 31) & 1);
+        if (meta) full = full && mapped && (__builtin_amdgcn_readfirstlane(map[(t - t0) / SPC]) >> (8 + (t - t0) % SPC) & 1);
         else full = full && k0 + 31 <= wmin;
-        if (full || meta || k0 <= wmax) {
-            MaskWords mk;
-            if constexpr (SHAPED) {
-                if (mrow) mk.load(mrow, t * (TK / 32) + ks, h, a.T);
-            }
-            float x[16];
-            keyScores<D, Q4, TK>(cur + ks * 32 * G::KRow, cur + G::oS + ks * 128, j, h, qh, ql, x);
+        const bool work = full || meta || k0 <= wmax;
+        MaskWords mk;
+        if constexpr (SHAPED) {
+            if (mrow && work) mk.load(mrow, t * (TK / 32) + ks, h, a.T);
+        }
+        float x[16];
+        if (work) keyScores<D, Q4>(cur + ks * 32 * G::KRow, cur + G::oScale + ks * NB * 64, j, h, qh, ql, x);
+        // the next step into the other buffer (last read before the barrier that ended the step before this one)
+        if (tn < t1) store(tn, lds + ((it + 1) & 1) * G::Buf, wildAt + 2 * sn);
+        if (tnn < t1) fetch(tnn);
+        if (work) {
+            const int wildBits = wildAt[2 * slot + ks];
             const int* kp = reinterpret_cast<const int*>(cur + G::oMeta) + 32 * ks + 4 * h;
             if constexpr (SHAPED) shapeScores(x, c, shape, row, meta ? kp : nullptr, k0 + 4 * h, mrow ? &mk : nullptr);
             if (!full) {
@@ -301,10 +321,10 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
             for (int v = 1; v < 16; ++v) bm = fmaxf(bm, x[v]);
             bm = swap32Max(bm);
             if constexpr (!SHAPED) bm *= c2;
-            const float mn = fmaxf(m, bm);
-            const float off = kPBits - (mn == -INFINITY ? 0.0f : mn);  // (nothing seen yet: every p is 0)
-            if (__any(mn > m)) {
-                const float alpha = ex2(m + off - kPBits);
+            // a row's m follows its maximum only when that is more than kLag ahead: after the first keys hardly ever
+            const bool ahead = bm > m + kLag;
+            if (__any(ahead)) {
+                const float mn = ahead ? bm : m, alpha = ahead ? ex2(m - mn) : 1.0f;
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -312,6 +332,7 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                     for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
                 m = mn;
             }
+            const float off = kPBits - (m == -INFINITY ? 0.0f : m);  // (nothing seen yet: every p is 0)
             float ls = 0.0f;
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
@@ -319,20 +340,32 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                 ls += x[v];
             }
             l += ls;
-            uint32_t wild = __builtin_amdgcn_readfirstlane(misc[4 + 2 * slot + ks]);
-            while (__builtin_expect(wild != 0, 0)) {  // values that are no matrix operands, for the rows that see them
-                const int key = __builtin_ctz(wild);
-                wild &= wild - 1;
-                const float p = __shfl(pick<16>(x, (key >> 3) * 4 + (key & 3)), j + 32 * ((key >> 2) & 1));
-                if (!__any(p != 0.0f)) continue;
-                const char* vr = vb + (size_t)(k0 + key) * a.v_row;
+            uint32_t wild = __builtin_amdgcn_readfirstlane(wildBits);
+            if (__builtin_expect(wild != 0, 0)) {  // values that are no matrix operands, for the rows that see them
+                float* zr = reinterpret_cast<float*>(lds + G::oZ) + wave * D;
+#pragma unroll 1
+                while (wild) {
+                    const int key = __builtin_ctz(wild);
+                    wild &= wild - 1;
+                    const float p = __shfl(pick<16>(x, (key >> 3) * 4 + (key & 3)), j + 32 * ((key >> 2) & 1));
+                    if (!__any(p != 0.0f)) continue;
+                    const char* vr = vb + (size_t)(k0 + key) * a.v_row;
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
+                    for (int e = 0; e < D / 64; ++e) zr[lane + 64 * e] = wildValue<Q4>(vr, lane + 64 * e);
+                    waveLds();
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const float z = wildValue<Q4>(vr, 32 * d + 8 * (v >> 2) + 4 * h + (v & 3));
-                        if (p != 0.0f && z != 0.0f) o[d][v] = fmaf(p, z, o[d][v]);
-                    }
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const f32x4 z = *reinterpret_cast<const f32x4*>(zr + 32 * d + 8 * g + 4 * h);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float y = fmaf(p, z[e], o[d][4 * g + e]);
+                                o[d][4 * g + e] = p != 0.0f ? y : o[d][4 * g + e];
+                            }
+                        }
+                    waveLds();
+                }
             }
             h8 ph[2], pl[2];
             splitParts<16>(x, ph, pl);
@@ -348,7 +381,7 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[mm], o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[mm], o[d], 0, 0, 0);
                     if constexpr (Q4) {
-                        const _Float16* vq = vp + (G::oVl - G::oV) / 2;
+                        const _Float16* vq = vp + G::oLow / 2;
                         const s4 y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)vq);
                         const s4 y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(vq + 8 * (G::VRow / 2)));
                         const h8 vl = __builtin_bit_cast(h8, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -356,12 +389,10 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                     }
                 }
         }
-        // the next step into the other buffer (last read before the barrier that ended the step before this one)
-        const int sn = slot == 2 ? 0 : slot + 1, sc = sn == 2 ? 0 : sn + 1;
-        if (tn < t1) store(lds + ((it + 1) & 1) * G::Buf, &misc[4 + 2 * sn]);
-        if (tid < 2) misc[4 + 2 * sc + tid] = 0;
+        if (tid < 2) wildAt[2 * sc + tid] = 0;
         slot = sn;
         t = tn;
+        tn = tnn;
         __syncthreads();
     }
 
@@ -434,18 +465,12 @@ struct FewGeo {
     static constexpr int VRow = 2 * D + 32;  // of an fp16 row
     static constexpr int oV = 64 * Row, oS = 2 * oV, oD = oS + NB * 256;  // 4-bit: codes of K, of V, K scales, V scales
     static constexpr int oMeta = Q4 ? oD + NB * 128 : 32 * VRow;  // positions, document numbers
-    static constexpr int Wave = oMeta + TK * 8;
+    static constexpr int oZ = oMeta + TK * 8;  // a wild key's values
+    static constexpr int Wave = oZ + D * 4;
     static constexpr int ORow = D + 4;       // join: floats per row
     static constexpr int Join = 4 * NR * 16 * (ORow + 2) * 4;
     static constexpr int Lds = 4 * Wave > Join ? 4 * Wave : Join;
 };
-
-// The lanes' loads and stores of LDS before this are done before those after it (a wavefront's own LDS accesses run in
-// order: only the compiler has to keep them so).
-__device__ __forceinline__ void waveLds() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 
 template <int D, bool Q4, bool SHAPED, int NR>
 __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_few_kernel(FxParams a) {
@@ -479,8 +504,8 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         if constexpr (SHAPED) {
             if (meta && lane < TK) {
                 const int key = (int)row0 + lane;
-                rkp = key < a.T ? (kpos ? kpos[key] : key) : kNoKey;
-                rkd = kdoc && key < a.T ? kdoc[key] : 0;
+                rkp = kpos ? kpos[min(key, a.T - 1)] : key;
+                rkd = kdoc ? kdoc[min(key, a.T - 1)] : 0;
             }
         }
         if (row0 + TK <= a.T) {
@@ -490,9 +515,9 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 if constexpr (Q4) {
                     const char* kp = kb + (row0 + 64 / PR * n) * a.k_row + klane;
                     kr[n] = *reinterpret_cast<const u4a2*>(kp + 2);
-                    kscale[n] = loadHalf(kp);
+                    kscale[n] = *reinterpret_cast<const u32a2*>(kp);
                     vr[n] = *reinterpret_cast<const u4a2*>(vp + 2);
-                    vscale[n] = loadHalf(vp);
+                    vscale[n] = *reinterpret_cast<const u32a2*>(vp);
                 } else {
                     kr[n] = *reinterpret_cast<const u4a4*>(kb + (row0 + 16 * (n / NB)) * a.k_row + 64 * (n % NB) + klane);
                     vr[n] = *reinterpret_cast<const u4a4*>(vp);
@@ -506,14 +531,13 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 if constexpr (Q4) {
                     const char* kp = kb + (size_t)min(vkey, a.T - 1) * a.k_row + 18 * part;
                     kr[n] = *reinterpret_cast<const u4a2*>(kp + 2);
-                    kscale[n] = loadHalf(kp);
+                    kscale[n] = *reinterpret_cast<const u32a2*>(kp);
                     vr[n] = *reinterpret_cast<const u4a2*>(vp + 2);
-                    vscale[n] = vkey < a.T ? loadHalf(vp) : 0u;
+                    vscale[n] = *reinterpret_cast<const u32a2*>(vp);
                 } else {
                     const int kkey = min((int)row0 + 16 * (n / NB) + i, a.T - 1);
                     kr[n] = *reinterpret_cast<const u4a4*>(kb + (size_t)kkey * a.k_row + 64 * (n % NB) + 16 * kg);
                     vr[n] = *reinterpret_cast<const u4a4*>(vp);
-                    if (vkey >= a.T) vr[n] = u4{0, 0, 0, 0};
                 }
             }
         }
@@ -592,8 +616,8 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             if constexpr (Q4) {
                 *reinterpret_cast<u4*>(mine + key * G::Row + 16 * part) = kr[n];
                 *reinterpret_cast<u4*>(mine + G::oV + key * G::Row + 16 * part) = vr[n];
-                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = halfBits(kscale[n]);
-                uint32_t s = vscale[n];
+                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = halfBits(kscale[n] & 0xFFFFu);
+                uint32_t s = t * TK + key < a.T ? vscale[n] & 0xFFFFu : 0u;
                 if (wildScale(s)) {
                     s = 0;
                     wild = true;
@@ -603,6 +627,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 reinterpret_cast<unsigned short*>(mine + G::oD)[at] = (unsigned short)s;
             } else {
                 u4 x = vr[n];
+                if (t * TK + key >= a.T) x = u4{0, 0, 0, 0};
                 if (wildHalves(x[0]) | wildHalves(x[1]) | wildHalves(x[2]) | wildHalves(x[3])) {
                     wild = true;
 #pragma unroll
@@ -615,7 +640,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         if constexpr (SHAPED) {
             if (meta && lane < TK) {
                 int* mt = reinterpret_cast<int*>(mine + G::oMeta);
-                mt[lane] = rkp < 0 ? kNoKey : rkp;
+                mt[lane] = rkp < 0 || t * TK + lane >= a.T ? kNoKey : rkp;
                 mt[TK + lane] = rkd;
             }
         }
@@ -710,15 +735,15 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             for (int v = 1; v < U * 4; ++v) bm = fmaxf(bm, x[n][v]);
             bm = swap32Max(swap16Max(bm));
             if constexpr (!SHAPED) bm *= c2;
-            const float mn = fmaxf(m[n], bm);
-            const float off = kPBits - (mn == -INFINITY ? 0.0f : mn);
-            if (__any(mn > m[n])) {
-                const float alpha = ex2(m[n] + off - kPBits);
+            const bool ahead = bm > m[n] + kLag;
+            if (__any(ahead)) {
+                const float mn = ahead ? bm : m[n], alpha = ahead ? ex2(m[n] - mn) : 1.0f;
                 l[n] *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[n][d] *= alpha;
                 m[n] = mn;
             }
+            const float off = kPBits - (m[n] == -INFINITY ? 0.0f : m[n]);
             float ls = 0.0f;
 #pragma unroll
             for (int v = 0; v < U * 4; ++v) {
@@ -729,10 +754,14 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             splitParts<U * 4>(x[n], ph[n], pl[n]);
         }
         if (__builtin_expect(__any(wild), 0)) {  // values that are no matrix operands, for the rows that see them
+            float* zr = reinterpret_cast<float*>(mine + G::oZ);
 #pragma unroll 1
             for (int key = 0; key < TK; ++key) {
                 const char* vrow = vb + (size_t)min(t * TK + key, a.T - 1) * a.v_row;
                 const int xi = 4 * (key >> 4) + (key & 3), from = i + 16 * ((key >> 2) & 3);
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) zr[lane + 64 * e] = wildValue<Q4>(vrow, lane + 64 * e);
+                waveLds();
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
                     const float p = __shfl(pick<U * 4>(x[n], xi), from);
@@ -742,10 +771,11 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
                             const int rr = 4 * kg + v;
-                            const float z = wildValue<Q4>(vrow, Q4 ? 32 * (d >> 1) + 8 * (d & 1) + (rr >> 1) + 16 * (rr & 1) : 16 * d + rr);
-                            if (p != 0.0f && z != 0.0f) o[n][d][v] = fmaf(p, z, o[n][d][v]);
+                            const float y = fmaf(p, zr[Q4 ? 32 * (d >> 1) + 8 * (d & 1) + (rr >> 1) + 16 * (rr & 1) : 16 * d + rr], o[n][d][v]);
+                            o[n][d][v] = p != 0.0f ? y : o[n][d][v];
                         }
                 }
+                waveLds();
             }
         }
         if constexpr (Q4) {
@@ -838,43 +868,80 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
 
 // ---------------------------------------------------------------------------------------------- joining key ranges
 // o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) for each row. A thread takes four of a row's values in every SG-th range,
-// its loads issued without waiting for the weights; the SG sums are added in order through LDS. What counts is the
-// latency of one round trip.
+// the first of its loads issued before the weights are known; the row's threads share the weights, and the SG sums are
+// added in order through LDS. What counts is the latency of a round trip.
 template <int D, int SG>
 __global__ __launch_bounds__(256) void flash_ext_join_kernel(FxParams a) {
-    constexpr int LP = D / 4, RPB = 256 / LP / SG;  // lanes to a row, rows to a workgroup
+    constexpr int LP = D / 4, RT = LP * SG, RPB = 256 / RT;  // lanes to a row's values, threads to a row, rows to a workgroup
+    constexpr int Ahead = 8, Most = 512;                     // (fxPlan: no more ranges)
     __shared__ f32x4 sum[SG > 1 ? 256 : 1];
-    __shared__ float den[SG > 1 ? 256 / LP : 1];
-    const int tid = threadIdx.x, at = tid % LP, g = tid / LP % SG, x = tid / LP / SG;
-    const int total = a.H_kv * a.rows, n = blockIdx.x * RPB + x, nr = min(n, total - 1);  // row n / .. of KV head n / rows
+    __shared__ float wt[SG > 1 ? RPB : 1][SG > 1 ? Most : 1], red[2][4];
+    const int tid = threadIdx.x, q = tid % RT, at = q % LP, g = q / LP, x = tid / RT;
+    const int total = a.H_kv * a.rows, n = blockIdx.x * RPB + x, nr = min(n, total - 1);  // row n % rows of KV head n / rows
     const float* po = a.part + (size_t)nr * D + 4 * at;
     const float* ml = a.part + (size_t)a.splits * total * D + 2 * (size_t)nr;
-    float M = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[(size_t)s * total * 2]);
-    float L = 0.0f;
-    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int s = g; s < a.splits; s += SG) {
-        const f32x4 z = *reinterpret_cast<const f4a4*>(po + (size_t)s * total * D);
-        const float ms = ml[(size_t)s * total * 2], f = ms == -INFINITY ? 0.0f : ex2(ms - M);
-        L = fmaf(f, ml[(size_t)s * total * 2 + 1], L);
+    f32x4 z[Ahead];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = f != 0.0f ? fmaf(f, z[e], y[e]) : y[e];
-    }
-    if constexpr (SG > 1) {
+    for (int k = 0; k < Ahead; ++k) z[k] = *reinterpret_cast<const f4a4*>(po + (size_t)min(g + SG * k, a.splits - 1) * total * D);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (SG == 1) {
+        float ms[4], ls[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            ms[s] = s < a.splits ? ml[(size_t)s * total * 2] : -INFINITY;
+            ls[s] = s < a.splits ? ml[(size_t)s * total * 2 + 1] : 0.0f;
+            M = fmaxf(M, ms[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const float f = ms[s] == -INFINITY ? 0.0f : ex2(ms[s] - M);
+            L = fmaf(f, ls[s], L);
+            if (f != 0.0f) y += f * z[s];
+        }
+    } else {
+        for (int s = q; s < a.splits; s += RT) {
+            const float ms = ml[(size_t)s * total * 2];
+            wt[x][s] = ms;
+            M = fmaxf(M, ms);
+        }
+        M = waveMaxF(M);
+        if ((tid & 63) == 0) red[0][tid >> 6] = M;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < RT / 64; ++w) M = fmaxf(M, red[0][x * (RT / 64) + w]);
+        for (int s = q; s < a.splits; s += RT) {
+            const float ms = wt[x][s], f = ms == -INFINITY ? 0.0f : ex2(ms - M);
+            L = fmaf(f, ml[(size_t)s * total * 2 + 1], L);
+            wt[x][s] = f;
+        }
+        L = waveSumF(L);
+        if ((tid & 63) == 0) red[1][tid >> 6] = L;
+        __syncthreads();
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < RT / 64; ++w) L += red[1][x * (RT / 64) + w];
+#pragma unroll
+        for (int k = 0; k < Ahead; ++k) {
+            const int s = g + SG * k;
+            const float f = s < a.splits ? wt[x][s] : 0.0f;
+            if (f != 0.0f) y += f * z[k];
+        }
+        for (int s = g + SG * Ahead; s < a.splits; s += SG) {
+            const float f = wt[x][s];
+            const f32x4 w = *reinterpret_cast<const f4a4*>(po + (size_t)s * total * D);
+            if (f != 0.0f) y += f * w;
+        }
         sum[tid] = y;
-        if (at == 0) den[tid / LP] = L;
         __syncthreads();
         if (g) return;
-        for (int k = 1; k < SG; ++k) {
-            y += sum[tid + k * LP];
-            L += den[tid / LP + k];
-        }
+#pragma unroll
+        for (int k = 1; k < SG; ++k) y += sum[tid + k * LP];
     }
     if (n >= total) return;
     const int kvh = n / a.rows, r = n - kvh * a.rows, token = r / a.G, head = kvh * a.G + (r - token * a.G);
     const float f = L == 0.0f ? 0.0f : 1.0f / L;
-    *reinterpret_cast<f4a4*>(a.out + ((size_t)token * a.H + head) * D + 4 * at) = f32x4{y[0] * f, y[1] * f, y[2] * f, y[3] * f};
+    *reinterpret_cast<f4a4*>(a.out + ((size_t)token * a.H + head) * D + 4 * at) = y * f;
     if (a.lse && at == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
 }
 

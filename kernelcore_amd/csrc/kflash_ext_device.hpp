@@ -29,6 +29,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // loads and stores at the alignment the callers' strides leave
 typedef u4 u4a4 __attribute__((aligned(4)));
 typedef u4 u4a2 __attribute__((aligned(2)));
+typedef uint32_t u32a2 __attribute__((aligned(2)));
 typedef f32x4 f4a4 __attribute__((aligned(4)));
 struct __attribute__((packed, aligned(4))) int4a4 {
     int x, y, z, w;
@@ -100,6 +101,9 @@ struct Row {
     int pos, doc;
     float slope;
 };
+__device__ __forceinline__ int limitOf(const FxParams& a, int pos) {
+    return a.causal ? min(max(pos, a.prefix - 1), INT_MAX - 1) : INT_MAX - 1;
+}
 __device__ __forceinline__ Row rowOf(const FxParams& a, int kvh, int r) {
     Row w;
     w.live = r < a.rows;
@@ -107,7 +111,7 @@ __device__ __forceinline__ Row rowOf(const FxParams& a, int kvh, int r) {
     w.token = rr / a.G;
     w.head = kvh * a.G + (rr - w.token * a.G);
     w.pos = a.qpos ? a.qpos[w.token] : a.pos0 + w.token;
-    w.limit = a.causal ? min(max(w.pos, a.prefix - 1), INT_MAX - 1) : INT_MAX - 1;
+    w.limit = limitOf(a, w.pos);
     w.doc = a.qdoc ? a.qdoc[w.token] : 0;
     w.slope = a.slopes ? a.slopes[w.head] : 0.0f;
     return w;
@@ -186,20 +190,21 @@ __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x)
 __device__ __forceinline__ float factor2(float c) { return fmaxf(c * kLog2e, 1.17549435e-38f); }
 
 // Maxima over the lanes 32 (16) apart, without LDS: a swap of one register's upper half (odd rows of 16) with a copy's lower half
-// (even rows). The swap may read a register two wait states after its write; the two sides of the compiler's builtin
-// come out as one value here, hence the instruction itself.
+// (even rows). (The results are copied before they are cast: a bit cast of a vector's element takes its first one.)
 __device__ __forceinline__ float swap32Max(float x) {
-    float y = x;
-    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-    return fmaxf(x, y);
+    const int y = __builtin_bit_cast(int, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    const int a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 __device__ __forceinline__ float swap16Max(float x) {
-    float y = x;
-    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-    return fmaxf(x, y);
+    const int y = __builtin_bit_cast(int, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+    const int a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
-// N values (p 2^15) as fp16 parts hi + lo
+// N values (p 2^11) as fp16 parts hi + lo
 template <int N>
 __device__ __forceinline__ void splitParts(const float (&x)[N], h8 (&hi)[N / 8], h8 (&lo)[N / 8]) {
 #pragma unroll
@@ -242,6 +247,17 @@ __device__ __forceinline__ int waveMax(int x) {
 __device__ __forceinline__ float halfBits(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (unsigned short)b); }
 __device__ __forceinline__ uint32_t loadHalf(const char* p) { return *reinterpret_cast<const unsigned short*>(p); }
 
+
+__device__ __forceinline__ float waveMaxF(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ float waveSumF(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
+    return x;
+}
 
 // ---- tiles of 32 keys x 32 rows (v_mfma_f32_32x32x16_f16; lane (j, h) = row j, lane half h)
 
@@ -295,9 +311,30 @@ __device__ __forceinline__ void blockCodes(const u4& raw, h8 (&code)[4]) {
         }
 }
 
+// Eight bytes of a block: the low codes and the high ones.
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void byteCodes8(const u2& raw, h8& lo, h8& hi) {
+    h2 x[8];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        byteCodes(raw[w], x[2 * w], x[2 * w + 1]);
+        byteCodes(raw[w] >> 4, x[4 + 2 * w], x[5 + 2 * w]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        lo[2 * e] = x[e][0];
+        lo[2 * e + 1] = x[e][1];
+        hi[2 * e] = x[4 + e][0];
+        hi[2 * e + 1] = x[4 + e][1];
+    }
+}
+
+// Where the fp16 scale of block b of key `key` of a tile lies in LDS: the 16 keys of a lane half in the order of its scores.
+__device__ __forceinline__ int scaleAt(int b, int key) { return (2 * b + ((key >> 2) & 1)) * 16 + (key >> 3) * 4 + (key & 3); }
+
 // Sums of scaled products of the lane's 16 keys, 8 (v / 4) + 4 h + v % 4, from key rows in LDS (fp16 values, or codes - 8
-// and f32 scales [block][key], SK keys to a block).
-template <int D, bool Q4, int SK = 32>
+// and their blocks' scales as scaleAt places them: eight of them a read, each taken as fp16 by the multiply-add).
+template <int D, bool Q4>
 __device__ __forceinline__ void keyScores(const char* keys, const char* scales, int j, int h, const h8 (&qh)[D / 16],
                                           const h8 (&ql)[D / 16], float (&x)[16]) {
     f32x16 zero;
@@ -314,12 +351,11 @@ __device__ __forceinline__ void keyScores(const char* keys, const char* scales, 
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[2 * b + 1], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[2 * b], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[2 * b + 1], s, 0, 0, 0);
-            const float* ks = reinterpret_cast<const float*>(scales) + SK * b + 4 * h;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 d = *reinterpret_cast<const f32x4*>(ks + 8 * g);
+            for (int g = 0; g < 2; ++g) {
+                const h8 d = *reinterpret_cast<const h8*>(scales + (2 * b + h) * 32 + 16 * g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * g + e] = fmaf(d[e], s[4 * g + e], x[4 * g + e]);
+                for (int e = 0; e < 8; ++e) x[8 * g + e] = fmaf((float)d[e], s[8 * g + e], x[8 * g + e]);
             }
         }
     } else {

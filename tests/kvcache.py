@@ -111,9 +111,9 @@ class Case:
         mag = np.stack([w[:, h] @ np.abs(safe[:, h]) for h in range(H)], 1)
         err = self.score_error(terms)
         bound = (2 * err + 2.0 ** -20 + 4 * math.sqrt(max(T, 1)) * 2.0 ** -24) * mag
-        # each p (largest 1, sum at least 1) is two fp16 parts of 2^15 p, of which the second is a multiple of 2^-24: off by
-        # up to half of that where it is subnormal, 2^-25 2^-15 = 2^-40 of p
-        bound += 2.0 ** -40 * np.stack([seen[:, h].astype(np.float64) @ np.abs(safe[:, h]) for h in range(H)], 1)
+        # each p (the largest between 1 and 16, so the sum at least 1) is two fp16 parts of 2^11 p, of which the second is a
+        # multiple of 2^-24: off by up to half of that where it is subnormal, 2^-25 2^-11 = 2^-36
+        bound += 2.0 ** -36 * np.stack([seen[:, h].astype(np.float64) @ np.abs(safe[:, h]) for h in range(H)], 1)
         lse = np.where(any_, top + np.log(np.where(any_, total, 1.0)), -np.inf)
         lse_bound = err + 2.0 ** -20 + 4 * math.sqrt(max(T, 1)) * 2.0 ** -24 + 2.0 ** -22 * np.abs(np.where(any_, lse, 0.0))
         return out, bound, lse, lse_bound
