@@ -192,14 +192,24 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
             x = *reinterpret_cast<const __attribute__((aligned(4))) Item*>(p);
         }
     };
+    const long long klane = key0 * a.k_row + pb, vlane0 = key0 * a.v_row + pb;
     auto fetch = [&](int t) {
         if (!idle) {
+            const char *kt = kb + (long long)t * TK * a.k_row, *vt = vb + (long long)t * TK * a.v_row;
+            if (t * TK + TK <= a.T) {
 #pragma unroll
-            for (int n = 0; n < NL; ++n) {
-                long long at = (long long)t * TK + NT / PR * n;
-                if (t * TK + TK > a.T) at = min(at, (long long)a.T - 1 - key0);  // (rows past the end reread the last one)
-                load(kb + at * a.k_row + (key0 * a.k_row + pb), kraw[n], ksc[Q4 ? n : 0]);
-                load(vb + at * a.v_row + (key0 * a.v_row + pb), vraw[n], vsc[Q4 ? n : 0]);
+                for (int n = 0; n < NL; ++n) {
+                    load(kt + NT / PR * n * a.k_row + klane, kraw[n], ksc[Q4 ? n : 0]);
+                    load(vt + NT / PR * n * a.v_row + vlane0, vraw[n], vsc[Q4 ? n : 0]);
+                }
+            } else {
+                asm volatile("" ::: "memory");  // (a branch: as selects, its products would be every step's)
+#pragma unroll
+                for (int n = 0; n < NL; ++n) {  // rows past the end reread the last one
+                    const long long at = min(NT / PR * n + key0, a.T - 1 - t * TK);
+                    load(kt + at * a.k_row + pb, kraw[n], ksc[Q4 ? n : 0]);
+                    load(vt + at * a.v_row + pb, vraw[n], vsc[Q4 ? n : 0]);
+                }
             }
         }
         if constexpr (SHAPED) {
@@ -213,6 +223,7 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     // (whatever is done to a loaded value is done here: done in fetch, it would wait for the loads there)
     auto store = [&](int t, char* buf, int* wild) {
         if (t * TK + TK > a.T) {  // values past the end are 0
+            asm volatile("" ::: "memory");
 #pragma unroll
             for (int n = 0; n < NL; ++n)
                 if (t * TK + NT / PR * n + key0 >= a.T) {
@@ -294,15 +305,19 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         if (meta) full = full && mapped && (__builtin_amdgcn_readfirstlane(map[(t - t0) / SPC]) >> (8 + (t - t0) % SPC) & 1);
         else full = full && k0 + 31 <= wmin;
         const bool work = full || meta || k0 <= wmax;
+        // the next step into the other buffer (last read before the barrier that ended the step before this one): the second set
+        // now, beside the first one's products, the first set at the end, beside the second one's
+        auto stage = [&]() {
+            if (tn < t1) store(tn, lds + ((it + 1) & 1) * G::Buf, wildAt + 2 * sn);
+            if (tnn < t1) fetch(tnn);
+        };
+        if (ks == 1) stage();
         MaskWords mk;
         if constexpr (SHAPED) {
             if (mrow && work) mk.load(mrow, t * (TK / 32) + ks, h, a.T);
         }
         float x[16];
         if (work) keyScores<D, Q4>(cur + ks * 32 * G::KRow, cur + G::oScale + ks * NB * 64, j, h, qh, ql, x);
-        // the next step into the other buffer (last read before the barrier that ended the step before this one)
-        if (tn < t1) store(tn, lds + ((it + 1) & 1) * G::Buf, wildAt + 2 * sn);
-        if (tnn < t1) fetch(tnn);
         if (work) {
             const int wildBits = wildAt[2 * slot + ks];
             const int* kp = reinterpret_cast<const int*>(cur + G::oMeta) + 32 * ks + 4 * h;
@@ -389,6 +404,7 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                     }
                 }
         }
+        if (ks == 0) stage();
         if (tid < 2) wildAt[2 * sc + tid] = 0;
         slot = sn;
         t = tn;

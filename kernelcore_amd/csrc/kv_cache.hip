@@ -15,6 +15,7 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f4a4 __attribute__((aligned(4)));
 typedef uint32_t u32a2 __attribute__((aligned(2)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ long long index64(const int* idx, long long i) {
@@ -129,7 +130,9 @@ __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restri
 // One workgroup per head. The weight of rank `want` among the free positions by a radix search from the top (four
 // digits of eight bits over order-preserving codes), then the positions above it and the first of those equal to it, written
 // in ascending order: each wavefront owns a contiguous piece of the row, so that ballots and one prefix over the
-// wavefronts give every position its place.
+// wavefronts give every position its place. Up to R x 1024 positions are read once and held in registers through the six
+// sweeps, so that what is left is the latency of the load and of the steps between barriers; longer rows (R = 0) are read by
+// each sweep.
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 
 __device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first
@@ -137,9 +140,10 @@ __device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0
     return w != w ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
+template <int R>
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __restrict__ w, int* __restrict__ keep, int T,
                                                                int w_row, int n_keep, int keep_row, int first, int recent) {
-    __shared__ unsigned hist[256];
+    __shared__ unsigned hist[2][256];
     __shared__ unsigned found[2];
     __shared__ int above[kKeepWaves], equal[kKeepWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -147,26 +151,48 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
     int* out = keep + (size_t)blockIdx.x * keep_row;
     const int lo = first, hi = T - recent;      // the free positions
     unsigned want = n_keep - first - recent;    // how many of them stay
+    const int piece = ((hi - lo + kKeepWaves - 1) / kKeepWaves + 63) / 64 * 64;
+    const int p0 = (int)min((long long)hi, lo + (long long)wave * piece), p1 = min(hi, p0 + piece);
+    const int n = (p1 - p0 + 63) / 64;          // (at most R where R > 0)
+    uint32_t held[R > 0 ? R : 1];
+    if constexpr (R > 0) {
+        float x[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) x[k] = k < n ? wr[min(p0 + 64 * k + lane, p1 - 1)] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < R; ++k) held[k] = rankCode(x[k]);
+    }
+    // f(k, position, code) for this wavefront's positions, 64 at a time (in a last, partial 64 the lanes past it with position p1)
+    auto sweep = [&](auto&& f) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (k < n) f(min(p0 + 64 * k + lane, p1), held[k]);
+        } else {
+#pragma unroll 4
+            for (int k = 0; k < n; ++k) {
+                const int i = p0 + 64 * k + lane;
+                f(min(i, p1), rankCode(wr[min(i, p1 - 1)]));
+            }
+        }
+    };
     for (int i = tid; i < first; i += kKeepThreads) out[i] = i;
     for (int i = tid; i < recent; i += kKeepThreads) out[n_keep - recent + i] = T - recent + i;
     if (want == 0) return;
-    const int piece = ((hi - lo + kKeepWaves - 1) / kKeepWaves + 63) / 64 * 64;
-    const int p0 = (int)min((long long)hi, lo + (long long)wave * piece), p1 = min(hi, p0 + piece);
+    if (tid < 256) hist[0][tid] = 0;
+    __syncthreads();
 
     uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-#pragma unroll 4
-        for (int i = p0 + lane; i < p1; i += 64) {
-            const uint32_t u = rankCode(wr[i]);
-            if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[u >> shift & 255u], 1u);
-        }
+    for (int shift = 24, side = 0; shift >= 0; shift -= 8, side ^= 1) {
+        sweep([&](int i, uint32_t u) {
+            if (i < p1 && (shift == 24 || (u >> (shift + 8)) == prefix)) atomicAdd(&hist[side][u >> shift & 255u], 1u);
+        });
+        if (tid >= 256 && tid < 512) hist[side ^ 1][tid - 256] = 0;
         __syncthreads();
         if (wave == 0) {  // the digit at which the count from the top reaches `want`
             unsigned c[4], sum = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += c[e] = hist[255 - (4 * lane + e)];
+            for (int e = 0; e < 4; ++e) sum += c[e] = hist[side][255 - (4 * lane + e)];
             unsigned upto = sum;
 #pragma unroll
             for (int o = 1; o < 64; o *= 2) {
@@ -189,17 +215,10 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
     }
     // prefix: the code of the last weight that stays; want: how many equal to it stay
     int gt = 0, eq = 0;
-#pragma unroll 4
-    for (int i = p0 + lane; i < p1; i += 64) {
-        const uint32_t u = rankCode(wr[i]);
-        gt += u > prefix;
-        eq += u == prefix;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        gt += __shfl_xor(gt, o);
-        eq += __shfl_xor(eq, o);
-    }
+    sweep([&](int i, uint32_t u) {
+        gt += (int)__popcll(__ballot(i < p1 && u > prefix));
+        eq += (int)__popcll(__ballot(i < p1 && u == prefix));
+    });
     if (lane == 0) {
         above[wave] = gt;
         equal[wave] = eq;
@@ -211,27 +230,26 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
         ties += equal[x];
     }
     at += min(ties, (int)want);
-    for (int i0 = p0; i0 < p1; i0 += 64) {
-        const int i = i0 + lane;
-        const uint32_t u = i < p1 ? rankCode(wr[i]) : 0u;
-        const unsigned long long below = (1ull << lane) - 1;
+    const unsigned long long below = (1ull << lane) - 1;
+    sweep([&](int i, uint32_t u) {
         const unsigned long long e = __ballot(i < p1 && u == prefix);
         const bool stays = i < p1 && (u > prefix || (u == prefix && ties + (int)__popcll(e & below) < (int)want));
         const unsigned long long s = __ballot(stays);
-        if (stays) out[at + __popcll(s & below)] = i;
-        at += __popcll(s);
-        ties += __popcll(e);
-    }
+        if (stays) out[at + (int)__popcll(s & below)] = i;
+        at += (int)__popcll(s);
+        ties += (int)__popcll(e);
+    });
 }
 
 // ---------------------------------------------------------------------------------------------- kept rows
-// One grid over planes, heads and the rows' units (the widest of 16, 4 and 2 bytes that all addresses of a plane
-// allow); eight units per thread in flight. Bound by memory.
+// One grid over planes, heads and rows. A row's units (the widest of 16, 8, 4 and 2 bytes that all addresses of a plane
+// allow) lie on the next power of two of lanes, up to 256; each thread moves up to eight units whose loads are all in flight
+// before the first store. Bound by memory.
 struct GatherPlane {
     const char* src;
     char* dst;
     long long src_row, src_head, dst_row, dst_head;
-    int units, unit;  // of a row
+    int units, unit, lanes;  // units of a row, bytes of a unit, log2 of the lanes to a row
 };
 struct GatherArgs {
     GatherPlane p[4];
@@ -241,41 +259,40 @@ struct GatherArgs {
 constexpr int kGather = 8;
 
 template <class U>
-__device__ __forceinline__ void gatherRows(const GatherPlane& p, const int* keep, int n_keep, int T, long long i0, int g) {
-    const long long total = (long long)n_keep * p.units;
-    U x[kGather];
+__device__ __forceinline__ void gatherRows(const GatherPlane& p, const int* keep, int n_keep, int T, int g) {
+    const int per = 256 >> p.lanes, u0 = threadIdx.x & ((1 << p.lanes) - 1);  // rows of a pass, this thread's unit
+    const long long r0 = (long long)blockIdx.x * per * kGather + (threadIdx.x >> p.lanes);
+    if (r0 >= n_keep) return;
+    const char* src = p.src + g * p.src_head;
+    char* dst = p.dst + g * p.dst_head;
     int from[kGather];
 #pragma unroll
     for (int k = 0; k < kGather; ++k) {
-        const long long i = i0 + 256 * k;
         from[k] = -1;
-        if (i < total) {
-            const int s = keep[i / p.units];
+        if (r0 + per * k < n_keep) {
+            const int s = keep[r0 + per * k];
             from[k] = s < T ? s : -1;
         }
     }
+    for (int u = u0; u < p.units; u += 256) {  // (more than once only in rows of more than 256 units)
+        U x[kGather];
 #pragma unroll
-    for (int k = 0; k < kGather; ++k) {
-        const long long i = i0 + 256 * k;
-        if (from[k] >= 0)
-            x[k] = *reinterpret_cast<const U*>(p.src + (long long)from[k] * p.src_row + g * p.src_head + (i % p.units) * (long long)sizeof(U));
-    }
+        for (int k = 0; k < kGather; ++k)
+            if (from[k] >= 0) x[k] = *reinterpret_cast<const U*>(src + (long long)from[k] * p.src_row + (long long)u * (int)sizeof(U));
 #pragma unroll
-    for (int k = 0; k < kGather; ++k) {
-        const long long i = i0 + 256 * k;
-        if (from[k] >= 0)
-            *reinterpret_cast<U*>(p.dst + (i / p.units) * p.dst_row + g * p.dst_head + (i % p.units) * (long long)sizeof(U)) = x[k];
+        for (int k = 0; k < kGather; ++k)
+            if (from[k] >= 0) *reinterpret_cast<U*>(dst + (r0 + per * k) * p.dst_row + (long long)u * (int)sizeof(U)) = x[k];
     }
 }
 
 __global__ __launch_bounds__(256) void kv_gather_kernel(GatherArgs a) {
     const GatherPlane& p = a.p[blockIdx.z];
     const int g = blockIdx.y;
-    const long long i0 = (long long)blockIdx.x * 256 * kGather + threadIdx.x;
     const int* keep = a.keep + (size_t)g * a.keep_row;
-    if (p.unit == 16) gatherRows<u4>(p, keep, a.n_keep, a.T, i0, g);
-    else if (p.unit == 4) gatherRows<uint32_t>(p, keep, a.n_keep, a.T, i0, g);
-    else gatherRows<unsigned short>(p, keep, a.n_keep, a.T, i0, g);
+    if (p.unit == 16) gatherRows<u4>(p, keep, a.n_keep, a.T, g);
+    else if (p.unit == 8) gatherRows<u2>(p, keep, a.n_keep, a.T, g);
+    else if (p.unit == 4) gatherRows<uint32_t>(p, keep, a.n_keep, a.T, g);
+    else gatherRows<unsigned short>(p, keep, a.n_keep, a.T, g);
 }
 
 }  // namespace
@@ -284,13 +301,14 @@ int launchSetRowsQ40(const kcSetRowsQ40Args& a, hipStream_t s) {
     if (a.rows == 0) return 0;
     const int nb = a.n / 32;
     char* dst = static_cast<char*>(a.dst);
-    // few rows: a workgroup each; more: eight per workgroup, which then share the search for repeated indices
-    if (a.rows <= 64)
-        hipLaunchKernelGGL(set_rows_q4_0_kernel<1>, dim3((nb + 31) / 32, a.rows), dim3(256), 0, s, a.src, a.idx, dst, nb, a.rows,
-                           a.src_row, a.dst_rows, a.dst_row);
-    else
-        hipLaunchKernelGGL(set_rows_q4_0_kernel<8>, dim3((nb + 31) / 32, (a.rows + 7) / 8), dim3(256), 0, s, a.src, a.idx, dst, nb,
-                           a.rows, a.src_row, a.dst_rows, a.dst_row);
+    auto run = [&](auto kernel, int r) {
+        hipLaunchKernelGGL(kernel, dim3((nb + 31) / 32, (a.rows + r - 1) / r), dim3(256), 0, s, a.src, a.idx, dst, nb, a.rows, a.src_row,
+                           a.dst_rows, a.dst_row);
+    };
+    // rows of a workgroup share its search for repeated indices, which grows with the rows; few rows fill the GPU one each
+    if (a.rows <= 2048) run(set_rows_q4_0_kernel<1>, 1);
+    else if (a.rows <= 8192) run(set_rows_q4_0_kernel<2>, 2);
+    else run(set_rows_q4_0_kernel<8>, 8);
     return fromHip(hipGetLastError(), "set_rows_q4_0");
 }
 
@@ -304,8 +322,15 @@ int launchGetRowsQ40(const kcGetRowsQ40Args& a, hipStream_t s) {
 
 int launchKvKeep(const kcKvKeepArgs& a, hipStream_t s) {
     if (a.n_keep == 0) return 0;
-    hipLaunchKernelGGL(kv_keep_kernel, dim3(a.heads), dim3(kKeepThreads), 0, s, a.w, a.keep, a.T, a.w_row, a.n_keep, a.keep_row,
-                       a.first, a.recent);
+    auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(a.heads), dim3(kKeepThreads), 0, s, a.w, a.keep, a.T, a.w_row, a.n_keep, a.keep_row, a.first,
+                           a.recent);
+    };
+    // (a wavefront's piece is a sixteenth of the free positions, rounded up to 64: R 64 at most)
+    if (a.T <= 5 * kKeepThreads - 1024) run(kv_keep_kernel<5>);
+    else if (a.T <= 17 * kKeepThreads - 1024) run(kv_keep_kernel<17>);
+    else if (a.T <= 33 * kKeepThreads - 1024) run(kv_keep_kernel<33>);
+    else run(kv_keep_kernel<0>);
     return fromHip(hipGetLastError(), "kv_keep");
 }
 
@@ -317,10 +342,13 @@ int launchKvGather(const kcKvGatherArgs& a, hipStream_t s) {
         const kcKvPlane& p = a.planes[i];
         const auto all = reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.dst) | uintptr_t(p.src_row) |
                          uintptr_t(p.src_head) | uintptr_t(p.dst_row) | uintptr_t(p.dst_head) | uintptr_t(p.bytes);
-        const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
+        const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2, units = p.bytes / unit;
+        int lanes = 0;
+        while (lanes < 8 && (1 << lanes) < units) ++lanes;
         g.p[i] = GatherPlane{static_cast<const char*>(p.src), static_cast<char*>(p.dst), p.src_row, p.src_head, p.dst_row,
-                             p.dst_head, p.bytes / unit, unit};
-        blocks = std::max(blocks, ((long long)a.n_keep * (p.bytes / unit) + 256 * kGather - 1) / (256 * kGather));
+                             p.dst_head, units, unit, lanes};
+        const int rows = (256 >> lanes) * kGather;
+        blocks = std::max(blocks, ((long long)a.n_keep + rows - 1) / rows);
     }
     g.keep = a.keep;
     g.n_keep = a.n_keep;
