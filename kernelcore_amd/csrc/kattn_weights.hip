@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxP
     constexpr int NB = G::NB, KW = 4 / RW, KT = KW * TP, PR = Q4 ? NB : D / 8, KS = D / 16;
     extern __shared__ int4 lds4[];
     __shared__ float part[4][TP][32];
-    __shared__ float4 rows4[4][32];  // factor, lse (base 2), slope, -
+    __shared__ float4 rows4[4][32];  // factor of the sums (base 2 unless capped), lse (base 2), slope, -
     __shared__ int4 rows4i[4][32];   // limit, position, document, token
     char* lds = reinterpret_cast<char*>(lds4);
     const int kvh = blockIdx.y;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxP
         const float c = loadRow32<D>(a, row, h, qh, ql);
         const float lse = row.live ? a.lse[(size_t)row.token * a.H + row.head] : -INFINITY;
         if (h == 0) {  // (a row that saw nothing gives nothing: its factor's place holds the mark)
-            rows4[wave][j] = make_float4(c, lse == -INFINITY ? INFINITY : lse * kLog2e, row.slope, 0.0f);
+            rows4[wave][j] = make_float4(shape.inv_cap > 0.0f ? c : factor2(c), lse == -INFINITY ? INFINITY : lse * kLog2e, row.slope, 0.0f);
             rows4i[wave][j] = make_int4(lse == -INFINITY ? -1 : row.limit, row.pos, row.doc, row.token);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxP
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const float2 cl = *reinterpret_cast<const float2*>(&rows4[wave][8 * (v >> 2) + 4 * h + (v & 3)]);
-                    acc[p] += ex2(fmaf(x[v], factor2(cl.x), -cl.y));
+                    acc[p] += ex2(fmaf(x[v], cl.x, -cl.y));
                 }
                 continue;
             }
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxP
                 capScores<16>(x, shape.inv_cap, shape);
             } else {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] *= factor2(rf[v].x);
+                for (int v = 0; v < 16; ++v) x[v] *= rf[v].x;
             }
 #pragma unroll
             for (int v = 0; v < 16; ++v) {

@@ -169,7 +169,6 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
             for (int k = 0; k < R; ++k)
                 if (k < n) f(min(p0 + 64 * k + lane, p1), held[k]);
         } else {
-#pragma unroll 4
             for (int k = 0; k < n; ++k) {
                 const int i = p0 + 64 * k + lane;
                 f(min(i, p1), rankCode(wr[min(i, p1 - 1)]));
