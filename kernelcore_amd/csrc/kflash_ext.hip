@@ -45,13 +45,6 @@ __device__ __forceinline__ uint32_t tameHalves(uint32_t w) {
     return w & ~((z >> 15 & 1u) * 0xFFFFu | (z >> 31) * 0xFFFF0000u);
 }
 
-// The lanes' loads and stores of LDS before this are done before those after it (a wavefront's own LDS accesses run in
-// order: only the compiler has to keep them so).
-__device__ __forceinline__ void waveLds() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // ---------------------------------------------------------------------------------------------- many rows
 // Workgroup: 128 rows of a KV head (four wavefronts of 32 rows) over one range of keys. A step takes KS tiles of 32 keys; with
 // KS = 2 two sets of four wavefronts take a tile each, joined through LDS at the end. Matrix form (v_mfma_f32_32x32x16_f16,
@@ -73,12 +66,14 @@ struct Geo {
     static constexpr int oScale = TK * KRow;                              // 4-bit: the keys' scales
     static constexpr int oV = oScale + (Q4 ? NB * TK * 2 : 0), oLow = TK * VRow;  // values, 4-bit: their rests
     static constexpr int oMeta = oV + TK * VRow * (Q4 ? 2 : 1);           // positions, document numbers
-    static constexpr int Buf = oMeta + TK * 8, oMap = 2 * Buf;
+    static constexpr int QRow = 2 * D + 16;                           // a row of q: fp16 values hi, their lo parts
+    static constexpr int Buf = oMeta + TK * 8, oMap = 2 * Buf > 256 * QRow ? 2 * Buf : 256 * QRow;
     static constexpr int MapEntries = 2048;      // 256 keys each: the steps with a key that some row may see, those all rows see
     static constexpr int oWild = oMap + 2 * MapEntries;  // 3 x the step's wild keys
     static constexpr int oZ = oWild + 32;                // a wild key's values, for each wavefront
-    static constexpr int ORow = D / 2 + 4;       // the join of the two sets: floats per lane
-    static constexpr int Join = KS == 2 ? 256 * ORow * 4 : 0;
+    static constexpr int oTops = oZ;                     // and, before the first step, the rows' largest |q|
+    static constexpr int OV = D / 16;            // the join of the two sets: vectors of four per lane
+    static constexpr int Join = KS == 2 ? 512 * (OV * 16 + 8) : 0;
     static constexpr int End = oZ + 4 * KS * D * 4;
     static constexpr int Lds = End > Join ? End : Join;
 };
@@ -96,8 +91,8 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     const int j = lane & 31, h = lane >> 5, rw = wave & 3, ks = wave >> 2;
     const int r0 = rb * 128 + rw * 32, r = r0 + j;
     const Row row = rowOf(a, kvh, r);
-    h8 qh[D / 16], ql[D / 16];
-    const float c = loadRow32<D>(a, row, h, qh, ql), c2 = factor2(c);
+    RowQ<D / G::KS> q;  // (each set takes its part of the values)
+    q.load(a.q + ks * (D / G::KS), (long long)row.token * a.q_tok + (long long)row.head * a.q_head, lane);
     const unsigned short* mrow = SHAPED && a.mask ? a.mask + (size_t)row.token * a.m_row2 : nullptr;
     const bool meta = SHAPED && (a.kpos || a.kdoc);
     const int* kpos = SHAPED && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
@@ -126,31 +121,36 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     const bool mapped = meta && (t1 - t0 + SPC - 1) / SPC <= G::MapEntries;
     if constexpr (SHAPED) {
         if (mapped) {  // a wavefront takes 256 keys, four a lane
-            if (a.qdoc) {
-                const int d0 = a.qdoc[min(b0 + lane, b1)], d1 = a.qdoc[min(b0 + 64 + lane, b1)];
-                dmin = waveMin(min(d0, d1));
-                dmax = waveMax(max(d0, d1));
-            }
             constexpr int LPT = TK / 4;  // lanes to a step
-            const int key1 = min(a.T, t1 * TK);
-            for (int at = wave; at * 256 < key1 - t0 * TK; at += NT / 64) {
+            const int key1 = min(a.T, t1 * TK), n = (key1 - t0 * TK + 255) / 256;
+            int p[4], x[4];
+            auto keysOf = [&](int at) {
                 const int key = t0 * TK + at * 256 + 4 * lane;
-                int p[4] = {key, key + 1, key + 2, key + 3}, x[4] = {dmin, dmin, dmin, dmin};
                 if (key + 3 < key1) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = key + e;
                     if (kpos) *reinterpret_cast<int4*>(p) = *reinterpret_cast<const int4a4*>(kpos + key);
                     if (kdoc) *reinterpret_cast<int4*>(x) = *reinterpret_cast<const int4a4*>(kdoc + key);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if (kpos && key + e < key1) p[e] = kpos[key + e];
-                        if (kdoc && key + e < key1) x[e] = kdoc[key + e];
-                        if (key + e >= key1) p[e] = -1;
+                        p[e] = key + e >= key1 ? -1 : kpos ? kpos[key + e] : key + e;
+                        x[e] = kdoc && key + e < key1 ? kdoc[key + e] : 0;
                     }
                 }
+            };
+            int at = wave;
+            if (at < n) keysOf(at);
+            if (a.qdoc) {
+                const int d0 = a.qdoc[min(b0 + lane, b1)], d1 = a.qdoc[min(b0 + 64 + lane, b1)];
+                dmin = waveMin(min(d0, d1));
+                dmax = waveMax(max(d0, d1));
+            }
+            for (; at < n; at += NT / 64) {
                 bool some = false, all = true;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool in = p[e] >= 0 && p[e] <= bmax && x[e] >= dmin && x[e] <= dmax;
+                    const bool in = p[e] >= 0 && p[e] <= bmax && (!kdoc || (x[e] >= dmin && x[e] <= dmax));
                     some |= in;
                     all &= in && p[e] <= bmin && dmin == dmax;
                 }
@@ -158,10 +158,14 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                 const unsigned long long sb = __ballot(lane < SPC && (s >> (lane % SPC * LPT) & group)),
                                          wb = __ballot(lane < SPC && (w >> (lane % SPC * LPT) & group) == group);
                 if (lane == 0) map[at] = (unsigned short)(sb | wb << 8);
+                if (at + NT / 64 < n) keysOf(at + NT / 64);
             }
-            __syncthreads();
         }
     }
+    float* tops = reinterpret_cast<float*>(lds + G::oTops) + rw * 32;
+    q.tops(tops + ks * 128, lane);
+    if (tid < 8) wildAt[tid] = 0;
+    __syncthreads();
     auto next = [&](int t) -> int {  // the first step from t on that is to be computed; t1 if none
         if (!mapped) return min(t, t1);
         while (t < t1) {
@@ -289,8 +293,22 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     float m = -INFINITY, l = 0.0f;
 
     int t = next(t0), tn = t < t1 ? next(t + 1) : t1;
-    if (tid < 8) wildAt[tid] = 0;
     if (t < t1) fetch(t);
+    h8 qh[D / 16], ql[D / 16];
+    auto topOf = [&](int r) { return G::KS == 2 ? fmaxf(tops[r], tops[128 + r]) : tops[r]; };
+    const float c = qScale(topOf(j), a.scale).c, c2 = factor2(c);
+    {
+        _Float16* qr = reinterpret_cast<_Float16*>(lds) + rw * 32 * G::QRow;
+        h4 low[RowQ<D / G::KS>::N];
+        q.split(a, qr + ks * (D / G::KS), G::QRow, lane, topOf, low);
+        q.place(qr + D + 8 + ks * (D / G::KS), G::QRow, lane, low);
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            qh[n] = *reinterpret_cast<const h8*>(qr + j * G::QRow + 16 * n + 8 * h);
+            ql[n] = *reinterpret_cast<const h8*>(qr + j * G::QRow + D + 8 + 16 * n + 8 * h);
+        }
+    }
     __syncthreads();
     if (t < t1) store(t, lds, wildAt);
     if (tn < t1) fetch(tn);
@@ -412,31 +430,39 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         __syncthreads();
     }
 
+    // the two sets swap halves of their sums, each joins and writes one half of the values
     l += __shfl_xor(l, 32);
-    if constexpr (G::KS == 2) {  // the second set's (o, m, l) to the first
-        float* mg = reinterpret_cast<float*>(lds) + (size_t)(rw * 64 + lane) * G::ORow;
-        if (ks == 1) {
+    constexpr int OB = DB / G::KS;  // blocks of 32 values that a wavefront writes
+    const int d0 = ks * OB;
+    if constexpr (G::KS == 2) {
+        f32x4* mg = reinterpret_cast<f32x4*>(lds) + (size_t)wave * 64 * G::OV + lane;
+        float2* ml = reinterpret_cast<float2*>(lds + 8 * 64 * G::OV * 16) + wave * 64 + lane;
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(mg + 16 * d + 4 * g) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-            mg[D / 2] = m;
-            mg[D / 2 + 1] = l;
-        }
-        __syncthreads();
-        if (ks == 1) return;
-        const float m1 = mg[D / 2], l1 = mg[D / 2 + 1], M = fmaxf(m, m1);
-        const float f0 = m == -INFINITY ? 0.0f : ex2(m - M), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - M);
-        l = l * f0 + l1 * f1;
-        m = M;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < OB; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 y = *reinterpret_cast<const f32x4*>(mg + 16 * d + 4 * g);
+                const f32x16 &u = o[d], &w = o[OB + d];
+                mg[64 * (4 * d + g)] = ks ? f32x4{u[4 * g], u[4 * g + 1], u[4 * g + 2], u[4 * g + 3]}
+                                          : f32x4{w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]};
+            }
+        *ml = make_float2(m, l);
+        __syncthreads();
+        mg += ks ? -4 * 64 * G::OV : 4 * 64 * G::OV;
+        ml += ks ? -256 : 256;
+        const float m1 = ml->x, l1 = ml->y, M = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.0f : ex2(m - M), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - M);
+        l = ks ? l1 * f1 + l * f0 : l * f0 + l1 * f1;
+        m = M;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[d][4 * g + e] = o[d][4 * g + e] * f0 + y[e] * f1;
+        for (int d = 0; d < OB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 y = mg[64 * (4 * d + g)];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float own = ks ? o[OB + d][4 * g + e] : o[d][4 * g + e];
+                    o[d][4 * g + e] = own * f0 + y[e] * f1;
+                }
             }
     }
     if (!row.live) return;
@@ -445,23 +471,23 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     if (a.splits == 1) {
         dst = a.out + ((size_t)row.token * a.H + row.head) * D;
         f = l == 0.0f ? 0.0f : 1.0f / l;
-        if (a.lse && h == 0) a.lse[(size_t)row.token * a.H + row.head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l * kPInv));
+        if (a.lse && h == 0 && ks == 0) a.lse[(size_t)row.token * a.H + row.head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l * kPInv));
     } else {
         const size_t at = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
         dst = a.part + at * D;
         f = kPInv;
-        if (h == 0) {
+        if (h == 0 && ks == 0) {
             float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * at;
             ml[0] = m;
             ml[1] = l * kPInv;
         }
     }
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < OB; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4 y = {o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f};
-            *reinterpret_cast<f4a4*>(dst + 32 * d + 8 * g + 4 * h) = y;
+            *reinterpret_cast<f4a4*>(dst + 32 * (d0 + d) + 8 * g + 4 * h) = y;
         }
 }
 

@@ -27,6 +27,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef int i2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // loads and stores at the alignment the callers' strides leave
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef u4 u4a4 __attribute__((aligned(4)));
 typedef u4 u4a2 __attribute__((aligned(2)));
 typedef uint32_t u32a2 __attribute__((aligned(2)));
@@ -266,36 +267,102 @@ __device__ __forceinline__ float waveSumF(float x) {
     return x;
 }
 
+// The lanes' loads and stores of LDS before this are done before those after it (a wavefront's own LDS accesses run in
+// order: only the compiler has to keep them so).
+__device__ __forceinline__ void waveLds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- tiles of 32 keys x 32 rows (v_mfma_f32_32x32x16_f16; lane (j, h) = row j, lane half h)
 
 // LDS bytes of a key's row as fp16: one pad chunk puts consecutive rows on different banks
 template <int D>
 constexpr int kKeyRow = 2 * D + 16;
 
-// q as the B operand: values 16 ks + 8 h .. + 8 of the lane's row; returns the factor of its scores
-template <int D>
-__device__ __forceinline__ float loadRow32(const FxParams& a, const Row& row, int h, h8 (&qh)[D / 16], h8 (&ql)[D / 16]) {
-    constexpr int KS = D / 16;
-    const float* qp = a.q + (size_t)row.token * a.q_tok + (size_t)row.head * a.q_head + 8 * h;
-    float x[KS][8], top = 0.0f;
+// q of 32 rows, W values of each, on its way to operands: loaded with consecutive lanes on consecutive values (a lane half per
+// row instead, as the operands have it, touches 32 cache lines an instruction and comes back to each four times: 4 us of a
+// workgroup's start), divided into hi and lo there, and turned into operands (values 16 ks + 8 h .. + 8 of the lane's row)
+// through LDS, as fp16.
+template <int W>
+struct RowQ {
+    static constexpr int LPR = W / 4, RPI = 64 / LPR, N = 32 / RPI;  // lanes to a row, rows to an instruction, instructions
+    f32x4 x[N];
+    // at: where the q of row lane % 32 begins, in floats
+    __device__ __forceinline__ void load(const float* q, long long at, int lane) {
+        const int lo = (int)at, hi = (int)(at >> 32);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const f32x4 u = *reinterpret_cast<const f4a4*>(qp + 16 * ks), w = *reinterpret_cast<const f4a4*>(qp + 16 * ks + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[ks][e] = u[e];
-            x[ks][4 + e] = w[e];
-            top = fmaxf(top, fmaxf(fabsf(u[e]), fabsf(w[e])));
+        for (int n = 0; n < N; ++n) {
+            const int src = n * RPI + lane / LPR;
+            const long long o = (long long)(((unsigned long long)(unsigned)__shfl(hi, src) << 32) | (unsigned)__shfl(lo, src));
+            x[n] = *reinterpret_cast<const f4a4*>(q + o + 4 * (lane % LPR));
         }
     }
+    // the rows' largest magnitudes to top[row]
+    __device__ __forceinline__ void tops(float* top, int lane) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float m = fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+            m = fmaxf(m, dpp<0xB1>(m));   // lane ^ 1
+            m = fmaxf(m, dpp<0x4E>(m));   // ^ 2
+            m = fmaxf(m, dpp<0x141>(m));  // the other four of eight
+            if constexpr (LPR >= 16) m = fmaxf(m, dpp<0x140>(m));  // the other eight of 16
+            if constexpr (LPR >= 32) m = swap16Max(m);
+            if constexpr (LPR >= 64) m = swap32Max(m);
+            if (lane % LPR == 0) top[n * RPI + lane / LPR] = m;
+        }
+    }
+    template <int CTRL>
+    static __device__ __forceinline__ float dpp(float v) {
+        const int u = __builtin_bit_cast(int, v);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, CTRL, 0xF, 0xF, false));
+    }
+    // the hi parts of row r's values to rows of `stride` fp16, the lo parts to `low`; topOf(r): the row's largest magnitude
+    template <class F>
+    __device__ __forceinline__ void split(const FxParams& a, _Float16* hi, int stride, int lane, F&& topOf, h4 (&low)[N]) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = n * RPI + lane / LPR, shift = qScale(topOf(r), a.scale).shift;
+            h4 u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                _Float16 y, z;
+                qSplit(x[n][e], a.scale < 0.0f, shift, y, z);
+                u[e] = y;
+                low[n][e] = z;
+            }
+            *reinterpret_cast<h4*>(hi + r * stride + 4 * (lane % LPR)) = u;
+        }
+    }
+    __device__ __forceinline__ void place(_Float16* to, int stride, int lane, const h4 (&v)[N]) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) *reinterpret_cast<h4*>(to + (n * RPI + lane / LPR) * stride + 4 * (lane % LPR)) = v[n];
+    }
+};
+
+// The same for a wavefront alone (few rows, whose lines the lanes share): values 16 ks + 8 h .. + 8 of the lane's row, loaded first, divided
+// into hi and lo when they are there; returns the factor of the row's scores.
+template <int D>
+__device__ __forceinline__ void loadRow32(const FxParams& a, const Row& row, int h, f32x4 (&x)[D / 8]) {
+    const float* qp = a.q + (size_t)row.token * a.q_tok + (size_t)row.head * a.q_head + 8 * h;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) x[n] = *reinterpret_cast<const f4a4*>(qp + 16 * (n >> 1) + 4 * (n & 1));
+}
+template <int D>
+__device__ __forceinline__ float splitRow32(const FxParams& a, const f32x4 (&x)[D / 8], h8 (&qh)[D / 16], h8 (&ql)[D / 16]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[n][e]));
     top = fmaxf(top, __shfl_xor(top, 32));
     const QScale qs = qScale(top, a.scale);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             _Float16 hi, lo;
-            qSplit(x[ks][e], a.scale < 0.0f, qs.shift, hi, lo);
+            qSplit(x[2 * ks + (e >> 2)][e & 3], a.scale < 0.0f, qs.shift, hi, lo);
             qh[ks][e] = hi;
             ql[ks][e] = lo;
         }
