@@ -127,24 +127,23 @@ __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restri
 }
 
 // ---------------------------------------------------------------------------------------------- positions to keep
-// One workgroup per head. The weight of rank `want` among the free positions by a radix search from the top (four
-// digits of eight bits over order-preserving codes), then the positions above it and the first of those equal to it, written
+// One workgroup per head. The weight of rank `want` among the free positions by a radix search from the top (digits of 11, 11
+// and 10 bits over order-preserving codes), then the positions above it and the first of those equal to it, written
 // in ascending order: each wavefront owns a contiguous piece of the row, so that ballots and one prefix over the
-// wavefronts give every position its place. Up to R x 1024 positions are read once and held in registers through the six
-// sweeps, so that what is left is the latency of the load and of the steps between barriers; longer rows (R = 0) are read by
-// each sweep.
+// wavefronts give every position its place. Up to R x 1024 positions are read once and held in registers through the five
+// sweeps; longer rows (R = 0) are read by each sweep. A head has one compute unit, and the sweeps' instructions bound it.
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 
-__device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first
+__device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first; never 0
     const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.0f ? 0.0f : w);
-    return w != w ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+    return w != w ? 1u : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
 template <int R>
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __restrict__ w, int* __restrict__ keep, int T,
                                                                int w_row, int n_keep, int keep_row, int first, int recent) {
-    __shared__ unsigned hist[2][256];
-    __shared__ unsigned found[2];
+    __shared__ uint2 hist[2][kKeepThreads];  // of 2048 digits
+    __shared__ unsigned waves[kKeepWaves], found[2];
     __shared__ int above[kKeepWaves], equal[kKeepWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* wr = w + (size_t)blockIdx.x * w_row;
@@ -160,63 +159,68 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
 #pragma unroll
         for (int k = 0; k < R; ++k) x[k] = k < n ? wr[min(p0 + 64 * k + lane, p1 - 1)] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < R; ++k) held[k] = rankCode(x[k]);
+        for (int k = 0; k < R; ++k) held[k] = p0 + 64 * k + lane < p1 ? rankCode(x[k]) : 0u;
     }
-    // f(k, position, code) for this wavefront's positions, 64 at a time (in a last, partial 64 the lanes past it with position p1)
+    // f(position, code) for this wavefront's positions, 64 at a time; code 0, less than any weight's, for the lanes past its piece
     auto sweep = [&](auto&& f) {
         if constexpr (R > 0) {
 #pragma unroll
             for (int k = 0; k < R; ++k)
-                if (k < n) f(min(p0 + 64 * k + lane, p1), held[k]);
+                if (k < n) f(p0 + 64 * k + lane, held[k]);
         } else {
             for (int k = 0; k < n; ++k) {
                 const int i = p0 + 64 * k + lane;
-                f(min(i, p1), rankCode(wr[min(i, p1 - 1)]));
+                const uint32_t u = rankCode(wr[min(i, p1 - 1)]);
+                f(i, i < p1 ? u : 0u);
             }
         }
     };
     for (int i = tid; i < first; i += kKeepThreads) out[i] = i;
     for (int i = tid; i < recent; i += kKeepThreads) out[n_keep - recent + i] = T - recent + i;
     if (want == 0) return;
-    if (tid < 256) hist[0][tid] = 0;
+    hist[0][tid] = make_uint2(0, 0);
     __syncthreads();
 
     uint32_t prefix = 0;
-    for (int shift = 24, side = 0; shift >= 0; shift -= 8, side ^= 1) {
-        sweep([&](int i, uint32_t u) {
-            if (i < p1 && (shift == 24 || (u >> (shift + 8)) == prefix)) atomicAdd(&hist[side][u >> shift & 255u], 1u);
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        constexpr int kShift[3] = {21, 10, 0};
+        const int shift = kShift[pass], bits = pass < 2 ? 11 : 10;
+        unsigned* digits = reinterpret_cast<unsigned*>(hist[pass & 1]);
+        sweep([&](int, uint32_t u) {
+            if (pass == 0 || u >> (shift + bits) == prefix) atomicAdd(digits + (u >> shift & ((1u << bits) - 1)), 1u);
         });
-        if (tid >= 256 && tid < 512) hist[side ^ 1][tid - 256] = 0;
+        if (pass < 2) hist[~pass & 1][tid] = make_uint2(0, 0);
         __syncthreads();
-        if (wave == 0) {  // the digit at which the count from the top reaches `want`
-            unsigned c[4], sum = 0;
+        // the digit at which the count from the top reaches `want`: two digits a thread
+        const int d = kKeepThreads - 1 - tid;
+        const uint2 c = hist[pass & 1][d];
+        unsigned upto = c.x + c.y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += c[e] = hist[side][255 - (4 * lane + e)];
-            unsigned upto = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o *= 2) {
-                const unsigned x = __shfl_up(upto, o);
-                if (lane >= o) upto += x;
-            }
-            unsigned before = upto - sum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (before < want && before + c[e] >= want) {
-                    found[0] = 255 - (4 * lane + e);
-                    found[1] = want - before;
-                }
-                before += c[e];
-            }
+        for (int o = 1; o < 64; o *= 2) {
+            const unsigned x = __shfl_up(upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 63) waves[wave] = upto;
+        __syncthreads();
+        unsigned before = upto - c.x - c.y;
+        for (int x = 0; x < wave; ++x) before += waves[x];
+        if (before < want && before + c.y >= want) {
+            found[0] = 2 * d + 1;
+            found[1] = want - before;
+        } else if (before + c.y < want && before + c.y + c.x >= want) {
+            found[0] = 2 * d;
+            found[1] = want - before - c.y;
         }
         __syncthreads();
-        prefix = prefix << 8 | found[0];
+        prefix = prefix << bits | found[0];
         want = found[1];
     }
     // prefix: the code of the last weight that stays; want: how many equal to it stay
     int gt = 0, eq = 0;
-    sweep([&](int i, uint32_t u) {
-        gt += (int)__popcll(__ballot(i < p1 && u > prefix));
-        eq += (int)__popcll(__ballot(i < p1 && u == prefix));
+    sweep([&](int, uint32_t u) {
+        gt += (int)__popcll(__ballot(u > prefix));
+        eq += (int)__popcll(__ballot(u == prefix));
     });
     if (lane == 0) {
         above[wave] = gt;
@@ -231,8 +235,8 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
     at += min(ties, (int)want);
     const unsigned long long below = (1ull << lane) - 1;
     sweep([&](int i, uint32_t u) {
-        const unsigned long long e = __ballot(i < p1 && u == prefix);
-        const bool stays = i < p1 && (u > prefix || (u == prefix && ties + (int)__popcll(e & below) < (int)want));
+        const unsigned long long e = __ballot(u == prefix);
+        const bool stays = u > prefix || (u == prefix && ties + (int)__popcll(e & below) < (int)want);
         const unsigned long long s = __ballot(stays);
         if (stays) out[at + (int)__popcll(s & below)] = i;
         at += (int)__popcll(s);
