@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
 // wavefronts over one range of keys of a KV head, each with its own tiles (64 keys of a 4-bit cache, 32 of an fp16
 // one), joined through LDS at the end. v_mfma_f32_16x16x32_f16, lane (i, kg) = column i, group kg of 16 lanes:
 //   S^T = K Q^T: fp16 keys are loaded as the A operand straight from memory; 4-bit keys go through LDS as they are, lane (i, kg)
-//   takes word kg of a block of key i, the 32 values of a block are one step of the products, and its scale multiplies the
+//   unpacks word kg of a block of key i, the 32 values of a block are one step of the products, and its scale multiplies the
 //   step's f32 sums. Lane (i, kg) then holds keys 16 u + 4 kg + v of row i.
 //   O^T += V^T P^T: 4-bit values are transposed as they are (ds_read_b64_tr_b4: 16 keys of one value per lane), then unpacked
 //   and scaled; fp16 values through 16-bit transposed reads.
@@ -602,11 +602,8 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     wmax = waveMax(wmax);
     if (!kpos) t1 = wmax < 0 ? t0 : min(t1, wmax / TK + 1);
 
-    // q as the B operand of step b (32 values): fp16 keys: values 32 b + 8 kg + e; 4-bit keys: the order nibbles() gives. 4-bit keys
-    // are not even unpacked: a masked nibble is an fp16 number, 2^-24 code, and one four bits up 2^-20 code (q / 16 there);
-    // the sums start from the -8 of every code, -8 2^-24 (sum of the block's q), and the scales carry 2^24.
+    // q as the B operand of step b (32 values): fp16 keys: values 32 b + 8 kg + e; 4-bit keys: the order nibbles() gives
     h8 qh[NR][NB], ql[NR][NB];
-    f32x4 start[NR][NB];
     float c[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -626,23 +623,14 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         const QScale qs = qScale(top, a.scale);
         c[n] = qs.c;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float sum = 0.0f;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 _Float16 hi, lo;
-                qSplit(x[b][e], a.scale < 0.0f, qs.shift - (Q4 && (e & 2) ? 4 : 0), hi, lo);
+                qSplit(x[b][e], a.scale < 0.0f, qs.shift, hi, lo);
                 qh[n][b][e] = hi;
                 ql[n][b][e] = lo;
-                sum += ldexpf(a.scale < 0.0f ? -x[b][e] : x[b][e], qs.shift);
             }
-            if constexpr (Q4) {
-                sum += __shfl_xor(sum, 16);
-                sum += __shfl_xor(sum, 32);
-                sum *= -8.0f * 0x1p-24f;
-                start[n][b] = f32x4{sum, sum, sum, sum};
-            }
-        }
     }
     const Shape shape = SHAPED ? shapeOf(a) : Shape{};
     const NibbleMagic magic = nibbleMagic();
@@ -671,7 +659,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             if constexpr (Q4) {
                 *reinterpret_cast<u4*>(mine + key * G::Row + 16 * part) = kr[n];
                 *reinterpret_cast<u4*>(mine + G::oV + key * G::Row + 16 * part) = vr[n];
-                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = halfBits(kscale[n] & 0xFFFFu) * 0x1p24f;
+                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = halfBits(kscale[n] & 0xFFFFu);
                 uint32_t s = t * TK + key < a.T ? vscale[n] & 0xFFFFu : 0u;
                 if (wildScale(s)) {
                     s = 0;
@@ -708,10 +696,10 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 f32x4 s[NR][NB];  // all blocks' products before their sums are taken: the matrix unit's latency overlaps
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const h8 kk = rawNibbles(*reinterpret_cast<const uint32_t*>(mine + (16 * u + i) * G::Row + 16 * b + 4 * kg), magic);
+                    const h8 kk = nibbles(*reinterpret_cast<const uint32_t*>(mine + (16 * u + i) * G::Row + 16 * b + 4 * kg), magic);
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
-                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[n][b], start[n][b], 0, 0, 0);
+                        s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[n][b], zero, 0, 0, 0);
                         s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[n][b], s[n][b], 0, 0, 0);
                     }
                 }

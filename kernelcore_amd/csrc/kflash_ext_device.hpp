@@ -66,13 +66,6 @@ __device__ __forceinline__ h8 nibbles(uint32_t w, const NibbleMagic& k) {
     const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w8 & k.high) | k.base), by16, off16);
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-// The codes themselves, in the same order, as the fp16 numbers that the masked nibbles are: 2^-24 code (subnormal), and 2^-20
-// code of nibbles 1, 5, 3 and 7.
-__device__ __forceinline__ h8 rawNibbles(uint32_t w, const NibbleMagic& k) {
-    const uint32_t w8 = w >> 8;
-    const u4 r = {w & k.low, w & k.high, w8 & k.low, w8 & k.high};
-    return __builtin_bit_cast(h8, r);
-}
 // The codes - 8 of a word's low (or, of w >> 4, high) nibbles as fp16, in the order of its bytes
 __device__ __forceinline__ void byteCodes(uint32_t w, h2& a, h2& b) {
     const h2 off = {(_Float16)1032.0f, (_Float16)1032.0f};
