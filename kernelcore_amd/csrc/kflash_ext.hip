@@ -589,17 +589,20 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     if (t < t1) fetch(t);  // (before it is known whether a row sees these keys: what it reads is there)
 
     Row row[NR];
-    int wmin = INT_MAX, wmax = -1;
+    int wmin = limitOf(a, a.pos0), wmax = limitOf(a, a.pos0 + (a.rows - 1) / a.G);  // (without positions: ascending with the rows)
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        row[n] = rowOf(a, kvh, 16 * n + i);
-        if (row[n].live) {
+    for (int n = 0; n < NR; ++n) row[n] = rowOf(a, kvh, 16 * n + i);
+    if (SHAPED && a.qpos) {
+        wmin = INT_MAX;
+        wmax = -1;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {  // (rows past the last one repeat it)
             wmin = min(wmin, row[n].limit);
             wmax = max(wmax, row[n].limit);
         }
+        wmin = waveMin(wmin);
+        wmax = waveMax(wmax);
     }
-    wmin = waveMin(wmin);
-    wmax = waveMax(wmax);
     if (!kpos) t1 = wmax < 0 ? t0 : min(t1, wmax / TK + 1);
 
     // q as the B operand of step b (32 values): fp16 keys: values 32 b + 8 kg + e; 4-bit keys: the order nibbles() gives
@@ -879,32 +882,48 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         }
     }
     __syncthreads();
-    const int total = a.rows * D;
-    for (int x = tid; x < total; x += 256) {
-        const int r = x / D, at = x % D;
-        float M = -INFINITY, f[4], L = 0.0f, y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, jm[2 * (w * NR * 16 + r)]);
+    for (int x = tid; x < a.rows * (D / 4); x += 256) {  // four values each
+        const int r = x / (D / 4), at = x % (D / 4) * 4;
+        float mw[4], lw[4], M = -INFINITY, L = 0.0f;
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, ow[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float mw = jm[2 * (w * NR * 16 + r)];
-            f[w] = mw == -INFINITY ? 0.0f : ex2(mw - M);
-            L = fmaf(f[w], jm[2 * (w * NR * 16 + r) + 1], L);
-            if (f[w] != 0.0f) y = fmaf(f[w], jo[(w * NR * 16 + r) * G::ORow + at], y);
+            const float2 ml = *reinterpret_cast<const float2*>(jm + 2 * (w * NR * 16 + r));
+            mw[w] = ml.x;
+            lw[w] = ml.y;
+            ow[w] = *reinterpret_cast<const f32x4*>(jo + (w * NR * 16 + r) * G::ORow + at);
         }
-        const int b = at >> 5, rr = at & 15, dd = Q4 ? 32 * b + 8 * ((at >> 4) & 1) + (rr >> 1) + 16 * (rr & 1) : at;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, mw[w]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = mw[w] == -INFINITY ? 0.0f : ex2(mw[w] - M);
+            L = fmaf(f, lw[w], L);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = f != 0.0f ? fmaf(f, ow[w][e], y[e]) : y[e];
+        }
+        float* dst;
         if (a.splits == 1) {
             const int token = r / a.G, head = kvh * a.G + (r - token * a.G);
-            a.out[((size_t)token * a.H + head) * D + dd] = L == 0.0f ? 0.0f : y * (1.0f / L);
+            dst = a.out + ((size_t)token * a.H + head) * D;
+            y *= L == 0.0f ? 0.0f : 1.0f / L;
             if (a.lse && at == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L * kPInv));
         } else {
             const size_t pr = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
-            a.part[pr * D + dd] = y * kPInv;
+            dst = a.part + pr * D;
+            y *= kPInv;
             if (at == 0) {
                 float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * pr;
                 ml[0] = M;
                 ml[1] = L * kPInv;
             }
+        }
+        if constexpr (Q4) {  // values 8 (rr / 16) + rr / 2 + 16 (rr % 2) of the block, rr = at .. at + 3 in the block
+            float* to = dst + (at & ~31) + 8 * ((at >> 4) & 1) + ((at & 15) >> 1);
+            *reinterpret_cast<f2a4*>(to) = f32x2{y[0], y[2]};
+            *reinterpret_cast<f2a4*>(to + 16) = f32x2{y[1], y[3]};
+        } else {
+            *reinterpret_cast<f4a4*>(dst + at) = y;
         }
     }
 }

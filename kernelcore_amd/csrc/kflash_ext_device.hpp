@@ -32,6 +32,8 @@ typedef u4 u4a4 __attribute__((aligned(4)));
 typedef u4 u4a2 __attribute__((aligned(2)));
 typedef uint32_t u32a2 __attribute__((aligned(2)));
 typedef f32x4 f4a4 __attribute__((aligned(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef f32x2 f2a4 __attribute__((aligned(4)));
 struct __attribute__((packed, aligned(4))) int4a4 {
     int x, y, z, w;
     __device__ operator int4() const { return {x, y, z, w}; }
@@ -235,29 +237,38 @@ __device__ __forceinline__ float pick(const float (&x)[N], int i) {
     return r;
 }
 
+// Over the wavefront, in registers: lanes ^ 1, ^ 2, mirrored in eight and 16, then rows and halves swapped.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false); }
+template <int CTRL>
+__device__ __forceinline__ float dppF(float v) { return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(int, v))); }
+template <class T, class F>
+__device__ __forceinline__ T waveAll(T x, F&& op) {
+    auto with = [&](int y) { x = op(x, __builtin_bit_cast(T, y)); };
+    with(dpp<0xB1>(__builtin_bit_cast(int, x)));
+    with(dpp<0x4E>(__builtin_bit_cast(int, x)));
+    with(dpp<0x141>(__builtin_bit_cast(int, x)));
+    with(dpp<0x140>(__builtin_bit_cast(int, x)));
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+    const int a = r[0], b = r[1];
+    x = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+    const int c = s[0], d = s[1];
+    return op(__builtin_bit_cast(T, c), __builtin_bit_cast(T, d));
+}
 __device__ __forceinline__ int waveMin(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = min(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
+    return __builtin_amdgcn_readfirstlane(waveAll(x, [](int a, int b) { return min(a, b); }));
 }
 __device__ __forceinline__ int waveMax(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = max(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
+    return __builtin_amdgcn_readfirstlane(waveAll(x, [](int a, int b) { return max(a, b); }));
 }
 __device__ __forceinline__ float halfBits(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (unsigned short)b); }
 __device__ __forceinline__ uint32_t loadHalf(const char* p) { return *reinterpret_cast<const unsigned short*>(p); }
-
-
 __device__ __forceinline__ float waveMaxF(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+    return waveAll(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float waveSumF(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
-    return x;
+    return waveAll(x, [](float a, float b) { return a + b; });
 }
 
 // The lanes' loads and stores of LDS before this are done before those after it (a wavefront's own LDS accesses run in
@@ -296,19 +307,14 @@ struct RowQ {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             float m = fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
-            m = fmaxf(m, dpp<0xB1>(m));   // lane ^ 1
-            m = fmaxf(m, dpp<0x4E>(m));   // ^ 2
-            m = fmaxf(m, dpp<0x141>(m));  // the other four of eight
-            if constexpr (LPR >= 16) m = fmaxf(m, dpp<0x140>(m));  // the other eight of 16
+            m = fmaxf(m, dppF<0xB1>(m));   // lane ^ 1
+            m = fmaxf(m, dppF<0x4E>(m));   // ^ 2
+            m = fmaxf(m, dppF<0x141>(m));  // the other four of eight
+            if constexpr (LPR >= 16) m = fmaxf(m, dppF<0x140>(m));  // the other eight of 16
             if constexpr (LPR >= 32) m = swap16Max(m);
             if constexpr (LPR >= 64) m = swap32Max(m);
             if (lane % LPR == 0) top[n * RPI + lane / LPR] = m;
         }
-    }
-    template <int CTRL>
-    static __device__ __forceinline__ float dpp(float v) {
-        const int u = __builtin_bit_cast(int, v);
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, CTRL, 0xF, 0xF, false));
     }
     // the hi parts of row r's values to rows of `stride` fp16, the lo parts to `low`; topOf(r): the row's largest magnitude
     template <class F>
