@@ -496,8 +496,8 @@ int getRowsQ40Launch(const void* p, void* s) { return kcamd::launchGetRowsQ40(*s
 // The sizes alone (no pointers): what kcFlashExtPartBytes accepts too.
 int fxShape(const kcFlashExtDims& d) {
     if (d.H <= 0 || d.H_kv <= 0 || d.H % d.H_kv || d.H_kv > 65535 || (d.D != 64 && d.D != 128 && d.D != 256) || d.N < 0 || d.T < 0 ||
-        d.T > INT32_MAX - 64)
-        return invalid("flash_ext: H a positive multiple of H_kv, D 64, 128 or 256, N and T not negative");
+        d.T > INT32_MAX - 1024)  // (the kernels count positions in 32 bits, up to 512 past the last one)
+        return invalid("flash_ext: H a positive multiple of H_kv, D 64, 128 or 256, N and T not negative, T below 2^31 - 1024");
     if (d.q_tok < 0 || d.q_head < 0 || d.m_row < 0 || d.key_row < 0 || d.k_row < 0 || d.k_head < 0 || d.v_row < 0 || d.v_head < 0)
         return invalid("flash_ext: negative strides");
     if ((d.causal != 0 && d.causal != 1) || d.prefix < 0) return invalid("flash_ext: causal 0 or 1, prefix not negative");

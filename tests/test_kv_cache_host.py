@@ -71,7 +71,7 @@ for q4 in (False, True):
             return cls(d=kc.FlashExtDims(**d), **k)
         return make
 
-    shared = [(dict(H=0), IV), (dict(H=7), IV), (dict(H_kv=0), IV), (dict(D=96), IV), (dict(D=0), IV), (dict(N=-1), IV), (dict(T=-1), IV), (dict(T=2**31 - 1), IV),
+    shared = [(dict(H=0), IV), (dict(H=7), IV), (dict(H_kv=0), IV), (dict(D=96), IV), (dict(D=0), IV), (dict(N=-1), IV), (dict(T=-1), IV), (dict(T=2**31 - 1), IV), (dict(T=2**31 - 1024), IV),
               (dict(q_tok=-1), IV), (dict(q_head=-4), IV), (dict(k_row=-2), IV), (dict(key_row=-1), IV), (dict(key_row=699), IV), (dict(causal=2), IV),
               (dict(prefix=-1), IV), (dict(pos0=-1), IV), (dict(pos0=2**31 - 3), IV), (dict(N=1 << 24), IV), (dict(k_row=2 * hb + 1), IV), (dict(k_head=hb + 1), IV),
               (dict(k_row=1 << 61), IV), (dict(scale=NAN), IV), (dict(scale=INF), IV), (dict(softcap=-1.0), IV), (dict(softcap=NAN), IV), (dict(softcap=INF), IV),
