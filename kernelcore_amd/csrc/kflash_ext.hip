@@ -52,10 +52,15 @@ __device__ __forceinline__ uint32_t tameHalves(uint32_t w) {
 //   S^T = K Q^T: A = key rows (LDS), B = q hi / lo (registers). Lane (j, h) holds keys 8 (v / 4) + 4 h + v % 4 of row j.
 //   O^T += V^T P^T: A = V^T through transposed LDS reads, B = p hi / lo, the score registers as they are (the products'
 //   index runs over the keys in the order those registers hold).
-// 4-bit keys and values are unpacked once per workgroup, on the way to LDS; a step's keys and values lie in one of two
+// 4-bit keys and values are unpacked once per workgroup, on the way to LDS (by each wavefront, after reads of the codes: 176
+// against 165 us for 1000 tokens over 3577 positions); a step's keys and values lie in one of two
 // buffers, the next step's stored while the present one is computed and the loads of the one after in flight, one barrier a step. The
 // two wavefronts of a SIMD drift apart within a step, and one's softmax runs beside the other's products. (Keeping them half
-// a step apart by a second barrier, the values' products a step behind, was slower: 103 against 94 us for 2048 tokens.)
+// a step apart by a second barrier, the values' products a step behind, was slower: 103 against 94 us for 2048 tokens. So was one
+// set to a workgroup: 101 against 78 us.)
+// Bound by the products, staging and softmax, which overlap little: 2048 causal tokens, 24 heads of 128, fp16: 75 us, 0.69
+// PFLOP/s counting both parts of q and p (a large fp16 product of the library: 1.19); 1000 tokens over 3577 4-bit positions,
+// 32 heads: 150 us, 0.84 PFLOP/s.
 template <int D, bool Q4>
 struct Geo {
     static constexpr int KS = D == 256 ? 1 : 2;  // (256 values: one wavefront's registers fill a SIMD)
@@ -492,7 +497,9 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
-// Up to 32 rows (NR columns of 16): single tokens and a few drafted ones, where the cache's bytes count. Workgroup: four
+// Up to 32 rows (NR columns of 16): single tokens and a few drafted ones, where the cache's bytes count. One token of 32 heads over
+// 131072 4-bit positions: 47 us, 3.2 TB/s of cache, bound by unpacking (about 600 VALU instructions per 64 keys and wavefront); over 8191:
+// 8.5 us, of which 2 are the first tile's latency and 3 its computation. Workgroup: four
 // wavefronts over one range of keys of a KV head, each with its own tiles (64 keys of a 4-bit cache, 32 of an fp16
 // one), joined through LDS at the end. v_mfma_f32_16x16x32_f16, lane (i, kg) = column i, group kg of 16 lanes:
 //   S^T = K Q^T: fp16 keys are loaded as the A operand straight from memory; 4-bit keys go through LDS as they are, lane (i, kg)
@@ -931,7 +938,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
 // ---------------------------------------------------------------------------------------------- joining key ranges
 // o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) for each row. A thread takes four of a row's values in every SG-th range,
 // the first of its loads issued before the weights are known; the row's threads share the weights, and the SG sums are
-// added in order through LDS. What counts is the latency of a round trip.
+// added in order through LDS. What counts is the latency of a round trip: 2.9 to 4.2 us for 32 rows of 32 or 64 ranges.
 template <int D, int SG>
 __global__ __launch_bounds__(256) void flash_ext_join_kernel(FxParams a) {
     constexpr int LP = D / 4, RT = LP * SG, RPB = 256 / RT;  // lanes to a row's values, threads to a row, rows to a workgroup

@@ -23,7 +23,8 @@ __device__ __forceinline__ long long index64(const int* idx, long long i) {
 }
 
 // ---------------------------------------------------------------------------------------------- 4-bit rows
-// Eight lanes per block of 32 values, four values each; R rows per workgroup. Bound by reading the f32 rows.
+// Eight lanes per block of 32 values, four values each; R rows per workgroup. Bound by reading the f32 rows, and by the search for
+// repeated indices: 1777 rows of 1024 values 5.3 us, 1.6 TB/s; one row 1.9 us.
 // Code of x: floor(x / d + 8.5), d = xm / -8. With a = |d| and y = x sign(d) that is the largest c with (c - 8.5) a <= y:
 // the product c' a of a half-integer and an f32 is rounded by the fma only after y is subtracted, so the sign of
 // y - c' a is exact and settles a guess from the rounded quotient.
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(256) void set_rows_q4_0_kernel(const float* __restr
     }
 }
 
-// Eight lanes per block, four values (16 bytes of y) each. Bound by writing y.
+// Eight lanes per block, four values (16 bytes of y) each. Bound by writing y: 1777 rows of 1024 values 4.8 us, 1.7 TB/s.
 __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restrict__ src, const int* __restrict__ idx,
                                                             float* __restrict__ y, int nb, int rows, int src_rows,
                                                             long long src_row) {
@@ -131,7 +132,8 @@ __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restri
 // and 10 bits over order-preserving codes), then the positions above it and the first of those equal to it, written
 // in ascending order: each wavefront owns a contiguous piece of the row, so that ballots and one prefix over the
 // wavefronts give every position its place. Up to R x 1024 positions are read once and held in registers through the five
-// sweeps; longer rows (R = 0) are read by each sweep. A head has one compute unit, and the sweeps' instructions bound it.
+// sweeps; longer rows (R = 0) are read by each sweep. A head has one compute unit, and the sweeps' instructions bound it: 16384
+// positions 13.4 us (with digits of 8 bits, a sweep more, 14.7), 1500 positions 6.5 us, its barriers and the load.
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 
 __device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first; never 0
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
 // ---------------------------------------------------------------------------------------------- kept rows
 // One grid over planes, heads and rows. A row's units (the widest of 16, 8, 4 and 2 bytes that all addresses of a plane
 // allow) lie on the next power of two of lanes, up to 256; each thread moves up to eight units whose loads are all in flight
-// before the first store. Bound by memory.
+// before the first store. Bound by memory: 4096 rows of 256 bytes of K and V and 8 heads 8.6 us, 3.9 TB/s read and written.
 struct GatherPlane {
     const char* src;
     char* dst;
