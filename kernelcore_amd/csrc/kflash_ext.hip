@@ -633,14 +633,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         const QScale qs = qScale(top, a.scale);
         c[n] = qs.c;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                _Float16 hi, lo;
-                qSplit(x[b][e], a.scale < 0.0f, qs.shift, hi, lo);
-                qh[n][b][e] = hi;
-                ql[n][b][e] = lo;
-            }
+        for (int b = 0; b < NB; ++b) qSplit8(x[b], qs, qh[n][b], ql[n][b]);
     }
     const Shape shape = SHAPED ? shapeOf(a) : Shape{};
     const NibbleMagic magic = nibbleMagic();

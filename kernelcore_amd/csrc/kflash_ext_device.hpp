@@ -81,19 +81,44 @@ __device__ __forceinline__ bool wildScale(uint32_t bits) { return (bits & 0x7FFF
 // Which of two fp16 values of a word is an infinity or NaN: bits 15 and 31.
 __device__ __forceinline__ uint32_t wildHalves(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-// q values of one row as fp16 hi / lo parts: x 2^shift
+// q values of one row as fp16 hi / lo parts of x 2^shift, with the scale's sign. 2^shift is a factor f and, for rows of numbers so
+// small that f would overflow, 2^more.
 struct QScale {
-    int shift;
+    float f;
+    int more;
     float c;  // the factor that makes a sum of scaled products a score
 };
 __device__ __forceinline__ QScale qScale(float top, float scale) {
-    const int e = top > 0.0f && top < INFINITY ? 8 - __builtin_amdgcn_frexp_expf(top) : 0;
-    return {e, ldexpf(fabsf(scale), -e)};
+    const int shift = top > 0.0f && top < INFINITY ? 8 - __builtin_amdgcn_frexp_expf(top) : 0, first = min(shift, 126);
+    return {ldexpf(scale < 0.0f ? -1.0f : 1.0f, first), shift - first, ldexpf(fabsf(scale), -shift)};
 }
-__device__ __forceinline__ void qSplit(float x, bool neg, int shift, _Float16& hi, _Float16& lo) {
-    const float y = ldexpf(neg ? -x : x, shift);
-    hi = (_Float16)y;
-    lo = (_Float16)(y - (float)hi);
+// Two numbers as fp16 parts hi + lo. (x - hi in one instruction each; x must not come straight from a matrix instruction.)
+__device__ __forceinline__ void splitTwo(float x0, float x1, h2& hi, h2& lo) {
+    hi = h2{(_Float16)x0, (_Float16)x1};
+    const uint32_t hb = __builtin_bit_cast(uint32_t, hi);
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hb), "v"(x0));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hb), "v"(x1));
+    lo = h2{(_Float16)r0, (_Float16)r1};
+}
+template <int N>
+__device__ __forceinline__ void qSplit(const float (&x)[N], const QScale& s, h2 (&hi)[N / 2], h2 (&lo)[N / 2]) {
+    float y[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = x[e] * s.f;
+    if (__builtin_expect(__any(s.more > 0), 0)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = ldexpf(y[e], s.more);
+    }
+#pragma unroll
+    for (int e = 0; e < N; e += 2) splitTwo(y[e], y[e + 1], hi[e / 2], lo[e / 2]);
+}
+
+__device__ __forceinline__ void qSplit8(const float (&x)[8], const QScale& s, h8& hi, h8& lo) {
+    h2 h[4], l[4];
+    qSplit<8>(x, s, h, l);
+    hi = h8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+    lo = h8{l[0][0], l[0][1], l[1][0], l[1][1], l[2][0], l[2][1], l[3][0], l[3][1]};
 }
 
 // What a query row brings to its scores.
@@ -212,12 +237,8 @@ template <int N>
 __device__ __forceinline__ void splitParts(const float (&x)[N], h8 (&hi)[N / 8], h8 (&lo)[N / 8]) {
 #pragma unroll
     for (int v = 0; v < N; v += 2) {
-        const h2 h = {(_Float16)x[v], (_Float16)x[v + 1]};
-        const uint32_t hb = __builtin_bit_cast(uint32_t, h);
-        float r0, r1;  // x - hi in one instruction each
-        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hb), "v"(x[v]));
-        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hb), "v"(x[v + 1]));
-        const h2 l = {(_Float16)r0, (_Float16)r1};
+        h2 h, l;
+        splitTwo(x[v], x[v + 1], h, l);
         hi[v >> 3][v & 7] = h[0];
         hi[v >> 3][(v & 7) + 1] = h[1];
         lo[v >> 3][v & 7] = l[0];
@@ -321,16 +342,12 @@ struct RowQ {
     __device__ __forceinline__ void split(const FxParams& a, _Float16* hi, int stride, int lane, F&& topOf, h4 (&low)[N]) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int r = n * RPI + lane / LPR, shift = qScale(topOf(r), a.scale).shift;
-            h4 u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                _Float16 y, z;
-                qSplit(x[n][e], a.scale < 0.0f, shift, y, z);
-                u[e] = y;
-                low[n][e] = z;
-            }
-            *reinterpret_cast<h4*>(hi + r * stride + 4 * (lane % LPR)) = u;
+            const int r = n * RPI + lane / LPR;
+            const float y[4] = {x[n][0], x[n][1], x[n][2], x[n][3]};
+            h2 u[2], w[2];
+            qSplit<4>(y, qScale(topOf(r), a.scale), u, w);
+            low[n] = h4{w[0][0], w[0][1], w[1][0], w[1][1]};
+            *reinterpret_cast<h4*>(hi + r * stride + 4 * (lane % LPR)) = h4{u[0][0], u[0][1], u[1][0], u[1][1]};
         }
     }
     __device__ __forceinline__ void place(_Float16* to, int stride, int lane, const h4 (&v)[N]) const {
@@ -357,14 +374,12 @@ __device__ __forceinline__ float splitRow32(const FxParams& a, const f32x4 (&x)[
     top = fmaxf(top, __shfl_xor(top, 32));
     const QScale qs = qScale(top, a.scale);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
+    for (int ks = 0; ks < D / 16; ++ks) {
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            _Float16 hi, lo;
-            qSplit(x[2 * ks + (e >> 2)][e & 3], a.scale < 0.0f, qs.shift, hi, lo);
-            qh[ks][e] = hi;
-            ql[ks][e] = lo;
-        }
+        for (int e = 0; e < 8; ++e) y[e] = x[2 * ks + (e >> 2)][e & 3];
+        qSplit8(y, qs, qh[ks], ql[ks]);
+    }
     return qs.c;
 }
 
