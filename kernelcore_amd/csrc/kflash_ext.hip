@@ -730,7 +730,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                     for (int v = 0; v < 4; ++v) x[n][4 * u + v] = sh[v] + sl[v];
                 }
         }
-        const bool full = !meta && !(SHAPED && a.mask) && t * TK + TK - 1 <= wmin && t * TK + TK - 1 < a.T;
+        const bool full = t * TK + TK - 1 <= wmin && t * TK + TK - 1 < a.T;  // (without positions)
         h8 ph[NR][TT], pl[NR][TT];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -742,36 +742,46 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
 #pragma unroll
                     for (int v = 0; v < U * 4; ++v) x[n][v] *= c2;
                 }
-                const float slope = -row[n].slope * kLog2e;
                 const int* mt = reinterpret_cast<const int*>(mine + G::oMeta) + 4 * kg;
+                if (shape.bias) {
+                    const float slope = -row[n].slope * kLog2e;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int key = t * TK + 16 * u + 4 * kg;
-                    int4 p4 = {key, key + 1, key + 2, key + 3}, d4 = {row[n].doc, row[n].doc, row[n].doc, row[n].doc};
-                    if (meta) {
-                        p4 = *reinterpret_cast<const int4*>(mt + 16 * u);
-                        d4 = *reinterpret_cast<const int4*>(mt + TK + 16 * u);
+                    for (int u = 0; u < U; ++u) {
+                        const int key = t * TK + 16 * u + 4 * kg;
+                        int4 p = {key, key + 1, key + 2, key + 3};
+                        if (meta) p = *reinterpret_cast<const int4*>(mt + 16 * u);
+                        x[n][4 * u] = fmaf(slope, fabsf((float)(row[n].pos - p.x)), x[n][4 * u]);
+                        x[n][4 * u + 1] = fmaf(slope, fabsf((float)(row[n].pos - p.y)), x[n][4 * u + 1]);
+                        x[n][4 * u + 2] = fmaf(slope, fabsf((float)(row[n].pos - p.z)), x[n][4 * u + 2]);
+                        x[n][4 * u + 3] = fmaf(slope, fabsf((float)(row[n].pos - p.w)), x[n][4 * u + 3]);
                     }
-                    const int p[4] = {p4.x, p4.y, p4.z, p4.w}, dd[4] = {d4.x, d4.y, d4.z, d4.w};
-                    if (shape.bias) {
+                }
+                if (a.mask) {
+                    const unsigned short* mrow = a.mask + (size_t)row[n].token * a.m_row2;
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) x[n][4 * u + v] = fmaf(slope, fabsf((float)(row[n].pos - p[v])), x[n][4 * u + v]);
-                    }
-                    if (a.mask) {
-                        const uint32_t* mr = reinterpret_cast<const uint32_t*>(a.mask + (size_t)row[n].token * a.m_row2) + key / 2;
+                    for (int u = 0; u < U; ++u) {
+                        const int key = t * TK + 16 * u + 4 * kg;
+                        const uint32_t* mr = reinterpret_cast<const uint32_t*>(mrow) + key / 2;
                         const uint32_t w0 = key < a.T ? mr[0] : 0xFC00FC00u, w1 = key + 2 < a.T ? mr[1] : 0xFC00FC00u;
                         x[n][4 * u] = addMask(x[n][4 * u], w0 & 0xFFFFu);
                         x[n][4 * u + 1] = addMask(x[n][4 * u + 1], w0 >> 16);
                         x[n][4 * u + 2] = addMask(x[n][4 * u + 2], w1 & 0xFFFFu);
                         x[n][4 * u + 3] = addMask(x[n][4 * u + 3], w1 >> 16);
                     }
-                    if (!full) {
+                }
+                if (meta) {  // (keys past the end are at kNoKey)
+                    auto unseen = [&](int pos, int doc) { return bool((pos > row[n].limit) | (doc != row[n].doc)); };
 #pragma unroll
-                        for (int v = 0; v < 4; ++v)
-                            if (p[v] > row[n].limit || dd[v] != row[n].doc || key + v >= a.T) x[n][4 * u + v] = -INFINITY;
+                    for (int u = 0; u < U; ++u) {
+                        const int4 p = *reinterpret_cast<const int4*>(mt + 16 * u), d = *reinterpret_cast<const int4*>(mt + TK + 16 * u);
+                        x[n][4 * u] = unseen(p.x, d.x) ? -INFINITY : x[n][4 * u];
+                        x[n][4 * u + 1] = unseen(p.y, d.y) ? -INFINITY : x[n][4 * u + 1];
+                        x[n][4 * u + 2] = unseen(p.z, d.z) ? -INFINITY : x[n][4 * u + 2];
+                        x[n][4 * u + 3] = unseen(p.w, d.w) ? -INFINITY : x[n][4 * u + 3];
                     }
                 }
-            } else if (!full) {
+            }
+            if (!meta && !full) {
                 const int last = min(row[n].limit, a.T - 1) - t * TK - 4 * kg;
 #pragma unroll
                 for (int v = 0; v < U * 4; ++v) x[n][v] = 16 * (v >> 2) + (v & 3) <= last ? x[n][v] : -INFINITY;

@@ -193,6 +193,7 @@ __device__ __forceinline__ void capScores(float (&x)[N], float k, const Shape& s
 #pragma unroll
             for (int i = 3; i >= 0; --i) r = fmaf(u, r, s.p5[i]);
             x[v] *= r;
+            if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time are enough to fill the unit; all at once take registers)
         }
     } else {
 #pragma unroll
@@ -207,6 +208,7 @@ __device__ __forceinline__ void capScores(float (&x)[N], float k, const Shape& s
             p = fmaf(u, p, s.p[0]);
             q = fmaf(u, q, 1.0f);
             x[v] = y * p * __builtin_amdgcn_rcpf(q);
+            if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
