@@ -5,7 +5,7 @@
 //   m_i = max_j x_ij, l_i = sum_j 2^(x_ij - m_i)
 // over the keys that i sees, in one pass over the keys with running m and l.
 //
-// Three kernels: few rows (up to 32: single and drafted tokens), many rows (prompts), and the join of key ranges where
+// Three kernels: few rows (single and drafted tokens, short calls), many rows (prompts), and the join of key ranges where
 // a call's rows alone do not fill the GPU.
 #include <hip/hip_runtime.h>
 
@@ -497,7 +497,8 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
-// Up to 32 rows (NR columns of 16): single tokens and a few drafted ones, where the cache's bytes count. One token of 32 heads over
+// Groups of up to 32 rows (NR columns of 16): single tokens and a few drafted ones, where the cache's bytes count, and more rows over
+// short ranges, where latency does (fxPlan). One token of 32 heads over
 // 131072 4-bit positions: 47 us, 3.2 TB/s of cache, bound by unpacking (about 600 VALU instructions per 64 keys and wavefront); over 8191:
 // 8.5 us, of which 2 are the first tile's latency and 3 its computation. Workgroup: four
 // wavefronts over one range of keys of a KV head, each with its own tiles (64 keys of a 4-bit cache, 32 of an fp16
@@ -527,7 +528,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     constexpr int NB = G::NB, TK = G::TK, U = TK / 16, TT = TK / 32, DT = D / 16;
     extern __shared__ int4 lds4[];
     char* lds = reinterpret_cast<char*>(lds4);
-    const int sp = blockIdx.x, kvh = blockIdx.y;
+    const int sp = blockIdx.x, kvh = blockIdx.y, row0 = blockIdx.z * 16 * NR, rows = min(a.rows - row0, 16 * NR);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int i = lane & 15, kg = lane >> 4;
     char* mine = lds + wave * G::Wave;
@@ -596,9 +597,10 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     if (t < t1) fetch(t);  // (before it is known whether a row sees these keys: what it reads is there)
 
     Row row[NR];
-    int wmin = limitOf(a, a.pos0), wmax = limitOf(a, a.pos0 + (a.rows - 1) / a.G);  // (without positions: ascending with the rows)
+    // (without positions: ascending with the rows)
+    int wmin = limitOf(a, a.pos0 + row0 / a.G), wmax = limitOf(a, a.pos0 + (row0 + rows - 1) / a.G);
 #pragma unroll
-    for (int n = 0; n < NR; ++n) row[n] = rowOf(a, kvh, 16 * n + i);
+    for (int n = 0; n < NR; ++n) row[n] = rowOf(a, kvh, row0 + 16 * n + i);
     if (SHAPED && a.qpos) {
         wmin = INT_MAX;
         wmax = -1;
@@ -892,7 +894,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         }
     }
     __syncthreads();
-    for (int x = tid; x < a.rows * (D / 4); x += 256) {  // four values each
+    for (int x = tid; x < rows * (D / 4); x += 256) {  // four values each
         const int r = x / (D / 4), at = x % (D / 4) * 4;
         float mw[4], lw[4], M = -INFINITY, L = 0.0f;
         f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, ow[4];
@@ -914,12 +916,12 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         }
         float* dst;
         if (a.splits == 1) {
-            const int token = r / a.G, head = kvh * a.G + (r - token * a.G);
+            const int token = (row0 + r) / a.G, head = kvh * a.G + (row0 + r - token * a.G);
             dst = a.out + ((size_t)token * a.H + head) * D;
             y *= L == 0.0f ? 0.0f : 1.0f / L;
             if (a.lse && at == 0) a.lse[(size_t)token * a.H + head] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L * kPInv));
         } else {
-            const size_t pr = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
+            const size_t pr = ((size_t)sp * a.H_kv + kvh) * a.rows + row0 + r;
             dst = a.part + pr * D;
             y *= kPInv;
             if (at == 0) {
@@ -1033,8 +1035,8 @@ int join(const FxParams& p, hipStream_t s) {
 template <int D, bool Q4, bool SHAPED>
 int run(const FxParams& p, const FxPlan& plan, hipStream_t s) {
     if (plan.few) {
-        const dim3 grid(p.splits, p.H_kv);
-        constexpr int NR2 = D == 256 ? 1 : 2;  // (fxPlan: no more than 16 rows of 256)
+        constexpr int NR2 = D == 256 ? 1 : 2;  // (16 rows of 256 values fill the registers)
+        const dim3 grid(p.splits, p.H_kv, (p.rows + 16 * NR2 - 1) / (16 * NR2));
         if (p.rows <= 16) {
             constexpr int lds = FewGeo<D, Q4, 1>::Lds;
             static const int ok = allow(flash_ext_few_kernel<D, Q4, SHAPED, 1>, lds);

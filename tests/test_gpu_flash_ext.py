@@ -25,16 +25,22 @@ SIZES = [(8, 8, 64, 1, 1), (4, 1, 64, 1, 31), (6, 2, 64, 2, 33), (8, 2, 128, 1, 
          (16, 2, 256, 2, 640), (16, 2, 256, 3, 129), (33, 1, 64, 1, 100), (8, 2, 64, 33, 33), (6, 2, 128, 40, 97), (8, 2, 128, 129, 641),
          (4, 4, 128, 70, 64), (4, 2, 256, 65, 130), (2, 1, 256, 257, 400), (5, 1, 64, 200, 1001)]
 
+# sizes that the many-rows kernel takes (more than four units of 64 keys for each of 256 compute units and each group of 32 rows, heads of 256:
+# eight and 16): one range and several, ragged, more tokens than positions
+MANY = [(32, 32, 64, 290, 256), (16, 16, 64, 257, 500), (16, 8, 128, 200, 641), (5, 1, 128, 700, 1111), (16, 16, 128, 300, 421), (16, 16, 256, 260, 501),
+        (8, 2, 256, 330, 900), (10, 2, 64, 333, 1030)]
+
 
 @CACHES
-@pytest.mark.parametrize("H,K,D,N,T", SIZES)
+@pytest.mark.parametrize("H,K,D,N,T", SIZES + MANY)
 def test_causal(q4, H, K, D, N, T):
     print(f"flash_ext q4={q4} H={H}/{K} D={D} N={N} T={T}", flush=True)
     Case(q4, H, K, D, N, T).check()
 
 
 @CACHES
-@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 333), (6, 2, 64, 4, 95), (8, 2, 128, 50, 333), (4, 2, 256, 40, 77), (24, 8, 128, 9, 513)])
+@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 333), (6, 2, 64, 4, 95), (8, 2, 128, 50, 333), (4, 2, 256, 40, 77), (24, 8, 128, 9, 513),
+                                       (32, 32, 64, 290, 256), (16, 16, 128, 300, 421), (16, 16, 256, 260, 501)])
 @pytest.mark.parametrize("shape", ["cap", "bias", "prefix", "docs", "open", "all"])
 def test_shaped(q4, H, K, D, N, T, shape):
     print(f"flash_ext q4={q4} H={H}/{K} D={D} N={N} T={T} {shape}", flush=True)
@@ -44,7 +50,8 @@ def test_shaped(q4, H, K, D, N, T, shape):
 
 
 @CACHES
-@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 70), (8, 2, 64, 3, 129), (6, 2, 128, 45, 131), (4, 4, 256, 34, 65)])
+@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 70), (8, 2, 64, 3, 129), (6, 2, 128, 45, 131), (4, 4, 256, 34, 65),
+                                       (32, 32, 64, 290, 256), (16, 16, 128, 300, 421), (16, 16, 256, 260, 501)])
 def test_mask(q4, H, K, D, N, T):
     """ggml's mask: biases, -infinity, the type's lowest value, a row that leaves nothing, rows longer than T."""
     r = np.random.default_rng(T)
@@ -62,7 +69,7 @@ def test_mask(q4, H, K, D, N, T):
 
 
 @CACHES
-@pytest.mark.parametrize("N", [1, 3, 37])
+@pytest.mark.parametrize("N", [1, 3, 37, 1100])
 def test_positions(q4, N):
     """A thinned cache: each head its own positions, empty slots, queries at positions of their own."""
     H, K, D, T = 8, 2, 128, 201
@@ -88,7 +95,7 @@ def test_no_keys_and_no_queries(q4):
 
 
 @CACHES
-@pytest.mark.parametrize("N,T", [(1, 150), (5, 200), (70, 200), (140, 260)])
+@pytest.mark.parametrize("N,T", [(1, 150), (5, 200), (70, 200), (140, 260), (700, 705)])
 def test_what_is_not_seen_does_not_reach_the_result(q4, N, T):
     """NaN and infinities in keys and values that some queries do not see: those queries' results stay as they were; the
     others' become what the definition says."""
@@ -137,7 +144,7 @@ def test_what_is_not_seen_does_not_reach_the_result(q4, N, T):
 
 def test_large_scales_of_4_bit_values():
     """Scales whose values leave fp16's range (d up to 65504: values up to 524032) stay exact."""
-    for N in (1, 40):
+    for N in (1, 40, 4200):
         c = Case(True, 4, 2, 64, N, 100)
         b = c.v.reshape(100, 2, -1, 18)
         for j, d in ((0, 8188.0), (1, 8192.0), (50, 65504.0), (60, -30000.0)):
@@ -148,7 +155,7 @@ def test_large_scales_of_4_bit_values():
 @CACHES
 def test_query_magnitudes(q4):
     """q far above and below fp16's range, a negative scale, zeros."""
-    for N in (2, 40):
+    for N in (2, 40, 4200):
         for spread, scale in ((1e6, 1e-7), (1e-9, 1e8), (1e30, 1e-31), (1.0, -0.1)):
             Case(q4, 4, 2, 64, N, 90, spread=spread, scale=scale).check()
         c = Case(q4, 4, 2, 64, N, 90)
@@ -158,7 +165,7 @@ def test_query_magnitudes(q4):
 
 
 @CACHES
-@pytest.mark.parametrize("N", [1, 60])
+@pytest.mark.parametrize("N", [1, 60, 1400])
 def test_strides(q4, N):
     """Head-major caches at odd offsets, q heads and tokens apart, against the packed layout's bits."""
     H, K, D, T = 8, 2, 128, 150
@@ -188,7 +195,7 @@ def test_strides(q4, N):
 def test_offsets_past_32_bits(q4):
     """Rows 1.5 GiB apart: the last ones lie past 4 GiB."""
     H, K, D, T = 4, 2, 64, 4
-    for N in (1, 40):
+    for N in (1, 40, 8300):
         c = Case(q4, H, K, D, N, T, causal=0, pos0=0)
         want, _ = c.attend()
         step = 3 << 29
@@ -289,15 +296,16 @@ def test_a_weight_row_past_nothing_seen_is_zero():
 
 
 @CACHES
-def test_graph_replays(q4):
+@pytest.mark.parametrize("N", [2, 700])
+def test_graph_replays(q4, N):
     """Two captured graphs with workspaces of their own, replayed in turn over changing inputs, eager calls between."""
-    c = Case(q4, 8, 2, 128, 2, 700)
+    c = Case(q4, 8, 2, 128, N, 700)
     s = C.c_void_p()
     kc.call("kcStreamCreate", C.byref(s))
     made = []
     for _ in range(2):
         b, d = c.upload(), c.dims()
-        out, part = kc.Buffer(4 * 2 * 8 * 128), kc.Buffer(kc.flash_ext_part_bytes(d))
+        out, part = kc.Buffer(4 * N * 8 * 128), kc.Buffer(kc.flash_ext_part_bytes(d))
         args = kc.FlashExtArgs(v=b["v"].ptr, out=out.ptr, part=part.ptr, **c.shape_args(b, d))
         kc.call("kcStreamBeginCapture", s)
         kc.launch(c.name("flash_ext"), args, s)
@@ -325,7 +333,7 @@ def test_graph_replays(q4):
 
 def test_one_result_for_every_run():
     """The same call gives the same bits, whatever ran before (no atomics in the sums)."""
-    for N, T in ((1, 3000), (90, 900)):
+    for N, T in ((1, 3000), (90, 900), (700, 900)):
         c = Case(True, 8, 2, 128, N, T)
         a, b = c.attend(), c.attend()
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
