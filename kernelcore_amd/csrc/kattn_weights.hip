@@ -2,9 +2,9 @@
 //   w_gj = decay w_in_gj + sum over rows r of KV head g of exp(y_rj - lse_r),
 // with the scores y of flash_ext (kflash_ext_device.hpp). Tiles of 32 rows x 32 keys on the matrix cores, S = Q K^T (A = q rows, B =
 // keys): lane (j, h) holds rows 8 (v / 4) + 4 h + v % 4 of key j, so a key's sum over the rows is a sum of registers and
-// nothing crosses lanes until the end. A workgroup stages its key tiles once; then its wavefronts share the rows (RW of them
-// to a tile) and walk over the row tiles without a barrier, q read once for all of the tiles. Sums in one order, no atomics.
-// A single token's call reads K once and is bound by a tile's latency (4099 fp16 positions, 8 KV heads of 128: 7.3 us, 1.2 TB/s); with
+// nothing crosses lanes until the end. A workgroup stages key tiles, and its wavefronts share the rows (RW of them
+// to a tile). Sums in one order, no atomics.
+// A single token's call reads K once and is bound by that, or by a tile's latency (4099 fp16 positions, 8 KV heads of 128: 6.8 us); with
 // many rows the scaling of the sums and the exponentials bound it, and q, split anew for every 128 keys (64 tokens of 32 heads over
 // 8192 4-bit positions: 19 us, 0.45 PFLOP/s counting both parts of q).
 #include <hip/hip_runtime.h>
@@ -26,9 +26,12 @@ struct WGeo {
     static constexpr int oS = 32 * kKeyRow<D>, oMeta = oS + (Q4 ? NB * 128 : 0), Tile = oMeta + 256;
 };
 
-// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup.
+// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup. Up to 64 rows (RW < 4) stay in registers, and the
+// workgroup walks over the keys, the next ones' loads under way (131072 fp16 positions of 8 heads of 128, one token: 45 us, 6 TB/s;
+// a workgroup for every 128 keys, each with q of its own, 95); with more rows it walks over them, and has its keys only once. Two workgroups to a
+// compute unit are worth some spilled registers at 256 values (64 tokens over 8192: 34 against 47 us), but for a walk over fp16 keys (15 against 20).
 template <int D, bool Q4, int RW, int TP>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxParams a) {
+__global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_weights_kernel(FxParams a) {
     using G = WGeo<D, Q4>;
     constexpr int NB = G::NB, KW = 4 / RW, KT = KW * TP, PR = Q4 ? NB : D / 8, KS = D / 16;
     extern __shared__ int4 lds4[];
@@ -40,165 +43,195 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_weights_kernel(FxP
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, h = lane >> 5;
     const int kw = wave / RW, rw = wave % RW;
-    const int t0 = blockIdx.x * KT;
     const char* kb = a.k + (size_t)kvh * a.k_head;
     const int* kpos = a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
     const int* kdoc = a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
     constexpr int IT = KT * 32 * PR, NL = (IT + 255) / 256;
     u4 raw[NL];
     uint32_t sc[Q4 ? NL : 1];
+    int rpos[TP], rdoc[TP];  // this lane's keys: key j of each of the wavefront's tiles
+    auto load = [&](int t0) {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) {
-        const int i = tid + 256 * n;
-        if (i >= IT) break;
-        const char* p = kb + (size_t)min((long long)t0 * 32 + i / PR, (long long)a.T - 1) * a.k_row + (Q4 ? 18 : 16) * (i % PR);
-        if constexpr (Q4) {
-            raw[n] = *reinterpret_cast<const u4a2*>(p + 2);
-            sc[n] = loadHalf(p);
-        } else {
-            raw[n] = *reinterpret_cast<const u4a4*>(p);
+        for (int n = 0; n < NL; ++n) {
+            const int i = tid + 256 * n;
+            if (i >= IT) break;
+            const char* p = kb + (size_t)min((long long)t0 * 32 + i / PR, (long long)a.T - 1) * a.k_row + (Q4 ? 18 : 16) * (i % PR);
+            if constexpr (Q4) {
+                raw[n] = *reinterpret_cast<const u4a2*>(p + 2);
+                sc[n] = loadHalf(p);
+            } else {
+                raw[n] = *reinterpret_cast<const u4a4*>(p);
+            }
         }
-    }
-    // a row tile's q: a wavefront's only one while the keys are staged (8.6 -> 8.0 us for a token over 4099 positions; where it
-    // walks over several, the registers for it are worth more to the tiles: 24.5 against 27.2 us for 64 tokens over 8192)
-    int r0 = 32 * rw;
-    Row row;
-    f32x4 q[D / 8];
-    float lse;
-    auto fetch = [&]() {
-        row = rowOf(a, kvh, r0 + j);
-        loadRow32<D>(a, row, h, q);
-        lse = a.lse[(size_t)row.token * a.H + row.head];
+#pragma unroll
+        for (int p = 0; p < TP; ++p) {
+            const int key = (int)min((long long)(t0 + kw * TP + p) * 32 + j, (long long)a.T - 1);
+            rpos[p] = kpos ? kpos[key] : 0;
+            rdoc[p] = kdoc ? kdoc[key] : 0;
+        }
     };
-    if (RW < 4 && r0 < a.rows) fetch();
-    // this lane's keys: key j of each of the wavefront's tiles
-    int pos[TP], doc[TP];
+    auto store = [&]() {
 #pragma unroll
-    for (int p = 0; p < TP; ++p) {
-        const long long key = (long long)(t0 + kw * TP + p) * 32 + j;
-        pos[p] = key < a.T ? (kpos ? kpos[key] : (int)key) : kNoKey;
-        if (pos[p] < 0) pos[p] = kNoKey;
-        doc[p] = kdoc && key < a.T ? kdoc[key] : 0;
-    }
+        for (int n = 0; n < NL; ++n) {
+            const int i = tid + 256 * n, key = i / PR, b = i % PR;
+            if (i >= IT) break;
+            char* tile = lds + (key >> 5) * G::Tile;
+            if constexpr (Q4) {
+                h8 code[4];
+                blockCodes(raw[n], code);
+                h8* dst = reinterpret_cast<h8*>(tile + (key & 31) * kKeyRow<D> + 64 * b);
 #pragma unroll
-    for (int n = 0; n < NL; ++n) {
-        const int i = tid + 256 * n, key = i / PR, b = i % PR;
-        if (i >= IT) break;
-        char* tile = lds + (key >> 5) * G::Tile;
-        if constexpr (Q4) {
-            h8 code[4];
-            blockCodes(raw[n], code);
-            h8* dst = reinterpret_cast<h8*>(tile + (key & 31) * kKeyRow<D> + 64 * b);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = code[e];
-            reinterpret_cast<float*>(tile + G::oS)[b * 32 + (key & 31)] = halfBits(sc[n]);
-        } else {
-            *reinterpret_cast<u4*>(tile + (key & 31) * kKeyRow<D> + 16 * b) = raw[n];
+                for (int e = 0; e < 4; ++e) dst[e] = code[e];
+                reinterpret_cast<float*>(tile + G::oS)[b * 32 + (key & 31)] = halfBits(sc[n]);
+            } else {
+                *reinterpret_cast<u4*>(tile + (key & 31) * kKeyRow<D> + 16 * b) = raw[n];
+            }
         }
-    }
+    };
     const Shape shape = shapeOf(a);
-    __syncthreads();
     f32x16 zero;
 #pragma unroll
     for (int v = 0; v < 16; ++v) zero[v] = 0.0f;
-    float acc[TP];
-#pragma unroll
-    for (int p = 0; p < TP; ++p) acc[p] = 0.0f;
-    const int key0 = (t0 + kw * TP) * 32;
-    for (; r0 < a.rows; r0 += 32 * RW) {  // (RW < 4: once)
-        if constexpr (RW == 4) fetch();
-        const int wmax = waveMax(row.live ? row.limit : -1), wmin = waveMin(row.live ? row.limit : INT_MAX);
-        if (!kpos && key0 > wmax) continue;
-        const bool easy = !kpos && !kdoc && !a.mask && !__any(lse == -INFINITY) && r0 + 32 <= a.rows;
-        if (!row.live) lse = -INFINITY;
-        h8 qh[KS], ql[KS];
+
+    // a row tile: q as operands, what else its rows bring to LDS
+    int r0 = 32 * rw, wmax, wmin;
+    bool easy;  // whole, each of its rows saw something, and keys are hidden by position alone
+    h8 qh[KS], ql[KS];
+    auto rows = [&]() {
+        const Row row = rowOf(a, kvh, r0 + j);
+        f32x4 q[D / 8];
+        loadRow32<D>(a, row, h, q);
+        const float lse = a.lse[(size_t)row.token * a.H + row.head];
+        wmax = waveMax(row.live ? row.limit : -1);
+        wmin = waveMin(row.live ? row.limit : INT_MAX);
+        easy = !kpos && !kdoc && !a.mask && !__any(lse == -INFINITY) && r0 + 32 <= a.rows;
         const float c = splitRow32<D>(a, q, qh, ql);
         if (h == 0) {  // (a row that saw nothing gives nothing: its factor's place holds the mark)
-            rows4[wave][j] = make_float4(shape.inv_cap > 0.0f ? c : factor2(c), lse == -INFINITY ? INFINITY : lse * kLog2e, row.slope, 0.0f);
-            rows4i[wave][j] = make_int4(lse == -INFINITY ? -1 : row.limit, row.pos, row.doc, row.token);
+            const bool none = !row.live || lse == -INFINITY;
+            rows4[wave][j] = make_float4(shape.inv_cap > 0.0f ? c : factor2(c), none ? INFINITY : lse * kLog2e, row.slope, 0.0f);
+            rows4i[wave][j] = make_int4(none ? -1 : row.limit, row.pos, row.doc, row.token);
         }
         waveLds();
+    };
+    const int tiles = a.T / 32 + (a.T % 32 != 0);
+    int t0 = blockIdx.x * KT;
+    load(t0);
+    if (RW < 4 && r0 < a.rows) rows();  // (the only one)
+    while (true) {
+        const int key0 = (t0 + kw * TP) * 32, next = t0 + (int)gridDim.x * KT;
+        const bool more = RW < 4 && next < tiles;
+        store();
+        int pos[TP], doc[TP];
 #pragma unroll
         for (int p = 0; p < TP; ++p) {
-            const int k0 = key0 + 32 * p;
-            if (!kpos && k0 > wmax) continue;
-            const char* tile = lds + (kw * TP + p) * G::Tile;
-            const char* kr = tile + j * kKeyRow<D> + 16 * h;
-            float x[16];
-            if constexpr (Q4) {
+            const long long key = (long long)key0 + 32 * p + j;
+            pos[p] = key >= a.T ? kNoKey : kpos ? (rpos[p] < 0 ? kNoKey : rpos[p]) : (int)key;
+            doc[p] = rdoc[p];
+        }
+        if (more) load(next);
+        __syncthreads();
+        float acc[TP];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const h8 ka = *reinterpret_cast<const h8*>(kr + 64 * b), kc = *reinterpret_cast<const h8*>(kr + 64 * b + 32);
-                    f32x16 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[2 * b], ka, zero, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[2 * b + 1], kc, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[2 * b], ka, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[2 * b + 1], kc, s, 0, 0, 0);
-                    const float d = reinterpret_cast<const float*>(tile + G::oS)[b * 32 + j];
+        for (int p = 0; p < TP; ++p) acc[p] = 0.0f;
+        const auto products = [&]() {
+            const int left = RW < 4 ? a.rows - r0 : 32;  // (groups of eight rows past the last one are left out)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) x[v] = b ? fmaf(d, s[v], x[v]) : d * s[v];
+            for (int p = 0; p < TP; ++p) {
+                const int k0 = key0 + 32 * p;
+                if (!kpos && k0 > wmax) continue;
+                const char* tile = lds + (kw * TP + p) * G::Tile;
+                const char* kr = tile + j * kKeyRow<D> + 16 * h;
+                float x[16];
+                if constexpr (Q4) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const h8 ka = *reinterpret_cast<const h8*>(kr + 64 * b), kc = *reinterpret_cast<const h8*>(kr + 64 * b + 32);
+                        f32x16 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[2 * b], ka, zero, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[2 * b + 1], kc, s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[2 * b], ka, s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[2 * b + 1], kc, s, 0, 0, 0);
+                        const float d = reinterpret_cast<const float*>(tile + G::oS)[b * 32 + j];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            if (8 * g >= left) break;
+#pragma unroll
+                            for (int v = 4 * g; v < 4 * g + 4; ++v) x[v] = b ? fmaf(d, s[v], x[v]) : d * s[v];
+                        }
+                    }
+                } else {
+                    f32x16 s = zero;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const h8 ka = *reinterpret_cast<const h8*>(kr + 32 * k);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[k], ka, s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[k], ka, s, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) x[v] = s[v];
                 }
-            } else {
-                f32x16 s = zero;
+                const bool full = easy && k0 + 31 <= wmin && k0 + 31 < a.T;
+                if (full && shape.inv_cap == 0.0f && !shape.bias) {
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const h8 ka = *reinterpret_cast<const h8*>(kr + 32 * k);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[k], ka, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[k], ka, s, 0, 0, 0);
+                    for (int v = 0; v < 16; ++v) {
+                        const float2 cl = *reinterpret_cast<const float2*>(&rows4[wave][8 * (v >> 2) + 4 * h + (v & 3)]);
+                        acc[p] += ex2(fmaf(x[v], cl.x, -cl.y));
+                    }
+                    continue;
                 }
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] = s[v];
+                for (int g = 0; g < 4; ++g) {  // rows 8 g + 4 h .. + 4
+                    if (8 * g >= left) break;
+                    float y[4];
+                    float4 rf[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        rf[v] = rows4[wave][8 * g + 4 * h + v];
+                        y[v] = x[4 * g + v] * rf[v].x;
+                    }
+                    if (shape.inv_cap > 0.0f) capScores<4>(y, shape.inv_cap, shape);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        const int4 ri = rows4i[wave][8 * g + 4 * h + v];
+                        if (shape.bias) y[v] = fmaf(-rf[v].z * kLog2e, fabsf((float)(ri.y - pos[p])), y[v]);
+                        bool seen = pos[p] <= ri.x && doc[p] == ri.z;
+                        if (a.mask && seen) {
+                            const uint32_t mv = a.mask[(size_t)ri.w * a.m_row2 + k0 + j];
+                            seen = mv != 0xFC00u;
+                            y[v] = addMask(y[v], mv);
+                        }
+                        acc[p] += seen ? ex2(y[v] - rf[v].y) : 0.0f;
+                    }
+                }
             }
-            const bool full = easy && k0 + 31 <= wmin && k0 + 31 < a.T;
-            if (full && shape.inv_cap == 0.0f && !shape.bias) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const float2 cl = *reinterpret_cast<const float2*>(&rows4[wave][8 * (v >> 2) + 4 * h + (v & 3)]);
-                    acc[p] += ex2(fmaf(x[v], cl.x, -cl.y));
-                }
-                continue;
-            }
-            float4 rf[16];
-#pragma unroll
-            for (int v = 0; v < 16; ++v) rf[v] = rows4[wave][8 * (v >> 2) + 4 * h + (v & 3)];
-            if (shape.inv_cap > 0.0f) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] *= rf[v].x;
-                capScores<16>(x, shape.inv_cap, shape);
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] *= rf[v].x;
-            }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int4 ri = rows4i[wave][8 * (v >> 2) + 4 * h + (v & 3)];
-                if (shape.bias) x[v] = fmaf(-rf[v].z * kLog2e, fabsf((float)(ri.y - pos[p])), x[v]);
-                bool seen = pos[p] <= ri.x && doc[p] == ri.z;
-                if (a.mask && seen) {
-                    const uint32_t mv = a.mask[(size_t)ri.w * a.m_row2 + k0 + j];
-                    seen = mv != 0xFC00u;
-                    x[v] = addMask(x[v], mv);
-                }
-                acc[p] += seen ? ex2(x[v] - rf[v].y) : 0.0f;
+        };
+        if constexpr (RW < 4) {
+            if (r0 < a.rows) products();
+        } else {
+            for (r0 = 32 * rw; r0 < a.rows; r0 += 32 * RW) {
+                rows();
+                if (kpos || key0 <= wmax) products();
+                waveLds();
             }
         }
-        waveLds();
-    }
 #pragma unroll
-    for (int p = 0; p < TP; ++p) {
-        acc[p] += __shfl_xor(acc[p], 32);
-        if (h == 0) part[wave][p][j] = acc[p];
-    }
-    __syncthreads();
-    if (tid < 32 * KT) {
-        const int g = tid >> 5, w0 = g / TP * RW;
-        const long long key = (long long)(t0 + g) * 32 + (tid & 31);
-        if (key < a.T) {
-            float s = part[w0][g % TP][tid & 31];
-#pragma unroll
-            for (int x = 1; x < RW; ++x) s += part[w0 + x][g % TP][tid & 31];
-            const size_t at = (size_t)kvh * a.w_row + key;
-            a.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], s) : s;
+        for (int p = 0; p < TP; ++p) {
+            acc[p] += __shfl_xor(acc[p], 32);
+            if (h == 0) part[wave][p][j] = acc[p];
         }
+        __syncthreads();
+        if (tid < 32 * KT) {
+            const int g = tid >> 5, w0 = g / TP * RW;
+            const long long key = (long long)(t0 + g) * 32 + (tid & 31);
+            if (key < a.T) {
+                float s = part[w0][g % TP][tid & 31];
+#pragma unroll
+                for (int x = 1; x < RW; ++x) s += part[w0 + x][g % TP][tid & 31];
+                const size_t at = (size_t)kvh * a.w_row + key;
+                a.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], s) : s;
+            }
+        }
+        if (!more) break;
+        t0 = next;
     }
 }
 
@@ -208,8 +241,9 @@ int run(const FxParams& p, hipStream_t s) {
     static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_weights_kernel<D, Q4, RW, TP>),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds), "attn_weights: LDS size");
     if (ok) return ok;
-    const int tiles = p.T / 32 + (p.T % 32 != 0);
-    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP>), dim3((tiles + kt - 1) / kt, p.H_kv), dim3(256), lds, s, p);
+    const int tiles = p.T / 32 + (p.T % 32 != 0), all = (tiles + kt - 1) / kt;
+    const int grid = RW < 4 ? std::min(all, std::max(1, (512 + p.H_kv - 1) / p.H_kv)) : all;  // (two workgroups to a compute unit)
+    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP>), dim3(grid, p.H_kv), dim3(256), lds, s, p);
     return fromHip(hipGetLastError(), "attn_weights");
 }
 

@@ -240,7 +240,8 @@ def test_more_positions_than_are_mapped(q4):
 
 @CACHES
 @pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 1), (8, 2, 128, 1, 333), (8, 8, 64, 3, 130), (6, 2, 128, 20, 97), (8, 2, 64, 16, 200), (4, 2, 256, 70, 130),
-                                       (4, 1, 128, 100, 65)])
+                                       (4, 1, 128, 100, 65),
+                                       (32, 32, 64, 1, 2300), (32, 8, 128, 9, 4201), (16, 16, 256, 2, 4300)])  # (walks over the keys)
 @pytest.mark.parametrize("shape", ["plain", "cap_bias", "docs", "mask", "kept"])
 def test_weights(q4, H, K, D, N, T, shape):
     print(f"attn_weights q4={q4} H={H}/{K} D={D} N={N} T={T} {shape}", flush=True)
