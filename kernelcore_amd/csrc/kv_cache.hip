@@ -141,12 +141,30 @@ __device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0
     return w != w ? 1u : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
+// The sum over this lane and those below it, in registers: within rows of 16, then from row to row.
+__device__ __forceinline__ unsigned scanUp(unsigned x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // from the lanes 1, 2, 4 and 8 below
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // lane 15 of a row to the odd row above it
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to the upper two
+    return x;
+}
+// The sum of the counts of the wavefronts before `wave`.
+__device__ __forceinline__ unsigned sumBelow(const u4* counts, int wave) {
+    unsigned sum = 0;
+#pragma unroll
+    for (int x = 0; x < kKeepWaves; ++x) sum += x < wave ? counts[x / 4][x % 4] : 0u;
+    return sum;
+}
+
 template <int R>
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __restrict__ w, int* __restrict__ keep, int T,
                                                                int w_row, int n_keep, int keep_row, int first, int recent) {
     __shared__ uint2 hist[2][kKeepThreads];  // of 2048 digits
-    __shared__ unsigned waves[kKeepWaves], found[2];
-    __shared__ int above[kKeepWaves], equal[kKeepWaves];
+    __shared__ unsigned found[2];
+    __shared__ u4 waves[kKeepWaves / 4], above[kKeepWaves / 4], equal[kKeepWaves / 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* wr = w + (size_t)blockIdx.x * w_row;
     int* out = keep + (size_t)blockIdx.x * keep_row;
@@ -198,15 +216,10 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
         const int d = kKeepThreads - 1 - tid;
         const uint2 c = hist[pass & 1][d];
         unsigned upto = c.x + c.y;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const unsigned x = __shfl_up(upto, o);
-            if (lane >= o) upto += x;
-        }
-        if (lane == 63) waves[wave] = upto;
+        upto = scanUp(upto);
+        if (lane == 63) reinterpret_cast<unsigned*>(waves)[wave] = upto;
         __syncthreads();
-        unsigned before = upto - c.x - c.y;
-        for (int x = 0; x < wave; ++x) before += waves[x];
+        const unsigned before = upto - c.x - c.y + sumBelow(waves, wave);
         if (before < want && before + c.y >= want) {
             found[0] = 2 * d + 1;
             found[1] = want - before;
@@ -225,16 +238,11 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(const float* __re
         eq += (int)__popcll(__ballot(u == prefix));
     });
     if (lane == 0) {
-        above[wave] = gt;
-        equal[wave] = eq;
+        reinterpret_cast<unsigned*>(above)[wave] = gt;
+        reinterpret_cast<unsigned*>(equal)[wave] = eq;
     }
     __syncthreads();
-    int at = first, ties = 0;  // of the pieces before this one
-    for (int x = 0; x < wave; ++x) {
-        at += above[x];
-        ties += equal[x];
-    }
-    at += min(ties, (int)want);
+    int ties = (int)sumBelow(equal, wave), at = first + (int)sumBelow(above, wave) + min(ties, (int)want);  // of the pieces before this one
     const unsigned long long below = (1ull << lane) - 1;
     sweep([&](int i, uint32_t u) {
         const unsigned long long e = __ballot(u == prefix);
