@@ -55,11 +55,15 @@ __global__ __launch_bounds__(256) void set_rows_q4_0_kernel(const float* __restr
     if (tid == 0) later = 0;
     __syncthreads();
     unsigned mine = 0;
-    for (int i = r0 + 1 + tid; i < rows; i += 256) {
-        const long long other = index64(idx, i);
+    for (int i0 = r0 + 1 + tid; i0 < rows; i0 += 4 * 256) {  // four loads at a time (past the end the last row's again)
+        long long other[4];
 #pragma unroll
-        for (int k = 0; k < R; ++k)
-            if (i > r0 + k && other == at[k]) mine |= 1u << k;
+        for (int n = 0; n < 4; ++n) other[n] = index64(idx, min(i0 + 256 * n, rows - 1));
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (min(i0 + 256 * n, rows - 1) > r0 + k && other[n] == at[k]) mine |= 1u << k;
     }
     if (mine) atomicOr(&later, mine);
     __syncthreads();
@@ -80,16 +84,18 @@ __global__ __launch_bounds__(256) void set_rows_q4_0_kernel(const float* __restr
                 first = 4 * l + e;
             }
         }
-#pragma unroll
-        for (int o = 1; o < 8; o *= 2) {
-            const float m2 = __shfl_xor(m, o);
-            const int f2 = __shfl_xor(first, o);
-            wild |= __shfl_xor((int)wild, o) != 0;
+        auto with = [&](auto from) {
+            const float m2 = __builtin_bit_cast(float, from(__builtin_bit_cast(int, m)));
+            const int f2 = from(first);
+            wild |= from((int)wild) != 0;
             if (fabsf(m2) > fabsf(m) || (fabsf(m2) == fabsf(m) && f2 < first)) {
                 m = m2;
                 first = f2;
             }
-        }
+        };
+        with([](int y) { return __builtin_amdgcn_update_dpp(y, y, 0xB1, 0xF, 0xF, false); });   // lane ^ 1
+        with([](int y) { return __builtin_amdgcn_update_dpp(y, y, 0x4E, 0xF, 0xF, false); });   // ^ 2
+        with([](int y) { return __builtin_amdgcn_update_dpp(y, y, 0x141, 0xF, 0xF, false); });  // the other four of eight
         const float d = m * -0.125f, up = fabsf(d) < 0x1p-100f ? 0x1p64f : 1.0f;  // (subnormal steps scaled: exact)
         const float a = fabsf(d) * up, inv = 1.0f / a;
         uint32_t w = 0;
