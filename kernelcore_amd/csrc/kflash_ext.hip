@@ -119,18 +119,20 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         bmax = waveMax(max(l0, l1));
     }
 
-    // this range's steps
-    const int t0 = sp * a.per * (64 / TK);
-    int t1 = (int)min((long long)t0 + (long long)a.per * (64 / TK), ((long long)a.T + TK - 1) / TK);
-    if (!kpos) t1 = bmax < 0 ? t0 : min(t1, bmax / TK + 1);
-    const bool mapped = meta && (t1 - t0 + SPC - 1) / SPC <= G::MapEntries;
+    // this range's steps, every splits-th of all (what the rows see is spread over the ranges): step i of the range is step
+    // stepOf(i); the range's end before i1
+    int t1 = a.T / TK + (a.T % TK != 0);
+    if (!kpos) t1 = bmax < 0 ? 0 : min(t1, bmax / TK + 1);
+    const int i1 = t1 > sp ? (t1 - sp + a.splits - 1) / a.splits : 0, chunks = (i1 + SPC - 1) / SPC;
+    auto stepOf = [&](int i) { return i * a.splits + sp; };
+    const bool mapped = meta && chunks <= G::MapEntries;
     if constexpr (SHAPED) {
         if (mapped) {  // a wavefront takes 256 keys, four a lane
             constexpr int LPT = TK / 4;  // lanes to a step
-            const int key1 = min(a.T, t1 * TK), n = (key1 - t0 * TK + 255) / 256;
+            const int key1 = min(a.T, t1 * TK), n = chunks;
             int p[4], x[4];
             auto keysOf = [&](int at) {
-                const int key = t0 * TK + at * 256 + 4 * lane;
+                const int key = stepOf(at * SPC + lane / LPT) * TK + 4 * (lane % LPT);
                 if (key + 3 < key1) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] = key + e;
@@ -171,14 +173,14 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
     q.tops(tops + ks * 128, lane);
     if (tid < 8) wildAt[tid] = 0;
     __syncthreads();
-    auto next = [&](int t) -> int {  // the first step from t on that is to be computed; t1 if none
-        if (!mapped) return min(t, t1);
-        while (t < t1) {
-            const uint32_t w = (__builtin_amdgcn_readfirstlane(map[(t - t0) / SPC]) & 0xFFu) >> ((t - t0) % SPC);
-            if (w) return min(t + __builtin_ctz(w), t1);
-            t = t0 + ((t - t0) / SPC + 1) * SPC;
+    auto next = [&](int i) -> int {  // the first step from i on that is to be computed; i1 if none
+        if (!mapped) return min(i, i1);
+        while (i < i1) {
+            const uint32_t w = (__builtin_amdgcn_readfirstlane(map[i / SPC]) & 0xFFu) >> (i % SPC);
+            if (w) return i + __builtin_ctz(w);
+            i = (i / SPC + 1) * SPC;
         }
-        return t1;
+        return i1;
     };
 
     // ---- staging, through registers: 16-byte chunks (fp16) or half blocks of 8 bytes (4-bit) of a step's K and V rows, of each NL
@@ -297,8 +299,8 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    int t = next(t0), tn = t < t1 ? next(t + 1) : t1;
-    if (t < t1) fetch(t);
+    int i = next(0), in = i < i1 ? next(i + 1) : i1;
+    if (i < i1) fetch(stepOf(i));
     h8 qh[D / 16], ql[D / 16];
     auto topOf = [&](int r) { return G::KS == 2 ? fmaxf(tops[r], tops[128 + r]) : tops[r]; };
     const float c = qScale(topOf(j), a.scale).c, c2 = factor2(c);
@@ -315,24 +317,25 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         }
     }
     __syncthreads();
-    if (t < t1) store(t, lds, wildAt);
-    if (tn < t1) fetch(tn);
+    if (i < i1) store(stepOf(i), lds, wildAt);
+    if (in < i1) fetch(stepOf(in));
     __syncthreads();
     const int vlane = ks * 32 * (G::VRow / 2) + (4 * (lane >> 5) + ((lane & 15) >> 2)) * (G::VRow / 2) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     int slot = 0;  // of the wild-key words: three pairs in turn, the one two steps on is cleared while none reads it
-    for (int it = 0; t < t1; ++it) {
+    for (int it = 0; i < i1; ++it) {
+        const int t = stepOf(i);
         char* cur = lds + (it & 1) * G::Buf;
-        const int sn = slot == 2 ? 0 : slot + 1, sc = sn == 2 ? 0 : sn + 1, tnn = tn < t1 ? next(tn + 1) : t1;
+        const int sn = slot == 2 ? 0 : slot + 1, sc = sn == 2 ? 0 : sn + 1, inn = in < i1 ? next(in + 1) : i1;
         const int k0 = t * TK + 32 * ks;  // this wavefront's 32 keys
         bool full = !(SHAPED && mrow) && k0 + 31 < a.T;
-        if (meta) full = full && mapped && (__builtin_amdgcn_readfirstlane(map[(t - t0) / SPC]) >> (8 + (t - t0) % SPC) & 1);
+        if (meta) full = full && mapped && (__builtin_amdgcn_readfirstlane(map[i / SPC]) >> (8 + i % SPC) & 1);
         else full = full && k0 + 31 <= wmin;
         const bool work = full || meta || k0 <= wmax;
         // the next step into the other buffer (last read before the barrier that ended the step before this one): the second set
         // now, beside the first one's products, the first set at the end, beside the second one's
         auto stage = [&]() {
-            if (tn < t1) store(tn, lds + ((it + 1) & 1) * G::Buf, wildAt + 2 * sn);
-            if (tnn < t1) fetch(tnn);
+            if (in < i1) store(stepOf(in), lds + ((it + 1) & 1) * G::Buf, wildAt + 2 * sn);
+            if (inn < i1) fetch(stepOf(inn));
         };
         if (ks == 1) stage();
         MaskWords mk;
@@ -430,8 +433,8 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         if (ks == 0) stage();
         if (tid < 2) wildAt[2 * sc + tid] = 0;
         slot = sn;
-        t = tn;
-        tn = tnn;
+        i = in;
+        in = inn;
         __syncthreads();
     }
 
@@ -534,8 +537,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     char* mine = lds + wave * G::Wave;
     const char* kb = a.k + (size_t)kvh * a.k_head;
     const char* vb = a.v + (size_t)kvh * a.v_head;
-    const int t0 = sp * a.per * (64 / TK);
-    int t1 = (int)min((long long)t0 + (long long)a.per * (64 / TK), ((long long)a.T + TK - 1) / TK);
+    int t1 = a.T / TK + (a.T % TK != 0);
 
     const bool meta = SHAPED && (a.kpos || a.kdoc);
     const int* kpos = SHAPED && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
@@ -593,7 +595,9 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         }
     };
 
-    int t = t0 + wave;
+    // every splits-th tile is this workgroup's, of those every fourth this wavefront's: what the rows see is spread over all
+    const int stride = 4 * a.splits;
+    int t = sp + a.splits * wave;
     if (t < t1) fetch(t);  // (before it is known whether a row sees these keys: what it reads is there)
 
     Row row[NR];
@@ -612,7 +616,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         wmin = waveMin(wmin);
         wmax = waveMax(wmax);
     }
-    if (!kpos) t1 = wmax < 0 ? t0 : min(t1, wmax / TK + 1);
+    if (!kpos) t1 = wmax < 0 ? 0 : min(t1, wmax / TK + 1);
 
     // q as the B operand of step b (32 values): fp16 keys: values 32 b + 8 kg + e; 4-bit keys: the order nibbles() gives
     h8 qh[NR][NB], ql[NR][NB];
@@ -655,7 +659,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
     const int xn = i & 7, en = 2 * (xn & 3) + (xn >> 2);
     const int trow = 32 * (i >> 3) + 16 * (en >> 2) + 4 * kg + (en & 3);
 
-    for (; t < t1; t += 4) {
+    for (; t < t1; t += stride) {
         bool wild = false;
         h8 ka[Q4 ? 1 : 2 * NB];
 #pragma unroll
@@ -692,7 +696,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
                 mt[TK + lane] = rkd;
             }
         }
-        if (t + 4 < t1) fetch(t + 4);
+        if (t + stride < t1) fetch(t + stride);
         waveLds();
         float x[NR][U * 4];
         if constexpr (Q4) {
@@ -1077,7 +1081,6 @@ int launchFlashExt(bool q4, const kcFlashExtArgs& a, hipStream_t s) {
     p.lse = a.lse;
     p.part = a.part;
     p.splits = plan.splits;
-    p.per = plan.per;
     const bool shaped = a.mask || a.kpos || a.kdoc || a.slopes || a.softcap > 0.0f;
     switch (a.d.D) {
         case 64: return runD<64>(q4, shaped, p, plan, s);

@@ -24,35 +24,36 @@ struct FxParams {
     float* w;
     long long k_row, k_head, v_row, v_head;
     int H, H_kv, G, N, T, q_tok, q_head, m_row2, key_row, pos0, causal, prefix, rows;
-    int splits, per;  // key ranges, units of 64 keys in each
+    int splits;  // key ranges
     int w_row;
     float scale, softcap, decay;
 };
 
 // How flash_ext splits a call. The few-rows kernel takes groups of 32 rows (16 of 256 values, beyond which it runs out of
-// registers), the many-rows kernel blocks of 128; the keys in `splits` ranges of `per` units of 64 keys. One group always runs on the
+// registers), the many-rows kernel blocks of 128; the keys go to `splits` ranges in turn. One group always runs on the
 // few-rows kernel, several while they leave a compute unit no more than four units of keys (256 values: eight): 64 tokens over 500
 // positions, 32 heads of 128 on 8, fp16: 14.3 us, on the many-rows kernel 18.0; over 8191: 9 tokens 26.4 and 20.3; 9 tokens over
 // 2048, heads of 256: 20.6 and 35.9.
 struct FxPlan {
     bool few;
-    int splits, per;
+    int splits;
     int64_t partFloats;
 };
 inline FxPlan fxPlan(const kcFlashExtDims& d) {
     const int64_t rows = int64_t(d.N) * (d.H / d.H_kv), units = (int64_t(d.T) + 63) / 64;
     const int64_t group = d.D == 256 ? 16 : 32, groups = (rows + group - 1) / group;
-    FxPlan p{groups <= 1 || d.H_kv * groups * units <= (d.D == 256 ? 2048 : 1024), 1, 1, 0};
+    FxPlan p{groups <= 1 || d.H_kv * groups * units <= (d.D == 256 ? 2048 : 1024), 1, 0};
     const int64_t base = int64_t(d.H_kv) * (p.few ? groups : (rows + 127) / 128);
     // few rows: ranges of two units while that is no more than a workgroup for each of the 256 compute units (a wavefront then
     // has one tile of an fp16 cache), of four beyond, up to two workgroups each; T 2049, 5 tokens: 17 ranges 13.3 us, 9 14.6;
-    // T 8191, 1 token: 64 ranges 14.2 us, 32 12.1
+    // T 8191, 1 token: 64 ranges 14.2 us, 32 12.1. Many rows, of which a compute unit holds one workgroup: as many ranges as fill the GPU
+    // once (300 tokens over 3577: three 55 us, six 73, two 67), of four units, or eight where the join of many blocks counts (500
+    // tokens over themselves: one 22.6 us, two 28.1).
     const int64_t one = std::max<int64_t>(1, 256 / std::max<int64_t>(1, base)), two = std::max<int64_t>(1, 512 / std::max<int64_t>(1, base));
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>(two, (units + 3) / 4));
-    if (p.few) splits = std::max<int64_t>(splits, std::min<int64_t>(one, (units + 1) / 2));
-    else splits = std::min<int64_t>(splits, 32);
-    p.per = int(std::max<int64_t>(1, (units + splits - 1) / splits));
-    p.splits = int(std::max<int64_t>(1, (units + p.per - 1) / p.per));
+    int64_t splits;
+    if (p.few) splits = std::max(std::min(two, (units + 3) / 4), std::min(one, (units + 1) / 2));
+    else splits = std::min(one, base > 64 ? (units + 7) / 8 : (units + 3) / 4);
+    p.splits = int(std::max<int64_t>(1, splits));
     p.partFloats = p.splits > 1 ? int64_t(p.splits) * d.H_kv * rows * (d.D + 2) : 0;
     return p;
 }
