@@ -30,7 +30,9 @@ struct WGeo {
 // workgroup walks over the keys, the next ones' loads under way (131072 fp16 positions of 8 heads of 128, one token: 45 us, 6 TB/s;
 // a workgroup for every 128 keys, each with q of its own, 95); with more rows it walks over them, and has its keys only once. Two workgroups to a
 // compute unit are worth some spilled registers at 256 values (64 tokens over 8192: 34 against 47 us), but for a walk over fp16 keys (15 against 20).
-template <int D, bool Q4, int RW, int TP>
+// META: keys have positions or documents of their own, and tiles that no row sees are left out (a form of its own, whose registers
+// cost the plain one 5%).
+template <int D, bool Q4, int RW, int TP, bool META>
 __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_weights_kernel(FxParams a) {
     using G = WGeo<D, Q4>;
     constexpr int NB = G::NB, KW = 4 / RW, KT = KW * TP, PR = Q4 ? NB : D / 8, KS = D / 16;
@@ -44,8 +46,8 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
     const int j = lane & 31, h = lane >> 5;
     const int kw = wave / RW, rw = wave % RW;
     const char* kb = a.k + (size_t)kvh * a.k_head;
-    const int* kpos = a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
-    const int* kdoc = a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
+    const int* kpos = META && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
+    const int* kdoc = META && a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
     constexpr int IT = KT * 32 * PR, NL = (IT + 255) / 256;
     u4 raw[NL];
     uint32_t sc[Q4 ? NL : 1];
@@ -93,17 +95,24 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
 #pragma unroll
     for (int v = 0; v < 16; ++v) zero[v] = 0.0f;
 
-    // a row tile: q as operands, what else its rows bring to LDS
-    int r0 = 32 * rw, wmax, wmin;
-    bool easy;  // whole, each of its rows saw something, and keys are hidden by position alone
+    // a row tile: its rows' limits and documents; q as operands, what else its rows bring to LDS
+    int r0 = 32 * rw, wmax = -1, wmin = INT_MAX, dmin = 0, dmax = 0;
+    bool easy = false;  // whole, each of its rows saw something, and keys are hidden by position alone
+    Row row;
     h8 qh[KS], ql[KS];
+    auto limits = [&]() {
+        row = rowOf(a, kvh, r0 + j);
+        wmax = waveMax(row.live ? row.limit : -1);
+        wmin = waveMin(row.live ? row.limit : INT_MAX);
+        if (kdoc) {
+            dmin = waveMin(row.doc);
+            dmax = waveMax(row.doc);
+        }
+    };
     auto rows = [&]() {
-        const Row row = rowOf(a, kvh, r0 + j);
         f32x4 q[D / 8];
         loadRow32<D>(a, row, h, q);
         const float lse = a.lse[(size_t)row.token * a.H + row.head];
-        wmax = waveMax(row.live ? row.limit : -1);
-        wmin = waveMin(row.live ? row.limit : INT_MAX);
         easy = !kpos && !kdoc && !a.mask && !__any(lse == -INFINITY) && r0 + 32 <= a.rows;
         const float c = splitRow32<D>(a, q, qh, ql);
         if (h == 0) {  // (a row that saw nothing gives nothing: its factor's place holds the mark)
@@ -116,7 +125,10 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
     const int tiles = a.T / 32 + (a.T % 32 != 0);
     int t0 = blockIdx.x * KT;
     load(t0);
-    if (RW < 4 && r0 < a.rows) rows();  // (the only one)
+    if (RW < 4 && r0 < a.rows) {  // (the only one)
+        limits();
+        rows();
+    }
     while (true) {
         const int key0 = (t0 + kw * TP) * 32, next = t0 + (int)gridDim.x * KT;
         const bool more = RW < 4 && next < tiles;
@@ -129,6 +141,14 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
             doc[p] = rdoc[p];
         }
         if (more) load(next);
+        int first[TP], dlo[TP], dhi[TP];  // a tile's least position and its documents
+#pragma unroll
+        for (int p = 0; p < TP; ++p) {
+            first[p] = kpos ? waveMin(pos[p]) : key0 + 32 * p;
+            dlo[p] = kdoc ? waveMin(doc[p]) : 0;
+            dhi[p] = kdoc ? waveMax(doc[p]) : 0;
+        }
+        auto seen = [&](int p) { return first[p] <= wmax && dlo[p] <= dmax && dhi[p] >= dmin; };  // by some row, perhaps
         __syncthreads();
         float acc[TP];
 #pragma unroll
@@ -138,7 +158,7 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
 #pragma unroll
             for (int p = 0; p < TP; ++p) {
                 const int k0 = key0 + 32 * p;
-                if (!kpos && k0 > wmax) continue;
+                if (!seen(p)) continue;
                 const char* tile = lds + (kw * TP + p) * G::Tile;
                 const char* kr = tile + j * kKeyRow<D> + 16 * h;
                 float x[16];
@@ -193,13 +213,13 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
                     for (int v = 0; v < 4; ++v) {
                         const int4 ri = rows4i[wave][8 * g + 4 * h + v];
                         if (shape.bias) y[v] = fmaf(-rf[v].z * kLog2e, fabsf((float)(ri.y - pos[p])), y[v]);
-                        bool seen = pos[p] <= ri.x && doc[p] == ri.z;
-                        if (a.mask && seen) {
+                        bool sees = pos[p] <= ri.x && doc[p] == ri.z;
+                        if (a.mask && sees) {
                             const uint32_t mv = a.mask[(size_t)ri.w * a.m_row2 + k0 + j];
-                            seen = mv != 0xFC00u;
+                            sees = mv != 0xFC00u;
                             y[v] = addMask(y[v], mv);
                         }
-                        acc[p] += seen ? ex2(y[v] - rf[v].y) : 0.0f;
+                        acc[p] += sees ? ex2(y[v] - rf[v].y) : 0.0f;
                     }
                 }
             }
@@ -208,8 +228,13 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
             if (r0 < a.rows) products();
         } else {
             for (r0 = 32 * rw; r0 < a.rows; r0 += 32 * RW) {
+                limits();
+                bool any = false;
+#pragma unroll
+                for (int p = 0; p < TP; ++p) any |= seen(p);
+                if (!any) continue;
                 rows();
-                if (kpos || key0 <= wmax) products();
+                products();
                 waveLds();
             }
         }
@@ -235,16 +260,21 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
     }
 }
 
-template <int D, bool Q4, int RW, int TP>
-int run(const FxParams& p, hipStream_t s) {
+template <int D, bool Q4, int RW, int TP, bool META>
+int runMeta(const FxParams& p, hipStream_t s) {
     constexpr int kt = 4 / RW * TP, lds = WGeo<D, Q4>::Tile * kt;
-    static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_weights_kernel<D, Q4, RW, TP>),
+    static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_weights_kernel<D, Q4, RW, TP, META>),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds), "attn_weights: LDS size");
     if (ok) return ok;
     const int tiles = p.T / 32 + (p.T % 32 != 0), all = (tiles + kt - 1) / kt;
     const int grid = RW < 4 ? std::min(all, std::max(1, (512 + p.H_kv - 1) / p.H_kv)) : all;  // (two workgroups to a compute unit)
-    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP>), dim3(grid, p.H_kv), dim3(256), lds, s, p);
+    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP, META>), dim3(grid, p.H_kv), dim3(256), lds, s, p);
     return fromHip(hipGetLastError(), "attn_weights");
+}
+
+template <int D, bool Q4, int RW, int TP>
+int run(const FxParams& p, hipStream_t s) {
+    return p.kpos || p.kdoc ? runMeta<D, Q4, RW, TP, true>(p, s) : runMeta<D, Q4, RW, TP, false>(p, s);
 }
 
 template <int D, bool Q4>

@@ -31,7 +31,7 @@ struct FxParams {
 
 // How flash_ext splits a call. The few-rows kernel takes groups of 32 rows (16 of 256 values, beyond which it runs out of
 // registers), the many-rows kernel blocks of 128; the keys go to `splits` ranges in turn. One group always runs on the
-// few-rows kernel, several while they leave a compute unit no more than four units of keys (256 values: eight): 64 tokens over 500
+// few-rows kernel, several while they leave a compute unit no more than four units of keys (128 values; eight otherwise): 64 tokens over 500
 // positions, 32 heads of 128 on 8, fp16: 14.3 us, on the many-rows kernel 18.0; over 8191: 9 tokens 26.4 and 20.3; 9 tokens over
 // 2048, heads of 256: 20.6 and 35.9.
 struct FxPlan {
@@ -42,7 +42,7 @@ struct FxPlan {
 inline FxPlan fxPlan(const kcFlashExtDims& d) {
     const int64_t rows = int64_t(d.N) * (d.H / d.H_kv), units = (int64_t(d.T) + 63) / 64;
     const int64_t group = d.D == 256 ? 16 : 32, groups = (rows + group - 1) / group;
-    FxPlan p{groups <= 1 || d.H_kv * groups * units <= (d.D == 256 ? 2048 : 1024), 1, 0};
+    FxPlan p{groups <= 1 || d.H_kv * groups * units <= (d.D == 128 ? 1024 : 2048), 1, 0};
     const int64_t base = int64_t(d.H_kv) * (p.few ? groups : (rows + 127) / 128);
     // few rows: ranges of two units while that is no more than a workgroup for each of the 256 compute units (a wavefront then
     // has one tile of an fp16 cache), of four beyond, up to two workgroups each; T 2049, 5 tokens: 17 ranges 13.3 us, 9 14.6;
