@@ -26,20 +26,22 @@ struct WGeo {
     static constexpr int oS = 32 * kKeyRow<D>, oMeta = oS + (Q4 ? NB * 128 : 0), Tile = oMeta + 256;
 };
 
-// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup. Up to 64 rows (RW < 4) stay in registers, and the
+// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup of four (RW = 8: eight) wavefronts. Up to 64 rows (RW < 4) stay in registers, and the
 // workgroup walks over the keys, the next ones' loads under way (131072 fp16 positions of 8 heads of 128, one token: 45 us, 6 TB/s;
 // a workgroup for every 128 keys, each with q of its own, 95); with more rows it walks over them, and has its keys only once. Two workgroups to a
 // compute unit are worth some spilled registers at 256 values (64 tokens over 8192: 34 against 47 us), but for a walk over fp16 keys (15 against 20).
 // META: keys have positions or documents of their own, and tiles that no row sees are left out (a form of its own, whose registers
 // cost the plain one 5%).
+template <int RW>
+constexpr int kWaves = RW > 4 ? RW : 4;
 template <int D, bool Q4, int RW, int TP, bool META>
-__global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_weights_kernel(FxParams a) {
+__global__ __launch_bounds__(64 * kWaves<RW>, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_weights_kernel(FxParams a) {
     using G = WGeo<D, Q4>;
-    constexpr int NB = G::NB, KW = 4 / RW, KT = KW * TP, PR = Q4 ? NB : D / 8, KS = D / 16;
+    constexpr int NB = G::NB, W = kWaves<RW>, NT = 64 * W, KW = W / RW, KT = KW * TP, PR = Q4 ? NB : D / 8, KS = D / 16;
     extern __shared__ int4 lds4[];
-    __shared__ float part[4][TP][32];
-    __shared__ float4 rows4[4][32];  // factor of the sums (base 2 unless capped), lse (base 2), slope, -
-    __shared__ int4 rows4i[4][32];   // limit, position, document, token
+    __shared__ float part[W][TP][32];
+    __shared__ float4 rows4[W][32];  // factor of the sums (base 2 unless capped), lse (base 2), slope, -
+    __shared__ int4 rows4i[W][32];   // limit, position, document, token
     char* lds = reinterpret_cast<char*>(lds4);
     const int kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -48,14 +50,14 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
     const char* kb = a.k + (size_t)kvh * a.k_head;
     const int* kpos = META && a.kpos ? a.kpos + (size_t)kvh * a.key_row : nullptr;
     const int* kdoc = META && a.kdoc ? a.kdoc + (size_t)kvh * a.key_row : nullptr;
-    constexpr int IT = KT * 32 * PR, NL = (IT + 255) / 256;
+    constexpr int IT = KT * 32 * PR, NL = (IT + NT - 1) / NT;
     u4 raw[NL];
     uint32_t sc[Q4 ? NL : 1];
     int rpos[TP], rdoc[TP];  // this lane's keys: key j of each of the wavefront's tiles
     auto load = [&](int t0) {
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-            const int i = tid + 256 * n;
+            const int i = tid + NT * n;
             if (i >= IT) break;
             const char* p = kb + (size_t)min((long long)t0 * 32 + i / PR, (long long)a.T - 1) * a.k_row + (Q4 ? 18 : 16) * (i % PR);
             if constexpr (Q4) {
@@ -75,7 +77,7 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
     auto store = [&]() {
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-            const int i = tid + 256 * n, key = i / PR, b = i % PR;
+            const int i = tid + NT * n, key = i / PR, b = i % PR;
             if (i >= IT) break;
             char* tile = lds + (key >> 5) * G::Tile;
             if constexpr (Q4) {
@@ -262,13 +264,13 @@ __global__ __launch_bounds__(256, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_
 
 template <int D, bool Q4, int RW, int TP, bool META>
 int runMeta(const FxParams& p, hipStream_t s) {
-    constexpr int kt = 4 / RW * TP, lds = WGeo<D, Q4>::Tile * kt;
+    constexpr int W = kWaves<RW>, kt = W / RW * TP, lds = WGeo<D, Q4>::Tile * kt;
     static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_weights_kernel<D, Q4, RW, TP, META>),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds), "attn_weights: LDS size");
     if (ok) return ok;
     const int tiles = p.T / 32 + (p.T % 32 != 0), all = (tiles + kt - 1) / kt;
     const int grid = RW < 4 ? std::min(all, std::max(1, (512 + p.H_kv - 1) / p.H_kv)) : all;  // (two workgroups to a compute unit)
-    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP, META>), dim3(grid, p.H_kv), dim3(256), lds, s, p);
+    hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP, META>), dim3(grid, p.H_kv), dim3(64 * W), lds, s, p);
     return fromHip(hipGetLastError(), "attn_weights");
 }
 
@@ -281,8 +283,12 @@ template <int D, bool Q4>
 int runRows(const FxParams& p, hipStream_t s) {
     if (p.rows <= 32) return run<D, Q4, 1, 1>(p, s);
     if (p.rows <= 64) return run<D, Q4, 2, 1>(p, s);
-    // four tiles to a wavefront, q read a quarter as often, where that leaves a workgroup for every compute unit
-    return (long long)p.T * p.H_kv >= 128 * 256 ? run<D, Q4, 4, 4>(p, s) : run<D, Q4, 4, 1>(p, s);
+    // four tiles to a wavefront, q read a quarter as often, where that leaves a workgroup for every compute unit; eight wavefronts
+    // to a tile where there is no more than a tile for each (189 tokens over 759 positions, 24 heads of 128: 25 -> 16 us; 64 over
+    // 2000, of 32: 12 -> 14)
+    const long long keys = (long long)p.T * p.H_kv;
+    if (keys >= 128 * 256) return run<D, Q4, 4, 4>(p, s);
+    return p.rows > 128 && keys <= 32 * 256 ? run<D, Q4, 8, 1>(p, s) : run<D, Q4, 4, 1>(p, s);
 }
 
 }  // namespace

@@ -6,6 +6,7 @@
 #include <kernelcore/llm_kernels.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 namespace kcamd {
@@ -39,6 +40,27 @@ struct FxPlan {
     int splits;
     int64_t partFloats;
 };
+// Key ranges of the many-rows kernel, of four units at least: the least estimate, in steps (64 keys in 2 us, of 256 values 32 in 3.5).
+// A compute unit holds one workgroup, which takes four steps to set up and write; ranges are written and read again by the join.
+// Causal rows' workgroups, the longest first, fill the GPU evenly as they are, and are divided only where they do not fill it; equal
+// ones run in whole rounds. 300 tokens over 3577: three ranges 55 us, six 73, two 67; 500 tokens over themselves: one 22.6, two
+// 28.1; 82 over 3169: ten 30.1, thirteen 40.2; 1500 over 3000: one 88, two 98.
+inline int64_t fxRanges(const kcFlashExtDims& d, int64_t base, int64_t units) {
+    const double steps = d.D == 256 ? 2.0 * units : 1.0 * units;
+    const double join = double(d.N) * d.H * d.D * 8 / 4.75e12 / (d.D == 256 ? 3.5e-6 : 2e-6);
+    const int64_t most = std::min<int64_t>((units + 3) / 4, std::max<int64_t>(1, (d.causal ? 256 : 1024) / std::max<int64_t>(1, base)));
+    int64_t best = 1;
+    double least = 0.0;
+    for (int64_t s = 1; s <= std::min<int64_t>(most, 256); ++s) {
+        const double rounds = std::ceil(double(base) * s / 256.0);
+        const double cost = rounds * (std::ceil(steps / s) + 4.0) + (s > 1 ? 2.0 + s * join : 0.0);
+        if (s == 1 || cost < least) {
+            best = s;
+            least = cost;
+        }
+    }
+    return best;
+}
 inline FxPlan fxPlan(const kcFlashExtDims& d) {
     const int64_t rows = int64_t(d.N) * (d.H / d.H_kv), units = (int64_t(d.T) + 63) / 64;
     const int64_t group = d.D == 256 ? 16 : 32, groups = (rows + group - 1) / group;
@@ -46,13 +68,9 @@ inline FxPlan fxPlan(const kcFlashExtDims& d) {
     const int64_t base = int64_t(d.H_kv) * (p.few ? groups : (rows + 127) / 128);
     // few rows: ranges of two units while that is no more than a workgroup for each of the 256 compute units (a wavefront then
     // has one tile of an fp16 cache), of four beyond, up to two workgroups each; T 2049, 5 tokens: 17 ranges 13.3 us, 9 14.6;
-    // T 8191, 1 token: 64 ranges 14.2 us, 32 12.1. Many rows, of which a compute unit holds one workgroup: as many ranges as fill the GPU
-    // once (300 tokens over 3577: three 55 us, six 73, two 67), of four units, or eight where the join of many blocks counts (500
-    // tokens over themselves: one 22.6 us, two 28.1).
+    // T 8191, 1 token: 64 ranges 14.2 us, 32 12.1
     const int64_t one = std::max<int64_t>(1, 256 / std::max<int64_t>(1, base)), two = std::max<int64_t>(1, 512 / std::max<int64_t>(1, base));
-    int64_t splits;
-    if (p.few) splits = std::max(std::min(two, (units + 3) / 4), std::min(one, (units + 1) / 2));
-    else splits = std::min(one, base > 64 ? (units + 7) / 8 : (units + 3) / 4);
+    int64_t splits = p.few ? std::max(std::min(two, (units + 3) / 4), std::min(one, (units + 1) / 2)) : fxRanges(d, base, units);
     p.splits = int(std::max<int64_t>(1, splits));
     p.partFloats = p.splits > 1 ? int64_t(p.splits) * d.H_kv * rows * (d.D + 2) : 0;
     return p;

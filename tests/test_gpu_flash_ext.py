@@ -214,10 +214,11 @@ def test_offsets_past_32_bits(q4):
 
 
 @CACHES
-def test_more_positions_than_are_mapped(q4):
+@pytest.mark.parametrize("N", [32800, 131200])
+def test_more_positions_than_are_mapped(q4, N):
     """Key positions are mapped 256 at a time, 2048 entries of a workgroup's range; with so many queries that the keys are one
-    range, more go unmapped. A few filled slots among empty ones."""
-    D, N, T = 64, 32800, 2048 * 256 + 300
+    range (the second size), more go unmapped. A few filled slots among empty ones."""
+    D, T = 64, 2048 * 256 + 300
     at = np.unique(np.r_[0, 255, T - 301, T - 300, T - 1, np.random.default_rng(5).integers(0, T, 35)])
     c = Case(q4, 1, 1, D, N, len(at), kpos=np.arange(len(at), dtype=np.int32)[None] * 900, qpos=np.arange(N, dtype=np.int32))
     hb = c.head_bytes()
@@ -228,20 +229,21 @@ def test_more_positions_than_are_mapped(q4):
     for b, x in ((q, c.q), (qpos, c.qpos), (dk, k), (dv, v), (dp, kpos)):
         b.upload(x.ravel())
     d = c.dims(T=T, k_row=hb, k_head=hb, v_row=hb, v_head=hb)
-    assert kc.flash_ext_part_bytes(d) == 0
-    out = kc.Buffer(4 * N * D)
-    kc.launch(c.name("flash_ext"), kc.FlashExtArgs(q=q.ptr, k=dk.ptr, v=dv.ptr, qpos=qpos.ptr, kpos=dp.ptr, out=out.ptr, d=d, scale=c.scale))
+    assert N < 131200 or kc.flash_ext_part_bytes(d) == 0
+    out, part = kc.Buffer(4 * N * D), kc.Buffer(kc.flash_ext_part_bytes(d) + 4)
+    kc.launch(c.name("flash_ext"), kc.FlashExtArgs(q=q.ptr, k=dk.ptr, v=dv.ptr, qpos=qpos.ptr, kpos=dp.ptr, out=out.ptr, part=part.ptr, d=d, scale=c.scale))
     want, bound, _, _ = c.expected()
     got = out.download(np.float32).reshape(N, 1, D)
     assert not (~(np.abs(got - want) <= bound)).any(), np.abs(got - want).max()
-    for x in (q, qpos, dk, dv, dp, out):
+    for x in (q, qpos, dk, dv, dp, out, part):
         x.free()
 
 
 @CACHES
 @pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 1), (8, 2, 128, 1, 333), (8, 8, 64, 3, 130), (6, 2, 128, 20, 97), (8, 2, 64, 16, 200), (4, 2, 256, 70, 130),
                                        (4, 1, 128, 100, 65),
-                                       (32, 32, 64, 1, 2300), (32, 8, 128, 9, 4201), (16, 16, 256, 2, 4300)])  # (walks over the keys)
+                                       (32, 32, 64, 1, 2300), (32, 8, 128, 9, 4201), (16, 16, 256, 2, 4300),  # (walks over the keys)
+                                       (8, 2, 128, 25, 150), (16, 8, 128, 40, 4201), (8, 2, 64, 80, 300)])  # (four wavefronts to a tile, to four, eight to one)
 @pytest.mark.parametrize("shape", ["plain", "cap_bias", "docs", "mask", "kept"])
 def test_weights(q4, H, K, D, N, T, shape):
     print(f"attn_weights q4={q4} H={H}/{K} D={D} N={N} T={T} {shape}", flush=True)
