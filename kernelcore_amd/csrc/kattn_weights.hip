@@ -4,7 +4,7 @@
 // keys): lane (j, h) holds rows 8 (v / 4) + 4 h + v % 4 of key j, so a key's sum over the rows is a sum of registers and
 // nothing crosses lanes until the end. A workgroup stages key tiles, and its wavefronts share the rows (RW of them
 // to a tile). Sums in one order, no atomics.
-// A single token's call reads K once and is bound by that, or by a tile's latency (4099 fp16 positions, 8 KV heads of 128: 6.8 us); with
+// A single token's call reads K once and is bound by that, or by a tile's latency (4099 fp16 positions, 8 KV heads of 128: 6.1 us); with
 // many rows the scaling of the sums and the exponentials bound it, and q, split anew for every 128 keys (64 tokens of 32 heads over
 // 8192 4-bit positions: 19 us, 0.45 PFLOP/s counting both parts of q).
 #include <hip/hip_runtime.h>
@@ -23,7 +23,7 @@ using namespace fx;
 template <int D, bool Q4>
 struct WGeo {
     static constexpr int NB = D / 32;
-    static constexpr int oS = 32 * kKeyRow<D>, oMeta = oS + (Q4 ? NB * 128 : 0), Tile = oMeta + 256;
+    static constexpr int oS = 32 * kKeyRow<D>, Tile = oS + (Q4 ? NB * 128 : 0);  // key rows, 4-bit: their blocks' scales
 };
 
 // RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup of four (RW = 8: eight) wavefronts. Up to 64 rows (RW < 4) stay in registers, and the

@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t tameHalves(uint32_t w) {
 // set to a workgroup: 101 against 78 us.)
 // Bound by the products, staging and softmax, which overlap little: 2048 causal tokens, 24 heads of 128, fp16: 75 us, 0.69
 // PFLOP/s counting both parts of q and p (a large fp16 product of the library: 1.19); 1000 tokens over 3577 4-bit positions,
-// 32 heads: 150 us, 0.84 PFLOP/s.
+// 32 heads: 143 us, 0.88 PFLOP/s.
 template <int D, bool Q4>
 struct Geo {
     static constexpr int KS = D == 256 ? 1 : 2;  // (256 values: one wavefront's registers fill a SIMD)

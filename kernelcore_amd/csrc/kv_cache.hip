@@ -24,7 +24,7 @@ __device__ __forceinline__ long long index64(const int* idx, long long i) {
 
 // ---------------------------------------------------------------------------------------------- 4-bit rows
 // Eight lanes per block of 32 values, four values each; R rows per workgroup. Bound by reading the f32 rows, and by the search for
-// repeated indices: 1777 rows of 1024 values 5.3 us, 1.6 TB/s; one row 1.9 us.
+// repeated indices: 1777 rows of 1024 values 5.4 us, 1.5 TB/s; one row 1.7 us.
 // Code of x: floor(x / d + 8.5), d = xm / -8. With a = |d| and y = x sign(d) that is the largest c with (c - 8.5) a <= y:
 // the product c' a of a half-integer and an f32 is rounded by the fma only after y is subtracted, so the sign of
 // y - c' a is exact and settles a guess from the rounded quotient.
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restri
 // in ascending order: each wavefront owns a contiguous piece of the row, so that ballots and one prefix over the
 // wavefronts give every position its place. Up to R x 1024 positions are read once and held in registers through the five
 // sweeps; longer rows (R = 0) are read by each sweep. A head has one compute unit, and the sweeps' instructions bound it: 16384
-// positions 13.4 us (with digits of 8 bits, a sweep more, 14.7), 1500 positions 6.5 us, its barriers and the load.
+// positions 12.1 us (digits of 8 bits, a sweep more: 1.3 us more), 1500 positions 5.4 us, its barriers and the load.
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 
 __device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first; never 0
