@@ -349,7 +349,8 @@ typedef struct kcFlashExtDims {
 /* flash_ext_f16 / flash_ext_q4_0: out[N][H][D] = sum_j softmax_j(score) v_j over the seen keys, for single
  * tokens and for prompts; a query that sees none gets zeros. lse (may be null): [N][H], the natural
  * logarithm of the sum of exp(score), -infinity for such a query. part: kcFlashExtPartBytes bytes of
- * workspace, which calls that may overlap must not share; null where that is 0. */
+ * workspace, which calls that may overlap must not share; null where that is 0. (Ask for each call's sizes: fewer
+ * tokens or positions may need more; a smaller part is refused.) */
 typedef struct kcFlashExtArgs {
     const float* q;
     const void* k;

@@ -26,10 +26,11 @@ struct WGeo {
     static constexpr int oS = 32 * kKeyRow<D>, Tile = oS + (Q4 ? NB * 128 : 0);  // key rows, 4-bit: their blocks' scales
 };
 
-// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup of four (RW = 8: eight) wavefronts. Up to 64 rows (RW < 4) stay in registers, and the
-// workgroup walks over the keys, the next ones' loads under way (131072 fp16 positions of 8 heads of 128, one token: 45 us, 6 TB/s;
-// a workgroup for every 128 keys, each with q of its own, 95); with more rows it walks over them, and has its keys only once. Two workgroups to a
-// compute unit are worth some spilled registers at 256 values (64 tokens over 8192: 34 against 47 us), but for a walk over fp16 keys (15 against 20).
+// RW wavefronts to a key tile, TP tiles to a wavefront: 4 / RW TP tiles to a workgroup of four (RW = 8: eight) wavefronts. Up to
+// 64 rows (RW < 4) stay in registers, and the workgroup walks over the keys, the next ones' loads under way (131072 fp16
+// positions of 8 heads of 128, one token: 45 us, 6 TB/s; a workgroup for every 128 keys, each with q of its own, 95); with more
+// rows it walks over them, and has its keys only once. Two workgroups to a compute unit are worth some spilled registers at 256
+// values (64 tokens over 8192: 34 against 47 us), but for a walk over fp16 keys (15 against 20).
 // META: keys have positions or documents of their own, and tiles that no row sees are left out (a form of its own, whose registers
 // cost the plain one 5%).
 template <int RW>

@@ -64,7 +64,7 @@ inline int64_t fxRanges(const kcFlashExtDims& d, int64_t base, int64_t units) {
 inline FxPlan fxPlan(const kcFlashExtDims& d) {
     const int64_t rows = int64_t(d.N) * (d.H / d.H_kv), units = (int64_t(d.T) + 63) / 64;
     const int64_t group = d.D == 256 ? 16 : 32, groups = (rows + group - 1) / group;
-    FxPlan p{groups <= 1 || d.H_kv * groups * units <= (d.D == 128 ? 1024 : 2048), 1, 0};
+    FxPlan p{groups <= 1 || d.H_kv * groups * std::max<int64_t>(1, units) <= (d.D == 128 ? 1024 : 2048), 1, 0};
     const int64_t base = int64_t(d.H_kv) * (p.few ? groups : (rows + 127) / 128);
     // few rows: ranges of two units while that is no more than a workgroup for each of the 256 compute units (a wavefront then
     // has one tile of an fp16 cache), of four beyond, up to two workgroups each; T 2049, 5 tokens: 17 ranges 13.3 us, 9 14.6;

@@ -94,6 +94,20 @@ def test_no_keys_and_no_queries(q4):
     Case(q4, 4, 2, 64, 0, 17, pos0=17).attend()
 
 
+def test_many_queries_and_no_keys():
+    """More rows than a grid's third dimension counts in groups of 32 (all tokens read the same q)."""
+    N, D = 2_100_000, 64
+    q, out, lse = kc.Buffer.of(np.ones(D, np.float32)), kc.Buffer(4 * N * D), kc.Buffer(4 * N)
+    d = kc.FlashExtDims(H=1, H_kv=1, D=D, N=N, T=0, causal=1, k_row=128, v_row=128)
+    assert kc.flash_ext_part_bytes(d) == 0
+    kc.launch("flash_ext_f16", kc.FlashExtArgs(q=q.ptr, k=q.ptr, v=q.ptr, out=out.ptr, lse=lse.ptr, d=d, scale=0.1))
+    assert np.isneginf(lse.download(np.float32, N)).all()
+    for at in (0, N // 2, N - 1000):
+        assert (out.download(np.float32, 1000 * D, 4 * at * D) == 0).all()
+    for x in (q, out, lse):
+        x.free()
+
+
 @CACHES
 @pytest.mark.parametrize("N,T", [(1, 150), (5, 200), (70, 200), (140, 260), (700, 705)])
 def test_what_is_not_seen_does_not_reach_the_result(q4, N, T):
@@ -332,6 +346,28 @@ def test_graph_replays(q4, N):
         for x in (out, part, *b.values()):
             x.free()
     kc.call("kcStreamDestroy", s)
+
+
+def test_two_streams_at_once():
+    """Calls under way together, each with a workspace of its own."""
+    cases = [Case(q4, 8, 2, 128, N, T, seed=n) for n, (q4, N, T) in enumerate([(True, 1, 9000), (False, 700, 900), (False, 1, 9000), (True, 700, 900)])]
+    want = [c.attend()[0] for c in cases]
+    made = []
+    for c in cases:
+        s = C.c_void_p()
+        kc.call("kcStreamCreate", C.byref(s))
+        b, d = c.upload(), c.dims()
+        out, part = kc.Buffer(want[len(made)].nbytes), kc.Buffer(kc.flash_ext_part_bytes(d) + 4)
+        made.append((s, b, out, part, kc.FlashExtArgs(v=b["v"].ptr, out=out.ptr, part=part.ptr, **c.shape_args(b, d))))
+    for _ in range(3):
+        for c, (s, _, _, _, args) in zip(cases, made):
+            kc.launch(c.name("flash_ext"), args, s)
+    kc.synchronize()
+    for w, (s, b, out, part, _) in zip(want, made):
+        assert np.array_equal(out.download(np.float32).reshape(w.shape), w)
+        kc.call("kcStreamDestroy", s)
+        for x in (out, part, *b.values()):
+            x.free()
 
 
 def test_one_result_for_every_run():
