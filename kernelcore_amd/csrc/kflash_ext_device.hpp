@@ -466,6 +466,16 @@ struct MaskWords {
     uint32_t w[8];
     __device__ __forceinline__ void load(const unsigned short* mrow, int t, int h, int T) {
         const int words = (T + 1) / 2;
+        if ((t + 1) * 16 <= words) {  // (the same for the wavefront)
+            const uint32_t* at = reinterpret_cast<const uint32_t*>(mrow) + t * 16 + 2 * h;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const u2 two = *reinterpret_cast<const __attribute__((aligned(4))) u2*>(at + 4 * g);
+                w[2 * g] = two[0];
+                w[2 * g + 1] = two[1];
+            }
+            return;
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
