@@ -337,11 +337,11 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
             if (in < i1) store(stepOf(in), lds + ((it + 1) & 1) * G::Buf, wildAt + 2 * sn);
             if (inn < i1) fetch(stepOf(inn));
         };
-        if (ks == 1) stage();
         MaskWords mk;
         if constexpr (SHAPED) {
             if (mrow && work) mk.load(mrow, t * (TK / 32) + ks, h, a.T);
         }
+        if (ks == 1) stage();
         float x[16];
         if (work) keyScores<D, Q4>(cur + ks * 32 * G::KRow, cur + G::oScale + ks * NB * 64, j, h, qh, ql, x);
         if (work) {
