@@ -1081,7 +1081,8 @@ int launchFlashExt(bool q4, const kcFlashExtArgs& a, hipStream_t s) {
     p.lse = a.lse;
     p.part = a.part;
     p.splits = plan.splits;
-    const bool shaped = a.mask || a.kpos || a.kdoc || a.slopes || a.softcap > 0.0f;
+    // (positions of queries too: the unshaped kernels take what their rows see from pos0)
+    const bool shaped = a.mask || a.qpos || a.kpos || a.kdoc || a.slopes || a.softcap > 0.0f;
     switch (a.d.D) {
         case 64: return runD<64>(q4, shaped, p, plan, s);
         case 128: return runD<128>(q4, shaped, p, plan, s);

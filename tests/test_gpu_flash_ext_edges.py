@@ -1,0 +1,40 @@
+"""flash_ext_* and attn_weights_* where their definition is easily missed, against plain forms in 64 bits (tests/kvcache.py)."""
+import numpy as np
+import pytest
+
+import kernelcore_amd as kc
+from tests.kvcache import Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def runtime():
+    kc.init()
+    yield
+    kc.synchronize()
+
+
+CACHES = pytest.mark.parametrize("q4", [False, True], ids=["f16", "q4_0"])
+# one row tile and several on the few-rows kernel, then the many-rows kernel, of each head size
+ROWS = [(8, 2, 128, 1, 2000), (6, 2, 64, 5, 700), (4, 2, 256, 3, 333), (8, 2, 128, 60, 330), (32, 32, 64, 290, 450), (16, 16, 128, 300, 421),
+        (16, 16, 256, 260, 501)]
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", ROWS)
+@pytest.mark.parametrize("how", ["last", "ascending", "shuffled", "early", "outside", "prefix"])
+def test_query_positions_alone(q4, H, K, D, N, T, how):
+    """qpos stands in for pos0 + i, whatever pos0 is, where nothing else shapes the scores."""
+    print(f"flash_ext q4={q4} H={H}/{K} D={D} N={N} T={T} {how}", flush=True)
+    r = np.random.default_rng([N, T])
+    spread = np.sort(r.integers(0, T, N))
+    qpos, pos0 = {"last": (np.full(N, T - 1), 0), "ascending": (spread, 0), "shuffled": (r.permutation(spread), 3), "early": (spread // 3, T),
+                  "outside": (np.where(np.arange(N) % 2 == 0, -1 - spread, T + spread), 0),  # (a negative one sees nothing)
+                  "prefix": (spread // 2, T)}[how]
+    c = Case(q4, H, K, D, N, T, qpos=qpos.astype(np.int32), pos0=pos0, prefix=T // 2 + 1 if how == "prefix" else 0)
+    _, sums = c.check()
+    if how in ("last", "outside"):  # and the weights of the same call
+        lse = c.expected()[2].astype(np.float32)
+        want, bound = c.expected_weights(lse, None, 0.0)
+        assert (np.abs(c.weights(lse) - want) <= bound).all()
