@@ -23,8 +23,8 @@ struct FxParams {
     float* part;
     const float* w_in;  // attn_weights
     float* w;
-    long long k_row, k_head, v_row, v_head;
-    int H, H_kv, G, N, T, q_tok, q_head, m_row2, key_row, pos0, causal, prefix, rows;
+    long long k_row, k_head, v_row, v_head, m_row2;  // (m_row2: fp16 values between mask rows, past 32 bits for rows 4 GiB apart)
+    int H, H_kv, G, N, T, q_tok, q_head, key_row, pos0, causal, prefix, rows;
     int splits;  // key ranges
     int w_row;
     float scale, softcap, decay;
@@ -103,7 +103,7 @@ inline FxParams fxParams(const kcFlashExtDims& d, const float* q, const void* k,
     p.T = d.T;
     p.q_tok = d.q_tok;
     p.q_head = d.q_head;
-    p.m_row2 = 2 * d.m_row;
+    p.m_row2 = 2ll * d.m_row;
     p.key_row = d.key_row;
     p.pos0 = d.pos0;
     p.causal = d.causal;

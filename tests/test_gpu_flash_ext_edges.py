@@ -38,3 +38,28 @@ def test_query_positions_alone(q4, H, K, D, N, T, how):
         lse = c.expected()[2].astype(np.float32)
         want, bound = c.expected_weights(lse, None, 0.0)
         assert (np.abs(c.weights(lse) - want) <= bound).all()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,T", [(4, 2, 64, 91), (8, 2, 128, 5000), (256, 2, 64, 8300)])
+def test_mask_rows_far_apart(q4, H, K, D, T):
+    """Mask rows 4 GiB apart, two of them, against packed ones: few rows in one range and in several, many rows."""
+    r = np.random.default_rng(T)
+    m = r.standard_normal((2, T + T % 2)).astype(np.float16)
+    m[r.random(m.shape) < 0.4] = -np.inf
+    c = Case(q4, H, K, D, 2, T, causal=0, mask=m)
+    want, lse = c.attend()
+    w_want = c.weights(lse)
+    step = 4 << 30
+    far = kc.Buffer(step + m[0].nbytes)
+    for i in range(2):
+        far.upload(m[i], i * step)
+    b, d = c.upload(), c.dims(m_row=step // 4)
+    out, part, w, bl = kc.Buffer(want.nbytes), kc.Buffer(kc.flash_ext_part_bytes(d) + 4), kc.Buffer(w_want.nbytes), kc.Buffer.of(lse)
+    shape = dict(c.shape_args(b, d), mask=far.ptr)
+    kc.launch(c.name("flash_ext"), kc.FlashExtArgs(v=b["v"].ptr, out=out.ptr, part=part.ptr, **shape))
+    assert np.array_equal(out.download(np.float32).reshape(want.shape), want)
+    kc.launch(c.name("attn_weights"), kc.AttnWeightsArgs(lse=bl.ptr, w=w.ptr, w_row=T, **shape))
+    assert np.array_equal(w.download(np.float32).reshape(w_want.shape), w_want)
+    for x in (far, out, part, w, bl, *b.values()):
+        x.free()
