@@ -174,9 +174,29 @@ __device__ __forceinline__ Shape shapeOf(const FxParams& a) {
     return s;
 }
 // x[v] = cap log2 e tanh(x[v] k), k = score factor / cap. Two relative minimax fits of tanh(y) / y in y^2: a polynomial for |y| <= 3/4
-// (3e-8), taken where all of a wavefront's scores are that small (they mostly are: caps lie well above the scores), else a
-// quotient for |y| <= 9 (2e-8; beyond, tanh is 1 within 3e-8). A form through exp would lose the small arguments' last bits.
-// NaN stays NaN.
+// (3e-8) and above that a quotient for |y| <= 9 (2e-8; beyond, tanh is 1 within 3e-8). A score's own size decides between them, so
+// that no other key or query reaches its bits (one form for a wavefront, by its largest score, would let them); the quotient is
+// branched around where no lane has use for it (mostly: caps lie well above the scores. 2048 tokens, 24 heads, cap 30: 89 us; cap
+// 4, where a score in 400 takes it: 101). A form through exp would lose the small arguments' last bits. NaN stays NaN.
+__device__ __forceinline__ float smallTanh(float y, const Shape& s) {  // over y
+    const float u = y * y;
+    float r = fmaf(u, s.p5[5], s.p5[4]);
+#pragma unroll
+    for (int i = 3; i >= 0; --i) r = fmaf(u, r, s.p5[i]);
+    return r;
+}
+__device__ __forceinline__ float largeTanh(float x, const Shape& s) {
+    const float y = __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 9.0f), -9.0f);
+    const float u = y * y;
+    float p = fmaf(u, s.p[4], s.p[3]), q = fmaf(u, s.q[3], s.q[2]);
+    p = fmaf(u, p, s.p[2]);
+    q = fmaf(u, q, s.q[1]);
+    p = fmaf(u, p, s.p[1]);
+    q = fmaf(u, q, s.q[0]);
+    p = fmaf(u, p, s.p[0]);
+    q = fmaf(u, q, 1.0f);
+    return y * p * __builtin_amdgcn_rcpf(q);
+}
 template <int N>
 __device__ __forceinline__ void capScores(float (&x)[N], float k, const Shape& s) {
     float top = 0.0f;
@@ -185,31 +205,24 @@ __device__ __forceinline__ void capScores(float (&x)[N], float k, const Shape& s
         x[v] *= k;
         top = fmaxf(top, fabsf(x[v]));
     }
-    if (!__any(top > 0.75f)) {
+    const bool some = __any(top > 0.75f);
 #pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const float u = x[v] * x[v];
-            float r = fmaf(u, s.p5[5], s.p5[4]);
+    for (int v = 0; v < N; v += 4) {  // (four at a time are enough to fill the unit; all at once take registers)
+        float r[4], most = 0.0f;
 #pragma unroll
-            for (int i = 3; i >= 0; --i) r = fmaf(u, r, s.p5[i]);
-            x[v] *= r;
-            if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time are enough to fill the unit; all at once take registers)
+        for (int e = 0; e < 4; ++e) r[e] = x[v + e] * smallTanh(x[v + e], s);
+        if (some) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[v + e]));
+            if (N == 4 || __any(most > 0.75f)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!(fabsf(x[v + e]) <= 0.75f)) r[e] = largeTanh(x[v + e], s);
+            }
         }
-    } else {
 #pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const float y = __builtin_elementwise_maximum(__builtin_elementwise_minimum(x[v], 9.0f), -9.0f);
-            const float u = y * y;
-            float p = fmaf(u, s.p[4], s.p[3]), q = fmaf(u, s.q[3], s.q[2]);
-            p = fmaf(u, p, s.p[2]);
-            q = fmaf(u, q, s.q[1]);
-            p = fmaf(u, p, s.p[1]);
-            q = fmaf(u, q, s.q[0]);
-            p = fmaf(u, p, s.p[0]);
-            q = fmaf(u, q, 1.0f);
-            x[v] = y * p * __builtin_amdgcn_rcpf(q);
-            if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int e = 0; e < 4; ++e) x[v + e] = r[e];
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 

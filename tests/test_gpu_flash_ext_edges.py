@@ -63,3 +63,51 @@ def test_mask_rows_far_apart(q4, H, K, D, T):
     assert np.array_equal(w.download(np.float32).reshape(w_want.shape), w_want)
     for x in (far, out, part, w, bl, *b.values()):
         x.free()
+
+
+def enlarge(c, name, at, head, factor):
+    """The key or value rows `at` of a KV head, multiplied by a power of two."""
+    a = getattr(c, name)
+    if c.q4:
+        d = a.reshape(c.T, c.K, -1, 18)[at, head, :, :2]
+        a.reshape(c.T, c.K, -1, 18)[at, head, :, :2] = (np.ascontiguousarray(d).view(np.float16) * np.float16(factor)).view(np.uint8)
+    else:
+        a[at, head] *= np.float16(factor)
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", ROWS)
+def test_a_cap_keeps_rows_and_keys_apart(q4, H, K, D, N, T):
+    """Under a cap a score's bits depend on its own query and key: not on keys that the query does not see, nor on other queries,
+    however large (their tanh takes another form)."""
+    r = np.random.default_rng(N)
+    c = Case(q4, H, K, D, N, T, cap=20.0)
+    at, few = T - max(1, N // 2), N == 1
+    if few:  # hidden by a mask
+        at = T // 2
+        c.mask = np.zeros((1, T + T % 2), np.float16)
+        c.mask[0, at] = -np.inf
+    clean, sums = c.check()
+    lse = c.expected()[2].astype(np.float32)
+    weights = c.weights(lse)
+    enlarge(c, "k", at, 0, 1024)
+    got, got_sums = c.check()
+    hidden = np.arange(N) + T - N < at if not few else np.array([True])
+    assert hidden.any()
+    assert np.array_equal(got[hidden], clean[hidden]) and np.array_equal(got_sums[hidden], sums[hidden])
+    others = np.arange(T) != at
+    assert np.array_equal(c.weights(lse)[:, others], weights[:, others])
+    if N > 1:
+        c = Case(q4, H, K, D, N, T, cap=20.0)
+        c.q[N // 2] *= 1024
+        got, got_sums = c.check()
+        rest = np.arange(N) != N // 2
+        assert np.array_equal(got[rest], clean[rest]) and np.array_equal(got_sums[rest], sums[rest])
+
+
+@CACHES
+@pytest.mark.parametrize("spread", [1.0, 8.0])
+def test_caps_among_the_scores(q4, spread):
+    """Scores on both sides of the border between the forms of tanh."""
+    for N, T in ((1, 500), (40, 300), (1100, 200)):
+        Case(q4, 8, 2, 128, N, T, cap=2.0, spread=spread).check()
