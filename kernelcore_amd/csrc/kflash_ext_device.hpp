@@ -177,7 +177,7 @@ __device__ __forceinline__ Shape shapeOf(const FxParams& a) {
 // (3e-8) and above that a quotient for |y| <= 9 (2e-8; beyond, tanh is 1 within 3e-8). A score's own size decides between them, so
 // that no other key or query reaches its bits (one form for a wavefront, by its largest score, would let them); the quotient is
 // branched around where no lane has use for it (mostly: caps lie well above the scores. 2048 tokens, 24 heads, cap 30: 89 us; cap
-// 4, where a score in 400 takes it: 101). A form through exp would lose the small arguments' last bits. NaN stays NaN.
+// 4, where a score in 400 takes it: 100). A form through exp would lose the small arguments' last bits. NaN stays NaN.
 __device__ __forceinline__ float smallTanh(float y, const Shape& s) {  // over y
     const float u = y * y;
     float r = fmaf(u, s.p5[5], s.p5[4]);
@@ -205,24 +205,20 @@ __device__ __forceinline__ void capScores(float (&x)[N], float k, const Shape& s
         x[v] *= k;
         top = fmaxf(top, fabsf(x[v]));
     }
-    const bool some = __any(top > 0.75f);
+    if (!__any(top > 0.75f)) {
 #pragma unroll
-    for (int v = 0; v < N; v += 4) {  // (four at a time are enough to fill the unit; all at once take registers)
-        float r[4], most = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = x[v + e] * smallTanh(x[v + e], s);
-        if (some) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[v + e]));
-            if (N == 4 || __any(most > 0.75f)) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!(fabsf(x[v + e]) <= 0.75f)) r[e] = largeTanh(x[v + e], s);
-            }
+        for (int v = 0; v < N; ++v) {
+            x[v] *= smallTanh(x[v], s);
+            if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time are enough to fill the unit; all at once take registers)
         }
+        return;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[v + e] = r[e];
-        __builtin_amdgcn_sched_barrier(0);
+    for (int v = 0; v < N; ++v) {
+        float r = x[v] * smallTanh(x[v], s);
+        if (!(fabsf(x[v]) <= 0.75f)) r = largeTanh(x[v], s);
+        x[v] = r;
+        if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
