@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
         if (work) {
             const int wildBits = wildAt[2 * slot + ks];
             const int* kp = reinterpret_cast<const int*>(cur + G::oMeta) + 32 * ks + 4 * h;
-            if constexpr (SHAPED) shapeScores(x, c, shape, row, meta ? kp : nullptr, k0 + 4 * h, mrow ? &mk : nullptr);
+            if constexpr (SHAPED) shapeScores(x, c, shape, row, meta ? kp : nullptr, k0 + 4 * h, mrow != nullptr, mk);
             if (!full) {
                 if (meta) {
                     hideKeys(x, row, kp, kp + TK);

@@ -501,9 +501,10 @@ __device__ __forceinline__ float addMask(float x, uint32_t bits) {
 }
 
 // Sums of products into shaped scores in base 2. c: the factor of the row's scores; kp: the keys' positions where they are not the
-// tile's own (LDS, in groups of four at 8 g + 4 h), key0 the first of the lane's; mk the mask's values, null without.
+// tile's own (LDS, in groups of four at 8 g + 4 h), key0 the first of the lane's; mk the mask's values where there is one (a
+// pointer to them, null without, would put them into memory).
 __device__ __forceinline__ void shapeScores(float (&x)[16], float c, const Shape& shape, const Row& row, const int* kp, int key0,
-                                            const MaskWords* mk) {
+                                            bool masked, const MaskWords& mk) {
     if (shape.inv_cap > 0.0f) {
         capScores(x, c * shape.inv_cap, shape);
     } else {
@@ -523,9 +524,9 @@ __device__ __forceinline__ void shapeScores(float (&x)[16], float c, const Shape
             x[4 * g + 3] = fmaf(slope, fabsf((float)(row.pos - p.w)), x[4 * g + 3]);
         }
     }
-    if (mk) {
+    if (masked) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) x[v] = addMask(x[v], (v & 1) ? mk->w[v >> 1] >> 16 : mk->w[v >> 1] & 0xFFFFu);
+        for (int v = 0; v < 16; ++v) x[v] = addMask(x[v], (v & 1) ? mk.w[v >> 1] >> 16 : mk.w[v >> 1] & 0xFFFFu);
     }
 }
 
