@@ -330,7 +330,8 @@ typedef struct kcGetRowsQ40Args {
  * qpos may be null: token i is at pos0 + i; kpos may be null: row j is position j. kpos and kdoc hold T
  * values, for each KV head its own (key_row ints apart) or one list for all (key_row 0). Positions are
  * below 2^31 - 1. mask: ggml's f16 mask, rows m_row 32-bit words apart, of which (T + 1) / 2 are read. What a
- * key holds that a query does not see (NaN and infinities too) does not reach that query's result. */
+ * key holds that a query does not see (NaN and infinities too) does not reach that query's result; what it sees counts
+ * as above: a score of -infinity has weight 0, one of +infinity or NaN makes the query's out and lse NaN. */
 typedef struct kcFlashExtDims {
     int H;
     int H_kv;
@@ -347,7 +348,7 @@ typedef struct kcFlashExtDims {
     long long k_row, k_head, v_row, v_head; /* bytes */
 } kcFlashExtDims;
 /* flash_ext_f16 / flash_ext_q4_0: out[N][H][D] = sum_j softmax_j(score) v_j over the seen keys, for single
- * tokens and for prompts; a query that sees none gets zeros. lse (may be null): [N][H], the natural
+ * tokens and for prompts; a query that sees none (or only scores of -infinity) gets zeros. lse (may be null): [N][H], the natural
  * logarithm of the sum of exp(score), -infinity for such a query. part: kcFlashExtPartBytes bytes of
  * workspace, which calls that may overlap must not share; null where that is 0. (Ask for each call's sizes: fewer
  * tokens or positions may need more; a smaller part is refused.) */

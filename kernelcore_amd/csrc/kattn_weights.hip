@@ -20,6 +20,21 @@ namespace {
 
 using namespace fx;
 
+// What the rows gave a key whose sum came out NaN, from the definition, by a wavefront.
+template <int D, bool Q4>
+__device__ __forceinline__ void writePlainWeight(int kvh, int key, int lane) {
+    const FxParams a = paramsAgain();
+    float s = 0.0f;
+    for (int r0 = 0; r0 < a.rows; r0 += 64) {
+        const Row row = rowOf(a, kvh, r0 + lane);
+        const float lse = a.lse[(size_t)row.token * a.H + row.head];
+        if (row.live && lse != -INFINITY) s += expf(plainScore<D, Q4>(a, kvh, row, key) - lse);
+    }
+    s = waveSumF(s);
+    const size_t at = (size_t)kvh * a.w_row + key;
+    if (lane == 0) a.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], s) : s;
+}
+
 template <int D, bool Q4>
 struct WGeo {
     static constexpr int NB = D / 32;
@@ -35,6 +50,7 @@ struct WGeo {
 // cost the plain one 5%).
 template <int RW>
 constexpr int kWaves = RW > 4 ? RW : 4;
+constexpr int kWalk = 256;  // the most steps of a walk
 template <int D, bool Q4, int RW, int TP, bool META>
 __global__ __launch_bounds__(64 * kWaves<RW>, D == 256 && RW == 1 && !Q4 ? 1 : 2) void attn_weights_kernel(FxParams a) {
     using G = WGeo<D, Q4>;
@@ -43,6 +59,7 @@ __global__ __launch_bounds__(64 * kWaves<RW>, D == 256 && RW == 1 && !Q4 ? 1 : 2
     __shared__ float part[W][TP][32];
     __shared__ float4 rows4[W][32];  // factor of the sums (base 2 unless capped), lse (base 2), slope, -
     __shared__ int4 rows4i[W][32];   // limit, position, document, token
+    __shared__ unsigned long long lost[RW < 4 ? kWalk : 1][(KT + 1) / 2];  // a step's keys whose sums are NaN
     char* lds = reinterpret_cast<char*>(lds4);
     const int kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -87,7 +104,7 @@ __global__ __launch_bounds__(64 * kWaves<RW>, D == 256 && RW == 1 && !Q4 ? 1 : 2
                 h8* dst = reinterpret_cast<h8*>(tile + (key & 31) * kKeyRow<D> + 64 * b);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) dst[e] = code[e];
-                reinterpret_cast<float*>(tile + G::oS)[b * 32 + (key & 31)] = halfBits(sc[n]);
+                reinterpret_cast<float*>(tile + G::oS)[b * 32 + (key & 31)] = finiteOrNaN(halfBits(sc[n]));
             } else {
                 *reinterpret_cast<u4*>(tile + (key & 31) * kKeyRow<D> + 16 * b) = raw[n];
             }
@@ -126,7 +143,8 @@ __global__ __launch_bounds__(64 * kWaves<RW>, D == 256 && RW == 1 && !Q4 ? 1 : 2
         waveLds();
     };
     const int tiles = a.T / 32 + (a.T % 32 != 0);
-    int t0 = blockIdx.x * KT;
+    int t0 = blockIdx.x * KT, step = 0;
+    bool some = false;
     load(t0);
     if (RW < 4 && r0 < a.rows) {  // (the only one)
         limits();
@@ -247,19 +265,32 @@ __global__ __launch_bounds__(64 * kWaves<RW>, D == 256 && RW == 1 && !Q4 ? 1 : 2
             if (h == 0) part[wave][p][j] = acc[p];
         }
         __syncthreads();
-        if (tid < 32 * KT) {
+        if (wave < (KT + 1) / 2) {
             const int g = tid >> 5, w0 = g / TP * RW;
             const long long key = (long long)(t0 + g) * 32 + (tid & 31);
-            if (key < a.T) {
-                float s = part[w0][g % TP][tid & 31];
+            const bool live = g < KT && key < a.T;
+            float s = 0.0f;
+            if (live) {
 #pragma unroll
-                for (int x = 1; x < RW; ++x) s += part[w0 + x][g % TP][tid & 31];
+                for (int x = 0; x < RW; ++x) s += part[w0 + x][g % TP][tid & 31];
+            }
+            const unsigned long long nan = __ballot(s != s);
+            if (lane == 0) lost[step][wave] = nan;
+            some |= nan != 0;
+            if (live && s == s) {
                 const size_t at = (size_t)kvh * a.w_row + key;
                 a.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], s) : s;
             }
         }
+        ++step;
         if (!more) break;
         t0 = next;
+    }
+    if (__builtin_expect(some, 0)) {  // (each wavefront's own)
+        for (int i = 0; i < step; ++i) {
+            for (unsigned long long nan = lost[i][wave]; nan; nan &= nan - 1)
+                writePlainWeight<D, Q4>(kvh, (int)((blockIdx.x + i * gridDim.x) * KT + 2 * wave) * 32 + __builtin_ctzll(nan), lane);
+        }
     }
 }
 
@@ -270,7 +301,7 @@ int runMeta(const FxParams& p, hipStream_t s) {
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds), "attn_weights: LDS size");
     if (ok) return ok;
     const int tiles = p.T / 32 + (p.T % 32 != 0), all = (tiles + kt - 1) / kt;
-    const int grid = RW < 4 ? std::min(all, std::max(1, (512 + p.H_kv - 1) / p.H_kv)) : all;  // (two workgroups to a compute unit)
+    const int grid = RW < 4 ? std::min(all, std::max((all + kWalk - 1) / kWalk, (512 + p.H_kv - 1) / p.H_kv)) : all;  // (two workgroups to a compute unit)
     hipLaunchKernelGGL((attn_weights_kernel<D, Q4, RW, TP, META>), dim3(grid, p.H_kv), dim3(64 * W), lds, s, p);
     return fromHip(hipGetLastError(), "attn_weights");
 }

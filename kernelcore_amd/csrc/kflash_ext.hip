@@ -25,6 +25,28 @@ using namespace fx;
 // (x - m + 11 is what is exponentiated; l and o carry the factor until the end.)
 constexpr float kLag = 4.0f, kPBits = 11.0f, kPInv = 1.0f / 2048.0f;
 
+// Row r of a workgroup's range, whose sums came out NaN, from the definition: written as the kernels write their rows, by a wavefront.
+template <int D, bool Q4, int TK>
+__device__ __forceinline__ void writePlainRow(int kvh, int r, int sp, int lane) {
+    const FxParams a = paramsAgain();
+    float m, l, o[D / 64];
+    plainRow<D, Q4, TK>(a, kvh, r, sp, lane, m, l, o);
+    const int token = r / a.G, head = kvh * a.G + (r - token * a.G);
+    const size_t at = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
+    const bool whole = a.splits == 1;
+    float* dst = whole ? a.out + ((size_t)token * a.H + head) * D : a.part + at * D;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) dst[lane + 64 * e] = !whole ? o[e] : l == 0.0f ? 0.0f : o[e] / l;
+    if (lane) return;
+    if (!whole) {
+        float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * at;
+        ml[0] = m;
+        ml[1] = l;
+    } else if (a.lse) {
+        a.lse[(size_t)token * a.H + head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l));
+    }
+}
+
 // The value at dd of a V row that the matrix products left out (0 where they took it).
 template <bool Q4>
 __device__ float wildValue(const char* row, int dd) {
@@ -254,7 +276,8 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                     *reinterpret_cast<h8*>(pk) = lo;
                     *reinterpret_cast<h8*>(pk + 32) = hi;
                     if (!(part & 1))
-                        reinterpret_cast<unsigned short*>(buf + G::oScale)[(key >> 5) * NB * 32 + scaleAt(part >> 1, key & 31)] = (unsigned short)ksc[n];
+                        reinterpret_cast<_Float16*>(buf + G::oScale)[(key >> 5) * NB * 32 + scaleAt(part >> 1, key & 31)] =
+                            finiteOrNaN(__builtin_bit_cast(_Float16, (unsigned short)ksc[n]));
                     uint32_t s = vsc[n] & 0xFFFFu;
                     if (wildScale(s)) {
                         s = 0;
@@ -473,30 +496,33 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
                 }
             }
     }
-    if (!row.live) return;
-    float* dst;
-    float f;
-    if (a.splits == 1) {
-        dst = a.out + ((size_t)row.token * a.H + row.head) * D;
-        f = l == 0.0f ? 0.0f : 1.0f / l;
-        if (a.lse && h == 0 && ks == 0) a.lse[(size_t)row.token * a.H + row.head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l * kPInv));
-    } else {
-        const size_t at = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
-        dst = a.part + at * D;
-        f = kPInv;
-        if (h == 0 && ks == 0) {
-            float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * at;
-            ml[0] = m;
-            ml[1] = l * kPInv;
+    if (row.live && l == l) {
+        float* dst;
+        float f;
+        if (a.splits == 1) {
+            dst = a.out + ((size_t)row.token * a.H + row.head) * D;
+            f = l == 0.0f ? 0.0f : 1.0f / l;
+            if (a.lse && h == 0 && ks == 0) a.lse[(size_t)row.token * a.H + row.head] = l == 0.0f ? -INFINITY : fmaf(m, kLn2, logf(l * kPInv));
+        } else {
+            const size_t at = ((size_t)sp * a.H_kv + kvh) * a.rows + r;
+            dst = a.part + at * D;
+            f = kPInv;
+            if (h == 0 && ks == 0) {
+                float* ml = a.part + (size_t)a.splits * a.H_kv * a.rows * D + 2 * at;
+                ml[0] = m;
+                ml[1] = l * kPInv;
+            }
         }
+#pragma unroll
+        for (int d = 0; d < OB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 y = {o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f};
+                *reinterpret_cast<f4a4*>(dst + 32 * (d0 + d) + 8 * g + 4 * h) = y;
+            }
     }
-#pragma unroll
-    for (int d = 0; d < OB; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 y = {o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f};
-            *reinterpret_cast<f4a4*>(dst + 32 * (d0 + d) + 8 * g + 4 * h) = y;
-        }
+    unsigned again = (unsigned)__ballot(row.live && l != l && (G::KS == 1 || (j & 1) == ks));  // (the sets share them)
+    for (; __builtin_expect(again != 0, 0); again &= again - 1) writePlainRow<D, Q4, TK>(kvh, r0 + __builtin_ctz(again), sp, lane);
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
@@ -668,7 +694,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             if constexpr (Q4) {
                 *reinterpret_cast<u4*>(mine + key * G::Row + 16 * part) = kr[n];
                 *reinterpret_cast<u4*>(mine + G::oV + key * G::Row + 16 * part) = vr[n];
-                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = halfBits(kscale[n] & 0xFFFFu);
+                reinterpret_cast<float*>(mine + G::oS)[part * 64 + key] = finiteOrNaN(halfBits(kscale[n] & 0xFFFFu));
                 uint32_t s = t * TK + key < a.T ? vscale[n] & 0xFFFFu : 0u;
                 if (wildScale(s)) {
                     s = 0;
@@ -898,6 +924,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
         }
     }
     __syncthreads();
+    bool lost = false;
     for (int x = tid; x < rows * (D / 4); x += 256) {  // four values each
         const int r = x / (D / 4), at = x % (D / 4) * 4;
         float mw[4], lw[4], M = -INFINITY, L = 0.0f;
@@ -918,6 +945,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = f != 0.0f ? fmaf(f, ow[w][e], y[e]) : y[e];
         }
+        lost |= L != L;
         float* dst;
         if (a.splits == 1) {
             const int token = (row0 + r) / a.G, head = kvh * a.G + (row0 + r - token * a.G);
@@ -940,6 +968,14 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             *reinterpret_cast<f2a4*>(to + 16) = f32x2{y[1], y[3]};
         } else {
             *reinterpret_cast<f4a4*>(dst + at) = y;
+        }
+    }
+    if (__builtin_expect(__any(lost), 0)) {  // of the rows that this wavefront has written
+        __threadfence();
+        for (int r = 0; r < rows; ++r) {
+            float L = 0.0f;
+            for (int w = 0; w < 4; ++w) L += jm[2 * ((w * NR) * 16 + r) + 1];
+            if (r * (D / 4) / 64 % 4 == wave && L != L) writePlainRow<D, Q4, TK>(kvh, row0 + r, sp, lane);
         }
     }
 }

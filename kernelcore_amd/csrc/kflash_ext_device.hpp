@@ -90,7 +90,8 @@ struct QScale {
 };
 __device__ __forceinline__ QScale qScale(float top, float scale) {
     const int shift = top > 0.0f && top < INFINITY ? 8 - __builtin_amdgcn_frexp_expf(top) : 0, first = min(shift, 126);
-    return {ldexpf(scale < 0.0f ? -1.0f : 1.0f, first), shift - first, ldexpf(fabsf(scale), -shift)};
+    // (a scale of 0 in q itself: times an infinite key it is NaN)
+    return {scale == 0.0f ? 0.0f : ldexpf(scale < 0.0f ? -1.0f : 1.0f, first), shift - first, ldexpf(fabsf(scale), -shift)};
 }
 // Two numbers as fp16 parts hi + lo. (x - hi in one instruction each; x must not come straight from a matrix instruction.)
 __device__ __forceinline__ void splitTwo(float x0, float x1, h2& hi, h2& lo) {
@@ -538,6 +539,100 @@ __device__ __forceinline__ void hideKeys(float (&x)[16], const Row& row, const i
         const int p[4] = {a.x, a.y, a.z, a.w}, d[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[4 * g + e] = p[e] <= row.limit && d[e] == row.doc ? x[4 * g + e] : -INFINITY;
+    }
+}
+
+// ---- keys and queries that hold an infinity or NaN
+// On the matrix cores such a number makes a row's sum infinite or NaN, but NaN also where the definition says infinity: an infinite key meets
+// a low part of q that is 0 or of the other sign. A sum that comes out infinite is right (of a 4-bit block, whose scale multiplies
+// the sum of its products, an infinite scale is replaced by NaN: finiteOrNaN). So the kernels run on as they are, and a row
+// (attn_weights: a position) whose sum of weights is NaN at the end is made again from the definition in plain f32 by a wavefront: at
+// the first such score where it is NaN by definition too (1000 tokens of NaN over 1024 positions, 32 heads of 128: 0.2 ms), else
+// slowly (every row to be made again: 2.4 ms; of one token over 65536 positions 0.5). Corrected within the loops, the scores
+// cost every call of many rows 2 to 8%.
+__device__ __forceinline__ float finiteOrNaN(float x) { return fmaf(x, 0.0f, x); }
+__device__ __forceinline__ _Float16 finiteOrNaN(_Float16 x) { return __builtin_elementwise_fma(x, (_Float16)0.0f, x); }
+
+// A kernel's parameters loaded again (it has no other arguments): a use of them that is hardly ever reached keeps no registers.
+__device__ __forceinline__ FxParams paramsAgain() {
+    auto p = (const __attribute__((address_space(4))) FxParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    FxParams a;
+    __builtin_memcpy(&a, (const FxParams*)p, sizeof a);
+    return a;
+}
+
+// The score of a row and a key; -infinity where the row does not see it.
+template <int D, bool Q4>
+__device__ __forceinline__ float plainScore(const FxParams& a, int kvh, const Row& row, int key) {
+    const size_t meta = (size_t)kvh * a.key_row + key;
+    const int pos = a.kpos ? a.kpos[meta] : key;
+    const uint32_t mask = a.mask ? a.mask[(size_t)row.token * a.m_row2 + key] : 0u;
+    if (pos < 0 || pos > row.limit || (a.kdoc && a.kdoc[meta] != row.doc) || mask == 0xFC00u) return -INFINITY;
+    const float* q = a.q + (size_t)row.token * a.q_tok + (size_t)row.head * a.q_head;
+    const char* k = a.k + (size_t)kvh * a.k_head + (size_t)key * a.k_row;
+    float s = 0.0f;
+    if constexpr (Q4) {
+#pragma unroll 1
+        for (int b = 0; b < D / 32; ++b, k += 18, q += 32) {
+            const float d = halfBits(loadHalf(k));
+#pragma unroll 4
+            for (int e = 0; e < 16; ++e) {
+                const int c = (unsigned char)k[2 + e];
+                s = fmaf(q[e] * a.scale, d * (float)((c & 15) - 8), s);
+                s = fmaf(q[e + 16] * a.scale, d * (float)((c >> 4) - 8), s);
+            }
+        }
+    } else {
+#pragma unroll 4
+        for (int d = 0; d < D; ++d) s = fmaf(q[d] * a.scale, halfBits(loadHalf(k + 2 * d)), s);
+    }
+    if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
+    if (a.slopes) s = fmaf(-row.slope, fabsf((float)(row.pos - pos)), s);
+    return a.mask ? s + halfBits(mask) : s;
+}
+
+// Row r over the tiles of TK keys sp, sp + splits, ..: values lane + 64 e of the sum of 2^(x - m) v to o, x the scores in base 2.
+template <int D, bool Q4, int TK>
+__device__ __forceinline__ void plainRow(const FxParams& a, int kvh, int r, int sp, int lane, float& m, float& l, float (&o)[D / 64]) {
+    const Row row = rowOf(a, kvh, r);
+    const char* vb = a.v + (size_t)kvh * a.v_head;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
+    for (long long k0 = (long long)sp * TK; k0 < a.T; k0 += (long long)a.splits * TK) {
+        const int key = (int)min(k0 + lane, (long long)a.T - 1);
+        const float x = lane < TK && k0 + lane < a.T ? plainScore<D, Q4>(a, kvh, row, key) * kLog2e : -INFINITY;
+        if (__any(!(x < INFINITY))) {  // infinity over infinity
+            l = NAN;
+            return;
+        }
+        const float top = fmaxf(m, waveMaxF(x));
+        if (top == -INFINITY) continue;
+        const float f = ex2(m - top), p = ex2(x - top);
+        m = top;
+        l = fmaf(l, f, waveSumF(p));
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[e] *= f;
+        for (unsigned long long left = __ballot(p != 0.0f); left; left &= left - 1) {
+            const int at = __builtin_ctzll(left);
+            const float pk = __shfl(p, at);
+            const char* v = vb + (size_t)(k0 + at) * a.v_row;
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) {
+                const int d = lane + 64 * e;
+                float y;
+                if constexpr (Q4) {
+                    const char* b = v + 18 * (d >> 5);
+                    const int c = (unsigned char)b[2 + (d & 15)];
+                    y = halfBits(loadHalf(b)) * (float)(((d & 16) ? c >> 4 : c & 15) - 8);
+                } else {
+                    y = halfBits(loadHalf(v + 2 * d));
+                }
+                o[e] = fmaf(pk, y, o[e]);
+            }
+        }
     }
 }
 

@@ -111,3 +111,92 @@ def test_caps_among_the_scores(q4, spread):
     """Scores on both sides of the border between the forms of tanh."""
     for N, T in ((1, 500), (40, 300), (1100, 200)):
         Case(q4, 8, 2, 128, N, T, cap=2.0, spread=spread).check()
+
+
+class Infinite(Case):
+    """Keys with infinities and NaN: a score of -infinity has weight 0, one of +infinity or NaN makes the query's result NaN."""
+
+    def scores(self):
+        x, seen, terms = super().scores()
+        return np.where(np.isneginf(x), -np.inf, x), seen & ~np.isneginf(x), np.where(np.isfinite(terms), terms, self.cap)
+
+    def check(self):
+        out, sums = self.attend()
+        x, seen, _ = self.scores()
+        lost = (seen & ~np.isfinite(x)).any(-1)
+        with np.errstate(invalid="ignore", over="ignore"):
+            want, bound, lse, lse_bound = self.expected()
+            lse32 = np.where(lost, 0.0, lse).astype(np.float32)
+            w_in = np.random.default_rng(1).random((self.K, self.T)).astype(np.float32)
+            w, w_bound = self.expected_weights(lse32, w_in, 0.5)
+        assert np.isnan(out[lost]).all() and np.isnan(sums[lost]).all()
+        kept = ~lost
+        assert (np.abs(out[kept] - want[kept]) <= bound[kept]).all()
+        assert (np.isneginf(sums[kept]) == np.isneginf(lse[kept])).all()
+        fin = kept & np.isfinite(lse)
+        assert (np.abs(sums[fin] - lse[fin]) <= lse_bound[fin]).all()
+        got = self.weights(lse32, w_in, 0.5)
+        assert (np.isnan(got) == np.isnan(w)).all()
+        plain = np.isfinite(w)
+        assert (np.abs(got[plain] - w[plain]) <= w_bound[plain]).all() and (np.isinf(got) == np.isinf(w)).all()
+        return lost
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", ROWS + [(32, 32, 64, 1, 2300), (32, 8, 128, 9, 4201), (16, 16, 256, 2, 4300)])  # (weights: walks over the keys)
+@pytest.mark.parametrize("cap", [0.0, 15.0])
+def test_infinities_and_nan_in_seen_keys(q4, H, K, D, N, T, cap):
+    print(f"flash_ext q4={q4} H={H}/{K} D={D} N={N} T={T} cap={cap}", flush=True)
+    r = np.random.default_rng([N, T])
+    c = Infinite(q4, H, K, D, N, T, cap=cap, causal=0)
+    # q of every token: the values that meet the infinity positive (whose low parts are 0 or negative for some) or, of KV head 0's
+    # first query head, too small beside the others to be fp16 numbers
+    at = 35
+    c.q[:, :, 32:64] = np.abs(c.q[:, :, 32:64])
+    c.q[:, 0, at] = 1e-30
+    rows = sorted(set([0, T // 3, T - 1]))
+    for j in rows:
+        if q4:  # every product of the block negative: codes below 8
+            b = c.k.reshape(T, K, -1, 18)[j]
+            b[:, 1, :2] = np.frombuffer(np.float16(np.inf).tobytes(), np.uint8)
+            b[:, 1, 2:] = r.integers(0, 8, (K, 16)) + 16 * r.integers(0, 8, (K, 16))
+        else:
+            c.k[j, :, at] = -np.inf
+    lost = c.check()
+    assert not lost.any()
+    j = rows[len(rows) // 2]
+    m = np.zeros((N, T + T % 2), np.float16)
+    m[N // 2:, j] = -np.inf
+    if N == 1:
+        m[:] = 0
+    c.mask = m
+    for bad in (np.inf, np.nan):
+        if q4:
+            b = c.k.reshape(T, K, -1, 18)[j]
+            b[K - 1, 0, :2] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
+            b[K - 1, 0, 2:] = np.arange(16) * 17  # (a code of 8: 0 times infinity)
+        else:
+            c.k[j, K - 1, 7] = bad
+        lost = c.check()
+        seen = np.arange(N) < N // 2 if N > 1 else np.ones(1, bool)
+        assert not lost[~seen].any() and (np.isinf(bad) or lost[seen][:, (K - 1) * H // K:].all())
+
+
+@CACHES
+def test_zero_times_an_infinity(q4):
+    """A zero of q that meets an infinity, and a scale of zero: NaN, for the queries that see the key."""
+    for N, T in ((1, 200), (40, 200), (1100, 200)):
+        c = Infinite(q4, 8, 2, 128, N, T)
+        c.q[:, 3, 40] = 0
+        if q4:
+            b = c.k.reshape(T, 2, -1, 18)[0, 0, 1]
+            b[:2] = np.frombuffer(np.float16(np.inf).tobytes(), np.uint8)
+            b[2:] = 0x11
+            c.q[:, :, 32:64] = np.abs(c.q[:, :, 32:64])
+        else:
+            c.q[:, :3, 40] = np.abs(c.q[:, :3, 40])
+            c.k[0, 0, 40] = -np.inf
+        lost = c.check()
+        assert lost[:, 3].all() and not lost[:, :3].any() and not lost[:, 4:].any()
+        c.scale = 0.0
+        assert c.check()[:, :4].all()
