@@ -321,7 +321,7 @@ typedef struct kcGetRowsQ40Args {
 
 /* Sizes and rules of flash_ext_* and attn_weights_*: N query tokens of H heads over T cached positions of
  * H_kv heads (query head h reads KV head h / (H / H_kv)), D = 64, 128 or 256 values a head, T below 2^31 - 1024.
- *   score(i, h, j) = scale q_ih . k_j; softcap > 0: softcap tanh(score / softcap);
+ *   score(i, h, j) = scale q_ih . k_j; softcap > 0 (from 2^-100 to 2^100; 0: none): softcap tanh(score / softcap);
  *                    - slopes[h] |qpos_i - kpos_j| where slopes is given; + mask[i][j] where mask is given
  * and key j is seen by query i when
  *   kpos_j >= 0 (a negative position marks an empty slot), and

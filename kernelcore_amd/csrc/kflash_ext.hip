@@ -769,7 +769,7 @@ __global__ __launch_bounds__(256, D == 256 || NR == 2 ? 1 : 2) void flash_ext_fe
             const float c2 = factor2(c[n]);
             if constexpr (SHAPED) {
                 if (shape.inv_cap > 0.0f) {
-                    capScores<U * 4>(x[n], c[n] * shape.inv_cap, shape);
+                    capScores<U * 4>(x[n], capFactor(c[n], shape), shape);
                 } else {
 #pragma unroll
                     for (int v = 0; v < U * 4; ++v) x[n][v] *= c2;

@@ -12,6 +12,7 @@
 // bits, so it is an fp16 value and an exact fp16 rest (a third matrix chain instead of a rounded value).
 #pragma once
 
+#include <cfloat>
 #include <climits>
 
 #include "kflash_ext.hpp"
@@ -174,6 +175,8 @@ __device__ __forceinline__ Shape shapeOf(const FxParams& a) {
     }
     return s;
 }
+// A row's k below, finite: a sum of 0 stays a score of 0 beside the smallest caps and the largest q.
+__device__ __forceinline__ float capFactor(float c, const Shape& s) { return fminf(c * s.inv_cap, FLT_MAX); }
 // x[v] = cap log2 e tanh(x[v] k), k = score factor / cap. Two relative minimax fits of tanh(y) / y in y^2: a polynomial for |y| <= 3/4
 // (3e-8) and above that a quotient for |y| <= 9 (2e-8; beyond, tanh is 1 within 3e-8). A score's own size decides between them, so
 // that no other key or query reaches its bits (one form for a wavefront, by its largest score, would let them); the quotient is
@@ -507,7 +510,7 @@ __device__ __forceinline__ float addMask(float x, uint32_t bits) {
 __device__ __forceinline__ void shapeScores(float (&x)[16], float c, const Shape& shape, const Row& row, const int* kp, int key0,
                                             bool masked, const MaskWords& mk) {
     if (shape.inv_cap > 0.0f) {
-        capScores(x, c * shape.inv_cap, shape);
+        capScores(x, capFactor(c, shape), shape);
     } else {
         const float c2 = factor2(c);
 #pragma unroll

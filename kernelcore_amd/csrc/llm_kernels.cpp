@@ -517,8 +517,9 @@ int fxCache(const kcFlashExtDims& d, bool q4, const void* p, int64_t row, int64_
 int fxInputs(const kcFlashExtDims& d, bool q4, const float* q, const void* k, const int* mask, const int* qpos, const int* kpos,
              const int* qdoc, const int* kdoc, const float* slopes, float scale, float softcap) {
     KC_TRY(fxShape(d));
-    if (!(scale == scale) || scale - scale != 0.0f || !(softcap >= 0.0f) || softcap - softcap != 0.0f)
-        return invalid("flash_ext: scale finite, softcap finite and not negative");
+    // (caps whose reciprocals and products with scores keep their bits in f32)
+    if (!(scale == scale) || scale - scale != 0.0f || !(softcap == 0.0f || (softcap >= 0x1p-100f && softcap <= 0x1p100f)))
+        return invalid("flash_ext: scale finite, softcap 0 or from 2^-100 to 2^100");
     if ((qdoc != nullptr) != (kdoc != nullptr)) return invalid("flash_ext: qdoc and kdoc are both given or both null");
     if (d.key_row && d.key_row < d.T && d.H_kv > 1) return invalid("flash_ext: key_row is 0 or at least T");
     if (!aligned(q, 4) || !aligned(mask, 4) || !aligned(qpos, 4) || !aligned(kpos, 4) || !aligned(qdoc, 4) || !aligned(kdoc, 4) ||

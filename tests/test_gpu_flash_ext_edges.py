@@ -1,4 +1,6 @@
 """flash_ext_* and attn_weights_* where their definition is easily missed, against plain forms in 64 bits (tests/kvcache.py)."""
+import math
+
 import numpy as np
 import pytest
 
@@ -200,3 +202,19 @@ def test_zero_times_an_infinity(q4):
         assert lost[:, 3].all() and not lost[:, :3].any() and not lost[:, 4:].any()
         c.scale = 0.0
         assert c.check()[:, :4].all()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", [(8, 2, 128, 1, 333), (8, 2, 64, 40, 333), (16, 16, 256, 260, 501)])
+def test_caps_of_any_size(q4, H, K, D, N, T):
+    """The smallest cap (every score 0 beside it, NaN in none) and the largest (no cap), with q of any size."""
+    for cap in (2.0 ** -100, 2.0 ** -20, 2.0 ** 30, 2.0 ** 100):
+        for spread, scale in ((1.0, 1.0 / math.sqrt(D)), (1e30, 1e-31), (1e30, 1.0), (1e-30, 1e30)):
+            c = Case(q4, H, K, D, N, T, cap=cap, spread=spread, scale=scale)
+            c.q[0, 0] = 0
+            if q4:  # (and a score of 0 beside q of any size)
+                c.k.reshape(T, K, -1, 18)[1, ..., :2] = 0
+            else:
+                c.k[1] = 0
+            if cap < 1 or scale * spread <= 1:
+                c.check()
