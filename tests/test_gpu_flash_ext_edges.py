@@ -218,3 +218,43 @@ def test_caps_of_any_size(q4, H, K, D, N, T):
                 c.k[1] = 0
             if cap < 1 or scale * spread <= 1:
                 c.check()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,N,T", [(8, 2, 12, 400), (16, 16, 60, 200), (8, 2, 40, 300), (16, 16, 90, 1000), (16, 16, 90, 2500)])
+@pytest.mark.parametrize("shape", ["plain", "cap_bias", "kept"])
+def test_weights_of_heads_of_256(q4, H, K, N, T, shape):
+    """Two, eight and four wavefronts to a key tile, four to four, with and without positions of the keys' own."""
+    r = np.random.default_rng(T)
+    kw = dict(cap=10.0, bias=True, prefix=T // 3) if shape == "cap_bias" else {}
+    if shape == "kept":
+        kpos = np.sort(r.choice(3 * T + 1, (K, T)), axis=1).astype(np.int32)
+        kpos[r.random((K, T)) < 0.2] = -1
+        kw = dict(kpos=kpos, pos0=2 * T, bias=True)
+    c = Case(q4, H, K, 256, N, T, **kw)
+    lse = c.expected()[2].astype(np.float32)
+    w_in = r.random((K, T)).astype(np.float32)
+    want, bound = c.expected_weights(lse, w_in, 0.75)
+    assert (np.abs(c.weights(lse, w_in, 0.75) - want) <= bound).all()
+
+
+@CACHES
+@pytest.mark.parametrize("H,K,D,N,T", [(4, 2, 256, 3, 200), (16, 16, 256, 260, 501), (6, 2, 64, 5, 200), (32, 32, 64, 290, 450)])
+def test_infinities_in_values(q4, H, K, D, N, T):
+    """An infinite or NaN value: just its own column (of a 4-bit cache, its block's), for the queries that see it."""
+    c = Case(q4, H, K, D, N, T)
+    clean, sums = c.attend()
+    at = T - N // 2 - 1
+    if q4:
+        c.v.reshape(T, K, -1, 18)[at, 1, 1, :2] = np.frombuffer(np.float16(-np.inf).tobytes(), np.uint8)
+        cols = np.arange(32, 64)
+    else:
+        c.v[at, 1, [1, D - 2]] = np.nan, np.inf
+        cols = np.array([1, D - 2])
+    got, got_sums = c.attend()
+    hidden = np.arange(N) + T - N < at
+    others = np.setdiff1d(np.arange(D), cols)
+    assert np.array_equal(got[hidden], clean[hidden]) and np.array_equal(got[..., others], clean[..., others]) and np.array_equal(got_sums, sums)
+    G = H // K
+    assert np.array_equal(got[:, :G], clean[:, :G]) and np.array_equal(got[:, 2 * G:], clean[:, 2 * G:])
+    assert not np.isfinite(got[~hidden][:, G:2 * G][..., cols]).any()
