@@ -297,7 +297,7 @@ typedef struct kcFlashDecodeArgs {
  * of largest magnitude in a block (the first of several) d = xm / -8, and value x gets the code
  * floor(x / d + 8.5), at most 15 (8 where d is 0), decided without rounding; d is then stored as fp16. A
  * block that holds an infinity or NaN reads back as NaN. An index outside [0, dst_rows) stores nothing;
- * of rows with the same index the last one is stored. The rest of dst stays as it is. */
+ * of rows with the same index the last one is stored. The rest of dst stays as it is. Up to 524280 rows. */
 typedef struct kcSetRowsQ40Args {
     const float* src;
     const int* idx; /* rows int64 values */
@@ -329,9 +329,10 @@ typedef struct kcGetRowsQ40Args {
  *   qdoc_i == kdoc_j where document numbers are given (both or neither).
  * qpos may be null: token i is at pos0 + i; kpos may be null: row j is position j. kpos and kdoc hold T
  * values, for each KV head its own (key_row ints apart) or one list for all (key_row 0). Positions are
- * below 2^31 - 1. mask: ggml's f16 mask, rows m_row 32-bit words apart, of which (T + 1) / 2 are read. What a
- * key holds that a query does not see (NaN and infinities too) does not reach that query's result; what it sees counts
- * as above: a score of -infinity has weight 0, one of +infinity or NaN makes the query's out and lse NaN. */
+ * below 2^31 - 1, and less than 2^31 apart where slopes are given. mask: ggml's f16 mask, rows m_row 32-bit words
+ * apart, of which (T + 1) / 2 are read. What a key holds that a query does not see (NaN and infinities too) does not
+ * reach that query's result; what it sees counts as above: a score of -infinity has weight 0, one of +infinity or
+ * NaN makes the query's out and lse NaN. */
 typedef struct kcFlashExtDims {
     int H;
     int H_kv;
@@ -348,8 +349,8 @@ typedef struct kcFlashExtDims {
     long long k_row, k_head, v_row, v_head; /* bytes */
 } kcFlashExtDims;
 /* flash_ext_f16 / flash_ext_q4_0: out[N][H][D] = sum_j softmax_j(score) v_j over the seen keys, for single
- * tokens and for prompts; a query that sees none (or only scores of -infinity) gets zeros. lse (may be null): [N][H], the natural
- * logarithm of the sum of exp(score), -infinity for such a query. part: kcFlashExtPartBytes bytes of
+ * tokens and for prompts; a query that sees none (or only scores of -infinity) gets zeros. lse (may be null):
+ * [N][H], the natural logarithm of the sum of exp(score), -infinity for such a query. part: kcFlashExtPartBytes bytes of
  * workspace, which calls that may overlap must not share; null where that is 0. (Ask for each call's sizes: fewer
  * tokens or positions may need more; a smaller part is refused.) */
 typedef struct kcFlashExtArgs {
@@ -407,8 +408,9 @@ typedef struct kcKvKeepArgs {
     int recent;
 } kcKvKeepArgs;
 /* kv_gather: dst row r of head g = src row keep[g][r] of head g, r < n_keep, for 1 to 4 planes (K, V, weights,
- * positions) in one launch; rows are `bytes` bytes, strides in bytes (all multiples of 2). Planes' sources and
- * destinations must not overlap. An index outside [0, T) leaves its dst row as it is. */
+ * positions) in one launch; rows are `bytes` bytes, strides in bytes (all multiples of 2). No destination row may
+ * overlap another, and a destination that overlaps a source is refused. An index outside [0, T) leaves its dst row
+ * as it is. */
 typedef struct kcKvPlane {
     const void* src;
     void* dst;

@@ -4,8 +4,9 @@
 // keys): lane (j, h) holds rows 8 (v / 4) + 4 h + v % 4 of key j, so a key's sum over the rows is a sum of registers and
 // nothing crosses lanes until the end. A workgroup stages key tiles, and its wavefronts share the rows (RW of them
 // to a tile). Sums in one order, no atomics.
-// A single token's call reads K once and is bound by that, or by a tile's latency (4099 fp16 positions, 8 KV heads of 128: 6.1 us); with
-// many rows the scaling of the sums and the exponentials bound it, and q, split anew for every 128 keys (64 tokens of 32 heads over
+// A single token's call reads K once. Over fp16 keys it is bound by that, or by a tile's latency (4099 positions, 8 KV heads of 128:
+// 6.1 us); over 4-bit ones by unpacking them and multiplying tiles of 32 rows of which four are there (131072 positions: 38 us,
+// 2 TB/s). With many rows the scaling of the sums and the exponentials bound it, and q, split anew for every 128 keys (64 tokens of 32 heads over
 // 8192 4-bit positions: 19 us, 0.45 PFLOP/s counting both parts of q).
 #include <hip/hip_runtime.h>
 

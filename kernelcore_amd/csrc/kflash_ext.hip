@@ -82,7 +82,7 @@ __device__ __forceinline__ uint32_t tameHalves(uint32_t w) {
 // set to a workgroup: 101 against 78 us.)
 // Bound by the products, staging and softmax, which overlap little: 2048 causal tokens, 24 heads of 128, fp16: 75 us, 0.69
 // PFLOP/s counting both parts of q and p (a large fp16 product of the library: 1.19); 1000 tokens over 3577 4-bit positions,
-// 32 heads: 143 us, 0.88 PFLOP/s.
+// 32 heads: 147 us, 0.86 PFLOP/s.
 template <int D, bool Q4>
 struct Geo {
     static constexpr int KS = D == 256 ? 1 : 2;  // (256 values: one wavefront's registers fill a SIMD)
@@ -528,7 +528,8 @@ __global__ __launch_bounds__(256 * (D == 256 ? 1 : 2), D == 256 ? 1 : 2) void fl
 // ---------------------------------------------------------------------------------------------- few rows
 // Groups of up to 32 rows (NR columns of 16): single tokens and a few drafted ones, where the cache's bytes count, and more rows over
 // short ranges, where latency does (fxPlan). One token of 32 heads over
-// 131072 4-bit positions: 47 us, 3.2 TB/s of cache, bound by unpacking (about 600 VALU instructions per 64 keys and wavefront); over 8191:
+// 131072 4-bit positions: 47 us, 3.2 TB/s of cache, by its unpacking most of all (770 VALU instructions
+// per 64 keys, start and join included, half of the time); over 8191:
 // 8.5 us, of which 2 are the first tile's latency and 3 its computation. Workgroup: four
 // wavefronts over one range of keys of a KV head, each with its own tiles (64 keys of a 4-bit cache, 32 of an fp16
 // one), joined through LDS at the end. v_mfma_f32_16x16x32_f16, lane (i, kg) = column i, group kg of 16 lanes:

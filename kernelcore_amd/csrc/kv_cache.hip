@@ -23,8 +23,9 @@ __device__ __forceinline__ long long index64(const int* idx, long long i) {
 }
 
 // ---------------------------------------------------------------------------------------------- 4-bit rows
-// Eight lanes per block of 32 values, four values each; R rows per workgroup. Bound by reading the f32 rows, and by the search for
-// repeated indices: 1777 rows of 1024 values 5.4 us, 1.5 TB/s; one row 1.7 us.
+// Eight lanes per block of 32 values, four values each; R rows per workgroup. Bound by the search for repeated indices, in which a workgroup
+// reads those of all later rows, and by reading the f32 rows: 1777 rows of 1024 values 5.6 us, 1.3 TB/s; one row 1.7 us. The search
+// grows with the square of the rows: 8192 rows 16 us, 32768 85 (1.6 TB/s), 131072 0.96 ms (0.6), 524280 14 ms.
 // Code of x: floor(x / d + 8.5), d = xm / -8. With a = |d| and y = x sign(d) that is the largest c with (c - 8.5) a <= y:
 // the product c' a of a half-integer and an f32 is rounded by the fma only after y is subtracted, so the sign of
 // y - c' a is exact and settles a guess from the rounded quotient.
@@ -113,7 +114,8 @@ __global__ __launch_bounds__(256) void set_rows_q4_0_kernel(const float* __restr
     }
 }
 
-// Eight lanes per block, four values (16 bytes of y) each. Bound by writing y: 1777 rows of 1024 values 4.8 us, 1.7 TB/s.
+// Eight lanes per block, four values (16 bytes of y) each. 1777 rows of 1024 values 4.8 us, 1.7 TB/s of y, a row to a workgroup: an
+// index, then its block, then the store; 32768 rows 25 us, 5.4 TB/s, by writing y.
 __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restrict__ src, const int* __restrict__ idx,
                                                             float* __restrict__ y, int nb, int rows, int src_rows,
                                                             long long src_row) {
@@ -139,7 +141,8 @@ __global__ __launch_bounds__(256) void get_rows_q4_0_kernel(const char* __restri
 // in ascending order: each wavefront owns a contiguous piece of the row, so that ballots and one prefix over the
 // wavefronts give every position its place. Up to R x 1024 positions are read once and held in registers through the five
 // sweeps; longer rows (R = 0) are read by each sweep. A head has one compute unit, and the sweeps' instructions bound it: 16384
-// positions 12.1 us (digits of 8 bits, a sweep more: 1.3 us more), 1500 positions 5.4 us, its barriers and the load.
+// positions 12.4 us (digits of 8 bits, a sweep more: 1.3 us more), 1500 positions 5.6 us, its barriers and the load. Over 32768
+// the sweeps' loads count too, one at a time: 32768 positions 22 us, 65536 70, 131072 134.
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 
 __device__ __forceinline__ uint32_t rankCode(float w) {  // ascending with w; -0 as 0; NaN first; never 0
