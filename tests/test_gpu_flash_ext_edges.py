@@ -18,9 +18,9 @@ def runtime():
 
 
 CACHES = pytest.mark.parametrize("q4", [False, True], ids=["f16", "q4_0"])
-# one row tile and several on the few-rows kernel, then the many-rows kernel, of each head size
+# one row tile and several on the few-rows kernel, then the many-rows kernel, of each head size, and in several ranges
 ROWS = [(8, 2, 128, 1, 2000), (6, 2, 64, 5, 700), (4, 2, 256, 3, 333), (8, 2, 128, 60, 330), (32, 32, 64, 290, 450), (16, 16, 128, 300, 421),
-        (16, 16, 256, 260, 501)]
+        (16, 16, 256, 260, 501), (5, 1, 128, 700, 1111), (8, 2, 256, 330, 900)]
 
 
 @CACHES
