@@ -427,6 +427,153 @@ typedef struct kcKvGatherArgs {
     int T;
 } kcKvGatherArgs;
 
+/* ---- a step of many requests over a paged cache (no reference counterpart) --------------------------
+ * A paged cache holds the positions of `seqs` sequences in pages of `page` positions (a power of two from 16 to 65536):
+ * position p of sequence s is row (slot) table[s][p / page] * page + p % page of K and of V. Sequence s brings the step's
+ * tokens start[s] .. start[s + 1) - 1, its "nodes" 0, 1, ..: one decoded token, a chunk of a prompt or a drafted tree.
+ * The counts, tables and trees live on the device, so that one captured graph serves every step of the same n_tokens.
+ *
+ * kv_pages: what a step of add[s] tokens on top of have[s] needs, for s < seqs (negative counts count as 0; len and pos stop at 2^31 - 1):
+ *   start[s] = add[0] + .. + add[s - 1], s <= seqs; tokens from n_tokens on are left out, as if add ended there;
+ *   len[s] = have[s] + the tokens it brings;
+ *   new pages, those whose first position is one of these, are taken from free[0 .. n_free) in the order of the sequences and of
+ *   their positions and written to table[s][..]; past the end of the free list -1 is. Positions from max_pages * page on have
+ *   no page. used[0]: the pages that the step needs (more than n_free: the list was too short);
+ *   slots[t] (int64): the slot of token t's position, -1 without a page (a page number below 0 in table or free is none);
+ *   pos[t] (may be null) = have[s] + i for node i, or have[s] + the node's depth where parent is given.
+ * parent[t] (may be null): a node's parent by its number in its sequence, -1 (or any other number that is not a smaller node's) for
+ * a root; depth 0. tree[t] (given with it; tree_words 1 to 64 32-bit words): bit j of the words is set where node j of the
+ * sequence, j < 32 tree_words, is node i itself or one of its ancestors.
+ * Tokens from start[seqs] on get slot -1, pos 0 and no tree bit. Outputs overlap neither each other nor the inputs. */
+typedef struct kcKvPagesArgs {
+    const int* have;
+    const int* add;
+    const int* free;
+    const int* parent;
+    int* table;
+    int* start;
+    int* len;
+    int* slots;
+    int* pos;
+    int* used;
+    int* tree;
+    int seqs;
+    int n_tokens;
+    int n_free;
+    int page;
+    int max_pages; /* entries of a table row */
+    int table_row; /* ints between table rows */
+    int tree_words;
+} kcKvPagesArgs;
+
+/* kcRopeFreqs (host): the revolutions per position of the n_rot / 2 pairs of a rotated part of n_rot values, and the factor of
+ * cosine and sine: theta_i = base^(-2 i / n_rot), / ff[i] where ff (may be null) is given, / factor (a context stretched by it).
+ * yarn_ctx > 0: YaRN (Peng et al., 2023) over the original context yarn_ctx: pairs that turn more than beta_fast times
+ * within it keep their speed, those below beta_slow are slowed down by factor, those between are blended by their number; the
+ * scale is then 1 + 0.1 ln(factor), else 1. (beta_fast and beta_slow: 32 and 1 where 0.) */
+typedef struct kcRopeScaling {
+    int n_rot;
+    float base;
+    float factor;
+    int yarn_ctx;
+    float beta_fast;
+    float beta_slow;
+} kcRopeScaling;
+KC_API kcError_t kcRopeFreqs(const kcRopeScaling* scaling, const float* ff, double* freqs, float* scale) KC_NOEXCEPT;
+/* rope_ext: q's and k's first n_rot values of each head turned by 2 pi pos[t] freqs[i] and multiplied by scale, the others as they are:
+ * pairs (2 i, 2 i + 1) where interleaved is 1, (i, i + n_rot / 2) where it is 0; angles in 64 bits, so that far positions keep theirs.
+ * q (with q_out) or k (with k_cache) may be null, v too. q_out may be q with the same strides (k may not be written to).
+ * k, turned, and v, as it is, are rounded to fp16 and stored in rows slots[t] (int64) of the caches; slots outside [0, cache_rows) are
+ * not stored, and of tokens with the same slot the last one is. Strides of q, k, v and q_out are in floats, of the
+ * caches in bytes (multiples of 2; rows do not overlap). D even, at most 1024; n_rot even, at most D. */
+typedef struct kcRopeExtArgs {
+    const float* q;
+    const float* k;
+    const float* v;
+    const int* pos;
+    const double* freqs;
+    const int* slots;
+    float* q_out;
+    void* k_cache;
+    void* v_cache;
+    int n_tokens;
+    int H;
+    int H_kv;
+    int D;
+    int n_rot;
+    int interleaved;
+    int q_tok, q_head, k_tok, k_head, v_tok, v_head, out_tok, out_head;
+    int cache_rows;
+    long long kc_row, kc_head, vc_row, vc_head;
+    float scale;
+} kcRopeExtArgs;
+
+/* flash_pages_f16: attention of the step's tokens over an fp16 paged cache that holds their own keys and values too (len[s] positions,
+ * the last of them the sequence's nodes): out[t][h] = sum_j softmax_j(scale q_th . k_j) v_j over the positions j that token t, node i
+ * of sequence s, sees: those before the nodes, and of the nodes j <= i, or where tree (kv_pages') is given those of its bits
+ * (none from 32 tree_words on). Query head h reads KV head h / (H / H_kv); D = 64, 128 or 256. A position whose page is outside [0, n_pages), from
+ * len[s] or from max_pages * page on is not seen. A token that sees none gets zeros; lse (may be null): [N][H], the natural logarithm
+ * of the sum of exp(score), -infinity for such a token. Rows of tokens from start[seqs] (at most N) on are left as they are. What a position holds that a
+ * token does not see (NaN and infinities too) does not reach that token; what it sees counts as in flash_ext_f16.
+ * Rows, heads and base of K and V at multiples of 16 bytes; offsets are 64-bit, a page spans less than 2^31 bytes. part: kcFlashPagesPartBytes bytes of workspace,
+ * 16-byte aligned, which calls that may overlap must not share. */
+typedef struct kcFlashPagesDims {
+    int H;
+    int H_kv;
+    int D;
+    int N;    /* tokens that q and out hold */
+    int seqs;
+    int page;
+    int max_pages;
+    int n_pages;   /* pages that the cache holds */
+    int tree_words;
+    int q_tok;     /* floats between tokens of q */
+    int q_head;    /* floats between heads of q */
+    int table_row; /* ints between table rows */
+    long long k_row, k_head, v_row, v_head; /* bytes */
+} kcFlashPagesDims;
+typedef struct kcFlashPagesArgs {
+    const float* q;
+    const void* k;
+    const void* v;
+    const int* table;
+    const int* start;
+    const int* len;
+    const int* tree;
+    float* out;
+    float* lse;
+    float* part;
+    kcFlashPagesDims d;
+    float scale;
+} kcFlashPagesArgs;
+KC_API kcError_t kcFlashPagesPartBytes(const kcFlashPagesDims* dims, size_t* bytes) KC_NOEXCEPT;
+
+/* sample_rows: a token for each of `rows` rows of n_vocab logits (row floats apart), drawn with the given random number u[r]:
+ *   weights w_j = exp((l_j - max l) / temperature), tokens in the order of their logits, largest first, equal ones by their number;
+ *   kept are the first top_k of them (0 or less: all), of those the fewest whose weights reach top_p of the sum of the top_k ones (1 or
+ *   more, or NaN: all), and of those the ones with w_j >= min_p (0 or less, or NaN: all); the first always is;
+ *   tokens[r] = the first in that order at which the sum of the kept weights exceeds u[r] times their whole sum (u below 0 or NaN
+ *   counts as 0; from 1 on: the last with a weight); probs[r] (may be null) = its weight over that sum.
+ * A temperature of 0 or less, or NaN: the first token (u and the cuts do not matter). temperature, top_k, top_p and min_p hold a value for each row; null:
+ * 1, 0, 1 and 0. A logit of -infinity has weight 0. A row that holds NaN or +infinity, or -infinity alone, gives token -1 and
+ * probability 0. Weights and sums are held in 64 bits and added in a fixed order. n_vocab at most 2^20; part: kcSampleRowsPartBytes bytes of workspace, 16-byte
+ * aligned, which calls that may overlap must not share. */
+typedef struct kcSampleRowsArgs {
+    const float* logits;
+    const float* u;
+    const float* temperature;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    int* tokens;
+    float* probs;
+    void* part;
+    long long row;
+    int rows;
+    int n_vocab;
+} kcSampleRowsArgs;
+KC_API kcError_t kcSampleRowsPartBytes(int rows, int n_vocab, size_t* bytes) KC_NOEXCEPT;
+
 /* ---- K-quant weight streams (this device's layout; no reference counterpart beyond
  * llm::ref::repackQ4K/Q6K and the ggml backend's unpack_stream, ggml-kernelcore.cpp:124-154) ----
  * Rows are grouped in tiles of 16 and super-blocks in groups of 4 (padding rows and super-blocks
@@ -533,6 +680,12 @@ typedef ::kcAttnWeightsArgs AttnWeightsArgs;
 typedef ::kcKvKeepArgs KvKeepArgs;
 typedef ::kcKvPlane KvPlane;
 typedef ::kcKvGatherArgs KvGatherArgs;
+typedef ::kcKvPagesArgs KvPagesArgs;
+typedef ::kcRopeScaling RopeScaling;
+typedef ::kcRopeExtArgs RopeExtArgs;
+typedef ::kcFlashPagesDims FlashPagesDims;
+typedef ::kcFlashPagesArgs FlashPagesArgs;
+typedef ::kcSampleRowsArgs SampleRowsArgs;
 inline int scratchInts(int nb) { return nb * 11; }
 inline float* scratchScales(int* q, int nb) { return reinterpret_cast<float*>(q + nb * 8); }
 inline int scratchKInts(int nsb) { return nsb * 85; }

@@ -106,6 +106,22 @@ KvPlane = _struct("KvPlane", [("src", _p), ("dst", _p), ("src_row", _l), ("src_h
                               ("bytes", _i)])
 KvGatherArgs = _struct("KvGatherArgs", [("planes", KvPlane * 4), ("n_planes", _i), ("keep", _p), ("heads", _i), ("n_keep", _i),
                                         ("keep_row", _i), ("T", _i)])
+KvPagesArgs = _struct("KvPagesArgs", [(n, _p) for n in ("have", "add", "free", "parent", "table", "start", "len", "slots", "pos", "used",
+                                                        "tree")] +
+                      [(n, _i) for n in ("seqs", "n_tokens", "n_free", "page", "max_pages", "table_row", "tree_words")])
+RopeScaling = _struct("RopeScaling", [("n_rot", _i), ("base", _f), ("factor", _f), ("yarn_ctx", _i), ("beta_fast", _f),
+                                      ("beta_slow", _f)])
+RopeExtArgs = _struct("RopeExtArgs", [(n, _p) for n in ("q", "k", "v", "pos", "freqs", "slots", "q_out", "k_cache", "v_cache")] +
+                      [(n, _i) for n in ("n_tokens", "H", "H_kv", "D", "n_rot", "interleaved", "q_tok", "q_head", "k_tok", "k_head",
+                                         "v_tok", "v_head", "out_tok", "out_head", "cache_rows")] +
+                      [(n, _l) for n in ("kc_row", "kc_head", "vc_row", "vc_head")] + [("scale", _f)])
+FlashPagesDims = _struct("FlashPagesDims", [(n, _i) for n in ("H", "H_kv", "D", "N", "seqs", "page", "max_pages", "n_pages",
+                                                              "tree_words", "q_tok", "q_head", "table_row")] +
+                         [(n, _l) for n in ("k_row", "k_head", "v_row", "v_head")])
+FlashPagesArgs = _struct("FlashPagesArgs", [(n, _p) for n in ("q", "k", "v", "table", "start", "len", "tree", "out", "lse", "part")] +
+                         [("d", FlashPagesDims), ("scale", _f)])
+SampleRowsArgs = _struct("SampleRowsArgs", [(n, _p) for n in ("logits", "u", "temperature", "top_k", "top_p", "min_p", "tokens", "probs",
+                                                              "part")] + [("row", _l), ("rows", _i), ("n_vocab", _i)])
 GetRowsKquantArgs = _struct("GetRowsKquantArgs", [("qw", _p), ("ids", _p), ("y", _p), ("qtype", _i), ("rows", _i),
                                                   ("k", _i), ("n", _i)])
 QuantizeKquantArgs = _struct("QuantizeKquantArgs", [("x", _p), ("blocks", _p), ("qtype", _i), ("rows", _i), ("k", _i)])
@@ -163,6 +179,9 @@ def lib():
         L.kcLaunchKernelChunked.argtypes = [C.c_char_p, _p, C.c_uint, C.c_int64, _p]
         L.kcKquantStreamBytes.argtypes = [_i, _i, _i, C.POINTER(C.c_size_t)]
         L.kcFlashExtPartBytes.argtypes = [C.POINTER(FlashExtDims), C.POINTER(C.c_size_t)]
+        L.kcFlashPagesPartBytes.argtypes = [C.POINTER(FlashPagesDims), C.POINTER(C.c_size_t)]
+        L.kcSampleRowsPartBytes.argtypes = [_i, _i, C.POINTER(C.c_size_t)]
+        L.kcRopeFreqs.argtypes = [C.POINTER(RopeScaling), _p, _p, C.POINTER(_f)]
         L.kcEventElapsedTime.argtypes = [C.POINTER(_f), _p, _p]
         for n in ("kcEventRecord", "kcStreamWaitEvent"):
             getattr(L, n).argtypes = [_p, _p]
@@ -247,6 +266,31 @@ def flash_ext_part_bytes(dims):
     n = C.c_size_t()
     call("kcFlashExtPartBytes", C.byref(dims), C.byref(n))
     return n.value
+
+
+def flash_pages_part_bytes(dims):
+    """kcFlashPagesPartBytes (host only): the workspace flash_pages_f16 needs for these FlashPagesDims."""
+    n = C.c_size_t()
+    call("kcFlashPagesPartBytes", C.byref(dims), C.byref(n))
+    return n.value
+
+
+def sample_rows_part_bytes(rows, n_vocab):
+    """kcSampleRowsPartBytes (host only): the workspace sample_rows needs."""
+    n = C.c_size_t()
+    call("kcSampleRowsPartBytes", rows, n_vocab, C.byref(n))
+    return n.value
+
+
+def rope_freqs(n_rot, base, factor=1.0, yarn_ctx=0, beta_fast=0.0, beta_slow=0.0, ff=None):
+    """kcRopeFreqs (host only): (revolutions per position of the n_rot / 2 pairs, the factor of cosine and sine)."""
+    out, scale = np.zeros(max(0, n_rot // 2)), _f()
+    f = None if ff is None else np.ascontiguousarray(ff, np.float32)
+    if f is not None and f.size != n_rot // 2:
+        raise ValueError("ff holds n_rot / 2 values")
+    call("kcRopeFreqs", C.byref(RopeScaling(n_rot, base, factor, yarn_ctx, beta_fast, beta_slow)),
+         None if f is None else f.ctypes.data, out.ctypes.data, C.byref(scale))
+    return out, scale.value
 
 
 class Buffer:

@@ -1,0 +1,214 @@
+// krope_ext.hip -- rope_ext: rotary positions of q and k with the fp16 store of k and v into cache rows; kcRopeFreqs on the host.
+//
+// y0 = x0 cos - x1 sin, y1 = x0 sin + x1 cos for the pairs of a head's rotated part, angle 2 pi frac(pos f) with f in revolutions per
+// position: the product and its fraction are taken in 64 bits (at position 2^20 a 32-bit angle is off by 2^-5), cosine and sine in 32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "internal.hpp"
+#include "kserve.hpp"
+
+namespace kcamd {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f4a4 __attribute__((aligned(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef h4 h4a2 __attribute__((aligned(2)));
+
+constexpr int kThreads = 256, kPairs = 1024;  // pairs of a workgroup's tokens
+
+struct RopeArgs {
+    const float *q, *k, *v;
+    const int* pos;
+    const double* freqs;
+    const long long* slots;
+    float* q_out;
+    char *k_cache, *v_cache;
+    int n, H, H_kv, D, n_rot;
+    int q_tok, q_head, k_tok, k_head, v_tok, v_head, out_tok, out_head, cache_rows;
+    long long kc_row, kc_head, vc_row, vc_head;
+    float scale;
+    int q_tokens, kv_tokens, q_blocks;  // tokens of a workgroup, workgroups for q (the first ones)
+};
+
+// Eight values of a row: two groups of four that hold four pairs, or of its unturned part; n of each group are there.
+struct Unit {
+    int a, b, na, nb, pair;  // pair: the first one's number, -1 for unturned values
+};
+template <bool INTER>
+__device__ __forceinline__ Unit unitOf(int u, int n_rot, int D) {
+    const int half = n_rot / 2, turned = (half + 3) / 4;
+    Unit x;
+    if (u < turned) {
+        x.pair = 4 * u;
+        x.a = INTER ? 8 * u : 4 * u;
+        x.b = INTER ? x.a + 4 : x.a + half;
+        const int left = half - 4 * u;  // pairs
+        x.na = INTER ? min(4, 2 * left) : min(4, left);
+        x.nb = INTER ? max(0, min(4, 2 * left - 4)) : x.na;
+    } else {
+        x.pair = -1;
+        x.a = n_rot + 8 * (u - turned);
+        x.b = x.a + 4;
+        x.na = min(4, D - x.a);
+        x.nb = max(0, min(4, D - x.b));
+    }
+    return x;
+}
+
+__device__ __forceinline__ f32x4 loadPart(const float* p, int n) {
+    if (n == 4) return *reinterpret_cast<const f4a4*>(p);
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) x[e] = p[e];
+    return x;
+}
+__device__ __forceinline__ void storePart(float* p, f32x4 x, int n) {
+    if (n == 4) {
+        *reinterpret_cast<f4a4*>(p) = x;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = x[e];
+}
+__device__ __forceinline__ void storePart(_Float16* p, f32x4 x, int n) {
+    if (n == 4) {
+        *reinterpret_cast<h4a2*>(p) = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = (_Float16)x[e];
+}
+
+// The pairs' cosines and sines lie in cs from the unit's first pair on.
+template <bool INTER>
+__device__ __forceinline__ void turn(f32x4& a, f32x4& b, const float2* cs, int pairs) {
+    float2 z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = cs[min(e, pairs - 1)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f32x4& lo = INTER ? (e < 2 ? a : b) : a;
+        f32x4& hi = INTER ? (e < 2 ? a : b) : b;
+        const int i = INTER ? 2 * (e & 1) : e, j = INTER ? i + 1 : e;
+        const float x0 = lo[i], x1 = hi[j];
+        lo[i] = fmaf(x0, z[e].x, -(x1 * z[e].y));
+        hi[j] = fmaf(x0, z[e].y, x1 * z[e].x);
+    }
+}
+
+// A workgroup takes all heads of q, or all of k and v, of q_tokens or kv_tokens tokens: the angles once into LDS, then eight values a
+// thread at a time, loaded before the angles are there.
+template <bool INTER>
+__global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
+    __shared__ float2 cs[kPairs];
+    __shared__ int later[16], rowOf[16];
+    const int tid = threadIdx.x;
+    const bool isQ = (int)blockIdx.x < a.q_blocks;
+    const int per = isQ ? a.q_tokens : a.kv_tokens;
+    const int t0 = (isQ ? blockIdx.x : blockIdx.x - a.q_blocks) * per, n = min(per, a.n - t0);
+    const int pairs = a.n_rot / 2;
+    const int turned = (pairs + 3) / 4, units = turned + (a.D - a.n_rot + 7) / 8, vunits = (a.D + 7) / 8;
+    if (!isQ && tid < 16) {
+        later[tid] = 0;
+        const long long slot = tid < n ? a.slots[t0 + tid] : -1;
+        rowOf[tid] = slot >= 0 && slot < a.cache_rows ? (int)slot : -1;
+    }
+    for (int x = tid; x < n * pairs; x += kThreads) {
+        const int t = x / pairs, i = x - t * pairs;
+        const double r = (double)a.pos[t0 + t] * a.freqs[i];
+        const float f = 2.0f * (float)(r - rint(r));
+        cs[x] = make_float2(cospif(f) * a.scale, sinpif(f) * a.scale);
+    }
+    __syncthreads();
+    if (isQ) {
+        const int all = n * a.H * units;
+        for (int x = tid; x < all; x += kThreads) {
+            const int row = x / units, t = row / a.H, h = row - t * a.H;
+            const Unit u = unitOf<INTER>(x - row * units, a.n_rot, a.D);
+            const float* src = a.q + (long long)(t0 + t) * a.q_tok + (long long)h * a.q_head;
+            float* dst = a.q_out + (long long)(t0 + t) * a.out_tok + (long long)h * a.out_head;
+            f32x4 p = loadPart(src + u.a, u.na), q = loadPart(src + u.b, u.nb);
+            if (u.pair >= 0) turn<INTER>(p, q, cs + t * pairs + u.pair, pairs - u.pair);
+            storePart(dst + u.a, p, u.na);
+            storePart(dst + u.b, q, u.nb);
+        }
+        return;
+    }
+    // tokens whose slot a later one repeats are left to that one
+    for (int x = t0 + 1 + tid; x < a.n; x += kThreads) {
+        const long long slot = a.slots[x];
+        if (slot < 0 || slot >= a.cache_rows) continue;
+        for (int t = 0; t < n; ++t)
+            if (t0 + t < x && rowOf[t] == (int)slot) later[t] = 1;
+    }
+    __syncthreads();
+    const int kall = n * a.H_kv * units, vall = a.v ? n * a.H_kv * vunits : 0;
+    for (int x = tid; x < kall + vall; x += kThreads) {
+        const bool isV = x >= kall;
+        const int y = isV ? x - kall : x, uu = isV ? vunits : units;
+        const int row = y / uu, t = row / a.H_kv, h = row - t * a.H_kv;
+        if (rowOf[t] < 0 || later[t]) continue;
+        const Unit u = unitOf<INTER>(y - row * uu, isV ? 0 : a.n_rot, a.D);
+        const float* src = isV ? a.v + (long long)(t0 + t) * a.v_tok + (long long)h * a.v_head
+                               : a.k + (long long)(t0 + t) * a.k_tok + (long long)h * a.k_head;
+        char* to = isV ? a.v_cache + rowOf[t] * a.vc_row + h * a.vc_head : a.k_cache + rowOf[t] * a.kc_row + h * a.kc_head;
+        _Float16* dst = reinterpret_cast<_Float16*>(to);
+        f32x4 p = loadPart(src + u.a, u.na), q = loadPart(src + u.b, u.nb);
+        if (u.pair >= 0) turn<INTER>(p, q, cs + t * pairs + u.pair, pairs - u.pair);
+        storePart(dst + u.a, p, u.na);
+        storePart(dst + u.b, q, u.nb);
+    }
+}
+
+}  // namespace
+
+int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
+    if (a.n_tokens == 0) return 0;
+    RopeArgs p{a.q, a.k, a.v, a.pos, a.freqs, reinterpret_cast<const long long*>(a.slots), a.q_out, static_cast<char*>(a.k_cache),
+               static_cast<char*>(a.v_cache), a.n_tokens, a.H, a.H_kv, a.D, a.n_rot, a.q_tok, a.q_head, a.k_tok, a.k_head, a.v_tok, a.v_head,
+               a.out_tok, a.out_head, a.cache_rows, a.kc_row, a.kc_head, a.vc_row, a.vc_head, a.scale, 1, 1, 0};
+    // k and v: up to 16 tokens share the search for repeated slots, once there are enough to fill the GPU
+    const int most = std::max(1, std::min(16, kPairs / std::max(1, a.n_rot / 2)));
+    p.kv_tokens = std::max(1, std::min(most, a.n_tokens / 512));
+    p.q_blocks = a.q ? (a.n_tokens + p.q_tokens - 1) / p.q_tokens : 0;
+    const int kvBlocks = a.k ? (a.n_tokens + p.kv_tokens - 1) / p.kv_tokens : 0;
+    const dim3 grid(p.q_blocks + kvBlocks);
+    if (a.interleaved) hipLaunchKernelGGL(rope_ext_kernel<true>, grid, dim3(kThreads), 0, s, p);
+    else hipLaunchKernelGGL(rope_ext_kernel<false>, grid, dim3(kThreads), 0, s, p);
+    return fromHip(hipGetLastError(), "rope_ext");
+}
+
+}  // namespace kcamd
+
+kcError_t kcRopeFreqs(const kcRopeScaling* r, const float* ff, double* freqs, float* scale) noexcept {
+    if (!r || !freqs || !scale || r->n_rot <= 0 || r->n_rot % 2 || r->n_rot > 1024 || !(r->base > 1.0f) || !std::isfinite(r->base) ||
+        !(r->factor > 0.0f) || !std::isfinite(r->factor) || r->yarn_ctx < 0 || !(r->beta_fast >= 0.0f) || !(r->beta_slow >= 0.0f) ||
+        !std::isfinite(r->beta_fast) || !std::isfinite(r->beta_slow)) {
+        kcamd::setDetail("rope: n_rot even, from 2 to 1024, base above 1, factor positive, yarn_ctx and betas not negative");
+        return kc::Error::InvalidValue;
+    }
+    const int n = r->n_rot;
+    constexpr double kTwoPi = 6.283185307179586;
+    // the pair that turns beta times within the original context
+    const auto pairOf = [&](double beta) { return n * std::log(r->yarn_ctx / (beta * kTwoPi)) / (2 * std::log((double)r->base)); };
+    double low = 0, high = 0;
+    if (r->yarn_ctx) {
+        low = std::max(0.0, std::floor(pairOf(r->beta_fast > 0.0f ? r->beta_fast : 32.0)));
+        high = std::min(n - 1.0, std::ceil(pairOf(r->beta_slow > 0.0f ? r->beta_slow : 1.0)));
+    }
+    for (int i = 0; i < n / 2; ++i) {
+        const double theta = std::pow((double)r->base, -2.0 * i / n) / (ff ? (double)ff[i] : 1.0);
+        const double slow = r->yarn_ctx ? std::min(1.0, std::max(0.0, (i - low) / std::max(0.001, high - low))) : 1.0;
+        freqs[i] = (theta / r->factor * slow + theta * (1 - slow)) / kTwoPi;
+    }
+    *scale = r->yarn_ctx ? (float)(1 + 0.1 * std::log((double)r->factor)) : 1.0f;
+    return kc::Error::Success;
+}

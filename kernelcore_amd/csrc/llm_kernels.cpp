@@ -17,6 +17,7 @@
 #include "launch.hpp"
 #include "kquantize.hpp"
 #include "kdecode.hpp"
+#include "kserve.hpp"
 #include "kv_cache.hpp"
 #include "model_kernels.hpp"
 
@@ -614,6 +615,178 @@ int kvGatherValidate(const void* p, const kcLaunchContext*) {
 }
 int kvGatherLaunch(const void* p, void* s) { return kcamd::launchKvGather(*static_cast<const kcKvGatherArgs*>(p), hs(s)); }
 
+// ---- a step of many requests over a paged cache: kv_pages, rope_ext, flash_pages_f16, sample_rows
+
+bool pageSize(int p) { return p >= 16 && p <= 65536 && (p & (p - 1)) == 0; }
+// n ints (or nothing) at 4-byte alignment
+int intsAt(const void* p, int64_t n, const char* what) {
+    if (!aligned(p, 4)) return invalid("4-byte aligned arrays");
+    return checkRange(p, size_t(n) * 4, what);
+}
+struct Span {
+    uintptr_t at;
+    size_t bytes;
+};
+bool overlap(const Span& a, const Span& b) { return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+Span spanOf(const void* p, size_t bytes) { return {reinterpret_cast<uintptr_t>(p), p ? bytes : 0}; }
+
+int kvPagesValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcKvPagesArgs*>(p);
+    if (a.seqs < 0 || a.seqs > INT32_MAX - 65536 || a.n_tokens < 0 || a.n_tokens > INT32_MAX - 65536 || a.n_free < 0 || !pageSize(a.page) || a.max_pages < 0 ||
+        a.table_row < a.max_pages)
+        return invalid("kv_pages: counts not negative, page a power of two from 16 to 65536, table_row at least max_pages");
+    if ((a.parent != nullptr) != (a.tree != nullptr) || (a.tree ? a.tree_words < 1 || a.tree_words > 64 : a.tree_words != 0))
+        return invalid("kv_pages: parent and tree are both given, with 1 to 64 tree_words, or both null, with none");
+    if (!aligned(a.slots, 8)) return invalid("kv_pages: slots 8-byte aligned");
+    int64_t table;
+    if (!extent(a.seqs, int64_t(a.table_row) * 4, int64_t(a.max_pages) * 4, &table)) return invalid("kv_pages: table too large");
+    KC_TRY(intsAt(a.have, a.seqs, "have"));
+    KC_TRY(intsAt(a.add, a.seqs, "add"));
+    KC_TRY(intsAt(a.free, a.n_free, "free"));
+    KC_TRY(intsAt(a.table, table / 4, "table"));
+    KC_TRY(intsAt(a.start, int64_t(a.seqs) + 1, "start"));
+    KC_TRY(intsAt(a.len, a.seqs, "len"));
+    KC_TRY(intsAt(a.slots, int64_t(a.n_tokens) * 2, "slots"));
+    if (a.pos) KC_TRY(intsAt(a.pos, a.n_tokens, "pos"));
+    KC_TRY(intsAt(a.used, 1, "used"));
+    if (a.parent) {
+        KC_TRY(intsAt(a.parent, a.n_tokens, "parent"));
+        KC_TRY(intsAt(a.tree, int64_t(a.n_tokens) * a.tree_words, "tree"));
+    }
+    const size_t n = size_t(a.n_tokens), s = size_t(a.seqs);
+    const Span all[11] = {spanOf(a.table, size_t(table)), spanOf(a.start, 4 * s + 4), spanOf(a.len, 4 * s), spanOf(a.slots, 8 * n), spanOf(a.pos, 4 * n),
+                          spanOf(a.used, 4), spanOf(a.tree, 4 * n * size_t(a.tree_words)), spanOf(a.have, 4 * s), spanOf(a.add, 4 * s),
+                          spanOf(a.free, 4 * size_t(a.n_free)), spanOf(a.parent, 4 * n)};
+    for (int i = 0; i < 7; ++i)
+        for (int j = i + 1; j < 11; ++j)
+            if (overlap(all[i], all[j])) return invalid("kv_pages: an output overlaps another array");
+    return 0;
+}
+int kvPagesLaunch(const void* p, void* s) { return kcamd::launchKvPages(*static_cast<const kcKvPagesArgs*>(p), hs(s)); }
+
+// Rows of `heads` heads of D values, strides in units of `unit` bytes.
+int headRows(const void* p, int64_t n, int64_t row, int heads, int64_t head, int D, int unit, const char* what, Span* span) {
+    int64_t x, y;
+    if (row < 0 || head < 0 || !aligned(p, size_t(unit)) || !extent(heads, head, D, &x) || !extent(n, row, x, &y) || y > INT64_MAX / 8)
+        return invalid("rope_ext: strides not negative, arrays aligned to their values");
+    *span = spanOf(p, size_t(y) * size_t(unit));
+    return checkRange(p, size_t(y) * size_t(unit), what);
+}
+// Whether no two of n x heads rows share a value: heads within a row, or rows within a head. (After headRows or extent: no overflow.)
+bool rowsApart(int64_t n, int64_t row, int64_t heads, int64_t head, int64_t size) {
+    const bool inner = (heads <= 1 || head >= size) && (n <= 1 || row >= (heads - 1) * head + size);
+    const bool outer = (n <= 1 || row >= size) && (heads <= 1 || head >= (n - 1) * row + size);
+    return inner || outer;
+}
+int ropeExtValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcRopeExtArgs*>(p);
+    if (a.n_tokens < 0 || a.n_tokens > (1 << 29) || a.D <= 0 || a.D % 2 || a.D > 1024 || a.n_rot <= 0 || a.n_rot % 2 || a.n_rot > a.D ||
+        (a.interleaved != 0 && a.interleaved != 1))
+        return invalid("rope_ext: D even, at most 1024, n_rot even, from 2 to D, interleaved 0 or 1");
+    if ((a.q != nullptr) != (a.q_out != nullptr) || (a.k != nullptr) != (a.k_cache != nullptr) || (a.v != nullptr) != (a.v_cache != nullptr) || (a.v && !a.k))
+        return invalid("rope_ext: q with q_out, k with k_cache, v with v_cache, and v only with k");
+    if (!(a.scale - a.scale == 0.0f)) return invalid("rope_ext: scale is finite");
+    if (!aligned(a.freqs, 8) || !aligned(a.slots, 8)) return invalid("rope_ext: freqs and slots 8-byte aligned");
+    KC_TRY(intsAt(a.pos, a.n_tokens, "pos"));
+    KC_TRY(checkRange(a.freqs, size_t(a.n_rot / 2) * 8, "freqs"));
+    Span in[3]{}, out[3]{};
+    if (a.q) {
+        if (a.H <= 0 || a.H > 65536) return invalid("rope_ext: H from 1 to 65536");
+        KC_TRY(headRows(a.q, a.n_tokens, a.q_tok, a.H, a.q_head, a.D, 4, "q", &in[0]));
+        KC_TRY(headRows(a.q_out, a.n_tokens, a.out_tok, a.H, a.out_head, a.D, 4, "q_out", &out[0]));
+        if (!rowsApart(a.n_tokens, a.out_tok, a.H, a.out_head, a.D)) return invalid("rope_ext: rows of q_out overlap");
+    }
+    if (a.k) {
+        if (a.H_kv <= 0 || a.H_kv > 65536 || a.cache_rows < 0) return invalid("rope_ext: H_kv from 1 to 65536, cache_rows not negative");
+        KC_TRY(headRows(a.k, a.n_tokens, a.k_tok, a.H_kv, a.k_head, a.D, 4, "k", &in[1]));
+        if (a.v) KC_TRY(headRows(a.v, a.n_tokens, a.v_tok, a.H_kv, a.v_head, a.D, 4, "v", &in[2]));
+        KC_TRY(checkRange(a.slots, size_t(a.n_tokens) * 8, "slots"));
+        for (int i = 0; i < (a.v ? 2 : 1); ++i) {
+            const long long row = i ? a.vc_row : a.kc_row, head = i ? a.vc_head : a.kc_head;
+            const int64_t bytes = 2 * int64_t(a.D);
+            void* c = i ? a.v_cache : a.k_cache;
+            int64_t x, y;
+            if (row % 2 || head % 2 || row < 0 || head < 0 || !aligned(c, 2) || !extent(a.H_kv, head, bytes, &x) || !extent(a.cache_rows, row, x, &y))
+                return invalid("rope_ext: cache rows, heads and bases at multiples of 2 bytes");
+            if (!rowsApart(a.cache_rows, row, a.H_kv, head, bytes)) return invalid("rope_ext: cache rows overlap");
+            KC_TRY(checkRange(c, size_t(y), i ? "v_cache" : "k_cache"));
+            out[1 + i] = spanOf(c, size_t(y));
+        }
+    }
+    const Span small[3] = {spanOf(a.pos, size_t(a.n_tokens) * 4), spanOf(a.freqs, size_t(a.n_rot / 2) * 8), spanOf(a.k ? a.slots : nullptr, size_t(a.n_tokens) * 8)};
+    const bool inPlace = a.q && a.q_out == a.q && a.out_tok == a.q_tok && a.out_head == a.q_head;
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j < 3; ++j) {
+            if (overlap(out[i], small[j]) || (i < j && overlap(out[i], out[j])) || (overlap(out[i], in[j]) && !(i == 0 && j == 0 && inPlace)))
+                return invalid("rope_ext: an output overlaps another array");
+        }
+    return 0;
+}
+int ropeExtLaunch(const void* p, void* s) { return kcamd::launchRopeExt(*static_cast<const kcRopeExtArgs*>(p), hs(s)); }
+
+// The sizes alone: what kcFlashPagesPartBytes accepts too.
+int fpShape(const kcFlashPagesDims& d) {
+    if (d.H <= 0 || d.H_kv <= 0 || d.H % d.H_kv || d.H_kv > 65535 || (d.D != 64 && d.D != 128 && d.D != 256) || d.N < 0 || d.seqs < 0 || d.max_pages < 0 ||
+        d.n_pages < 0 || !pageSize(d.page))
+        return invalid("flash_pages: H a positive multiple of H_kv, D 64, 128 or 256, counts not negative, page a power of two from 16 to 65536");
+    if (int64_t(d.max_pages) * d.page > INT32_MAX - 65536 || d.table_row < d.max_pages)
+        return invalid("flash_pages: a sequence's pages hold less than 2^31 - 65536 positions, table_row at least max_pages");
+    if (d.tree_words < 0 || d.tree_words > 64) return invalid("flash_pages: tree_words from 0 to 64");
+    if (d.q_tok < 0 || d.q_head < 0 || d.k_row < 0 || d.k_head < 0 || d.v_row < 0 || d.v_head < 0) return invalid("flash_pages: negative strides");
+    const int64_t G = d.H / d.H_kv;
+    if (int64_t(d.N) * d.H * d.D > INT32_MAX || (int64_t(d.N) * G / 16 + d.seqs) * d.H_kv > (1 << 24))
+        return invalid("flash_pages: N H D below 2^31, (N H / H_kv / 16 + seqs) H_kv at most 2^24");
+    return 0;
+}
+int fpCache(const kcFlashPagesDims& d, const void* p, int64_t row, int64_t head, const char* what) {
+    int64_t a, b;
+    if (row % 16 || head % 16 || !aligned(p, 16)) return invalid("flash_pages: cache rows, heads and base at multiples of 16 bytes");
+    if (!extent(d.H_kv, head, int64_t(d.D) * 2, &a) || !extent(int64_t(d.n_pages) * d.page, row, a, &b) || row > INT32_MAX / d.page)
+        return invalid("flash_pages: strides too large");
+    return checkRange(p, size_t(b), what);
+}
+int flashPagesValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcFlashPagesArgs*>(p);
+    const kcFlashPagesDims& d = a.d;
+    KC_TRY(fpShape(d));
+    if (!(a.scale - a.scale == 0.0f)) return invalid("flash_pages: scale finite");
+    if (a.tree ? d.tree_words < 1 : d.tree_words != 0) return invalid("flash_pages: tree with tree_words, or neither");
+    if (!aligned(a.q, 4) || !aligned(a.out, 4) || !aligned(a.lse, 4) || !aligned(a.part, 16)) return invalid("flash_pages: 4-byte aligned arrays, part 16-byte");
+    int64_t x, y, t;
+    if (!extent(d.H, d.q_head, d.D, &x) || !extent(d.N, d.q_tok, x, &y)) return invalid("flash_pages: q strides too large");
+    if (!extent(d.seqs, int64_t(d.table_row) * 4, int64_t(d.max_pages) * 4, &t)) return invalid("flash_pages: table too large");
+    KC_TRY(checkRange(a.q, size_t(y) * 4, "q"));
+    KC_TRY(fpCache(d, a.k, d.k_row, d.k_head, "k"));
+    KC_TRY(fpCache(d, a.v, d.v_row, d.v_head, "v"));
+    KC_TRY(intsAt(a.table, t / 4, "table"));
+    KC_TRY(intsAt(a.start, d.seqs ? int64_t(d.seqs) + 1 : 0, "start"));
+    KC_TRY(intsAt(a.len, d.seqs, "len"));
+    if (a.tree) KC_TRY(intsAt(a.tree, int64_t(d.N) * d.tree_words, "tree"));
+    KC_TRY(checkRange(a.out, f32Bytes(int64_t(d.N) * d.H * d.D), "out"));
+    if (a.lse) KC_TRY(checkRange(a.lse, f32Bytes(int64_t(d.N) * d.H), "lse"));
+    return checkRange(a.part, kcamd::flashPagesPartBytes(d), "part");
+}
+int flashPagesLaunch(const void* p, void* s) { return kcamd::launchFlashPages(*static_cast<const kcFlashPagesArgs*>(p), hs(s)); }
+
+int sampleRowsValidate(const void* p, const kcLaunchContext*) {
+    const auto& a = *static_cast<const kcSampleRowsArgs*>(p);
+    int64_t x;
+    if (a.rows < 0 || a.rows > 65535 || a.n_vocab <= 0 || a.n_vocab > (1 << 20) || a.row < 0 || !extent(a.rows, a.row, a.n_vocab, &x))
+        return invalid("sample_rows: rows from 0 to 65535, n_vocab from 1 to 2^20, row not negative");
+    if (!aligned(a.part, 16)) return invalid("sample_rows: part 16-byte aligned");
+    if (!aligned(a.logits, 4)) return invalid("sample_rows: 4-byte aligned arrays");
+    KC_TRY(checkRange(a.logits, size_t(x) * 4, "logits"));
+    KC_TRY(intsAt(a.u, a.rows, "u"));
+    if (a.temperature) KC_TRY(intsAt(a.temperature, a.rows, "temperature"));
+    if (a.top_k) KC_TRY(intsAt(a.top_k, a.rows, "top_k"));
+    if (a.top_p) KC_TRY(intsAt(a.top_p, a.rows, "top_p"));
+    if (a.min_p) KC_TRY(intsAt(a.min_p, a.rows, "min_p"));
+    KC_TRY(intsAt(a.tokens, a.rows, "tokens"));
+    if (a.probs) KC_TRY(intsAt(a.probs, a.rows, "probs"));
+    return checkRange(a.part, kcamd::sampleRowsPartBytes(a.rows, a.n_vocab), "part");
+}
+int sampleRowsLaunch(const void* p, void* s) { return kcamd::launchSampleRows(*static_cast<const kcSampleRowsArgs*>(p), hs(s)); }
+
 // ---- quantize_kquant / fill_normal_f32 (synthetic weights; no reference kernel)
 
 int quantKquantValidate(const void* p, const kcLaunchContext*) {
@@ -682,6 +855,10 @@ const kcKernelEntry kTable[] = {
     {"attn_weights_q4_0", attnWeightsValidate<true>, attnWeightsLaunch<true>, 0},
     {"kv_keep", kvKeepValidate, kvKeepLaunch, 0},
     {"kv_gather", kvGatherValidate, kvGatherLaunch, 0},
+    {"kv_pages", kvPagesValidate, kvPagesLaunch, 0},
+    {"rope_ext", ropeExtValidate, ropeExtLaunch, 0},
+    {"flash_pages_f16", flashPagesValidate, flashPagesLaunch, 0},
+    {"sample_rows", sampleRowsValidate, sampleRowsLaunch, 0},
     {"repack_kquant", repackValidate<false>, repackLaunch<false>, 0},
     {"unpack_kquant", repackValidate<true>, repackLaunch<true>, 0},
     {"get_rows_kquant", getRowsValidate, getRowsLaunch, 0},
@@ -706,5 +883,17 @@ kcError_t kcKquantStreamBytes(int qtype, int rows, int k, size_t* bytes) noexcep
 kcError_t kcFlashExtPartBytes(const kcFlashExtDims* dims, size_t* bytes) noexcept {
     if (!dims || !bytes || fxShape(*dims)) return kc::Error::InvalidValue;
     *bytes = f32Bytes(kcamd::fxPlan(*dims).partFloats);
+    return kc::Error::Success;
+}
+
+kcError_t kcFlashPagesPartBytes(const kcFlashPagesDims* dims, size_t* bytes) noexcept {
+    if (!dims || !bytes || fpShape(*dims)) return kc::Error::InvalidValue;
+    *bytes = kcamd::flashPagesPartBytes(*dims);
+    return kc::Error::Success;
+}
+
+kcError_t kcSampleRowsPartBytes(int rows, int n_vocab, size_t* bytes) noexcept {
+    if (!bytes || rows < 0 || rows > 65535 || n_vocab <= 0 || n_vocab > (1 << 20)) return kc::Error::InvalidValue;
+    *bytes = kcamd::sampleRowsPartBytes(rows, n_vocab);
     return kc::Error::Success;
 }
