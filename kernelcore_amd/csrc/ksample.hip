@@ -2,12 +2,15 @@
 //
 // Kept tokens are a prefix of the tokens in descending order, and the drawn one is where the cumulated weights reach a target; so
 // all that is asked of the order is where in it a count or a weight is reached. With z = l log2 e / T, tokens fall into bins of
-// 1/32 octave of weight below an integer `ref` at or above the largest z; counts and sums of the bins give each border's bin, and only the members of
-// those few bins are looked at one by one. Two kernels: the bins of pieces of rows; then a workgroup per row, which adds up the
-// pieces' bins, collects the members of the bins that borders may fall into, and finds the borders among them.
+// 1/32 octave of weight below an integer `ref` at or above the largest z; counts and weights of the bins give each border's bin, and only
+// the members of those few bins are looked at one by one. Two kernels: the bins of pieces of rows; then a workgroup per row, which adds
+// up the pieces' bins, collects the members of the bins that borders may fall into, and finds the borders among them.
 //
-// Weights are 2^(z - ref) to about 2^-52, as integers in steps of 2^-43: sums of integers do not depend on their order. (Weights in
-// 32 bits would move the borders by about 2^-24 of the whole, and a border of 150000 flat weights comes every 2^-17.)
+// A weight is 2^-((b + 1/2) / 32), its bin's factor, times g = 2^-(s / 32) for the token's place s in the bin, |s| <= 1/2. A bin's sum of g
+// is held as an integer in steps of 2^-38 (integers do not depend on the order of the atomics that add them up), with the
+// count in the same word: one 64-bit atomic in LDS and a polynomial of degree 5 for each token. The bins' weights are added up
+// in 64 bits, always in the same order. (Weights in 32 bits would move the borders by about 2^-24 of the whole, and among 150000 flat
+// weights there is a border every 2^-17.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -22,10 +25,13 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f4a4 __attribute__((aligned(4)));
 typedef unsigned long long u64;
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kThreads = 1024, kWaves = 16, kBins = 1024, kList = 6144;
+// 64 octaves in bins; the last bin takes what is further (a millionth of millionths of millionths of the largest weight): counted, but of weight 0
+constexpr int kThreads = 1024, kWaves = 16, kBins = 2048, kFar = kBins - 1, kList = 5120, kPieces = 64;
 constexpr double kPerOctave = 32.0;
-constexpr int kUnitBits = 43;  // (2^20 weights of up to 1 stay below 2^63)
+constexpr int kUnitBits = 38, kCountBit = 48;
+constexpr u64 kUnit = 1ull << kUnitBits;
 
 struct SampleArgs {
     const float *logits, *u, *temperature, *top_p, *min_p;
@@ -38,59 +44,57 @@ struct SampleArgs {
 };
 
 // A piece's bins in the workspace.
-struct Piece {
-    u64 sum[kBins];
-    unsigned count[kBins];
-    double ref;  // -infinity: no finite logit
-    int wild;    // NaN or +infinity among the logits
-    float top;   // the largest logit
+struct __attribute__((aligned(16))) Piece {
+    u64 bins[kBins];  // the count from bit 48 on, below it the sum of 2^38 (g - 1) + 2^32
+    float top;        // the largest logit; -infinity: no finite one
+    int wild;         // NaN or +infinity among the logits
+    unsigned finite;  // finite logits
 };
 
-// Octaves of weight per unit of logit. (Rows that take the likeliest token count as temperature 1.)
+// (Rows that take the likeliest token count as temperature 1.)
 __device__ __forceinline__ bool greedy(float t) { return !(t > 0.0f); }
+// Octaves of weight per unit of logit.
 __device__ __forceinline__ double slopeOf(const SampleArgs& a, int r) {
     const float t = a.temperature ? a.temperature[r] : 1.0f;
     return greedy(t) ? 1.4426950408889634 : 1.4426950408889634 / (double)t;
 }
-// 2^x for x <= 0 in steps of 2^-43: the series of exp(r ln 2), |r| <= 1/2, whose 13th term is below 2^-52.
-__device__ __forceinline__ u64 weightOf(double x) {
-    if (x < -50.0) return 0;
-    const double n = rint(x), r = (x - n) * 0.6931471805599453;
-    double p = 1.0 / 479001600.0;
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    const double scale = __builtin_bit_cast(double, (u64)(1023 + kUnitBits + (int)n) << 52);
-    return (u64)fma(p, scale, 0.5);
+// ref, and what the largest logit lies below it, in bins: within an octave, also where z is so large that integers are far apart.
+__device__ __forceinline__ double refOf(float top, double slope) { return ceil((double)top * slope); }
+__device__ __forceinline__ double offsetOf(float top, double slope, double ref) {
+    return kPerOctave * fmin(fmax(fma(-(double)top, slope, ref), 0.0), 1.0);
 }
-// The bin below ref; the last one takes all that is further.
-__device__ __forceinline__ int binOf(double z, double ref) {
-    const double d = (ref - z) * kPerOctave;
-    return d < kBins - 1 ? (int)d : kBins - 1;
+// A token's distance below ref in bins (slope32 = 32 slope), its bin, and what it adds to the bin's word. g - 1 by the series of
+// exp, whose sixth term is below 2^-48; added to 2^14 + 1 / 64, so that the sum's last bit is 2^-38 and its bits but the
+// last 33 are known.
+__device__ __forceinline__ double distanceOf(float l, double top, double slope32, double offset) { return fma(top - (double)l, slope32, offset); }
+__device__ __forceinline__ int binOf(double d) { return min((int)d, kFar); }
+__device__ __forceinline__ u64 wordOf(double d) {
+    const double s = __builtin_amdgcn_fract(d) - 0.5;
+    constexpr double a = -0.6931471805599453 / kPerOctave;
+    double p = a * a * a * a * a / 120.0;
+    p = fma(p, s, a * a * a * a / 24.0);
+    p = fma(p, s, a * a * a / 6.0);
+    p = fma(p, s, a * a / 2.0);
+    p = fma(p, s, a);
+    p = fma(p, s, 16384.0 + 1.0 / 64.0);
+    return __builtin_bit_cast(u64, p) + ((1ull << kCountBit) - 0x40D0000000000000ull);
 }
+// The sum of g of a bin of n tokens, from the sum of its words.
+__device__ __forceinline__ u64 unitsOf(u64 words, unsigned n) { return words + (u64)n * (kUnit - (1ull << 32)); }
+// The weight of a bin's unit.
+__device__ __forceinline__ double factorOf(int b) { return b < kFar ? exp2(-(b + 0.5) / kPerOctave - kUnitBits) : 0.0; }
 
 // ---------------------------------------------------------------------------------------------- bins of the pieces
-// 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins by atomics in LDS (the
-// last one, into which all of a peaked row's tail falls, in registers).
+// 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins.
 template <int R>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
-    __shared__ u64 sum[kBins];
-    __shared__ unsigned count[kBins];
+    __shared__ u64 bins[kBins];
     __shared__ float tops[kWaves];
-    __shared__ int wilds[kWaves];
+    __shared__ unsigned wilds[kWaves], finites[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = blockIdx.y, p0 = blockIdx.x * a.piece, n = min(a.piece, a.n - p0);
     const float* x = a.logits + (long long)r * a.row + p0;
-    const double c = slopeOf(a, r);
+    const double slope = slopeOf(a, r);
     f32x4 v[R / 4];
 #pragma unroll
     for (int k = 0; k < R / 4; ++k) {
@@ -102,73 +106,66 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
             for (int e = 0; e < 4; ++e) v[k][e] = at + e < n ? x[at + e] : -INFINITY;
         }
     }
-    sum[tid] = 0;
-    count[tid] = 0;
+    bins[tid] = 0;
+    bins[tid + kThreads] = 0;
     float top = -INFINITY;
     bool wild = false;
+    unsigned finite = 0;
 #pragma unroll
     for (int k = 0; k < R / 4; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             wild |= !(v[k][e] < INFINITY);
             top = fmaxf(top, v[k][e]);
+            finite += v[k][e] > -INFINITY;
         }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if (lane == 0) tops[wave] = top;
-    if (lane == 0) wilds[wave] = 0;
-    if (__any(wild) && lane == 0) wilds[wave] = 1;
+    for (int o = 32; o; o >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, o));
+        finite += __shfl_xor(finite, o);
+    }
+    const bool any = __any(wild);
+    if (lane == 0) {
+        tops[wave] = top;
+        wilds[wave] = any;
+        finites[wave] = finite;
+    }
     __syncthreads();
-    int any = 0;
+    unsigned bad = 0;
+    finite = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         top = fmaxf(top, tops[w]);
-        any |= wilds[w];
+        bad |= wilds[w];
+        finite += finites[w];
     }
     Piece& out = reinterpret_cast<Piece*>(a.part)[(size_t)r * a.pieces + blockIdx.x];
-    const bool empty = top == -INFINITY || any;
-    const double ref = ceil((double)top * c);
-    if (tid == 0) {
-        out.ref = empty ? -INFINITY : ref;
-        out.wild = any;
-        out.top = top;
-    }
+    const bool empty = top == -INFINITY || bad;
+    const double top64 = top, slope32 = kPerOctave * slope, offset = offsetOf(top, slope, refOf(top, slope));
     if (!empty) {
-        u64 far = 0;
-        unsigned farCount = 0;
-#pragma unroll 4
+#pragma unroll
         for (int k = 0; k < R / 4; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (v[k][e] == -INFINITY) continue;
-                const double z = (double)v[k][e] * c;
-                const int b = binOf(z, ref);
-                const u64 w = weightOf(z - ref);
-                if (b == kBins - 1) {
-                    far += w;
-                    ++farCount;
-                } else {
-                    atomicAdd(sum + b, w);
-                    atomicAdd(count + b, 1u);
+                const float l = v[k][e];
+                if (l > -INFINITY) {
+                    const double d = distanceOf(l, top64, slope32, offset);
+                    const int b = binOf(d);
+                    if (b < kFar) atomicAdd(bins + b, wordOf(d));  // (the others: those finite that no bin counts)
                 }
             }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) {
-            far += __shfl_xor(far, o);
-            farCount += __shfl_xor(farCount, o);
-        }
-        if (lane == 0 && farCount) {
-            atomicAdd(sum + kBins - 1, far);
-            atomicAdd(count + kBins - 1, farCount);
-        }
     }
     __syncthreads();
-    out.sum[tid] = sum[tid];
-    out.count[tid] = count[tid];
+    if (tid == 0) {
+        out.top = top;
+        out.wild = bad;
+        out.finite = finite;
+    }
+    *reinterpret_cast<u64x2*>(out.bins + 2 * tid) = *reinterpret_cast<const u64x2*>(bins + 2 * tid);
 }
 
 // ---------------------------------------------------------------------------------------------- borders and the draw
-// Tokens in order: codes that ascend with (falling logit, rising number), unique.
+// Tokens in order: codes of 52 bits that ascend with (falling logit, rising number).
 __device__ __forceinline__ u64 codeOf(float l, int at) {
     const uint32_t u = __builtin_bit_cast(uint32_t, l == 0.0f ? 0.0f : l);
     const uint32_t up = u & 0x80000000u ? ~u : u | 0x80000000u;  // ascending with l
@@ -178,98 +175,146 @@ __device__ __forceinline__ float logitOf(u64 code) {
     const uint32_t up = ~(uint32_t)(code >> 20);
     return __builtin_bit_cast(float, up & 0x80000000u ? up & 0x7FFFFFFFu : ~up);
 }
+constexpr u64 kCode = (1ull << 52) - 1;
 
 struct Shared {
-    u64 sum[kBins];         // weights up to and with a bin
+    double sum[kBins];      // weights up to and with a bin
     unsigned count[kBins];  // tokens likewise
-    u64 dsum[kBins];        // the digits of a search
-    unsigned dcount[kBins];
-    u64 list[kList];        // members of the wanted bins
+    u64 dsum[kThreads];     // the digits of a search
+    unsigned dcount[kThreads];
+    u64 list[kList];        // members of the wanted bins, the bin from bit 52 on
     u64 few[64];
+    double top[kPieces], offset[kPieces];
+    int shift[kPieces];     // bins that a piece's lie further down
     u64 waves[kWaves], waves2[kWaves];
-    u64 found[4];
-    int bins[8];
-    int listed, nfew;
+    u64 found[4], cut[4];
+    float rowTop;
+    int wild, bins[8], listed, nfew;
 };
 
-__device__ __forceinline__ u64 waveScan(u64 x, int lane) {
+// Sums up to and with this thread's of x and y.
+template <class X, class Y>
+__device__ __forceinline__ void scanTwo(X& x, Y& y, u64* wx, u64* wy, int tid) {
+    const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-        const u64 y = __shfl_up(x, o);
-        if (lane >= o) x += y;
+        const X p = __shfl_up(x, o);
+        const Y q = __shfl_up(y, o);
+        if (lane >= o) {
+            x += p;
+            y += q;
+        }
     }
-    return x;
-}
-// Sums up to and with this thread's of x and y.
-__device__ __forceinline__ void scanTwo(u64& x, u64& y, u64* wx, u64* wy, int tid) {
-    const int lane = tid & 63, wave = tid >> 6;
-    x = waveScan(x, lane);
-    y = waveScan(y, lane);
     __syncthreads();
     if (lane == 63) {
-        wx[wave] = x;
-        wy[wave] = y;
+        reinterpret_cast<X*>(wx)[wave] = x;
+        reinterpret_cast<Y*>(wy)[wave] = y;
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        x += w < wave ? wx[w] : 0;
-        y += w < wave ? wy[w] : 0;
+    X xb = 0;
+    Y yb = 0;
+    for (int w = 0; w < wave; ++w) {
+        xb += reinterpret_cast<X*>(wx)[w];
+        yb += reinterpret_cast<Y*>(wy)[w];
     }
+    x += xb;
+    y += yb;
+}
+
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float same(float x) { return __builtin_bit_cast(float, same(__builtin_bit_cast(int, x))); }
+__device__ __forceinline__ double same(double x) {
+    const u64 u = __builtin_bit_cast(u64, x);
+    return __builtin_bit_cast(double, (u64)(unsigned)same((int)(u >> 32)) << 32 | (unsigned)same((int)u));
 }
 
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     extern __shared__ int4 lds4[];
     Shared& S = *reinterpret_cast<Shared*>(lds4);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x;
+    // (the last rows first: they were read last, and lie in the caches still)
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = a.rows - 1 - blockIdx.x;
     const Piece* pieces = reinterpret_cast<const Piece*>(a.part) + (size_t)r * a.pieces;
     const float* x = a.logits + (long long)r * a.row;
-    const double c = slopeOf(a, r);
-    S.sum[tid] = 0;
-    S.count[tid] = 0;
-    if (tid == 0) S.listed = 0;
-    double ref = -INFINITY;
-    float top = -INFINITY;
-    int wild = 0;
-    for (int p = 0; p < a.pieces; ++p) {
-        ref = fmax(ref, pieces[p].ref);
-        top = fmaxf(top, pieces[p].top);
-        wild |= pieces[p].wild;
+    const double slope = slopeOf(a, r), slope32 = kPerOctave * slope;
+    unsigned finite = 0;
+    if (wave == 0) {
+        const bool in = lane < a.pieces;
+        const float mine = in ? pieces[lane].top : -INFINITY;
+        const bool wild = __any(in && pieces[lane].wild);
+        finite = in ? pieces[lane].finite : 0;
+        float top = mine;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            top = fmaxf(top, __shfl_xor(top, o));
+            finite += __shfl_xor(finite, o);
+        }
+        const bool none = mine == -INFINITY;
+        const double ref = refOf(mine, slope);
+        S.top[lane] = mine;
+        S.offset[lane] = offsetOf(mine, slope, ref);
+        S.shift[lane] = none ? kBins : (int)fmin((refOf(top, slope) - ref) * kPerOctave, (double)kBins);
+        if (lane == 0) {
+            S.rowTop = top;
+            S.wild = wild;
+            S.found[0] = finite;
+            S.listed = 0;
+        }
     }
-    if (wild || ref == -INFINITY) {
+    if (tid < 8) S.bins[tid] = kBins;
+    __syncthreads();
+    if (S.wild || S.rowTop == -INFINITY) {
         if (tid == 0) {
             a.tokens[r] = -1;
             if (a.probs) a.probs[r] = 0.0f;
         }
         return;
     }
-    __syncthreads();
-    // bins of a piece lie (ref - its ref) octaves further
-    auto shiftOf = [&](double pref) { return (int)fmin((ref - pref) * kPerOctave, (double)kBins); };
-    for (int p = 0; p < a.pieces; ++p) {
-        const double pref = pieces[p].ref;
-        if (pref == -INFINITY) continue;
-        const unsigned n = pieces[p].count[tid];
-        if (!n) continue;
-        const int down = (int)fmin(ref - pref, 63.0), to = min(kBins - 1, tid + shiftOf(pref));
-        const u64 w = pieces[p].sum[tid];
-        atomicAdd(S.sum + to, down ? ((w >> (down - 1)) + 1) >> 1 : w);
-        atomicAdd(S.count + to, n);
+    const double top = same(S.rowTop);
+    finite = same((int)S.found[0]);
+
+    // ---- the row's bins: two a thread, of all pieces (their shifts are multiples of 32)
+    unsigned n0 = 0, n1 = 0;
+    u64 w0 = 0, w1 = 0;
+    for (int p0 = 0; p0 < a.pieces; p0 += 4) {
+        u64x2 y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = min(p0 + k, a.pieces - 1), at = 2 * tid - S.shift[p];
+            const bool in = p0 + k < a.pieces && at >= 0;
+            y[k] = *reinterpret_cast<const u64x2*>(pieces[p].bins + max(at, 0));
+            if (!in) y[k] = u64x2{0, 0};
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            n0 += (unsigned)(y[k][0] >> kCountBit);
+            n1 += (unsigned)(y[k][1] >> kCountBit);
+            w0 += y[k][0] & ((1ull << kCountBit) - 1);
+            w1 += y[k][1] & ((1ull << kCountBit) - 1);
+        }
+    }
+    if (tid == kThreads - 1) n1 = w1 = 0;  // (the last bin)
+    const double f0 = factorOf(2 * tid), f1 = factorOf(2 * tid + 1);
+    const double s0 = f0 * (double)unitsOf(w0, n0), s1 = f1 * (double)unitsOf(w1, n1);
+    {
+        double s = s0 + s1;
+        unsigned n = n0 + n1;
+        const unsigned nMine = n;
+        scanTwo(s, n, S.waves, S.waves2, tid);
+        S.sum[2 * tid + 1] = s;
+        S.count[2 * tid] = n - nMine + n0;
+        S.count[2 * tid + 1] = tid == kThreads - 1 ? finite : n;
     }
     __syncthreads();
-    const u64 binSum = S.sum[tid], binCount = S.count[tid];
-    u64 sumTo = binSum, countTo = binCount;
-    scanTwo(sumTo, countTo, S.waves, S.waves2, tid);
-    S.sum[tid] = sumTo;
-    S.count[tid] = (unsigned)countTo;
-    if (tid < 8) S.bins[tid] = kBins;
+    S.sum[2 * tid] = (tid ? S.sum[2 * tid - 1] : 0.0) + s0;
+    if (tid == kThreads - 1) n1 = finite - S.count[kFar - 1];
     __syncthreads();
-    const unsigned finite = S.count[kBins - 1];
-    auto sumBefore = [&](int b) { return b ? S.sum[b - 1] : 0ull; };
-    // the first bin at which cond(sum, count up to it) holds, among all threads' bins; kBins if none
-    auto firstBin = [&](int slot, bool here) {
-        const unsigned long long v = __ballot(here);
-        if (v && lane == 0) atomicMin(S.bins + slot, wave * 64 + __builtin_ctzll(v));
+    auto sumBefore = [&](int b) { return b ? S.sum[b - 1] : 0.0; };
+    auto countBefore = [&](int b) { return b ? S.count[b - 1] : 0u; };
+    // the first bin with a token at which cond(bin) holds, kBins if none; to S.bins[slot]
+    auto firstBin = [&](int slot, auto&& cond) {
+        const bool c0 = n0 && cond(2 * tid), c1 = n1 && cond(2 * tid + 1);
+        const unsigned long long v = __ballot(c0 || c1);
+        if (v && lane == __builtin_ctzll(v)) atomicMin(S.bins + slot, 2 * tid + (c0 ? 0 : 1));
     };
 
     // ---- the cuts
@@ -278,119 +323,147 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     const int tk = a.top_k ? a.top_k[r] : 0;
     unsigned K = tk > 0 ? min((unsigned)tk, finite) : finite;
     if (greedy(t) || p <= 0.0f || mp > 1.0f) K = 1;
-    const bool cutP = p < 1.0f && K > 1, cutM = mp > 0.0f && K > 1;
+    bool cutP = p < 1.0f && K > 1, cutM = mp > 0.0f && K > 1;
     double u = a.u[r];
-    u = u > 0.0 ? u : 0.0;
-    // the largest token lies in the first bin that has one
-    firstBin(0, S.count[tid] > 0);
-    firstBin(1, S.count[tid] >= K);
+    u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
+    firstBin(0, [&](int) { return true; });  // the largest token's
+    firstBin(1, [&](int b) { return S.count[b] >= K; });
     __syncthreads();
-    const int b0 = S.bins[0], bK = S.bins[1];
-    // what is kept of top_k: between kLo and kHi
-    const bool cutK = K < S.count[bK];  // (else its bin is whole, and so is the sum)
-    u64 kLo = cutK ? sumBefore(bK) : S.sum[bK], kHi = S.sum[bK];
-    auto targetP = [&](u64 s) { return max((u64)ceil((double)p * (double)s), 1ull); };
+    const int b0 = same(S.bins[0]), bK = same(S.bins[1]);
+    // what top_k keeps: between kLo and kHi
+    const bool cutK = K < S.count[bK] && bK < kFar;  // (else its bin is whole, or of no weight)
+    const double kHi = S.sum[bK], kLo = cutK ? sumBefore(bK) : kHi;
     int bP0 = kBins, bP1 = kBins;
     if (cutP) {
-        firstBin(2, S.sum[tid] >= targetP(kLo));
-        firstBin(3, S.sum[tid] >= targetP(kHi));
+        firstBin(2, [&](int b) { return S.sum[b] >= p * kLo; });
+        firstBin(3, [&](int b) { return S.sum[b] >= p * kHi; });
     }
     __syncthreads();
     if (cutP) {
-        bP0 = min(S.bins[2], bK);
-        bP1 = min(S.bins[3], bK);
+        bP0 = min(same(S.bins[2]), bK);
+        bP1 = min(same(S.bins[3]), bK);
     }
     // min_p: where 2^(z - largest z) comes to it, a bin or so
     int bM0 = kBins, bM1 = kBins;
     if (cutM) {
-        const double d = -log2((double)mp) * kPerOctave + b0;  // (bins below the largest token's upper end)
-        bM0 = max(0, (int)fmin(d, 2000.0) - 1);
-        bM1 = min(kBins - 1, bM0 + 3);
-        bM0 = min(bM0, kBins - 1);
+        const double d = b0 - log2((double)mp) * kPerOctave;  // (bins below the upper end of the largest token's)
+        cutM = d < kFar - 4;                                  // (else it cuts off nothing that has a weight)
+        if (cutM) {
+            bM0 = max(0, (int)d - 1);
+            bM1 = bM0 + 3;
+        }
+        if (cutM && cutP && bM1 < bP0) {  // (top_p cuts further down: it does not matter)
+            cutP = false;
+            bP0 = bP1 = kBins;
+        } else if (cutM && cutP && bP1 < bM0) {
+            cutM = false;
+            bM0 = bM1 = kBins;
+        }
     }
     // the whole sum, and the draw's target: between these
     const int lo = min(min(bK, bP0), bM0), hi = min(min(bK, bP1), bM1);
-    const u64 sLo = cutP || cutM ? sumBefore(lo) : kLo, sHi = cutP || cutM ? S.sum[hi] : kHi;
-    auto targetU = [&](u64 s) { return s ? min((u64)((double)s * u), s - 1) : 0ull; };
-    firstBin(4, S.sum[tid] > targetU(sLo));
-    firstBin(5, S.sum[tid] > targetU(sHi));
+    const double sLo = cutP || cutM ? sumBefore(lo) : kLo, sHi = cutP || cutM ? S.sum[hi] : kHi;
+    firstBin(4, [&](int b) { return S.sum[b] > u * sLo; });
+    firstBin(5, [&](int b) { return S.sum[b] > u * sHi; });
     __syncthreads();
-    const int bU0 = min(S.bins[4], hi), bU1 = min(S.bins[5], hi);
+    const int bU0 = min(same(S.bins[4]), hi), bU1 = min(same(S.bins[5]), hi);
 
-    // ---- the members of those bins
-    const int from[4] = {cutK ? bK : kBins, bP0, bM0, bU0}, to[4] = {cutK ? bK : -1, cutP ? bP1 : -1, cutM ? min(bM1, kBins - 1) : -1, bU1};
-    float least[4], most[4];  // logits of a range, a bin further on either side (of the last bin: all)
+    // ---- the members of those bins: of the draw's, the cuts' by weight (which overlap where there are two), the cut's by count
+    const int from[3] = {bU0, min(bP0, bM0), cutK ? bK : kBins};
+    const int to[3] = {bU1, max(cutP ? bP1 : -1, cutM ? bM1 : -1), cutK ? bK : -1};
+    const double offset = offsetOf(same(S.rowTop), slope, refOf(same(S.rowTop), slope));
+    float least[3], most[3];  // their logits, and what rounding may take off
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const bool none = to[k] < from[k];
-        most[k] = none ? -INFINITY : (float)((ref - (from[k] - 1) / kPerOctave) / c);
-        least[k] = none ? INFINITY : to[k] == kBins - 1 ? -INFINITY : (float)((ref - (to[k] + 2) / kPerOctave) / c);
-        if (!none && !(most[k] > -INFINITY)) most[k] = INFINITY;  // (a slope of 0: all logits are in one bin)
-        if (!none && !(least[k] < INFINITY)) least[k] = -INFINITY;
-        if (!none) {  // (what rounding to 32 bits may take off)
-            most[k] += fabsf(most[k]) * 2.4e-7f;
-            least[k] -= fabsf(least[k]) * 2.4e-7f;
-        }
+    for (int k = 0; k < 3; ++k) {
+        const float hiL = (float)(top - (from[k] - offset) / slope32), loL = (float)(top - (to[k] + 1 - offset) / slope32);
+        const float slack = 2.4e-7f * fmaxf((float)fabs(top), 1.2e-38f);
+        const bool none = to[k] < from[k], all = slope == 0.0;  // (a slope of 0: all logits lie in one bin)
+        most[k] = same(none ? -INFINITY : all ? INFINITY : fmaf(fabsf(hiL), 2.4e-7f, hiL) + slack);
+        least[k] = same(none ? INFINITY : all ? -INFINITY : fminf(fmaf(fabsf(loL), -2.4e-7f, loL) - slack, 3.4e38f));
     }
-    auto wanted = [&](int b) {
-        bool w = false;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w |= b >= from[k] && b <= to[k];
-        return w;
+    auto near = [&](float l) {
+        return ((l >= least[0]) & (l <= most[0])) | ((l >= least[1]) & (l <= most[1])) | ((l >= least[2]) & (l <= most[2]));
     };
-    // f(code, bin) for every finite logit in a wanted bin
-    auto overRow = [&](auto&& f) {
-        for (int pc = 0; pc < a.pieces; ++pc) {
-            const double pref = pieces[pc].ref;
-            if (pref == -INFINITY) continue;
-            const int shift = shiftOf(pref), p0 = pc * a.piece, n = min(a.piece, a.n - p0);
-            auto one = [&](float l, int at) {
-                bool maybe = false;
+    auto binAt = [&](float l, int at) {
+        const int pc = at / a.piece;
+        return min(binOf(distanceOf(l, S.top[pc], slope32, S.offset[pc])) + S.shift[pc], kFar);
+    };
+    for (int i0 = 0; i0 < a.n; i0 += 4 * kThreads * 8) {
+        f32x4 v[8];
+        unsigned mask = 0;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) maybe |= l >= least[k] && l <= most[k];
-                if (!maybe || l == -INFINITY) return;
-                const int b = min(kBins - 1, binOf((double)l * c, pref) + shift);
-                if (wanted(b)) f(codeOf(l, at), b);
-            };
-            for (int i = 4 * tid; i < n; i += 4 * kThreads) {
-                if (i + 3 < n) {
-                    const f32x4 v = *reinterpret_cast<const f4a4*>(x + p0 + i);
+        for (int k = 0; k < 8; ++k) {
+            const int at = i0 + 4 * (kThreads * k + tid);
+            if (at + 3 < a.n) {
+                v[k] = *reinterpret_cast<const f4a4*>(x + at);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) one(v[e], p0 + i + e);
-                } else {
-                    for (int e = 0; e < n - i; ++e) one(x[p0 + i + e], p0 + i + e);
-                }
+                for (int e = 0; e < 4; ++e) v[k][e] = at + e < a.n ? x[at + e] : -INFINITY;
             }
         }
-    };
-    overRow([&](u64 code, int b) {
-        const int at = atomicAdd(&S.listed, 1);
-        if (at < kList) S.list[at] = code | (u64)b << 52;
-    });
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mask |= near(v[k][e]) && v[k][e] > -INFINITY ? 1u << (4 * k + e) : 0u;
+        if (mask) {
+            int pos = atomicAdd(&S.listed, __builtin_popcount(mask));
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (mask >> (4 * k + e) & 1u) {
+                        if (pos < kList) S.list[pos] = codeOf(v[k][e], i0 + 4 * (kThreads * k + tid) + e);
+                        ++pos;
+                    }
+        }
+    }
     __syncthreads();
-    const int listed = S.listed;
-    constexpr u64 kCode = (1ull << 52) - 1;
-    // (longer lists are not kept: the row is gone over again each time)
+    const int listed = same(S.listed);
+    if (listed <= kList) {
+        for (int i = tid; i < listed; i += kThreads) {
+            const u64 code = S.list[i];
+            S.list[i] = code | (u64)binAt(logitOf(code), (int)(code & 0xFFFFF)) << 52;
+        }
+    }
+    __syncthreads();
+    // f(code, bin) for the members of the wanted bins (and some others). A list that is too long is not kept: the row is gone over
+    // again each time.
     auto overList = [&](auto&& f) {
-        if (listed <= kList) {
-            for (int i = tid; i < listed; i += kThreads) f(S.list[i] & kCode, (int)(S.list[i] >> 52));
-        } else {
-            overRow(f);
+        const bool kept = listed <= kList;
+        const int n = kept ? listed : a.n;
+#pragma unroll 1
+        for (int i = tid; i < n; i += kThreads) {
+            u64 e;
+            if (kept) {
+                e = S.list[i];
+            } else {
+                const float l = x[i];
+                if (!near(l) || l == -INFINITY) continue;
+                e = codeOf(l, i) | (u64)binAt(l, i) << 52;
+            }
+            f(e & kCode, (int)(e >> 52));
         }
     };
-    auto unitsOf = [&](u64 code) { return weightOf((double)logitOf(code) * c - ref); };
+    // a token's part of its bin's sum: what the first kernel added for it
+    auto unitOf = [&](u64 code) {
+        const int pc = (int)(code & 0xFFFFF) / a.piece;
+        const u64 w = wordOf(distanceOf(logitOf(code), S.top[pc], slope32, S.offset[pc]));
+        return unitsOf(w & ((1ull << kCountBit) - 1), 1);
+    };
 
-    // Among the members of bin b, in order: the one at which the count reaches `want` (byCount), or the weights exceed `want`; found[0]: the
-    // weights up to and with it, found[1] its code, found[2] its own weight. Where rounding leaves no such member: the last one with a weight.
+    // Among the members of bin b, in order, the one with which the count (byCount) or the sum reaches `want`, the last one if none does:
+    // found[0]: the sum up to and with it, found[1] its code, found[2] its own part.
     auto search = [&](int b, u64 want, bool byCount) {
         u64 lowest = 0, highest = kCode, before = 0;
-        unsigned n = S.count[b] - (b ? S.count[b - 1] : 0), nBefore = 0;
+        unsigned n = S.count[b] - countBefore(b), nBefore = 0;
         while (n > 64) {
             // the members' range, then the digits of ten bits from its top
             __syncthreads();
             if (tid == 0) {
                 S.found[0] = ~0ull;
                 S.found[1] = 0;
+                S.bins[6] = kBins;
+                S.bins[7] = -1;
             }
             S.dsum[tid] = 0;
             S.dcount[tid] = 0;
@@ -414,26 +487,25 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
             __syncthreads();
             lowest = S.found[0];
             highest = S.found[1];
-            const int bits = 64 - __builtin_clzll((highest - lowest) | 1), shift = max(0, bits - 10);
+            const int shift = max(0, 64 - __builtin_clzll((highest - lowest) | 1) - 10);
             overList([&](u64 code, int bb) {
                 if (bb == b && code >= lowest && code <= highest) {
                     const int d = (int)((code - lowest) >> shift);
-                    atomicAdd(S.dsum + d, unitsOf(code));
+                    atomicAdd(S.dsum + d, unitOf(code));
                     atomicAdd(S.dcount + d, 1u);
                 }
             });
             __syncthreads();
-            const u64 ds = S.dsum[tid], dc = S.dcount[tid];
-            u64 w = ds, k = dc;
+            const u64 ds = S.dsum[tid];
+            const unsigned dc = S.dcount[tid];
+            u64 w = ds;
+            unsigned k = dc;
             scanTwo(w, k, S.waves, S.waves2, tid);
-            // the first digit that reaches it; if none does, the last that has a weight (a member)
-            const bool here = dc && (byCount ? nBefore + k >= want : before + w > want);
-            if (tid < 8) S.bins[tid] = tid == 6 ? kBins : -1;
+            const unsigned long long here = __ballot(dc && (byCount ? nBefore + k >= want : before + w >= want)), some = __ballot(dc != 0);
+            if (here && lane == 0) atomicMin(S.bins + 6, wave * 64 + __builtin_ctzll(here));
+            if (some && lane == 0) atomicMax(S.bins + 7, wave * 64 + 63 - __builtin_clzll(some));
             __syncthreads();
-            firstBin(6, here);
-            if (ds || (byCount && dc)) atomicMax(S.bins + 7, tid);
-            __syncthreads();
-            const int digit = S.bins[6] < kBins ? S.bins[6] : max(S.bins[7], 0);
+            const int digit = S.bins[6] < kBins ? S.bins[6] : S.bins[7];
             if (tid == digit) {
                 S.found[0] = w - ds;
                 S.found[1] = k - dc;
@@ -445,7 +517,6 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
             n = (unsigned)S.found[2];
             lowest += (u64)digit << shift;
             highest = min(highest, lowest + (1ull << shift) - 1);
-            if (n == 0) break;  // (a bin without weights: nothing is drawn from it)
         }
         __syncthreads();
         if (tid == 0) S.nfew = 0;
@@ -460,7 +531,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         if (wave == 0) {
             const int m = min(S.nfew, 64);
             const u64 mine = lane < m ? S.few[lane] : ~0ull;
-            const u64 w = lane < m ? unitsOf(mine) : 0;
+            const u64 w = lane < m ? unitOf(mine) : 0;
             u64 upTo = before;
             unsigned rank = nBefore;
             for (int i = 0; i < m; ++i) {
@@ -470,16 +541,14 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
                     ++rank;
                 }
             }
-            const bool reached = lane < m && (byCount ? rank >= want : upTo > want);
-            // the first that reaches it, or else the last with a weight
-            u64 best = reached ? mine : ~0ull, last = lane < m && (w || byCount) ? mine : 0;
+            const bool reached = lane < m && (byCount ? rank >= want : upTo >= want);
+            u64 best = reached ? mine : ~0ull, last = lane < m ? mine : 0;
 #pragma unroll
             for (int o = 32; o; o >>= 1) {
                 best = min(best, (u64)__shfl_xor(best, o));
                 last = max(last, (u64)__shfl_xor(last, o));
             }
-            const u64 pick = best != ~0ull ? best : last;
-            if (lane < m && mine == pick) {
+            if (lane < m && mine == (best != ~0ull ? best : last)) {
                 S.found[0] = upTo;
                 S.found[1] = mine;
                 S.found[2] = w;
@@ -487,55 +556,62 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         }
         __syncthreads();
     };
+    // the first bin from b on, up to last, with a token and cond; else the last with a token
+    auto walk = [&](int b, int last, auto&& cond) {
+        while (b < last && !(S.count[b] > countBefore(b) && cond(b))) ++b;
+        while (b > 0 && S.count[b] == countBefore(b)) --b;
+        return b;
+    };
+    auto unitsTo = [&](int b, double target) { return fmax(0.0, fmin((target - sumBefore(b)) / factorOf(b), 0x1p60)); };
 
-    u64 kept = kLo;  // the sum of what is kept
-    if (cutK) {
-        search(bK, K - (bK ? S.count[bK - 1] : 0), true);
-        kept = sumBefore(bK) + S.found[0];
-        __syncthreads();
-    }
-    const u64 keptK = kept;
-    if (cutP) {
-        const u64 want = targetP(keptK);
-        // (between bP0 and bP1)
-        int b = bP0;
-        while (b < bP1 && S.sum[b] < want) ++b;
-        if (want > sumBefore(b)) {
-            search(b, want - 1 - sumBefore(b), false);
-            kept = min(kept, sumBefore(b) + S.found[0]);
-        }
-        __syncthreads();
-    }
-    if (cutM) {
-        // what of bins bM0 .. bM1 comes up to min_p of the largest logit's weight
-        __syncthreads();
-        if (tid == 0) S.found[0] = 0;
-        __syncthreads();
-        const double zTop = (double)top * c, least2 = log2((double)mp);
-        u64 w = 0;
-        overList([&](u64 code, int b) {
-            if (b >= bM0 && b <= bM1 && (double)logitOf(code) * c - zTop >= least2) w += unitsOf(code);
-        });
+    double kept = kLo;  // the weight of what is kept
+    for (int stage = 0; stage < 3; ++stage) {  // the cuts by count and by weight, the draw
+        int b = bK;
+        u64 want;
+        if (stage == 0) {
+            if (!cutK) continue;
+            want = K - countBefore(bK);
+        } else if (stage == 1) {
+            if (!cutP) continue;
+            const double target = p * kept;
+            b = walk(bP0, bP1, [&](int k) { return S.sum[k] >= target; });
+            want = max((u64)ceil(unitsTo(b, target)), 1ull);
+        } else {
+            if (cutM) {  // what of bins bM0 .. bM1 comes up to min_p of the largest logit's weight
+                __syncthreads();
+                if (tid < 4) S.cut[tid] = 0;
+                __syncthreads();
+                const double least2 = log2((double)mp);
+                overList([&](u64 code, int bb) {
+                    if (bb >= bM0 && bb <= bM1 && ((double)logitOf(code) - top) * slope >= least2) atomicAdd(S.cut + (bb - bM0), unitOf(code));
+                });
+                __syncthreads();
+                double s = sumBefore(bM0);
 #pragma unroll
-        for (int o = 32; o; o >>= 1) w += __shfl_xor(w, o);
-        if (lane == 0 && w) atomicAdd(S.found, w);
-        __syncthreads();
-        kept = min(kept, sumBefore(bM0) + S.found[0]);
-        __syncthreads();
-    }
-    // ---- the draw
-    const u64 want = targetU(kept);
-    int b = bU0;
-    while (b < bU1 && S.sum[b] <= want) ++b;
-    search(b, want >= sumBefore(b) ? want - sumBefore(b) : 0, false);
-    if (tid == 0) {
-        a.tokens[r] = (int)(S.found[1] & 0xFFFFF);
-        if (a.probs) a.probs[r] = (float)((double)S.found[2] / (double)kept);
+                for (int k = 0; k < 4; ++k) s += factorOf(bM0 + k) * (double)S.cut[k];
+                kept = fmin(kept, s);
+            }
+            const double target = u * kept;
+            b = walk(bU0, bU1, [&](int k) { return S.sum[k] > target; });
+            want = (u64)unitsTo(b, target) + 1;
+        }
+        b = same(b);
+        search(b, want, stage == 0);
+        if (stage == 2) {
+            if (tid == 0) {
+                a.tokens[r] = (int)(S.found[1] & 0xFFFFF);
+                if (a.probs) a.probs[r] = (float)(factorOf(b) * (double)S.found[2] / kept);
+            }
+        } else {
+            const double s = sumBefore(b) + factorOf(b) * (double)S.found[0];
+            kept = stage == 0 ? s : fmin(kept, s);
+            __syncthreads();
+        }
     }
 }
 
 int piecesOf(int rows, int n, int* piece) {
-    // pieces of 16384 logits until they fill the GPU twice, of 32768 beyond (a piece's bins are 12 KiB to write and read)
+    // pieces of 16384 logits until they fill the GPU twice, of 32768 beyond (a piece's bins are 16 KiB to write and read)
     const int64_t small = ((int64_t)n + 16383) / 16384;
     *piece = small * rows <= 512 ? 16384 : 32768;
     return (int)(((int64_t)n + *piece - 1) / *piece);
