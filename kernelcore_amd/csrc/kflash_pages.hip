@@ -131,7 +131,7 @@ __device__ __forceinline__ constexpr int rowBits(int row) { return (row & 3) << 
 // Keys and values come by buffer-to-LDS loads, a step ahead, with a resource for each 16 positions (a page holds 16 at least) that
 // ends with the last valid one: what lies behind it in the page reads as zeros.
 template <int D, int NR, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG) void flash_pages_kernel(FpParams a) {
+__global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kernel(FpParams a) {
     using G = FpGeo<D, NR, RG, KG>;
     constexpr int NB = D / 32, DT = D / 16, RT = G::RT, NT = G::Threads;
     extern __shared__ int4 lds4[];
@@ -356,6 +356,7 @@ __global__ __launch_bounds__(64 * RG * KG) void flash_pages_kernel(FpParams a) {
         }
 
         // ---- the steps
+        const bool idle = rg * NR * 16 >= rows;  // (it loads for the others)
         int slot = 0;
         for (int st = st0; st < end; ++st, slot ^= 1) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(64 * RG * KG) void flash_pages_kernel(FpParams a) {
             valid = validNext;
             if (st + 1 < end) validNext = issue(st + 1, slot ^ 1);
             const int key0 = st * G::Step + 32 * kg;
-            if (key0 >= vis) continue;
+            if (key0 >= vis || idle) continue;
             const char* kt = mine + slot * G::Tile;
             const char* vt = kt + G::Tile / 2;
             float x[NR][8];
@@ -625,17 +626,21 @@ __global__ __launch_bounds__(256) void flash_pages_join_kernel(FpParams a, int r
     if (a.lse && c == 0) a.lse[at] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
 }
 
-// How a call is launched: rows of an item, workgroups, and the largest number of items.
+// How a call is launched: a form of the kernel, workgroups (as many as run at once), and the largest number of items. The forms differ in
+// the rows of an item; those of a sequence should lie in one, or its keys and values are read several times.
 struct FpPlan {
-    int rt, groups, items;
+    int form, rt, groups, items;
     size_t bytes;
 };
 FpPlan planOf(const kcFlashPagesDims& d) {
     FpPlan p{};
     const int64_t G = d.H / d.H_kv, rows = int64_t(d.N) * G;
     const int64_t each = d.seqs ? (rows + d.seqs - 1) / d.seqs : 0;  // a sequence's rows on average
-    p.rt = each <= 16 || d.D == 256 ? 16 : 32;
-    p.groups = d.D == 64 ? 512 : 256;
+    const bool wide = d.D == 256;
+    p.form = each <= 16 ? 0 : !wide && each <= 32 ? 1 : each <= (wide ? 64 : 128) ? 2 : 3;
+    constexpr int kRows[2][4] = {{16, 32, 128, 256}, {16, 16, 64, 128}};
+    p.rt = kRows[wide][p.form];
+    p.groups = p.form == 2 || (d.D == 64 && p.form < 2) ? 512 : 256;
     p.items = int((rows / p.rt + d.seqs) * d.H_kv);
     p.bytes = 16 + size_t(p.items) * 32 + size_t(p.groups) * 2 * p.rt * (d.D + 2) * 4;
     return p;
@@ -657,6 +662,18 @@ int run(FpParams p, const FpPlan& plan, hipStream_t s) {
         hipLaunchKernelGGL((flash_pages_join_kernel<D, 1>), dim3(plan.items, (G::RT + Rows - 1) / Rows), dim3(256), 0, s, p, G::RT);
     }
     return fromHip(hipGetLastError(), "flash_pages (join)");
+}
+
+// (heads of 256: 16 rows of a wavefront fill its registers, 64 positions of a step the LDS)
+template <int D>
+int runD(const FpParams& p, const FpPlan& plan, hipStream_t s) {
+    constexpr int NR = D == 256 ? 1 : 2;
+    switch (plan.form) {
+        case 0: return run<D, 1, 1, D == 256 ? 2 : 4>(p, plan, s);
+        case 1: return run<D, NR, 1, D == 256 ? 2 : 4>(p, plan, s);
+        case 2: return run<D, NR, 4, 1>(p, plan, s);
+        default: return run<D, NR, 8, 1>(p, plan, s);
+    }
 }
 
 }  // namespace
@@ -699,9 +716,9 @@ int launchFlashPages(const kcFlashPagesArgs& a, hipStream_t s) {
     p.items = plan.items;
     p.scale = a.scale;
     switch (d.D) {
-        case 64: return plan.rt == 16 ? run<64, 1, 1, 4>(p, plan, s) : run<64, 2, 1, 4>(p, plan, s);
-        case 128: return plan.rt == 16 ? run<128, 1, 1, 4>(p, plan, s) : run<128, 2, 1, 4>(p, plan, s);
-        case 256: return run<256, 1, 1, 2>(p, plan, s);
+        case 64: return runD<64>(p, plan, s);
+        case 128: return runD<128>(p, plan, s);
+        case 256: return runD<256>(p, plan, s);
         default: return fromHip(hipErrorInvalidValue, "flash_pages: D");
     }
 }

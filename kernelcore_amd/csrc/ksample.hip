@@ -87,7 +87,7 @@ __device__ __forceinline__ double factorOf(int b) { return b < kFar ? exp2(-(b +
 // ---------------------------------------------------------------------------------------------- bins of the pieces
 // 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins.
 template <int R>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) {
     __shared__ u64 bins[kBins];
     __shared__ float tops[kWaves];
     __shared__ unsigned wilds[kWaves], finites[kWaves];
