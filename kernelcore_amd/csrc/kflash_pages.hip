@@ -104,18 +104,44 @@ __device__ __forceinline__ void plainRow(const FpParams& a, const Item& it, int 
     }
 }
 
-template <int D, int NR, int RG, int KG>
+// A form of the kernel: W wavefronts of 16 NR rows, at most KM of them side by side over the keys.
+typedef __attribute__((address_space(3))) void* LdsPtr;
+// V^T of 64 of the head's values (4 operands) from value 64 J on, and its products. The transposed reads are written out: before
+// each of the builtin's the compiler waits for all loads into LDS under way.
+template <int D, int NR, int J>
+__device__ __forceinline__ void valuesTimesP(const uint32_t (&at)[4], const h8 (&ph)[NR], const h8 (&pl)[NR], f32x4 (&o)[NR][D / 16]) {
+    s4 x[4], y[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %3, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(128 * J), "n"(128 * J + 16 * 2 * D)
+        : "memory");
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const h8 va = __builtin_bit_cast(h8, __builtin_shufflevector(x[d], y[d], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            o[n][4 * J + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[n], o[n][4 * J + d], 0, 0, 0);
+            o[n][4 * J + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[n], o[n][4 * J + d], 0, 0, 0);
+        }
+    }
+    if constexpr (64 * (J + 1) < D) valuesTimesP<D, NR, J + 1>(at, ph, pl, o);
+}
+
+template <int D, int NR, int W, int KM>
 struct FpGeo {
-    static constexpr int RT = 16 * NR * RG, Waves = RG * KG, Threads = 64 * Waves;
-    static constexpr int Step = 32 * KG;                  // positions of a step
-    static constexpr int Tile = 2 * 32 * 2 * D;           // bytes of 32 keys and values
-    static constexpr int ORow = D + 4;                    // the join of the wavefronts: floats of a row
-    static constexpr int Loop = 2 * KG * Tile, Join = KG > 1 ? KG * RT * (ORow + 2) * 4 : 0;
+    static constexpr int RT = 16 * NR * W, Threads = 64 * W;  // rows of an item, at most
+    static constexpr int Tile = 2 * 32 * 2 * D;               // bytes of 32 keys and values
+    static constexpr int ORow = D + 4;                        // the join of the wavefronts: floats of a row
+    static constexpr int Loop = 2 * KM * Tile, Join = KM > 1 ? RT * (ORow + 2) * 4 : 0;
     static constexpr int Lds = Loop > Join ? Loop : Join;
-    static constexpr int Part = RT * (D + 2);             // floats of a sum: rows of D values, then m and l of each
+    static constexpr int Part = RT * (D + 2);                 // floats of a sum: rows of D values, then m and l of each
 };
 
-typedef __attribute__((address_space(3))) void* LdsPtr;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t bufRes(const char* p, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, bytes, 0x00020000);
 }
@@ -123,61 +149,61 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t bufRes(const char* p, int byte
 // of one chunk, and four rows' transposed reads of two, are on different banks.
 __device__ __forceinline__ constexpr int rowBits(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
 
-// Workgroup: RG groups of wavefronts with 16 NR rows each, KG of them with 32 keys of a step each.
+// A sequence of few rows has them in few wavefronts, and the others take other keys: RG wavefronts (a power of two) with 16 NR rows each,
+// KG = W / RG of these groups with 32 keys of a step each, RG the least that holds the rows (and leaves KG at most KM, for
+// which there is LDS).
 // Matrix form (v_mfma_f32_16x16x32_f16; lane (i, g), i < 16, g < 4):
 //   S^T = K Q^T: A = 16 keys (LDS; lane: key i, values 32 b + 8 g ..), B = q hi / lo (registers; row i). Lane holds keys 4 g + v of row i.
 //   O^T += V^T P^T: A = V^T by transposed LDS reads, B = p hi / lo, the score registers as they are: the products' index 8 g + e
 //   stands for key 16 (e / 4) + 4 g + e % 4.
 // Keys and values come by buffer-to-LDS loads, a step ahead, with a resource for each 16 positions (a page holds 16 at least) that
 // ends with the last valid one: what lies behind it in the page reads as zeros.
-template <int D, int NR, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kernel(FpParams a) {
-    using G = FpGeo<D, NR, RG, KG>;
+template <int D, int NR, int W, int KM>
+__global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpParams a) {
+    using G = FpGeo<D, NR, W, KM>;
     constexpr int NB = D / 32, DT = D / 16, RT = G::RT, NT = G::Threads;
     extern __shared__ int4 lds4[];
     char* lds = reinterpret_cast<char*>(lds4);
     __shared__ long long found[4];
-    __shared__ long long scan[G::Waves];
+    __shared__ long long scan[2][W];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int i = lane & 15, g = lane >> 4, rg = wave % RG, kg = wave / RG;
+    const int i = lane & 15, g = lane >> 4;
     const int wg = blockIdx.x;
 
-    // ---- this workgroup's share
-    auto nodesOf = [&](int s) {
+    // ---- this workgroup's share. A unit is what a step of 32 positions costs: a step over KG x 32 has KG (the cache's bytes bound it; two
+    // where eight wavefronts have rows of their own, whose products take as long as 64 positions take to load).
+    constexpr int lgW = W == 8 ? 3 : W == 4 ? 2 : 1, lgMin = W / KM == 4 ? 2 : W / KM == 2 ? 1 : 0, lgRows = NR == 2 ? 5 : 4;
+    static_assert(1 << lgW == W && KM << lgMin == W && 1 << lgRows == 16 * NR);
+    struct Seq {
+        int nodes, len, lg, blocks, steps, weight;  // tokens, positions, log2 RG, blocks of rows, steps, a step's units
+        long long units;                            // of all its items
+    };
+    const int most = a.max_pages << a.shift;
+    auto sequence = [&](int s) {
+        Seq q;
         const int x = min(max(a.start[s], 0), a.N), y = min(max(a.start[s + 1], 0), a.N);
-        return max(0, y - x);
+        q.nodes = max(0, y - x);
+        q.len = min(max(a.len[s], 0), most);
+        const int waves = (q.nodes * a.G + (1 << lgRows) - 1) >> lgRows;
+        q.lg = min(max(waves > 1 ? 32 - __builtin_clz(waves - 1) : 0, lgMin), lgW);
+        q.blocks = (waves + (1 << q.lg) - 1) >> q.lg;
+        const int sh = 5 + lgW - q.lg;
+        q.steps = max(1, (q.len >> sh) + ((q.len & ((1 << sh) - 1)) != 0));
+        q.weight = W == 8 && q.lg == lgW ? 2 : W >> q.lg;
+        q.units = (long long)q.blocks * a.H_kv * ((long long)q.steps * q.weight);
+        return q;
     };
-    const long long most = (long long)a.max_pages << a.shift;
-    auto lenOf = [&](int s) { return (int)min((long long)max(a.len[s], 0), most); };
-    auto stepsOf = [&](int len) { return max(1, len / G::Step + (len % G::Step != 0)); };
-    auto blocksOf = [&](int nodes) { return (int)(((long long)nodes * a.G + RT - 1) / RT); };
-    auto unitsOf = [&](int s) -> long long {
-        const int n = nodesOf(s);
-        return n ? (long long)blocksOf(n) * a.H_kv * stepsOf(lenOf(s)) : 0;
-    };
-    auto waveSum64 = [&](long long x) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-        return x;
-    };
-    long long total = 0;
-    for (int s = tid; s < a.seqs; s += NT) total += unitsOf(s);
-    total = waveSum64(total);
-    if (lane == 0) scan[wave] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < G::Waves; ++w) total += scan[w];
-    const long long share = max(1ll, (total + a.groups - 1) / a.groups);
-    const long long u0 = wg * share, u1 = min(total, u0 + share);
-    // the sequence of unit u0, the units and items before it
-    long long before = 0, items = 0;
-    if (tid == 0) found[0] = -1;
-    for (int s0 = 0; s0 < a.seqs; s0 += NT) {
-        const int s = s0 + tid;
-        const long long mine = s < a.seqs ? unitsOf(s) : 0;
-        const long long it = s < a.seqs ? (long long)blocksOf(nodesOf(s)) * a.H_kv : 0;
-        long long x = mine, y = it;
+    // (sums up to and with this thread's of its sequences' units and items, and over all threads)
+    long long total = 0, items = 0, mine = 0, upTo = 0, itemsTo = 0;
+    int myItems = 0;
+    auto round = [&](int s0) {
+        mine = myItems = 0;
+        if (s0 + tid < a.seqs) {
+            const Seq q = sequence(s0 + tid);
+            mine = q.units;
+            myItems = q.blocks * a.H_kv;
+        }
+        long long x = mine, y = myItems;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const long long z = __shfl_up(x, o), w = __shfl_up(y, o);
@@ -188,82 +214,96 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
         }
         __syncthreads();
         if (lane == 63) {
-            scan[wave] = x;
-            reinterpret_cast<long long*>(lds)[wave] = y;
+            scan[0][wave] = x;
+            scan[1][wave] = y;
         }
         __syncthreads();
-        long long xb = before + x - mine, yb = items + y - it;
+        upTo = total + x;
+        itemsTo = items + y;
 #pragma unroll
-        for (int w = 0; w < G::Waves; ++w) {
-            const long long p = scan[w], q = reinterpret_cast<long long*>(lds)[w];
-            if (w < wave) {
-                xb += p;
-                yb += q;
-            }
-            before += p;
-            items += q;
+        for (int w = 0; w < W; ++w) {
+            upTo += w < wave ? scan[0][w] : 0;
+            itemsTo += w < wave ? scan[1][w] : 0;
+            total += scan[0][w];
+            items += scan[1][w];
         }
-        if (mine && u0 >= xb && u0 < xb + mine) {
-            found[0] = s;
-            found[1] = xb;
-            found[2] = yb;
+    };
+    for (int s0 = 0; s0 < a.seqs; s0 += NT) round(s0);
+    if (wg == 0 && tid == 0) a.head[0] = (int)min(items, (long long)a.items);
+    // (a workgroup's units hold a step at least of each item that they touch: more than a step has, and a power of two of workgroups)
+    const long long share = max((long long)W, (total + a.groups - 1) >> (31 - __builtin_clz(a.groups)));
+    const long long u0 = wg * share, u1 = min(total, u0 + share);
+    if (u0 >= u1) return;
+    // the sequence of unit u0, the units and items before it
+    auto find = [&](int s0) {
+        if (mine && u0 >= upTo - mine && u0 < upTo) {
+            found[0] = s0 + tid;
+            found[1] = upTo - mine;
+            found[2] = itemsTo - myItems;
+        }
+    };
+    if (a.seqs <= NT) {
+        find(0);
+    } else {
+        total = items = 0;
+        for (int s0 = 0; s0 < a.seqs; s0 += NT) {
+            round(s0);
+            find(s0);
         }
     }
     __syncthreads();
-    if (wg == 0 && tid == 0) a.head[0] = (int)min(items, (long long)a.items);
-    if (u0 >= u1) return;
     int s = __builtin_amdgcn_readfirstlane((int)found[0]);
     long long sBefore = found[1];
     int sItems = __builtin_amdgcn_readfirstlane((int)min(found[2], (long long)a.items));
+    // x / y, x mostly small
+    auto over = [](long long x, long long y) { return x >> 31 || y >> 31 ? (int)(x / y) : (int)((unsigned)x / (unsigned)y); };
 
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    char* mine = lds + kg * 2 * G::Tile;
-    // the lane's share of a load's addresses: rows of a load, and where the chunks' permutation differs among loads
-    constexpr int CPR = D / 8, RPL = 64 / CPR, VAR = 8 / RPL, LPT = 32 / RPL;
-    int kvo[VAR], vvo[VAR];
-#pragma unroll
-    for (int x = 0; x < VAR; ++x) {
-        const int row = x * RPL + lane / CPR, chunk = lane % CPR ^ rowBits(row);
-        kvo[x] = (lane / CPR) * (int)a.k_row + 16 * chunk;
-        vvo[x] = (lane / CPR) * (int)a.v_row + 16 * chunk;
-    }
+    // a lane's share of a load's addresses (64 chunks of 16 bytes: RPL rows)
+    constexpr int CPR = D / 8, RPL = 64 / CPR, LPT = 32 / RPL;
+    const int chunk = 16 * (lane % CPR ^ rowBits(lane / CPR)), klane = lane / CPR * (int)a.k_row, vlane = lane / CPR * (int)a.v_row;
 
     for (long long u = u0; u < u1;) {
         // ---- the item of unit u
-        int nodes = nodesOf(s);
-        while (u >= sBefore + unitsOf(s)) {
-            sBefore += unitsOf(s);
-            sItems += blocksOf(nodes) * a.H_kv;
-            ++s;
-            nodes = nodesOf(s);
+        Seq q = sequence(s);
+        while (u >= sBefore + q.units) {
+            sBefore += q.units;
+            sItems += q.blocks * a.H_kv;
+            q = sequence(++s);
         }
+        const int RG = 1 << q.lg, KG = W >> q.lg, Step = 32 * KG, rg = wave & (RG - 1), kg = wave >> q.lg;
+        const int rt = (16 * NR) << q.lg;
+        char* tiles = lds + kg * 2 * G::Tile;
         Item it;
         it.token0 = min(max(a.start[s], 0), a.N);
-        it.nodes = nodes;
-        it.len = lenOf(s);
-        it.base = a.len[s] - nodes;
-        it.rows = nodes * a.G;
+        it.nodes = q.nodes;
+        it.len = q.len;
+        it.base = a.len[s] - q.nodes;
+        it.rows = q.nodes * a.G;
         it.table = a.table + (size_t)s * a.table_row;
-        const int steps = stepsOf(it.len);
-        const int at = (int)((u - sBefore) / steps), st0 = (int)(u - sBefore - (long long)at * steps);
-        const int blocks = blocksOf(nodes), item = sItems + at;
-        it.kvh = at / blocks;
-        it.r0 = (at - it.kvh * blocks) * RT;
-        const long long i0 = u - st0, i1 = i0 + steps;  // the item's units
-        const int st1 = (int)(min(u1, i1) - i0);
-        const bool whole = st0 == 0 && st1 == steps;
-        const int rows = min(RT, it.rows - it.r0);
-        u = min(u1, i1);
+        const long long per = (long long)q.steps * q.weight;  // an item's units
+        const int at = over(u - sBefore, per);
+        const long long i0 = sBefore + at * per;
+        const int item = sItems + at;
+        it.kvh = at / q.blocks;
+        it.r0 = (at - it.kvh * q.blocks) * rt;
+        // the steps whose first unit is in this workgroup's share
+        const int st0 = (int)(u - i0 + q.weight - 1) / q.weight;
+        const int st1 = (int)(min(u1 - i0, per) + q.weight - 1) / q.weight;
+        const bool whole = st0 == 0 && st1 == q.steps;
+        const int rows = min(rt, it.rows - it.r0);
+        u = min(u1, i0 + per);
         if (item >= a.items) return;  // (more rows than N tokens have: sequences that overlap)
+        if (st0 >= st1) continue;     // (the item's last steps began in the share before)
         if (st0 == 0 && tid < 8) {
-            const int w0 = wg, w1 = (int)((i1 - 1) / share);
-            const int d[8] = {it.token0, it.r0, rows, it.kvh, w0, w1 - w0 + 1, 0, 0};
+            const int n = over(i0 + (long long)(q.steps - 1) * q.weight - u0, share) + 1;
+            const int d[8] = {it.token0, it.r0, rows, it.kvh, wg, n, 0, 0};
             a.head[4 + 8 * item + tid] = d[tid];
         }
         // steps that some row sees
         const int lastNode = (it.r0 + rows - 1) / a.G;
         const int vis = a.tree ? it.len : (int)min((long long)it.len, max(0ll, (long long)it.base + lastNode + 1));
-        const int end = min(st1, vis / G::Step + (vis % G::Step != 0));
+        const int end = min(st1, vis / Step + (vis % Step != 0));
 
         // ---- loads
         const char* kb = a.k + it.kvh * a.k_head;
@@ -271,8 +311,8 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
         int window = 0, win0 = -1000;  // entries win0 + lane of the table row
         // (returns which of the 32 positions there are)
         auto issue = [&](int st, int slot) -> uint32_t {
-            const int p0 = st * G::Step, first = p0 >> a.shift;
-            if (first < win0 || ((p0 + G::Step - 1) >> a.shift) >= win0 + 64) {
+            const int p0 = st * Step, first = p0 >> a.shift;
+            if (first < win0 || ((p0 + Step - 1) >> a.shift) >= win0 + 64) {
                 win0 = first;
                 window = it.table[min(win0 + lane, a.max_pages - 1)];
             }
@@ -280,34 +320,28 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
             if (key0 >= vis) return 0;
             uint32_t valid = 0;
             // 16 positions' first slot (0 without a page), and how many of them there are
-            auto half = [&](int h, long long& slot0) {
+            auto half = [&](int h, int& slot0) {
                 const int key = key0 + 16 * h;
                 const int page = __builtin_amdgcn_readlane(window, (key >> a.shift) - win0 & 63);
                 const bool in = key < it.len && page >= 0 && page < a.n_pages;
                 const int n = in ? min(16, it.len - key) : 0;
                 valid |= ((1u << n) - 1) << 16 * h;
-                slot0 = in ? ((long long)page << a.shift) + (key & ((1 << a.shift) - 1)) : 0;
+                slot0 = in ? (page << a.shift) + (key & ((1 << a.shift) - 1)) : 0;
                 return n;
             };
-            long long s0, s1;
+            int s0, s1;
             const int n0 = half(0, s0), n1 = half(1, s1);
-            const auto rk0 = bufRes(kb + s0 * a.k_row, n0 ? (n0 - 1) * (int)a.k_row + 2 * D : 0);
-            const auto rk1 = bufRes(kb + s1 * a.k_row, n1 ? (n1 - 1) * (int)a.k_row + 2 * D : 0);
-            const auto rv0 = bufRes(vb + s0 * a.v_row, n0 ? (n0 - 1) * (int)a.v_row + 2 * D : 0);
-            const auto rv1 = bufRes(vb + s1 * a.v_row, n1 ? (n1 - 1) * (int)a.v_row + 2 * D : 0);
-            char* to = mine + slot * G::Tile;
-#pragma unroll
-            for (int L = 0; L < LPT; ++L) {
-                if (RG > 1 && L % RG != rg) continue;
-                const int ko = kvo[L % VAR] + L * RPL % 16 * (int)a.k_row, vo = vvo[L % VAR] + L * RPL % 16 * (int)a.v_row;
+            char* to = tiles + slot * G::Tile;
+            for (int L = rg; L < LPT; L += RG) {
+                const bool second = L >= LPT / 2;
+                const int n = second ? n1 : n0, bits = 16 * rowBits(L * RPL & 7), row = L * RPL & 15;
+                const long long at = second ? s1 : s0;
+                // (the sizes in scalar registers: without it a load is a loop over the lanes' resources)
+                const auto rk = bufRes(kb + at * (int)a.k_row, __builtin_amdgcn_readfirstlane(n ? (n - 1) * (int)a.k_row + 2 * D : 0));
+                const auto rv = bufRes(vb + at * (int)a.v_row, __builtin_amdgcn_readfirstlane(n ? (n - 1) * (int)a.v_row + 2 * D : 0));
                 char *kl = to + L * 1024, *vl = kl + G::Tile / 2;
-                if (L < LPT / 2) {
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk0, (LdsPtr)kl, 16, ko, 0, 0, 0);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv0, (LdsPtr)vl, 16, vo, 0, 0, 0);
-                } else {
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk1, (LdsPtr)kl, 16, ko, 0, 0, 0);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv1, (LdsPtr)vl, 16, vo, 0, 0, 0);
-                }
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (LdsPtr)kl, 16, (chunk ^ bits) + klane + row * (int)a.k_row, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (LdsPtr)vl, 16, (chunk ^ bits) + vlane + row * (int)a.v_row, 0, 0, 0);
             }
             return valid;
         };
@@ -360,32 +394,31 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
         int slot = 0;
         for (int st = st0; st < end; ++st, slot ^= 1) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (RG > 1) __syncthreads();  // every wavefront's loads are there, and the other buffer has been read
+            if (KM < W || RG > 1) __syncthreads();  // every wavefront's loads are there, and the other buffer has been read
             valid = validNext;
             if (st + 1 < end) validNext = issue(st + 1, slot ^ 1);
-            const int key0 = st * G::Step + 32 * kg;
+            const int key0 = st * Step + 32 * kg;
             if (key0 >= vis || idle) continue;
-            const char* kt = mine + slot * G::Tile;
+            const char* kt = tiles + slot * G::Tile;
             const char* vt = kt + G::Tile / 2;
             float x[NR][8];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                f32x4 sh[NR], sl[NR];
+                f32x4 sc[NR];
 #pragma unroll
-                for (int n = 0; n < NR; ++n) sh[n] = sl[n] = zero;
+                for (int n = 0; n < NR; ++n) sc[n] = zero;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const h8 ka = *reinterpret_cast<const h8*>(kt + (16 * t + i) * 2 * D + 16 * ((4 * b + g) ^ rowBits(i)));
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) {
-                        sh[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[n][b], sh[n], 0, 0, 0);
-                        sl[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[n][b], sl[n], 0, 0, 0);
-                    }
+                    for (int n = 0; n < NR; ++n) sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[n][b], sc[n], 0, 0, 0);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[n][b], sc[n], 0, 0, 0);
                 }
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) x[n][4 * t + v] = sh[n][v] + sl[n][v];
+                    for (int v = 0; v < 4; ++v) x[n][4 * t + v] = sc[n][v];
             }
             // what is not seen
             if (valid != ~0u || key0 + 32 > it.base) {
@@ -406,12 +439,14 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
             h8 ph[NR], pl[NR];
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
+                // (a lane's own keys first: the row's maximum over its four lanes is only needed where one of them runs ahead)
                 float bm = x[n][0];
 #pragma unroll
                 for (int v = 1; v < 8; ++v) bm = fmaxf(bm, x[n][v]);
-                bm = swap32Max(swap16Max(bm)) * c2[n];
-                const bool ahead = bm > m[n] + kLag;
-                if (__any(ahead)) {
+                bm *= c2[n];
+                if (__any(bm > m[n] + kLag)) {
+                    bm = swap32Max(swap16Max(bm));
+                    const bool ahead = bm > m[n] + kLag;
                     const float mn = ahead ? bm : m[n], alpha = ahead ? ex2(m[n] - mn) : 1.0f;
                     l[n] *= alpha;
 #pragma unroll
@@ -432,18 +467,11 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
                 pl[n] = lo[0];
             }
             const int vr = 4 * g + (i >> 2);  // (rows vr and vr + 16 have the same bits)
+            uint32_t at[4];
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const char* vp = vt + vr * 2 * D + 16 * ((2 * d + (i >> 1 & 1)) ^ rowBits(vr)) + 8 * (i & 1);
-                const s4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)vp);
-                const s4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(vp + 16 * 2 * D));
-                const h8 va = __builtin_bit_cast(h8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[n], o[n][d], 0, 0, 0);
-                    o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[n], o[n][d], 0, 0, 0);
-                }
-            }
+            for (int d = 0; d < 4; ++d)
+                at[d] = (uint32_t)(uintptr_t)(LdsPtr)(vt + vr * 2 * D + 16 * ((2 * d + (i >> 1 & 1)) ^ rowBits(vr)) + 8 * (i & 1));
+            valuesTimesP<D, NR, 0>(at, ph, pl, o);
         }
 
         // ---- the item's rows: to out, or to this workgroup's sums
@@ -463,7 +491,7 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
         };
         auto again = [&](int r) {  // a row that met an infinity or NaN
             float M, L, y[D / 64], *dst;
-            plainRow<D>(a, it, it.r0 + r, st0 * G::Step, min(st1 * G::Step, vis), lane, M, L, y);
+            plainRow<D>(a, it, it.r0 + r, st0 * Step, min(st1 * Step, vis), lane, M, L, y);
             rowOut(r, dst);
 #pragma unroll
             for (int e = 0; e < D / 64; ++e) dst[lane + 64 * e] = !whole ? y[e] : L == 0.0f ? 0.0f : y[e] / L;
@@ -474,7 +502,7 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
             l[n] += __shfl_xor(l[n], 16);
             l[n] += __shfl_xor(l[n], 32);
         }
-        if constexpr (KG == 1) {
+        if (KG == 1) {
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 const int r = (rg * NR + n) * 16 + i;
@@ -501,13 +529,13 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
                 }
             }
             if (u < u1) __syncthreads();
-        } else {
+        } else if constexpr (KM > 1) {
             __syncthreads();
             float* jo = reinterpret_cast<float*>(lds);
-            float* jm = jo + KG * RT * G::ORow;
+            float* jm = jo + RT * G::ORow;  // (rt KG = RT)
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                const int x = kg * RT + (rg * NR + n) * 16 + i;
+                const int x = kg * rt + (rg * NR + n) * 16 + i;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(jo + x * G::ORow + 16 * d + 4 * g) = o[n][d];
                 if (g == 0) {
@@ -520,18 +548,13 @@ __global__ __launch_bounds__(64 * RG * KG, RG > 1 ? 2 : 1) void flash_pages_kern
             static_assert(NT % LP == 0 && LP <= 64);
             for (int r0 = 0; r0 < rows; r0 += NT / LP) {  // (the same for a wavefront's lanes but for the row)
                 const int r = r0 + tid / LP, c = 4 * (tid % LP), rr = min(r, rows - 1);
-                float M = -INFINITY, L = 0.0f, mw[KG];
+                float M = -INFINITY, L = 0.0f;
                 f32x4 y = zero;
-#pragma unroll
+                for (int w = 0; w < KG; ++w) M = fmaxf(M, jm[2 * (w * rt + rr)]);
                 for (int w = 0; w < KG; ++w) {
-                    mw[w] = jm[2 * (w * RT + rr)];
-                    M = fmaxf(M, mw[w]);
-                }
-#pragma unroll
-                for (int w = 0; w < KG; ++w) {
-                    const float f = mw[w] == -INFINITY ? 0.0f : ex2(mw[w] - M);
-                    const f32x4 ow = *reinterpret_cast<const f32x4*>(jo + (w * RT + rr) * G::ORow + c);
-                    L = fmaf(f, jm[2 * (w * RT + rr) + 1], L);
+                    const float mw = jm[2 * (w * rt + rr)], f = mw == -INFINITY ? 0.0f : ex2(mw - M);
+                    const f32x4 ow = *reinterpret_cast<const f32x4*>(jo + (w * rt + rr) * G::ORow + c);
+                    L = fmaf(f, jm[2 * (w * rt + rr) + 1], L);
                     y += f * ow;
                 }
                 float bad = L;
@@ -564,102 +587,103 @@ __global__ __launch_bounds__(256) void flash_pages_join_kernel(FpParams a, int r
     __shared__ f32x4 sum[SG > 1 ? 256 : 1];
     __shared__ float2 ml[SG > 1 ? 256 / LP : 1];
     const int tid = threadIdx.x, c = 4 * (tid % LP), y = tid / LP, x = y / SG, sg = y % SG;
-    const int item = blockIdx.x, r = blockIdx.y * RB + x;
+    const int item = blockIdx.x;
     const int total = a.head[0];
     const int* d = a.head + 4 + 8 * item;
     const int token0 = d[0], r0 = d[1], rows = d[2], kvh = d[3], w0 = d[4], n = d[5];
-    if (item >= total || n <= 1 || (int)blockIdx.y * RB >= rows) return;
-    const int rr = min(r, rows - 1);
+    if (item >= total || n <= 1) return;
     const long long stride = 2ll * rt * (D + 2);  // between workgroups; the first one's sum is its second, the others' their first
     const float* p0 = a.part + (long long)w0 * stride + rt * (D + 2);
     const float* pn = a.part + (long long)(w0 + 1) * stride;
-    float M = -INFINITY, L = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int Ahead = 4;
-    for (int s0 = sg; s0 < n; s0 += SG * Ahead) {
-        f32x4 z[Ahead];
-        float ms[Ahead], ls[Ahead];
+    for (int b = blockIdx.y * RB; b < rows; b += gridDim.y * RB) {
+        const int r = b + x, rr = min(r, rows - 1);
+        float M = -INFINITY, L = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int Ahead = 4;
+        for (int s0 = sg; s0 < n; s0 += SG * Ahead) {
+            f32x4 z[Ahead];
+            float ms[Ahead], ls[Ahead];
 #pragma unroll
-        for (int k = 0; k < Ahead; ++k) {
-            const int s = min(s0 + SG * k, n - 1);
-            const float* p = s == 0 ? p0 : pn + (s - 1) * stride;
-            z[k] = *reinterpret_cast<const f4a4*>(p + rr * D + c);
-            ms[k] = p[rt * D + 2 * rr];
-            ls[k] = p[rt * D + 2 * rr + 1];
-        }
+            for (int k = 0; k < Ahead; ++k) {
+                const int s = min(s0 + SG * k, n - 1);
+                const float* p = s == 0 ? p0 : pn + (s - 1) * stride;
+                z[k] = *reinterpret_cast<const f4a4*>(p + rr * D + c);
+                ms[k] = p[rt * D + 2 * rr];
+                ls[k] = p[rt * D + 2 * rr + 1];
+            }
 #pragma unroll
-        for (int k = 0; k < Ahead; ++k) {
-            if (s0 + SG * k >= n) continue;
-            const float top = fmaxf(M, ms[k]);  // (a NaN l comes with any m)
-            const float f = M == -INFINITY ? 0.0f : ex2(M - top), h = ms[k] == -INFINITY ? 0.0f : ex2(ms[k] - top);
-            L = ls[k] != ls[k] ? ls[k] : fmaf(h, ls[k], f * L);
-            if (f != 1.0f) o = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * f;
-            if (h != 0.0f) o += h * z[k];
-            M = top;
+            for (int k = 0; k < Ahead; ++k) {
+                if (s0 + SG * k >= n) continue;
+                const float top = fmaxf(M, ms[k]);  // (a NaN l comes with any m)
+                const float f = M == -INFINITY ? 0.0f : ex2(M - top), h = ms[k] == -INFINITY ? 0.0f : ex2(ms[k] - top);
+                L = ls[k] != ls[k] ? ls[k] : fmaf(h, ls[k], f * L);
+                if (f != 1.0f) o = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * f;
+                if (h != 0.0f) o += h * z[k];
+                M = top;
+            }
         }
+        if constexpr (SG > 1) {
+            __syncthreads();  // (the last row's sums are read)
+            sum[tid] = o;
+            if (c == 0) ml[y] = make_float2(M, L);
+            __syncthreads();
+            float2 q[SG];
+#pragma unroll
+            for (int k = 0; k < SG; ++k) {
+                q[k] = ml[y - sg + k];
+                M = fmaxf(M, q[k].x);
+            }
+            L = 0.0f;
+            o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < SG; ++k) {
+                const float f = q[k].x == -INFINITY ? 0.0f : ex2(q[k].x - M);
+                L = q[k].y != q[k].y ? q[k].y : fmaf(f, q[k].y, L);
+                if (f != 0.0f) o += f * sum[tid + (k - sg) * LP];
+            }
+        }
+        if (r >= rows || sg) continue;
+        const int row = r0 + r, node = row / a.G, head = kvh * a.G + (row - node * a.G);
+        const size_t at = (size_t)(token0 + node) * a.H + head;
+        if (L != L) o = f32x4{NAN, NAN, NAN, NAN};
+        *reinterpret_cast<f4a4*>(a.out + at * D + c) = L == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / L);
+        if (a.lse && c == 0) a.lse[at] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
     }
-    if constexpr (SG > 1) {
-        sum[tid] = o;
-        if (c == 0) ml[y] = make_float2(M, L);
-        __syncthreads();
-        if (sg) return;
-        float2 q[SG];
-#pragma unroll
-        for (int k = 0; k < SG; ++k) {
-            q[k] = ml[y + k];
-            M = fmaxf(M, q[k].x);
-        }
-        L = 0.0f;
-        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < SG; ++k) {
-            const float f = q[k].x == -INFINITY ? 0.0f : ex2(q[k].x - M);
-            L = q[k].y != q[k].y ? q[k].y : fmaf(f, q[k].y, L);
-            if (f != 0.0f) o += f * sum[tid + k * LP];
-        }
-    }
-    if (r >= rows) return;
-    const int row = r0 + r, node = row / a.G, head = kvh * a.G + (row - node * a.G);
-    const size_t at = (size_t)(token0 + node) * a.H + head;
-    if (L != L) o = f32x4{NAN, NAN, NAN, NAN};
-    *reinterpret_cast<f4a4*>(a.out + at * D + c) = L == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / L);
-    if (a.lse && c == 0) a.lse[at] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
 }
 
-// How a call is launched: a form of the kernel, workgroups (as many as run at once), and the largest number of items. The forms differ in
-// the rows of an item; those of a sequence should lie in one, or its keys and values are read several times.
+// How a call is launched: the form by a sequence's rows on average, workgroups (as many as run at once), and the largest number of items.
 struct FpPlan {
-    int form, rt, groups, items;
+    int form, rt, groups, items, each;
     size_t bytes;
 };
 FpPlan planOf(const kcFlashPagesDims& d) {
     FpPlan p{};
     const int64_t G = d.H / d.H_kv, rows = int64_t(d.N) * G;
-    const int64_t each = d.seqs ? (rows + d.seqs - 1) / d.seqs : 0;  // a sequence's rows on average
+    const int64_t each = d.seqs ? (rows + d.seqs - 1) / d.seqs : 0;
     const bool wide = d.D == 256;
     p.form = each <= 16 ? 0 : !wide && each <= 32 ? 1 : each <= (wide ? 64 : 128) ? 2 : 3;
-    constexpr int kRows[2][4] = {{16, 32, 128, 256}, {16, 16, 64, 128}};
+    constexpr int kRows[2][4] = {{64, 128, 128, 256}, {32, 32, 64, 128}};
     p.rt = kRows[wide][p.form];
     p.groups = p.form == 2 || (d.D == 64 && p.form < 2) ? 512 : 256;
     p.items = int((rows / p.rt + d.seqs) * d.H_kv);
+    p.each = int(std::min<int64_t>(each, p.rt));
     p.bytes = 16 + size_t(p.items) * 32 + size_t(p.groups) * 2 * p.rt * (d.D + 2) * 4;
     return p;
 }
 
-template <int D, int NR, int RG, int KG>
+template <int D, int NR, int W, int KM>
 int run(FpParams p, const FpPlan& plan, hipStream_t s) {
-    using G = FpGeo<D, NR, RG, KG>;
-    static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(flash_pages_kernel<D, NR, RG, KG>),
+    using G = FpGeo<D, NR, W, KM>;
+    static const int ok = fromHip(hipFuncSetAttribute(reinterpret_cast<const void*>(flash_pages_kernel<D, NR, W, KM>),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, G::Lds), "flash_pages: LDS size");
     if (ok) return ok;
-    hipLaunchKernelGGL((flash_pages_kernel<D, NR, RG, KG>), dim3(plan.groups), dim3(G::Threads), G::Lds, s, p);
+    hipLaunchKernelGGL((flash_pages_kernel<D, NR, W, KM>), dim3(plan.groups), dim3(G::Threads), G::Lds, s, p);
     if (int e = fromHip(hipGetLastError(), "flash_pages")) return e;
     constexpr int Rows = 256 / (D / 4);
-    if (plan.items < plan.groups) {  // several workgroups to an item
-        constexpr int SG = Rows;
-        hipLaunchKernelGGL((flash_pages_join_kernel<D, SG>), dim3(plan.items, G::RT), dim3(256), 0, s, p, G::RT);
+    if (plan.items * 8 <= plan.groups) {  // many workgroups to an item
+        hipLaunchKernelGGL((flash_pages_join_kernel<D, Rows>), dim3(plan.items, std::max(1, plan.each)), dim3(256), 0, s, p, G::RT);
     } else {
-        hipLaunchKernelGGL((flash_pages_join_kernel<D, 1>), dim3(plan.items, (G::RT + Rows - 1) / Rows), dim3(256), 0, s, p, G::RT);
+        hipLaunchKernelGGL((flash_pages_join_kernel<D, 1>), dim3(plan.items, (plan.each + Rows - 1) / Rows), dim3(256), 0, s, p, G::RT);
     }
     return fromHip(hipGetLastError(), "flash_pages (join)");
 }
@@ -667,12 +691,12 @@ int run(FpParams p, const FpPlan& plan, hipStream_t s) {
 // (heads of 256: 16 rows of a wavefront fill its registers, 64 positions of a step the LDS)
 template <int D>
 int runD(const FpParams& p, const FpPlan& plan, hipStream_t s) {
-    constexpr int NR = D == 256 ? 1 : 2;
+    constexpr bool wide = D == 256;
     switch (plan.form) {
-        case 0: return run<D, 1, 1, D == 256 ? 2 : 4>(p, plan, s);
-        case 1: return run<D, NR, 1, D == 256 ? 2 : 4>(p, plan, s);
-        case 2: return run<D, NR, 4, 1>(p, plan, s);
-        default: return run<D, NR, 8, 1>(p, plan, s);
+        case 0: return run<D, 1, wide ? 2 : 4, wide ? 2 : 4>(p, plan, s);
+        case 1: return run<D, wide ? 1 : 2, wide ? 2 : 4, wide ? 2 : 4>(p, plan, s);
+        case 2: return run<D, wide ? 1 : 2, 4, wide ? 1 : 2>(p, plan, s);
+        default: return run<D, wide ? 1 : 2, 8, wide ? 2 : 4>(p, plan, s);
     }
 }
 

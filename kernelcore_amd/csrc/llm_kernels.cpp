@@ -731,6 +731,7 @@ int fpShape(const kcFlashPagesDims& d) {
         return invalid("flash_pages: H a positive multiple of H_kv, D 64, 128 or 256, counts not negative, page a power of two from 16 to 65536");
     if (int64_t(d.max_pages) * d.page > INT32_MAX - 65536 || d.table_row < d.max_pages)
         return invalid("flash_pages: a sequence's pages hold less than 2^31 - 65536 positions, table_row at least max_pages");
+    if (int64_t(d.n_pages) * d.page > INT32_MAX) return invalid("flash_pages: the cache holds less than 2^31 positions");
     if (d.tree_words < 0 || d.tree_words > 64) return invalid("flash_pages: tree_words from 0 to 64");
     if (d.q_tok < 0 || d.q_head < 0 || d.k_row < 0 || d.k_head < 0 || d.v_row < 0 || d.v_head < 0) return invalid("flash_pages: negative strides");
     const int64_t G = d.H / d.H_kv;
