@@ -402,24 +402,36 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
             const char* kt = tiles + slot * G::Tile;
             const char* vt = kt + G::Tile / 2;
             float x[NR][8];
+            // (2 NR independent sums, and a wavefront in its products before one in its weights: 240 to 230 us for 64 nodes of 8 sequences
+            // of 100000 positions; two sums took the products' latency each time)
+            f32x4 sc[2][NR];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 sc[NR];
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int n = 0; n < NR; ++n) sc[n] = zero;
+                for (int n = 0; n < NR; ++n) sc[t][n] = zero;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const h8 ka = *reinterpret_cast<const h8*>(kt + (16 * t + i) * 2 * D + 16 * ((4 * b + g) ^ rowBits(i)));
+            for (int b = 0; b < NB; ++b) {
+                h8 ka[2];
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[n][b], sc[n], 0, 0, 0);
+                for (int t = 0; t < 2; ++t)
+                    ka[t] = *reinterpret_cast<const h8*>(kt + (16 * t + i) * 2 * D + 16 * ((4 * b + g) ^ rowBits(i)));
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[n][b], sc[n], 0, 0, 0);
-                }
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) sc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t], ql[n][b], sc[t][n], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) sc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t], qh[n][b], sc[t][n], 0, 0, 0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) x[n][4 * t + v] = sc[n][v];
-            }
+                    for (int v = 0; v < 4; ++v) x[n][4 * t + v] = sc[t][n][v];
             // what is not seen
             if (valid != ~0u || key0 + 32 > it.base) {
 #pragma unroll
