@@ -28,7 +28,7 @@ typedef unsigned long long u64;
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
 // 64 octaves in bins; the last bin takes what is further (a millionth of millionths of millionths of the largest weight): counted, but of weight 0
-constexpr int kThreads = 1024, kWaves = 16, kBins = 2048, kFar = kBins - 1, kList = 5120, kPieces = 64;
+constexpr int kThreads = 1024, kWaves = 16, kDraw = 512, kBins = 2048, kFar = kBins - 1, kList = 5120, kGroups = 2048, kPieces = 64;
 constexpr double kPerOctave = 32.0;
 constexpr int kUnitBits = 38, kCountBit = 48;
 constexpr u64 kUnit = 1ull << kUnitBits;
@@ -49,6 +49,7 @@ struct __attribute__((aligned(16))) Piece {
     float top;        // the largest logit; -infinity: no finite one
     int wild;         // NaN or +infinity among the logits
     unsigned finite;  // finite logits
+    float tops[kThreads];  // the largest of the logits that a thread held (4 each 4096)
 };
 
 // (Rows that take the likeliest token count as temperature 1.)
@@ -119,6 +120,8 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) 
             top = fmaxf(top, v[k][e]);
             finite += v[k][e] > -INFINITY;
         }
+    Piece& out = reinterpret_cast<Piece*>(a.part)[(size_t)r * a.pieces + blockIdx.x];
+    out.tops[tid] = top;
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
         top = fmaxf(top, __shfl_xor(top, o));
@@ -139,7 +142,6 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) 
         bad |= wilds[w];
         finite += finites[w];
     }
-    Piece& out = reinterpret_cast<Piece*>(a.part)[(size_t)r * a.pieces + blockIdx.x];
     const bool empty = top == -INFINITY || bad;
     const double top64 = top, slope32 = kPerOctave * slope, offset = offsetOf(top, slope, refOf(top, slope));
     if (!empty) {
@@ -180,20 +182,21 @@ constexpr u64 kCode = (1ull << 52) - 1;
 struct Shared {
     double sum[kBins];      // weights up to and with a bin
     unsigned count[kBins];  // tokens likewise
-    u64 dsum[kThreads];     // the digits of a search
-    unsigned dcount[kThreads];
+    u64 dsum[kDraw];        // the digits of a search
+    unsigned dcount[kDraw];
     u64 list[kList];        // members of the wanted bins, the bin from bit 52 on
+    unsigned groups[kGroups];
     u64 few[64];
     double top[kPieces], offset[kPieces];
     int shift[kPieces];     // bins that a piece's lie further down
-    u64 waves[kWaves], waves2[kWaves];
+    u64 waves[kDraw / 64], waves2[kDraw / 64];
     u64 found[4], cut[4];
     float rowTop;
-    int wild, bins[8], listed, nfew;
+    int wild, bins[8], listed, grouped, nfew;
 };
 
 // Sums up to and with this thread's of x and y.
-template <class X, class Y>
+template <int Waves, class X, class Y>
 __device__ __forceinline__ void scanTwo(X& x, Y& y, u64* wx, u64* wy, int tid) {
     const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
@@ -213,9 +216,10 @@ __device__ __forceinline__ void scanTwo(X& x, Y& y, u64* wx, u64* wy, int tid) {
     __syncthreads();
     X xb = 0;
     Y yb = 0;
-    for (int w = 0; w < wave; ++w) {
-        xb += reinterpret_cast<X*>(wx)[w];
-        yb += reinterpret_cast<Y*>(wy)[w];
+#pragma unroll
+    for (int w = 0; w < Waves; ++w) {
+        xb += w < wave ? reinterpret_cast<X*>(wx)[w] : 0;
+        yb += w < wave ? reinterpret_cast<Y*>(wy)[w] : 0;
     }
     x += xb;
     y += yb;
@@ -228,14 +232,21 @@ __device__ __forceinline__ double same(double x) {
     return __builtin_bit_cast(double, (u64)(unsigned)same((int)(u >> 32)) << 32 | (unsigned)same((int)u));
 }
 
-__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
+// (512 threads: two workgroups on a CU, one's reads beside the other's searches; 512 rows of 151936: 117 us, 130 with 1024. One row: the same.)
+__global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     extern __shared__ int4 lds4[];
     Shared& S = *reinterpret_cast<Shared*>(lds4);
     // (the last rows first: they were read last, and lie in the caches still)
+    constexpr int NT = kDraw, BPT = kBins / NT, kDigitBits = 9;
+    static_assert(1 << kDigitBits == NT);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = a.rows - 1 - blockIdx.x;
     const Piece* pieces = reinterpret_cast<const Piece*>(a.part) + (size_t)r * a.pieces;
     const float* x = a.logits + (long long)r * a.row;
     const double slope = slopeOf(a, r), slope32 = kPerOctave * slope;
+    const float t = a.temperature ? a.temperature[r] : 1.0f;
+    const float p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
+    const int tk = a.top_k ? a.top_k[r] : 0;
+    double u = a.u[r];
     unsigned finite = 0;
     if (wave == 0) {
         const bool in = lane < a.pieces;
@@ -257,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
             S.rowTop = top;
             S.wild = wild;
             S.found[0] = finite;
-            S.listed = 0;
+            S.listed = S.grouped = 0;
         }
     }
     if (tid < 8) S.bins[tid] = kBins;
@@ -272,59 +283,72 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     const double top = same(S.rowTop);
     finite = same((int)S.found[0]);
 
-    // ---- the row's bins: two a thread, of all pieces (their shifts are multiples of 32)
-    unsigned n0 = 0, n1 = 0;
-    u64 w0 = 0, w1 = 0;
-    for (int p0 = 0; p0 < a.pieces; p0 += 4) {
-        u64x2 y[4];
+    // ---- the row's bins: BPT a thread, of all pieces (their shifts are multiples of 32)
+    unsigned cnt[BPT] = {};
+    u64 words[BPT] = {};
+    for (int p0 = 0; p0 < a.pieces; p0 += 8) {
+        u64x2 y[8][BPT / 2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int p = min(p0 + k, a.pieces - 1), at = 2 * tid - S.shift[p];
+        for (int k = 0; k < 8; ++k) {
+            const int pc = min(p0 + k, a.pieces - 1), at = BPT * tid - S.shift[pc];
             const bool in = p0 + k < a.pieces && at >= 0;
-            y[k] = *reinterpret_cast<const u64x2*>(pieces[p].bins + max(at, 0));
-            if (!in) y[k] = u64x2{0, 0};
+#pragma unroll
+            for (int e = 0; e < BPT / 2; ++e) {
+                y[k][e] = *reinterpret_cast<const u64x2*>(pieces[pc].bins + max(at, 0) + 2 * e);
+                if (!in) y[k][e] = u64x2{0, 0};
+            }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            n0 += (unsigned)(y[k][0] >> kCountBit);
-            n1 += (unsigned)(y[k][1] >> kCountBit);
-            w0 += y[k][0] & ((1ull << kCountBit) - 1);
-            w1 += y[k][1] & ((1ull << kCountBit) - 1);
-        }
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int e = 0; e < BPT; ++e) {
+                cnt[e] += (unsigned)(y[k][e / 2][e % 2] >> kCountBit);
+                words[e] += y[k][e / 2][e % 2] & ((1ull << kCountBit) - 1);
+            }
     }
-    if (tid == kThreads - 1) n1 = w1 = 0;  // (the last bin)
-    const double f0 = factorOf(2 * tid), f1 = factorOf(2 * tid + 1);
-    const double s0 = f0 * (double)unitsOf(w0, n0), s1 = f1 * (double)unitsOf(w1, n1);
+    if (tid == NT - 1) cnt[BPT - 1] = words[BPT - 1] = 0;  // (the last bin)
     {
-        double s = s0 + s1;
-        unsigned n = n0 + n1;
-        const unsigned nMine = n;
-        scanTwo(s, n, S.waves, S.waves2, tid);
-        S.sum[2 * tid + 1] = s;
-        S.count[2 * tid] = n - nMine + n0;
-        S.count[2 * tid + 1] = tid == kThreads - 1 ? finite : n;
+        double sums[BPT], sum = 0.0, own = 0.0;
+        unsigned n = 0;
+#pragma unroll
+        for (int e = 0; e < BPT; ++e) {
+            own += factorOf(BPT * tid + e) * (double)unitsOf(words[e], cnt[e]);
+            sums[e] = own;
+            n += cnt[e];
+        }
+        sum = own;
+        unsigned upTo = n;
+        scanTwo<NT / 64>(sum, upTo, S.waves, S.waves2, tid);
+        S.sum[BPT * tid + BPT - 1] = sum;
+        unsigned c = upTo - n;
+#pragma unroll
+        for (int e = 0; e < BPT; ++e) {
+            c += cnt[e];
+            S.count[BPT * tid + e] = c;
+        }
+        if (tid == NT - 1) S.count[kFar] = finite;
+        __syncthreads();
+        const double before = tid ? S.sum[BPT * tid - 1] : 0.0;
+#pragma unroll
+        for (int e = 0; e < BPT - 1; ++e) S.sum[BPT * tid + e] = before + sums[e];
+        if (tid == NT - 1) cnt[BPT - 1] = finite - S.count[kFar - 1];
     }
-    __syncthreads();
-    S.sum[2 * tid] = (tid ? S.sum[2 * tid - 1] : 0.0) + s0;
-    if (tid == kThreads - 1) n1 = finite - S.count[kFar - 1];
     __syncthreads();
     auto sumBefore = [&](int b) { return b ? S.sum[b - 1] : 0.0; };
     auto countBefore = [&](int b) { return b ? S.count[b - 1] : 0u; };
     // the first bin with a token at which cond(bin) holds, kBins if none; to S.bins[slot]
     auto firstBin = [&](int slot, auto&& cond) {
-        const bool c0 = n0 && cond(2 * tid), c1 = n1 && cond(2 * tid + 1);
-        const unsigned long long v = __ballot(c0 || c1);
-        if (v && lane == __builtin_ctzll(v)) atomicMin(S.bins + slot, 2 * tid + (c0 ? 0 : 1));
+        int first = kBins;
+#pragma unroll
+        for (int e = BPT - 1; e >= 0; --e) first = cnt[e] && cond(BPT * tid + e) ? BPT * tid + e : first;
+        const unsigned long long v = __ballot(first < kBins);
+        if (v && lane == __builtin_ctzll(v)) atomicMin(S.bins + slot, first);
     };
 
     // ---- the cuts
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
-    const float p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
-    const int tk = a.top_k ? a.top_k[r] : 0;
     unsigned K = tk > 0 ? min((unsigned)tk, finite) : finite;
     if (greedy(t) || p <= 0.0f || mp > 1.0f) K = 1;
     bool cutP = p < 1.0f && K > 1, cutM = mp > 0.0f && K > 1;
-    double u = a.u[r];
     u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
     firstBin(0, [&](int) { return true; });  // the largest token's
     firstBin(1, [&](int b) { return S.count[b] >= K; });
@@ -388,51 +412,95 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         const int pc = at / a.piece;
         return min(binOf(distanceOf(l, S.top[pc], slope32, S.offset[pc])) + S.shift[pc], kFar);
     };
-    for (int i0 = 0; i0 < a.n; i0 += 4 * kThreads * 8) {
-        f32x4 v[8];
+    auto collect = [&](const f32x4& v, int at) {
         unsigned mask = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int at = i0 + 4 * (kThreads * k + tid);
-            if (at + 3 < a.n) {
-                v[k] = *reinterpret_cast<const f4a4*>(x + at);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[k][e] = at + e < a.n ? x[at + e] : -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mask |= near(v[k][e]) && v[k][e] > -INFINITY ? 1u << (4 * k + e) : 0u;
+        for (int e = 0; e < 4; ++e) mask |= near(v[e]) && v[e] > -INFINITY ? 1u << e : 0u;
         if (mask) {
             int pos = atomicAdd(&S.listed, __builtin_popcount(mask));
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int e = 0; e < 4; ++e)
+                if (mask >> e & 1u) {
+                    if (pos < kList) S.list[pos] = codeOf(v[e], at + e);
+                    ++pos;
+                }
+        }
+    };
+    auto fourAt = [&](int at) {
+        f32x4 v;
+        if (at + 3 < a.n) {
+            v = *reinterpret_cast<const f4a4*>(x + at);
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (mask >> (4 * k + e) & 1u) {
-                        if (pos < kList) S.list[pos] = codeOf(v[k][e], i0 + 4 * (kThreads * k + tid) + e);
-                        ++pos;
-                    }
+            for (int e = 0; e < 4; ++e) v[e] = at + e < a.n ? x[at + e] : -INFINITY;
+        }
+        return v;
+    };
+    // The groups whose largest logit is not below all of them: few where the borders are among a row's first tokens (one row of 128256
+    // with top_k 40: 4.5 us, 14 for all logits). Of more than there is room for all logits are read.
+    const float lowest = fminf(fminf(least[0], least[1]), least[2]);
+    for (int p0 = 0; p0 < a.pieces; p0 += 8) {
+        float tops[8];
+#pragma unroll
+        for (int h = 0; h < kThreads / NT; ++h) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) tops[k] = pieces[min(p0 + k, a.pieces - 1)].tops[tid + NT * h];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (p0 + k < a.pieces && tops[k] >= lowest) {
+                    const int at = atomicAdd(&S.grouped, 1);
+                    if (at < kGroups) S.groups[at] = (p0 + k) * a.piece + 4 * (tid + NT * h);
+                }
+        }
+    }
+    __syncthreads();
+    const int grouped = same(S.grouped);
+    if (grouped <= kGroups) {
+        const int per = a.piece / (4 * kThreads), lgPer = per == 8 ? 3 : 2;
+        for (int c0 = tid; c0 < grouped << lgPer; c0 += 4 * NT) {
+            f32x4 v[4];
+            int at[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = c0 + NT * k;
+                at[k] = c < grouped << lgPer ? (int)S.groups[c >> lgPer] + 4 * kThreads * (c & (per - 1)) : a.n;
+                v[k] = fourAt(at[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) collect(v[k], at[k]);
+        }
+    } else {
+        for (int i0 = 4 * tid; i0 < a.n; i0 += 4 * NT * 8) {
+            f32x4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = fourAt(i0 + 4 * NT * k);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) collect(v[k], i0 + 4 * NT * k);
         }
     }
     __syncthreads();
     const int listed = same(S.listed);
+    // (no more than a wavefront has lanes: the first one does the rest by itself)
+    const bool alone = listed <= 64;
+    if (alone && wave) return;
+    auto sync = [&]() {
+        if (!alone) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
     if (listed <= kList) {
-        for (int i = tid; i < listed; i += kThreads) {
+        for (int i = tid; i < listed; i += NT) {
             const u64 code = S.list[i];
             S.list[i] = code | (u64)binAt(logitOf(code), (int)(code & 0xFFFFF)) << 52;
         }
     }
-    __syncthreads();
+    sync();
     // f(code, bin) for the members of the wanted bins (and some others). A list that is too long is not kept: the row is gone over
     // again each time.
     auto overList = [&](auto&& f) {
         const bool kept = listed <= kList;
         const int n = kept ? listed : a.n;
 #pragma unroll 1
-        for (int i = tid; i < n; i += kThreads) {
+        for (int i = tid; i < n; i += NT) {
             u64 e;
             if (kept) {
                 e = S.list[i];
@@ -458,7 +526,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         unsigned n = S.count[b] - countBefore(b), nBefore = 0;
         while (n > 64) {
             // the members' range, then the digits of ten bits from its top
-            __syncthreads();
+            sync();
             if (tid == 0) {
                 S.found[0] = ~0ull;
                 S.found[1] = 0;
@@ -467,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
             }
             S.dsum[tid] = 0;
             S.dcount[tid] = 0;
-            __syncthreads();
+            sync();
             u64 mn = ~0ull, mx = 0;
             overList([&](u64 code, int bb) {
                 if (bb == b && code >= lowest && code <= highest) {
@@ -484,10 +552,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
                 atomicMin(S.found, mn);
                 atomicMax(S.found + 1, mx);
             }
-            __syncthreads();
+            sync();
             lowest = S.found[0];
             highest = S.found[1];
-            const int shift = max(0, 64 - __builtin_clzll((highest - lowest) | 1) - 10);
+            const int shift = max(0, 64 - __builtin_clzll((highest - lowest) | 1) - kDigitBits);
             overList([&](u64 code, int bb) {
                 if (bb == b && code >= lowest && code <= highest) {
                     const int d = (int)((code - lowest) >> shift);
@@ -495,39 +563,39 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
                     atomicAdd(S.dcount + d, 1u);
                 }
             });
-            __syncthreads();
+            sync();
             const u64 ds = S.dsum[tid];
             const unsigned dc = S.dcount[tid];
             u64 w = ds;
             unsigned k = dc;
-            scanTwo(w, k, S.waves, S.waves2, tid);
+            scanTwo<NT / 64>(w, k, S.waves, S.waves2, tid);
             const unsigned long long here = __ballot(dc && (byCount ? nBefore + k >= want : before + w >= want)), some = __ballot(dc != 0);
             if (here && lane == 0) atomicMin(S.bins + 6, wave * 64 + __builtin_ctzll(here));
             if (some && lane == 0) atomicMax(S.bins + 7, wave * 64 + 63 - __builtin_clzll(some));
-            __syncthreads();
+            sync();
             const int digit = S.bins[6] < kBins ? S.bins[6] : S.bins[7];
             if (tid == digit) {
                 S.found[0] = w - ds;
                 S.found[1] = k - dc;
                 S.found[2] = dc;
             }
-            __syncthreads();
+            sync();
             before += S.found[0];
             nBefore += (unsigned)S.found[1];
             n = (unsigned)S.found[2];
             lowest += (u64)digit << shift;
             highest = min(highest, lowest + (1ull << shift) - 1);
         }
-        __syncthreads();
+        sync();
         if (tid == 0) S.nfew = 0;
-        __syncthreads();
+        sync();
         overList([&](u64 code, int bb) {
             if (bb == b && code >= lowest && code <= highest) {
                 const int at = atomicAdd(&S.nfew, 1);
                 if (at < 64) S.few[at] = code;
             }
         });
-        __syncthreads();
+        sync();
         if (wave == 0) {
             const int m = min(S.nfew, 64);
             const u64 mine = lane < m ? S.few[lane] : ~0ull;
@@ -554,7 +622,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
                 S.found[2] = w;
             }
         }
-        __syncthreads();
+        sync();
     };
     // the first bin from b on, up to last, with a token and cond; else the last with a token
     auto walk = [&](int b, int last, auto&& cond) {
@@ -578,14 +646,14 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
             want = max((u64)ceil(unitsTo(b, target)), 1ull);
         } else {
             if (cutM) {  // what of bins bM0 .. bM1 comes up to min_p of the largest logit's weight
-                __syncthreads();
+                sync();
                 if (tid < 4) S.cut[tid] = 0;
-                __syncthreads();
+                sync();
                 const double least2 = log2((double)mp);
                 overList([&](u64 code, int bb) {
                     if (bb >= bM0 && bb <= bM1 && ((double)logitOf(code) - top) * slope >= least2) atomicAdd(S.cut + (bb - bM0), unitOf(code));
                 });
-                __syncthreads();
+                sync();
                 double s = sumBefore(bM0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s += factorOf(bM0 + k) * (double)S.cut[k];
@@ -605,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         } else {
             const double s = sumBefore(b) + factorOf(b) * (double)S.found[0];
             kept = stage == 0 ? s : fmin(kept, s);
-            __syncthreads();
+            sync();
         }
     }
 }
@@ -634,7 +702,7 @@ int launchSampleRows(const kcSampleRowsArgs& a, hipStream_t s) {
     if (p.piece == 16384) hipLaunchKernelGGL(sample_bins_kernel<16>, dim3(p.pieces, a.rows), dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL(sample_bins_kernel<32>, dim3(p.pieces, a.rows), dim3(kThreads), 0, s, p);
     if (int e = fromHip(hipGetLastError(), "sample_rows (bins)")) return e;
-    hipLaunchKernelGGL(sample_draw_kernel, dim3(a.rows), dim3(kThreads), sizeof(Shared), s, p);
+    hipLaunchKernelGGL(sample_draw_kernel, dim3(a.rows), dim3(kDraw), sizeof(Shared), s, p);
     return fromHip(hipGetLastError(), "sample_rows");
 }
 
