@@ -19,7 +19,7 @@ typedef f32x4 f4a4 __attribute__((aligned(4)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef h4 h4a2 __attribute__((aligned(2)));
 
-constexpr int kThreads = 256, kPairs = 1024;  // pairs of a workgroup's tokens
+constexpr int kThreads = 256, kAhead = 2, kPairs = 1024;  // pairs of a workgroup's tokens
 
 struct RopeArgs {
     const float *q, *k, *v;
@@ -104,8 +104,10 @@ __device__ __forceinline__ void turn(f32x4& a, f32x4& b, const float2* cs, int p
     }
 }
 
-// A workgroup takes all heads of q, or all of k and v, of q_tokens or kv_tokens tokens: the angles once into LDS, then eight values a
-// thread at a time, loaded before the angles are there.
+// A workgroup takes all heads of q, or all of k and v, of q_tokens or kv_tokens tokens, eight values a thread at a time. The first kAhead
+// of a thread's are loaded before the angles are computed (once, into LDS) and repeated slots looked for: what bounds it is the
+// bytes, and for few tokens the latency of one load and the angles. 3333 tokens of 24 + 2 x 8 heads of 128: 29.7 us, 4.1 TB/s (35 with
+// loads after the angles, 31 with four ahead); one token 3.9 us.
 template <bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
     __shared__ float2 cs[kPairs];
@@ -116,6 +118,40 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
     const int t0 = (isQ ? blockIdx.x : blockIdx.x - a.q_blocks) * per, n = min(per, a.n - t0);
     const int pairs = a.n_rot / 2;
     const int turned = (pairs + 3) / 4, units = turned + (a.D - a.n_rot + 7) / 8, vunits = (a.D + 7) / 8;
+    const int heads = isQ ? a.H : a.H_kv, first = n * heads * units, all = first + (!isQ && a.v ? n * heads * vunits : 0);
+    // where the x-th eight values are
+    struct Place {
+        const float* src;
+        Unit u;
+        int t, h;
+        bool isV;
+    };
+    auto placeOf = [&](int x) {
+        Place p;
+        p.isV = x >= first;
+        const int y = p.isV ? x - first : x, uu = p.isV ? vunits : units, row = y / uu;
+        p.t = row / heads;
+        p.h = row - p.t * heads;
+        p.u = unitOf<INTER>(y - row * uu, p.isV ? 0 : a.n_rot, a.D);
+        p.src = isQ ? a.q + (long long)(t0 + p.t) * a.q_tok + (long long)p.h * a.q_head
+              : p.isV ? a.v + (long long)(t0 + p.t) * a.v_tok + (long long)p.h * a.v_head
+                      : a.k + (long long)(t0 + p.t) * a.k_tok + (long long)p.h * a.k_head;
+        return p;
+    };
+    Place at[kAhead];
+    f32x4 lo[kAhead], hi[kAhead];
+    auto load = [&](int x0) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int x = x0 + kThreads * k;
+            if (x < all) {
+                at[k] = placeOf(x);
+                lo[k] = loadPart(at[k].src + at[k].u.a, at[k].u.na);
+                hi[k] = loadPart(at[k].src + at[k].u.b, at[k].u.nb);
+            }
+        }
+    };
+    load(tid);
     if (!isQ && tid < 16) {
         later[tid] = 0;
         const long long slot = tid < n ? a.slots[t0 + tid] : -1;
@@ -128,43 +164,35 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
         cs[x] = make_float2(cospif(f) * a.scale, sinpif(f) * a.scale);
     }
     __syncthreads();
-    if (isQ) {
-        const int all = n * a.H * units;
-        for (int x = tid; x < all; x += kThreads) {
-            const int row = x / units, t = row / a.H, h = row - t * a.H;
-            const Unit u = unitOf<INTER>(x - row * units, a.n_rot, a.D);
-            const float* src = a.q + (long long)(t0 + t) * a.q_tok + (long long)h * a.q_head;
-            float* dst = a.q_out + (long long)(t0 + t) * a.out_tok + (long long)h * a.out_head;
-            f32x4 p = loadPart(src + u.a, u.na), q = loadPart(src + u.b, u.nb);
-            if (u.pair >= 0) turn<INTER>(p, q, cs + t * pairs + u.pair, pairs - u.pair);
-            storePart(dst + u.a, p, u.na);
-            storePart(dst + u.b, q, u.nb);
+    if (!isQ) {
+        // tokens whose slot a later one repeats are left to that one
+        for (int x = t0 + 1 + tid; x < a.n; x += kThreads) {
+            const long long slot = a.slots[x];
+            if (slot < 0 || slot >= a.cache_rows) continue;
+            for (int t = 0; t < n; ++t)
+                if (t0 + t < x && rowOf[t] == (int)slot) later[t] = 1;
         }
-        return;
+        __syncthreads();
     }
-    // tokens whose slot a later one repeats are left to that one
-    for (int x = t0 + 1 + tid; x < a.n; x += kThreads) {
-        const long long slot = a.slots[x];
-        if (slot < 0 || slot >= a.cache_rows) continue;
-        for (int t = 0; t < n; ++t)
-            if (t0 + t < x && rowOf[t] == (int)slot) later[t] = 1;
-    }
-    __syncthreads();
-    const int kall = n * a.H_kv * units, vall = a.v ? n * a.H_kv * vunits : 0;
-    for (int x = tid; x < kall + vall; x += kThreads) {
-        const bool isV = x >= kall;
-        const int y = isV ? x - kall : x, uu = isV ? vunits : units;
-        const int row = y / uu, t = row / a.H_kv, h = row - t * a.H_kv;
-        if (rowOf[t] < 0 || later[t]) continue;
-        const Unit u = unitOf<INTER>(y - row * uu, isV ? 0 : a.n_rot, a.D);
-        const float* src = isV ? a.v + (long long)(t0 + t) * a.v_tok + (long long)h * a.v_head
-                               : a.k + (long long)(t0 + t) * a.k_tok + (long long)h * a.k_head;
-        char* to = isV ? a.v_cache + rowOf[t] * a.vc_row + h * a.vc_head : a.k_cache + rowOf[t] * a.kc_row + h * a.kc_head;
-        _Float16* dst = reinterpret_cast<_Float16*>(to);
-        f32x4 p = loadPart(src + u.a, u.na), q = loadPart(src + u.b, u.nb);
-        if (u.pair >= 0) turn<INTER>(p, q, cs + t * pairs + u.pair, pairs - u.pair);
-        storePart(dst + u.a, p, u.na);
-        storePart(dst + u.b, q, u.nb);
+    for (int x0 = tid; x0 < all; x0 += kThreads * kAhead) {
+        if (x0 != tid) load(x0);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (x0 + kThreads * k >= all) break;
+            const Unit& u = at[k].u;
+            const int t = at[k].t, h = at[k].h;
+            if (u.pair >= 0 && !at[k].isV) turn<INTER>(lo[k], hi[k], cs + t * pairs + u.pair, pairs - u.pair);
+            if (isQ) {
+                float* dst = a.q_out + (long long)(t0 + t) * a.out_tok + (long long)h * a.out_head;
+                storePart(dst + u.a, lo[k], u.na);
+                storePart(dst + u.b, hi[k], u.nb);
+            } else if (rowOf[t] >= 0 && !later[t]) {
+                char* to = at[k].isV ? a.v_cache + rowOf[t] * a.vc_row + h * a.vc_head : a.k_cache + rowOf[t] * a.kc_row + h * a.kc_head;
+                _Float16* dst = reinterpret_cast<_Float16*>(to);
+                storePart(dst + u.a, lo[k], u.na);
+                storePart(dst + u.b, hi[k], u.nb);
+            }
+        }
     }
 }
 
@@ -175,9 +203,13 @@ int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
     RopeArgs p{a.q, a.k, a.v, a.pos, a.freqs, reinterpret_cast<const long long*>(a.slots), a.q_out, static_cast<char*>(a.k_cache),
                static_cast<char*>(a.v_cache), a.n_tokens, a.H, a.H_kv, a.D, a.n_rot, a.q_tok, a.q_head, a.k_tok, a.k_head, a.v_tok, a.v_head,
                a.out_tok, a.out_head, a.cache_rows, a.kc_row, a.kc_head, a.vc_row, a.vc_head, a.scale, 1, 1, 0};
-    // k and v: up to 16 tokens share the search for repeated slots, once there are enough to fill the GPU
+    // k and v: up to 16 tokens share the search for repeated slots, once there are enough to fill the GPU twice (which reads all later
+    // tokens' slots in each workgroup)
     const int most = std::max(1, std::min(16, kPairs / std::max(1, a.n_rot / 2)));
     p.kv_tokens = std::max(1, std::min(most, a.n_tokens / 512));
+    // q: what a workgroup loads ahead, likewise
+    const int units = a.n_rot / 8 + (a.D - a.n_rot + 7) / 8;
+    p.q_tokens = std::max(1, std::min({most, a.n_tokens / 512, kAhead * kThreads / std::max(1, a.H * units)}));
     p.q_blocks = a.q ? (a.n_tokens + p.q_tokens - 1) / p.q_tokens : 0;
     const int kvBlocks = a.k ? (a.n_tokens + p.kv_tokens - 1) / p.kv_tokens : 0;
     const dim3 grid(p.q_blocks + kvBlocks);
