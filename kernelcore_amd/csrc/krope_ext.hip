@@ -32,30 +32,31 @@ struct RopeArgs {
     int q_tok, q_head, k_tok, k_head, v_tok, v_head, out_tok, out_head, cache_rows;
     long long kc_row, kc_head, vc_row, vc_head;
     float scale;
-    int q_tokens, kv_tokens, q_blocks;  // tokens of a workgroup, workgroups for q (the first ones)
+    int q_tokens, kv_tokens, kv_blocks;  // tokens of a workgroup, workgroups for k and v (the first ones, which take longest)
 };
 
-// Eight values of a row: two groups of four that hold four pairs, or of its unturned part; n of each group are there.
+// Eight values of a row: two groups of four that hold four pairs, or of its unturned part; na and nb of them are there. Neighbouring
+// threads' groups lie side by side.
 struct Unit {
-    int a, b, na, nb, pair;  // pair: the first one's number, -1 for unturned values
+    int a, b, na, nb, pa, pb;  // pa, pb: the groups' first pairs, -1 for unturned values
 };
 template <bool INTER>
 __device__ __forceinline__ Unit unitOf(int u, int n_rot, int D) {
     const int half = n_rot / 2, turned = (half + 3) / 4;
     Unit x;
-    if (u < turned) {
-        x.pair = 4 * u;
-        x.a = INTER ? 8 * u : 4 * u;
-        x.b = INTER ? x.a + 4 : x.a + half;
-        const int left = half - 4 * u;  // pairs
-        x.na = INTER ? min(4, 2 * left) : min(4, left);
-        x.nb = INTER ? max(0, min(4, 2 * left - 4)) : x.na;
+    if (u < turned && !INTER) {
+        x.pa = x.pb = 4 * u;
+        x.a = 4 * u;
+        x.b = x.a + half;
+        x.na = x.nb = min(4, half - 4 * u);
     } else {
-        x.pair = -1;
-        x.a = n_rot + 8 * (u - turned);
-        x.b = x.a + 4;
-        x.na = min(4, D - x.a);
-        x.nb = max(0, min(4, D - x.b));
+        const int from = u < turned ? 0 : n_rot, to = u < turned ? n_rot : D, y = u < turned ? u : u - turned;
+        x.a = from + 4 * y;
+        x.b = x.a + 4 * ((to - from + 7) / 8);
+        x.na = min(4, to - x.a);
+        x.nb = max(0, min(4, to - x.b));
+        x.pa = u < turned ? x.a / 2 : -1;
+        x.pb = x.b / 2;
     }
     return x;
 }
@@ -87,12 +88,12 @@ __device__ __forceinline__ void storePart(_Float16* p, f32x4 x, int n) {
         if (e < n) p[e] = (_Float16)x[e];
 }
 
-// The pairs' cosines and sines lie in cs from the unit's first pair on.
+// (cs: the token's cosines and sines)
 template <bool INTER>
-__device__ __forceinline__ void turn(f32x4& a, f32x4& b, const float2* cs, int pairs) {
+__device__ __forceinline__ void turn(f32x4& a, f32x4& b, const Unit& u, const float2* cs, int pairs) {
     float2 z[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] = cs[min(e, pairs - 1)];
+    for (int e = 0; e < 4; ++e) z[e] = cs[min(INTER && e >= 2 ? u.pb + e - 2 : u.pa + e, pairs - 1)];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         f32x4& lo = INTER ? (e < 2 ? a : b) : a;
@@ -113,9 +114,9 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
     __shared__ float2 cs[kPairs];
     __shared__ int later[16], rowOf[16];
     const int tid = threadIdx.x;
-    const bool isQ = (int)blockIdx.x < a.q_blocks;
+    const bool isQ = (int)blockIdx.x >= a.kv_blocks;
     const int per = isQ ? a.q_tokens : a.kv_tokens;
-    const int t0 = (isQ ? blockIdx.x : blockIdx.x - a.q_blocks) * per, n = min(per, a.n - t0);
+    const int t0 = (isQ ? blockIdx.x - a.kv_blocks : blockIdx.x) * per, n = min(per, a.n - t0);
     const int pairs = a.n_rot / 2;
     const int turned = (pairs + 3) / 4, units = turned + (a.D - a.n_rot + 7) / 8, vunits = (a.D + 7) / 8;
     const int heads = isQ ? a.H : a.H_kv, first = n * heads * units, all = first + (!isQ && a.v ? n * heads * vunits : 0);
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
             if (x0 + kThreads * k >= all) break;
             const Unit& u = at[k].u;
             const int t = at[k].t, h = at[k].h;
-            if (u.pair >= 0 && !at[k].isV) turn<INTER>(lo[k], hi[k], cs + t * pairs + u.pair, pairs - u.pair);
+            if (u.pa >= 0) turn<INTER>(lo[k], hi[k], u, cs + t * pairs, pairs);
             if (isQ) {
                 float* dst = a.q_out + (long long)(t0 + t) * a.out_tok + (long long)h * a.out_head;
                 storePart(dst + u.a, lo[k], u.na);
@@ -206,13 +207,13 @@ int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
     // k and v: up to 16 tokens share the search for repeated slots, once there are enough to fill the GPU twice (which reads all later
     // tokens' slots in each workgroup)
     const int most = std::max(1, std::min(16, kPairs / std::max(1, a.n_rot / 2)));
-    p.kv_tokens = std::max(1, std::min(most, a.n_tokens / 512));
+    p.kv_tokens = std::max(1, std::min(most, a.n_tokens / 1024));
     // q: what a workgroup loads ahead, likewise
     const int units = a.n_rot / 8 + (a.D - a.n_rot + 7) / 8;
     p.q_tokens = std::max(1, std::min({most, a.n_tokens / 512, kAhead * kThreads / std::max(1, a.H * units)}));
-    p.q_blocks = a.q ? (a.n_tokens + p.q_tokens - 1) / p.q_tokens : 0;
-    const int kvBlocks = a.k ? (a.n_tokens + p.kv_tokens - 1) / p.kv_tokens : 0;
-    const dim3 grid(p.q_blocks + kvBlocks);
+    const int qBlocks = a.q ? (a.n_tokens + p.q_tokens - 1) / p.q_tokens : 0;
+    p.kv_blocks = a.k ? (a.n_tokens + p.kv_tokens - 1) / p.kv_tokens : 0;
+    const dim3 grid(p.kv_blocks + qBlocks);
     if (a.interleaved) hipLaunchKernelGGL(rope_ext_kernel<true>, grid, dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL(rope_ext_kernel<false>, grid, dim3(kThreads), 0, s, p);
     return fromHip(hipGetLastError(), "rope_ext");
