@@ -12,7 +12,8 @@
  *
  * Weights arrive as raw ggml blocks (kcModelSetTensor) and are repacked on the GPU; the KV cache
  * is fp16 in HBM. kcModelGenerate runs greedy decode as replays of one captured hipGraph: the
- * next token, the position and the context length stay on the GPU between steps.
+ * next token, the position and the context length stay on the GPU between steps. kcModelSample does
+ * the same with tokens drawn under temperature, top-k, top-p and min-p.
  */
 #ifndef KERNELCORE_MODEL_H
 #define KERNELCORE_MODEL_H
@@ -89,6 +90,16 @@ KC_API kcError_t kcModelForward(kcModel_t model, const int* tokens, int n_tokens
 /* Greedy decode: starts from the argmax of the last forward's logits and generates `steps`
  * tokens (written to tokens_out, host), each one graph replay. */
 KC_API kcError_t kcModelGenerate(kcModel_t model, int steps, int* tokens_out) KC_NOEXCEPT;
+/* Sampled decode: as kcModelGenerate, but each token is drawn from the logits by sample_rows with the number us[i] (host, `steps`
+ * of them, from 0 up to 1) and the cuts of `how` (their meaning, and which values switch one off, as in kcSampleRowsArgs). The cuts may change
+ * from call to call. tokens_out holds -1 where a step's logits hold NaN or +infinity; the step after it goes on from token 0. */
+typedef struct kcModelSampling {
+    float temperature; /* 0: greedy */
+    int top_k;
+    float top_p;
+    float min_p;
+} kcModelSampling;
+KC_API kcError_t kcModelSample(kcModel_t model, const kcModelSampling* how, const float* us, int steps, int* tokens_out) KC_NOEXCEPT;
 /* Current position (tokens in the KV cache); kcModelReset empties the cache. */
 KC_API kcError_t kcModelPosition(kcModel_t model, int* pos) KC_NOEXCEPT;
 KC_API kcError_t kcModelReset(kcModel_t model) KC_NOEXCEPT;

@@ -132,6 +132,7 @@ DeviceProperties = _struct("DeviceProperties", [("name", C.c_char * 128), ("work
                                                 ("performance_workers", C.c_uint), ("total_memory", C.c_size_t),
                                                 ("is_hardware_gpu", C.c_bool), ("guard_pages", C.c_bool),
                                                 ("large_pages", C.c_bool), ("kernel_stack_bytes", C.c_size_t)])
+ModelSampling = _struct("ModelSampling", [("temperature", _f), ("top_k", _i), ("top_p", _f), ("min_p", _f)])
 ModelConfig = _struct("ModelConfig", [("n_layer", _i), ("n_embd", _i), ("n_head", _i), ("n_head_kv", _i),
                                       ("head_dim", _i), ("n_ff", _i), ("n_vocab", _i), ("norm_eps", _f),
                                       ("rope_theta", _f), ("rope_neox", _i), ("qk_norm", _i), ("max_ctx", _i),
@@ -206,6 +207,7 @@ def lib():
                                        C.POINTER(C.c_size_t), C.POINTER(_p)]
         L.kcModelForward.argtypes = [_p, _p, _i, _p]
         L.kcModelGenerate.argtypes = [_p, _i, _p]
+        L.kcModelSample.argtypes = [_p, C.POINTER(ModelSampling), _p, _i, _p]
         L.kcModelPosition.argtypes = [_p, C.POINTER(_i)]
         L.kcModelReset.argtypes = [_p]
         L.kcModelReadCache.argtypes = [_p, _i, _i, _i, _i, _p]
@@ -671,6 +673,14 @@ class Model:
     def generate(self, steps):
         out = np.zeros(steps, np.int32)
         call("kcModelGenerate", self.h, steps, out.ctypes.data)
+        return out
+
+    def sample(self, us, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """len(us) tokens drawn with the numbers us (from 0 up to 1): kcModelSample."""
+        us = np.ascontiguousarray(us, np.float32)
+        how = ModelSampling(temperature, top_k, top_p, min_p)
+        out = np.zeros(us.size, np.int32)
+        call("kcModelSample", self.h, C.byref(how), us.ctypes.data, us.size, out.ctypes.data)
         return out
 
     def position(self):

@@ -107,8 +107,8 @@ __device__ __forceinline__ void turn(f32x4& a, f32x4& b, const Unit& u, const fl
 
 // A workgroup takes all heads of q, or all of k and v, of q_tokens or kv_tokens tokens, eight values a thread at a time. The first kAhead
 // of a thread's are loaded before the angles are computed (once, into LDS) and repeated slots looked for: what bounds it is the
-// bytes, and for few tokens the latency of one load and the angles. 3333 tokens of 24 + 2 x 8 heads of 128: 29.7 us, 4.1 TB/s (35 with
-// loads after the angles, 31 with four ahead); one token 3.9 us.
+// bytes, and for few tokens the latency of one load and the angles. 3333 tokens of 24 + 2 x 8 heads of 128, from memory: 28 us, 4.4 TB/s
+// where a copy of as many bytes reaches 5.0 (35 us with loads after the angles and k and v last); one token 4 us.
 template <bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
     __shared__ float2 cs[kPairs];
@@ -204,8 +204,8 @@ int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
     RopeArgs p{a.q, a.k, a.v, a.pos, a.freqs, reinterpret_cast<const long long*>(a.slots), a.q_out, static_cast<char*>(a.k_cache),
                static_cast<char*>(a.v_cache), a.n_tokens, a.H, a.H_kv, a.D, a.n_rot, a.q_tok, a.q_head, a.k_tok, a.k_head, a.v_tok, a.v_head,
                a.out_tok, a.out_head, a.cache_rows, a.kc_row, a.kc_head, a.vc_row, a.vc_head, a.scale, 1, 1, 0};
-    // k and v: up to 16 tokens share the search for repeated slots, once there are enough to fill the GPU twice (which reads all later
-    // tokens' slots in each workgroup)
+    // k and v: up to 16 tokens share the search for repeated slots, which reads all later tokens' slots, once there are four workgroups
+    // for each CU (3333 tokens with three to a workgroup 28 us, with six 31, with one 33)
     const int most = std::max(1, std::min(16, kPairs / std::max(1, a.n_rot / 2)));
     p.kv_tokens = std::max(1, std::min(most, a.n_tokens / 1024));
     // q: what a workgroup loads ahead, likewise

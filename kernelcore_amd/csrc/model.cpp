@@ -20,6 +20,7 @@
 #include "internal.hpp"
 #include "kdecode.hpp"
 #include "kquant.hpp"
+#include "kserve.hpp"
 #include "launch.hpp"
 #include "model_kernels.hpp"
 
@@ -81,7 +82,11 @@ struct kcModel_st {
     long long* idx = nullptr;
     int max_gen = 4096;
     int pos_host = 0;
-    kcGraph_t step_graph = nullptr;
+    kcGraph_t step_graph = nullptr, sample_graph = nullptr;
+    // kcModelSample's, from its first call on: cuts, the draw's number, the drawn token, all steps' numbers, sample_rows' workspace
+    float *cuts = nullptr, *sample_u = nullptr, *sample_us = nullptr;
+    int* drawn = nullptr;
+    char* sample_part = nullptr;
     std::vector<void*> allocs;
 };
 
@@ -591,6 +596,7 @@ kcError_t kcModelDestroy(kcModel_t m) noexcept {
     if (!m) return kc::Error::Success;
     (void)kcStreamSynchronize(m->ks);
     if (m->step_graph) (void)kcGraphDestroy(m->step_graph);
+    if (m->sample_graph) (void)kcGraphDestroy(m->sample_graph);
     for (void* p : m->allocs) (void)kcFree(p);
     (void)kcStreamDestroy(m->ks);
     delete m;
@@ -754,6 +760,68 @@ kcError_t kcModelGenerate(kcModel_t m, int steps, int* tokens_out) noexcept {
         m->step_graph = g;
     }
     for (int i = 1; i < steps; ++i) KM_TRYE(kcGraphLaunch(m->step_graph, m->ks));
+    KM_TRYE(syncModel(m));
+    m->pos_host += steps - 1;
+    if (tokens_out) KM_TRYE(kcMemcpy(tokens_out, m->gen, sizeof(int) * steps, kc::CopyKind::DeviceToHost));
+    return ok;
+}
+
+// A draw from the logits, and what follows it (n_past: null where no position is consumed).
+static int sampleStep(kcModel_t m, int* n_past) {
+    kcSampleRowsArgs a{};
+    a.logits = m->logits;
+    a.u = m->sample_u;
+    a.temperature = m->cuts;
+    a.top_k = reinterpret_cast<const int*>(m->cuts + 1);
+    a.top_p = m->cuts + 2;
+    a.min_p = m->cuts + 3;
+    a.tokens = m->drawn;
+    a.part = m->sample_part;
+    a.row = m->c.n_vocab;
+    a.rows = 1;
+    a.n_vocab = m->c.n_vocab;
+    if (int e = kcamd::launchSampleRows(a, m->s)) return e;
+    return kcamd::launchSampleStep(m->drawn, m->sample_us, m->sample_u, m->tokens, m->gen, m->step, n_past, m->max_gen, m->s);
+}
+
+kcError_t kcModelSample(kcModel_t m, const kcModelSampling* how, const float* us, int steps, int* tokens_out) noexcept {
+    if (E e = checkModel(m); e != ok) return e;
+    if (E e = checkLoaded(m); e != ok) return e;
+    if (!how || !us || steps <= 0 || steps > m->max_gen || m->pos_host == 0 || m->pos_host + steps - 1 > m->c.max_ctx ||
+        m->c.n_vocab > (1 << 20)) {
+        kcamd::setDetail("steps must be in [1, 4096], after a forward, and fit the cache; n_vocab at most 2^20; how and us given");
+        return kc::Error::InvalidValue;
+    }
+    KM_TRYE(syncModel(m));
+    if (!m->sample_part) {
+        if (!m->cuts) KM_TRYE(allocT(m, &m->cuts, 4));
+        if (!m->sample_u) KM_TRYE(allocT(m, &m->sample_u, 1));
+        if (!m->sample_us) KM_TRYE(allocT(m, &m->sample_us, (size_t)m->max_gen));
+        if (!m->drawn) KM_TRYE(allocT(m, &m->drawn, 1));
+        KM_TRYE(allocT(m, &m->sample_part, kcamd::sampleRowsPartBytes(1, m->c.n_vocab)));
+    }
+    const int zero = 0;
+    static_assert(sizeof *how == 16);
+    KM_TRYE(kcMemcpy(m->step, &zero, sizeof(int), kc::CopyKind::HostToDevice));
+    KM_TRYE(kcMemcpy(m->n_past, &m->pos_host, sizeof(int), kc::CopyKind::HostToDevice));
+    KM_TRYE(kcMemcpy(m->cuts, how, sizeof *how, kc::CopyKind::HostToDevice));
+    KM_TRYE(kcMemcpy(m->sample_us, us, sizeof(float) * steps, kc::CopyKind::HostToDevice));
+    KM_TRYE(kcMemcpy(m->sample_u, us, sizeof(float), kc::CopyKind::HostToDevice));
+    KM_TRY(sampleStep(m, nullptr));  // the first token, from the last forward's logits (no position consumed)
+    if (!m->sample_graph) {
+        KM_TRYE(kcStreamBeginCapture(m->ks));
+        int e1 = decodeAny(m, m->s);
+        if (!e1) e1 = sampleStep(m, m->n_past);
+        kcGraph_t g = nullptr;
+        const E e2 = kcStreamEndCapture(m->ks, &g);
+        if (e1) {
+            if (g) (void)kcGraphDestroy(g);
+            return err(e1);
+        }
+        if (e2 != ok) return e2;
+        m->sample_graph = g;
+    }
+    for (int i = 1; i < steps; ++i) KM_TRYE(kcGraphLaunch(m->sample_graph, m->ks));
     KM_TRYE(syncModel(m));
     m->pos_host += steps - 1;
     if (tokens_out) KM_TRYE(kcMemcpy(tokens_out, m->gen, sizeof(int) * steps, kc::CopyKind::DeviceToHost));

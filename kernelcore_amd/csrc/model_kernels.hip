@@ -195,6 +195,18 @@ __global__ __launch_bounds__(1024) void argmax_step_kernel(const float* __restri
     }
 }
 
+// What follows a draw: tokens[0] = the drawn token (0 for none, -1), gen[*step] = it; ++*step; ++*n_past; u[0] = the next draw's
+// random number.
+__global__ void sample_step_kernel(const int* __restrict__ drawn, const float* __restrict__ us, float* u, int* tokens, int* gen, int* step,
+                                   int* n_past, int max_gen) {
+    const int t = drawn[0], st = *step;
+    tokens[0] = max(t, 0);
+    if (st < max_gen) gen[st] = t;
+    *step = st + 1;
+    u[0] = us[min(st + 1, max_gen - 1)];
+    if (n_past) *n_past = *n_past + 1;
+}
+
 // Positions of the n tokens of a step: pos[i] = *n_past + i, idx[i] (int64) the same, and the
 // context length the step attends over, n_ctx = *n_past + n.
 __global__ void positions_kernel(const int* __restrict__ n_past, int n, int* pos, long long* idx, int* n_ctx) {
@@ -684,6 +696,12 @@ int launchArgmaxStep(const float* logits, int n, int* tokens, int* gen, int* ste
                      hipStream_t s) {
     hipLaunchKernelGGL(argmax_step_kernel, dim3(1), dim3(1024), 0, s, logits, n, tokens, gen, step, n_past, max_gen);
     return fromHip(hipGetLastError(), "argmax");
+}
+
+int launchSampleStep(const int* drawn, const float* us, float* u, int* tokens, int* gen, int* step, int* n_past, int max_gen,
+                     hipStream_t s) {
+    hipLaunchKernelGGL(sample_step_kernel, dim3(1), dim3(1), 0, s, drawn, us, u, tokens, gen, step, n_past, max_gen);
+    return fromHip(hipGetLastError(), "sample step");
 }
 
 int launchPositions(const int* n_past, int n, int* pos, long long* idx, int* n_ctx, hipStream_t s) {

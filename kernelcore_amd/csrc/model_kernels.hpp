@@ -33,6 +33,8 @@ int launchAttnGqa(const float* q, const int* k, const int* v, float* out, const 
                   const unsigned short* mask, int m_row2, int t_host, int cache_rows, const int* msum, hipStream_t s);
 int launchArgmaxStep(const float* logits, int n, int* tokens, int* gen, int* step, int* n_past, int max_gen,
                      hipStream_t s);
+int launchSampleStep(const int* drawn, const float* us, float* u, int* tokens, int* gen, int* step, int* n_past, int max_gen,
+                     hipStream_t s);
 int launchPositions(const int* n_past, int n, int* pos, long long* idx, int* n_ctx, hipStream_t s);
 
 }  // namespace kcamd
