@@ -511,12 +511,14 @@ typedef struct kcRopeExtArgs {
 /* flash_pages_f16: attention of the step's tokens over an fp16 paged cache that holds their own keys and values too (len[s] positions,
  * the last of them the sequence's nodes): out[t][h] = sum_j softmax_j(scale q_th . k_j) v_j over the positions j that token t, node i
  * of sequence s, sees: those before the nodes, and of the nodes j <= i, or where tree (kv_pages') is given those of its bits
- * (none from 32 tree_words on). Query head h reads KV head h / (H / H_kv); D = 64, 128 or 256. A position whose page is outside [0, n_pages), from
- * len[s] or from max_pages * page on is not seen. A token that sees none gets zeros; lse (may be null): [N][H], the natural logarithm
- * of the sum of exp(score), -infinity for such a token. Rows of tokens from start[seqs] (at most N) on are left as they are. What a position holds that a
- * token does not see (NaN and infinities too) does not reach that token; what it sees counts as in flash_ext_f16.
- * Rows, heads and base of K and V at multiples of 16 bytes; offsets are 64-bit, a page spans less than 2^31 bytes. part: kcFlashPagesPartBytes bytes of workspace,
- * 16-byte aligned, which calls that may overlap must not share. */
+ * (none from 32 tree_words on). Query head h reads KV head h / (H / H_kv); D = 64, 128 or 256. A position whose page is outside
+ * [0, n_pages), from len[s] or from max_pages * page on is not seen. A token that sees none gets zeros; lse (may be null): [N][H], the
+ * natural logarithm of the sum of exp(score), -infinity for such a token. Rows of tokens from start[seqs] (at most N) on are left as they
+ * are. What a position holds that a token does not see (NaN and infinities too) does not reach that token; what it sees counts as in
+ * flash_ext_f16. The same call gives the same bits; N and seqs take part in how the work is split, so the same tokens among others may
+ * differ from themselves alone by roundings.
+ * Rows, heads and base of K and V at multiples of 16 bytes; offsets are 64-bit, a page spans less than 2^31 bytes, the cache holds less
+ * than 2^31 positions. part: kcFlashPagesPartBytes bytes of workspace, 16-byte aligned, which calls that may overlap must not share. */
 typedef struct kcFlashPagesDims {
     int H;
     int H_kv;
@@ -553,11 +555,12 @@ KC_API kcError_t kcFlashPagesPartBytes(const kcFlashPagesDims* dims, size_t* byt
  *   kept are the first top_k of them (0 or less: all), of those the fewest whose weights reach top_p of the sum of the top_k ones (1 or
  *   more, or NaN: all), and of those the ones with w_j >= min_p (0 or less, or NaN: all); the first always is;
  *   tokens[r] = the first in that order at which the sum of the kept weights exceeds u[r] times their whole sum (u below 0 or NaN
- *   counts as 0; from 1 on: the last with a weight); probs[r] (may be null) = its weight over that sum.
- * A temperature of 0 or less, or NaN: the first token (u and the cuts do not matter). temperature, top_k, top_p and min_p hold a value for each row; null:
- * 1, 0, 1 and 0. A logit of -infinity has weight 0. A row that holds NaN or +infinity, or -infinity alone, gives token -1 and
- * probability 0. Weights and sums are held in 64 bits, and results do not depend on the order of additions; a weight below 2^-63 of the largest counts as 0. n_vocab at most 2^20; part: kcSampleRowsPartBytes bytes of workspace, 16-byte
- * aligned, which calls that may overlap must not share. */
+ *   counts as 0, from 1 on as the largest double below 1); probs[r] (may be null) = its weight over that sum.
+ * A temperature of 0 or less, or NaN: the first token (u and the cuts do not matter). temperature, top_k, top_p and min_p hold a value
+ * for each row; null: 1, 0, 1 and 0. A logit of -infinity has weight 0. A row that holds NaN or +infinity, or -infinity alone, gives
+ * token -1 and probability 0. Weights and sums are held in 64 bits, and results do not depend on the order of additions; a weight below
+ * 2^-63 of the largest counts as 0. n_vocab at most 2^20; part: kcSampleRowsPartBytes bytes of workspace, 16-byte aligned, which calls
+ * that may overlap must not share. */
 typedef struct kcSampleRowsArgs {
     const float* logits;
     const float* u;

@@ -28,7 +28,7 @@ typedef unsigned long long u64;
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
 // 64 octaves in bins; the last bin takes what is further (a millionth of millionths of millionths of the largest weight): counted, but of weight 0
-constexpr int kThreads = 1024, kWaves = 16, kDraw = 512, kBins = 2048, kFar = kBins - 1, kList = 5120, kGroups = 2048, kPieces = 64;
+constexpr int kThreads = 1024, kWaves = 16, kDraw = 512, kBins = 2048, kFar = kBins - 1, kList = 5120, kGroups = 3 * kDraw, kPieces = 64;
 constexpr double kPerOctave = 32.0;
 constexpr int kUnitBits = 38, kCountBit = 48;
 constexpr u64 kUnit = 1ull << kUnitBits;
@@ -83,7 +83,10 @@ __device__ __forceinline__ u64 wordOf(double d) {
 // The sum of g of a bin of n tokens, from the sum of its words.
 __device__ __forceinline__ u64 unitsOf(u64 words, unsigned n) { return words + (u64)n * (kUnit - (1ull << 32)); }
 // The weight of a bin's unit.
-__device__ __forceinline__ double factorOf(int b) { return b < kFar ? exp2(-(b + 0.5) / kPerOctave - kUnitBits) : 0.0; }
+constexpr int kOctave = 32;  // bins of an octave: of the factors of its bins (by octaves[], in LDS), which are computed once
+__device__ __forceinline__ double factorOf(const double* octaves, int b) {
+    return b < kFar ? ldexp(octaves[b % kOctave], -(b / kOctave) - kUnitBits) : 0.0;
+}
 
 // ---------------------------------------------------------------------------------------------- bins of the pieces
 // 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins.
@@ -182,18 +185,23 @@ constexpr u64 kCode = (1ull << 52) - 1;
 struct Shared {
     double sum[kBins];      // weights up to and with a bin
     unsigned count[kBins];  // tokens likewise
-    u64 dsum[kDraw];        // the digits of a search
-    unsigned dcount[kDraw];
+    union {
+        unsigned groups[kGroups];
+        struct {
+            u64 dsum[kDraw];  // the digits of a search
+            unsigned dcount[kDraw];
+        };
+    };
     u64 list[kList];        // members of the wanted bins, the bin from bit 52 on
-    unsigned groups[kGroups];
     u64 few[64];
-    double top[kPieces], offset[kPieces];
+    double octaves[kOctave], top[kPieces], offset[kPieces];
     int shift[kPieces];     // bins that a piece's lie further down
     u64 waves[kDraw / 64], waves2[kDraw / 64];
     u64 found[4], cut[4];
     float rowTop;
     int wild, bins[8], listed, grouped, nfew;
 };
+static_assert(sizeof(Shared) <= 80 * 1024);  // two workgroups on a CU
 
 // Sums up to and with this thread's of x and y.
 template <int Waves, class X, class Y>
@@ -272,6 +280,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         }
     }
     if (tid < 8) S.bins[tid] = kBins;
+    if (wave == 1 && lane < kOctave) S.octaves[lane] = exp2(-(lane + 0.5) / kPerOctave);
     __syncthreads();
     if (S.wild || S.rowTop == -INFINITY) {
         if (tid == 0) {
@@ -312,7 +321,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         unsigned n = 0;
 #pragma unroll
         for (int e = 0; e < BPT; ++e) {
-            own += factorOf(BPT * tid + e) * (double)unitsOf(words[e], cnt[e]);
+            own += factorOf(S.octaves, BPT * tid + e) * (double)unitsOf(words[e], cnt[e]);
             sums[e] = own;
             n += cnt[e];
         }
@@ -457,17 +466,17 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     const int grouped = same(S.grouped);
     if (grouped <= kGroups) {
         const int per = a.piece / (4 * kThreads), lgPer = per == 8 ? 3 : 2;
-        for (int c0 = tid; c0 < grouped << lgPer; c0 += 4 * NT) {
-            f32x4 v[4];
-            int at[4];
+        for (int c0 = tid; c0 < grouped << lgPer; c0 += 2 * NT) {
+            f32x4 v[2];
+            int at[2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 const int c = c0 + NT * k;
                 at[k] = c < grouped << lgPer ? (int)S.groups[c >> lgPer] + 4 * kThreads * (c & (per - 1)) : a.n;
                 v[k] = fourAt(at[k]);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) collect(v[k], at[k]);
+            for (int k = 0; k < 2; ++k) collect(v[k], at[k]);
         }
     } else {
         for (int i0 = 4 * tid; i0 < a.n; i0 += 4 * NT * 8) {
@@ -480,20 +489,15 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     }
     __syncthreads();
     const int listed = same(S.listed);
-    // (no more than a wavefront has lanes: the first one does the rest by itself)
-    const bool alone = listed <= 64;
-    if (alone && wave) return;
-    auto sync = [&]() {
-        if (!alone) __syncthreads();
-        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    };
+    // (no more than a wavefront has lanes: the first one does the rest by itself; the barriers do not wait for the others, which have ended)
+    if (listed <= 64 && wave) return;
     if (listed <= kList) {
         for (int i = tid; i < listed; i += NT) {
             const u64 code = S.list[i];
             S.list[i] = code | (u64)binAt(logitOf(code), (int)(code & 0xFFFFF)) << 52;
         }
     }
-    sync();
+    __syncthreads();
     // f(code, bin) for the members of the wanted bins (and some others). A list that is too long is not kept: the row is gone over
     // again each time.
     auto overList = [&](auto&& f) {
@@ -526,7 +530,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         unsigned n = S.count[b] - countBefore(b), nBefore = 0;
         while (n > 64) {
             // the members' range, then the digits of ten bits from its top
-            sync();
+            __syncthreads();
             if (tid == 0) {
                 S.found[0] = ~0ull;
                 S.found[1] = 0;
@@ -535,7 +539,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             }
             S.dsum[tid] = 0;
             S.dcount[tid] = 0;
-            sync();
+            __syncthreads();
             u64 mn = ~0ull, mx = 0;
             overList([&](u64 code, int bb) {
                 if (bb == b && code >= lowest && code <= highest) {
@@ -552,7 +556,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
                 atomicMin(S.found, mn);
                 atomicMax(S.found + 1, mx);
             }
-            sync();
+            __syncthreads();
             lowest = S.found[0];
             highest = S.found[1];
             const int shift = max(0, 64 - __builtin_clzll((highest - lowest) | 1) - kDigitBits);
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
                     atomicAdd(S.dcount + d, 1u);
                 }
             });
-            sync();
+            __syncthreads();
             const u64 ds = S.dsum[tid];
             const unsigned dc = S.dcount[tid];
             u64 w = ds;
@@ -572,30 +576,30 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             const unsigned long long here = __ballot(dc && (byCount ? nBefore + k >= want : before + w >= want)), some = __ballot(dc != 0);
             if (here && lane == 0) atomicMin(S.bins + 6, wave * 64 + __builtin_ctzll(here));
             if (some && lane == 0) atomicMax(S.bins + 7, wave * 64 + 63 - __builtin_clzll(some));
-            sync();
+            __syncthreads();
             const int digit = S.bins[6] < kBins ? S.bins[6] : S.bins[7];
             if (tid == digit) {
                 S.found[0] = w - ds;
                 S.found[1] = k - dc;
                 S.found[2] = dc;
             }
-            sync();
+            __syncthreads();
             before += S.found[0];
             nBefore += (unsigned)S.found[1];
             n = (unsigned)S.found[2];
             lowest += (u64)digit << shift;
             highest = min(highest, lowest + (1ull << shift) - 1);
         }
-        sync();
+        __syncthreads();
         if (tid == 0) S.nfew = 0;
-        sync();
+        __syncthreads();
         overList([&](u64 code, int bb) {
             if (bb == b && code >= lowest && code <= highest) {
                 const int at = atomicAdd(&S.nfew, 1);
                 if (at < 64) S.few[at] = code;
             }
         });
-        sync();
+        __syncthreads();
         if (wave == 0) {
             const int m = min(S.nfew, 64);
             const u64 mine = lane < m ? S.few[lane] : ~0ull;
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
                 S.found[2] = w;
             }
         }
-        sync();
+        __syncthreads();
     };
     // the first bin from b on, up to last, with a token and cond; else the last with a token
     auto walk = [&](int b, int last, auto&& cond) {
@@ -630,7 +634,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         while (b > 0 && S.count[b] == countBefore(b)) --b;
         return b;
     };
-    auto unitsTo = [&](int b, double target) { return fmax(0.0, fmin((target - sumBefore(b)) / factorOf(b), 0x1p60)); };
+    auto unitsTo = [&](int b, double target) { return fmax(0.0, fmin((target - sumBefore(b)) / factorOf(S.octaves, b), 0x1p60)); };
 
     double kept = kLo;  // the weight of what is kept
     for (int stage = 0; stage < 3; ++stage) {  // the cuts by count and by weight, the draw
@@ -646,17 +650,17 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             want = max((u64)ceil(unitsTo(b, target)), 1ull);
         } else {
             if (cutM) {  // what of bins bM0 .. bM1 comes up to min_p of the largest logit's weight
-                sync();
+                __syncthreads();
                 if (tid < 4) S.cut[tid] = 0;
-                sync();
+                __syncthreads();
                 const double least2 = log2((double)mp);
                 overList([&](u64 code, int bb) {
                     if (bb >= bM0 && bb <= bM1 && ((double)logitOf(code) - top) * slope >= least2) atomicAdd(S.cut + (bb - bM0), unitOf(code));
                 });
-                sync();
+                __syncthreads();
                 double s = sumBefore(bM0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s += factorOf(bM0 + k) * (double)S.cut[k];
+                for (int k = 0; k < 4; ++k) s += factorOf(S.octaves, bM0 + k) * (double)S.cut[k];
                 kept = fmin(kept, s);
             }
             const double target = u * kept;
@@ -668,12 +672,12 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         if (stage == 2) {
             if (tid == 0) {
                 a.tokens[r] = (int)(S.found[1] & 0xFFFFF);
-                if (a.probs) a.probs[r] = (float)(factorOf(b) * (double)S.found[2] / kept);
+                if (a.probs) a.probs[r] = (float)(factorOf(S.octaves, b) * (double)S.found[2] / kept);
             }
         } else {
-            const double s = sumBefore(b) + factorOf(b) * (double)S.found[0];
+            const double s = sumBefore(b) + factorOf(S.octaves, b) * (double)S.found[0];
             kept = stage == 0 ? s : fmin(kept, s);
-            sync();
+            __syncthreads();
         }
     }
 }

@@ -92,7 +92,7 @@ def make(**k):
 
 checks("flash_pages_f16", make, good,
        [(dict(H=0), IV), (dict(H=7), IV), (dict(H_kv=0), IV), (dict(D=96), IV), (dict(D=0), IV), (dict(N=-1), IV), (dict(seqs=-1), IV), (dict(page=8), IV), (dict(page=33), IV),
-        (dict(max_pages=-1), IV), (dict(max_pages=7), IV), (dict(n_pages=-1), IV), (dict(tree_words=0), IV), (dict(tree_words=65), IV), (dict(tree=None), IV),
+        (dict(max_pages=-1), IV), (dict(max_pages=7), IV), (dict(n_pages=-1), IV), (dict(n_pages=1 << 26), IV), (dict(n_pages=(1 << 26) - 1), IP), (dict(tree_words=0), IV), (dict(tree_words=65), IV), (dict(tree=None), IV),
         (dict(tree=None, tree_words=0), OK), (dict(lse=None), OK), (dict(N=0), OK), (dict(seqs=0), OK), (dict(n_pages=0), OK), (dict(max_pages=0), OK),
         (dict(page=65536, max_pages=32768, table_row=32768), IV), (dict(q_tok=-1), IV), (dict(q_head=-4), IV), (dict(k_row=-16), IV), (dict(k_row=520), IV), (dict(k_head=250), IV),
         (dict(v_row=528, v_head=8), IV), (dict(k_row=1 << 61), IV), (dict(k_row=1 << 27), IV), (dict(scale=NAN), IV), (dict(scale=INF), IV), (dict(q=None), IP), (dict(k=None), IP),
