@@ -8,9 +8,14 @@
 //
 // A weight is 2^-((b + 1/2) / 32), its bin's factor, times g = 2^-(s / 32) for the token's place s in the bin, |s| <= 1/2. A bin's sum of g
 // is held as an integer in steps of 2^-38 (integers do not depend on the order of the atomics that add them up), with the
-// count in the same word: one 64-bit atomic in LDS and a polynomial of degree 5 for each token. The bins' weights are added up
+// count in the same word: one 64-bit atomic in LDS and a polynomial of degree 4 for each token. The bins' weights are added up
 // in 64 bits, always in the same order. (Weights in 32 bits would move the borders by about 2^-24 of the whole, and among 150000 flat
 // weights there is a border every 2^-17.)
+//
+// What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 72 us, 4.3 TB/s, the draws 117 us, of which
+// the second reading 57), for one row latencies, of one workgroup's steps one after the other (128256 logits, top_k 40: 5.5 and
+// 18 us). What is held of a row instead of reading it again, a byte for each logit, would be written and read for as much again as it saves
+// of the second reading's time.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,7 +35,7 @@ typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 // 64 octaves in bins; the last bin takes what is further (a millionth of millionths of millionths of the largest weight): counted, but of weight 0
 constexpr int kThreads = 1024, kWaves = 16, kDraw = 512, kBins = 2048, kFar = kBins - 1, kList = 5120, kGroups = 3 * kDraw, kPieces = 64;
 constexpr double kPerOctave = 32.0;
-constexpr int kUnitBits = 38, kCountBit = 48;
+constexpr int kUnitBits = 38;
 constexpr u64 kUnit = 1ull << kUnitBits;
 
 struct SampleArgs {
@@ -45,7 +50,7 @@ struct SampleArgs {
 
 // A piece's bins in the workspace.
 struct __attribute__((aligned(16))) Piece {
-    u64 bins[kBins];  // the count from bit 48 on, below it the sum of 2^38 (g - 1) + 2^32
+    u64 bins[kBins];  // sums of words: the count's multiple from bit 48 on, below it the sum of 2^38 (g - 1) + 2^32
     float top;        // the largest logit; -infinity: no finite one
     int wild;         // NaN or +infinity among the logits
     unsigned finite;  // finite logits
@@ -65,22 +70,30 @@ __device__ __forceinline__ double offsetOf(float top, double slope, double ref) 
     return kPerOctave * fmin(fmax(fma(-(double)top, slope, ref), 0.0), 1.0);
 }
 // A token's distance below ref in bins (slope32 = 32 slope), its bin, and what it adds to the bin's word. g - 1 by the series of
-// exp, whose sixth term is below 2^-48; added to 2^14 + 1 / 64, so that the sum's last bit is 2^-38 and its bits but the
-// last 33 are known.
+// exp to the fourth power, the fifth's term (at most 2^-39.6) by the polynomial of degree 3 nearest to it (off by 2^-43.5); added to
+// 2^14 + 2^10 + 1 / 64, so that the sum's last bit is 2^-38 and its bits but the last 33 are known.
 __device__ __forceinline__ double distanceOf(float l, double top, double slope32, double offset) { return fma(top - (double)l, slope32, offset); }
-__device__ __forceinline__ int binOf(double d) { return min((int)d, kFar); }
-__device__ __forceinline__ u64 wordOf(double d) {
-    const double s = __builtin_amdgcn_fract(d) - 0.5;
-    constexpr double a = -0.6931471805599453 / kPerOctave;
-    double p = a * a * a * a * a / 120.0;
-    p = fma(p, s, a * a * a * a / 24.0);
-    p = fma(p, s, a * a * a / 6.0);
-    p = fma(p, s, a * a / 2.0);
-    p = fma(p, s, a);
-    p = fma(p, s, 16384.0 + 1.0 / 64.0);
-    return __builtin_bit_cast(u64, p) + ((1ull << kCountBit) - 0x40D0000000000000ull);
+__device__ __forceinline__ int binOf(double d) { return (int)fmin(d, (double)kFar); }
+// The word's top 16 bits are the same for all, and odd: n words' sum gives n.
+struct Series {
+    double c[5];
+};
+__device__ __forceinline__ Series seriesOf() {
+    constexpr double a = -0.6931471805599453 / kPerOctave, h2 = a * a / 4.0;  // (as)^5 ~ 5/4 h^2 (as)^3 - 5/16 h^4 as, |as| <= h
+    Series r{{a * a * a * a / 24.0, a * a * a * (1.0 / 6.0 + 1.25 * h2 / 120.0), a * a / 2.0, a * (1.0 - 0.3125 * h2 * h2 / 120.0), 17408.0 + 1.0 / 64.0}};
+    // (kept in registers, where the compiler would write them again for each token)
+    asm("" : "+v"(r.c[0]), "+s"(r.c[1]), "+s"(r.c[2]), "+s"(r.c[3]), "+s"(r.c[4]));
+    return r;
 }
-// The sum of g of a bin of n tokens, from the sum of its words.
+__device__ __forceinline__ u64 wordOf(const Series& k, double d) {
+    const double s = __builtin_amdgcn_fract(d) - 0.5;
+    return __builtin_bit_cast(u64, fma(fma(fma(fma(k.c[0], s, k.c[1]), s, k.c[2]), s, k.c[3]), s, k.c[4]));
+}
+constexpr unsigned kTop = 0x40D1, kTopInverse = 0x1831;  // of modulo 2^16
+static_assert((kTop * kTopInverse & 0xFFFF) == 1);
+__device__ __forceinline__ unsigned countOf(u64 words) { return (unsigned)(words >> 48) * kTopInverse & 0xFFFF; }
+__device__ __forceinline__ u64 lowOf(u64 words) { return words & ((1ull << 48) - 1); }
+// The sum of g of a bin of n tokens, from the sum of its words' low bits.
 __device__ __forceinline__ u64 unitsOf(u64 words, unsigned n) { return words + (u64)n * (kUnit - (1ull << 32)); }
 // The weight of a bin's unit.
 constexpr int kOctave = 32;  // bins of an octave: of the factors of its bins (by octaves[], in LDS), which are computed once
@@ -89,7 +102,8 @@ __device__ __forceinline__ double factorOf(const double* octaves, int b) {
 }
 
 // ---------------------------------------------------------------------------------------------- bins of the pieces
-// 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins.
+// 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins. (15 vector instructions a
+// token, 40 us of the 72 above: what need not be is not done for each token.)
 template <int R>
 __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) {
     __shared__ u64 bins[kBins];
@@ -112,17 +126,26 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) 
     }
     bins[tid] = 0;
     bins[tid + kThreads] = 0;
-    float top = -INFINITY;
+    float top = -INFINITY, odd = 0.0f;  // odd: NaN if some logit is not finite
     bool wild = false;
-    unsigned finite = 0;
+    unsigned finite = R;
 #pragma unroll
     for (int k = 0; k < R / 4; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            wild |= !(v[k][e] < INFINITY);
+            odd = fmaf(v[k][e], 0.0f, odd);
             top = fmaxf(top, v[k][e]);
-            finite += v[k][e] > -INFINITY;
         }
+    if (odd != 0.0f) {
+        finite = 0;
+#pragma unroll
+        for (int k = 0; k < R / 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                wild |= !(v[k][e] < INFINITY);
+                finite += v[k][e] > -INFINITY;
+            }
+    }
     Piece& out = reinterpret_cast<Piece*>(a.part)[(size_t)r * a.pieces + blockIdx.x];
     out.tops[tid] = top;
 #pragma unroll
@@ -146,18 +169,15 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) 
         finite += finites[w];
     }
     const bool empty = top == -INFINITY || bad;
+    const Series series = seriesOf();
     const double top64 = top, slope32 = kPerOctave * slope, offset = offsetOf(top, slope, refOf(top, slope));
     if (!empty) {
 #pragma unroll
         for (int k = 0; k < R / 4; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float l = v[k][e];
-                if (l > -INFINITY) {
-                    const double d = distanceOf(l, top64, slope32, offset);
-                    const int b = binOf(d);
-                    if (b < kFar) atomicAdd(bins + b, wordOf(d));  // (the others: those finite that no bin counts)
-                }
+                const double d = distanceOf(v[k][e], top64, slope32, offset);  // (infinite for a logit of -infinity; a slope of 0: NaN)
+                if (d < kFar) atomicAdd(bins + (int)d, wordOf(series, d));  // (the others: those finite that no bin counts)
             }
     }
     __syncthreads();
@@ -311,8 +331,8 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         for (int k = 0; k < 8; ++k)
 #pragma unroll
             for (int e = 0; e < BPT; ++e) {
-                cnt[e] += (unsigned)(y[k][e / 2][e % 2] >> kCountBit);
-                words[e] += y[k][e / 2][e % 2] & ((1ull << kCountBit) - 1);
+                cnt[e] += countOf(y[k][e / 2][e % 2]);
+                words[e] += lowOf(y[k][e / 2][e % 2]);
             }
     }
     if (tid == NT - 1) cnt[BPT - 1] = words[BPT - 1] = 0;  // (the last bin)
@@ -517,10 +537,10 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         }
     };
     // a token's part of its bin's sum: what the first kernel added for it
+    const Series series = seriesOf();
     auto unitOf = [&](u64 code) {
         const int pc = (int)(code & 0xFFFFF) / a.piece;
-        const u64 w = wordOf(distanceOf(logitOf(code), S.top[pc], slope32, S.offset[pc]));
-        return unitsOf(w & ((1ull << kCountBit) - 1), 1);
+        return unitsOf(lowOf(wordOf(series, distanceOf(logitOf(code), S.top[pc], slope32, S.offset[pc]))), 1);
     };
 
     // Among the members of bin b, in order, the one with which the count (byCount) or the sum reaches `want`, the last one if none does:
