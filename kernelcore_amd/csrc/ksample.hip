@@ -57,6 +57,14 @@ struct __attribute__((aligned(16))) Piece {
     float tops[kThreads];  // the largest of the logits that a thread held (4 each 4096)
 };
 
+// Four logits from number `at` on of the n at x; zeros from n on. (A load under a condition would be waited for before the next one.)
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rowOf(const float* x, int n) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(x), (short)0, __builtin_amdgcn_readfirstlane(4 * n), 0x00020000);
+}
+__device__ __forceinline__ f32x4 fourAt(__amdgpu_buffer_rsrc_t x, int at) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(x, 4 * at, 0, 0));
+}
 // (Rows that take the likeliest token count as temperature 1.)
 __device__ __forceinline__ bool greedy(float t) { return !(t > 0.0f); }
 // Octaves of weight per unit of logit.
@@ -113,16 +121,15 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) 
     const int r = blockIdx.y, p0 = blockIdx.x * a.piece, n = min(a.piece, a.n - p0);
     const float* x = a.logits + (long long)r * a.row + p0;
     const double slope = slopeOf(a, r);
+    const auto row = rowOf(x, n);
     f32x4 v[R / 4];
 #pragma unroll
-    for (int k = 0; k < R / 4; ++k) {
-        const int at = 4 * (tid + kThreads * k);
-        if (at + 3 < n) {
-            v[k] = *reinterpret_cast<const f4a4*>(x + at);
-        } else {
+    for (int k = 0; k < R / 4; ++k) v[k] = fourAt(row, 4 * (tid + kThreads * k));
+    if (n < kThreads * R) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[k][e] = at + e < n ? x[at + e] : -INFINITY;
-        }
+        for (int k = 0; k < R / 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] = 4 * (tid + kThreads * k) + e < n ? v[k][e] : -INFINITY;
     }
     bins[tid] = 0;
     bins[tid + kThreads] = 0;
@@ -441,29 +448,22 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         const int pc = at / a.piece;
         return min(binOf(distanceOf(l, S.top[pc], slope32, S.offset[pc])) + S.shift[pc], kFar);
     };
-    auto collect = [&](const f32x4& v, int at) {
+    // Of the logits at at0 + step (i / 4) + i % 4 those whose bit i is set. (They are few, and read again: which register holds one is
+    // not known in advance.)
+    auto keep = [&](unsigned mask, int at0, int step) {
+        if (!mask) return;
+        int pos = atomicAdd(&S.listed, __builtin_popcount(mask));
+        for (; mask; mask &= mask - 1, ++pos) {
+            const int i = __builtin_ctz(mask), at = at0 + step * (i >> 2) + (i & 3);
+            if (pos < kList) S.list[pos] = codeOf(x[at], at);
+        }
+    };
+    const auto row = rowOf(x, a.n);
+    auto bitsOf = [&](const f32x4& v, int at) {
         unsigned mask = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) mask |= near(v[e]) && v[e] > -INFINITY ? 1u << e : 0u;
-        if (mask) {
-            int pos = atomicAdd(&S.listed, __builtin_popcount(mask));
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (mask >> e & 1u) {
-                    if (pos < kList) S.list[pos] = codeOf(v[e], at + e);
-                    ++pos;
-                }
-        }
-    };
-    auto fourAt = [&](int at) {
-        f32x4 v;
-        if (at + 3 < a.n) {
-            v = *reinterpret_cast<const f4a4*>(x + at);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = at + e < a.n ? x[at + e] : -INFINITY;
-        }
-        return v;
+        return at + 3 < a.n ? mask : mask & ((1u << max(a.n - at, 0)) - 1);
     };
     // The groups whose largest logit is not below all of them: few where the borders are among a row's first tokens (one row of 128256
     // with top_k 40: 4.5 us, 14 for all logits). Of more than there is room for all logits are read.
@@ -493,18 +493,31 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             for (int k = 0; k < 2; ++k) {
                 const int c = c0 + NT * k;
                 at[k] = c < grouped << lgPer ? (int)S.groups[c >> lgPer] + 4 * kThreads * (c & (per - 1)) : a.n;
-                v[k] = fourAt(at[k]);
+                v[k] = fourAt(row, at[k]);
             }
 #pragma unroll
-            for (int k = 0; k < 2; ++k) collect(v[k], at[k]);
+            for (int k = 0; k < 2; ++k) keep(bitsOf(v[k], at[k]), at[k], 0);
         }
     } else {
-        for (int i0 = 4 * tid; i0 < a.n; i0 += 4 * NT * 8) {
-            f32x4 v[8];
+        // (the next ones are under way while these are looked at)
+        constexpr int Step = 4 * NT;
+        f32x4 v[4], w[4];
+        auto load = [&](f32x4 (&z)[4], int i0) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = fourAt(i0 + 4 * NT * k);
+            for (int k = 0; k < 4; ++k) z[k] = fourAt(row, i0 + Step * k);
+        };
+        auto look = [&](const f32x4 (&z)[4], int i0) {
+            unsigned mask = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) collect(v[k], i0 + 4 * NT * k);
+            for (int k = 0; k < 4; ++k) mask |= bitsOf(z[k], i0 + Step * k) << 4 * k;
+            keep(mask, i0, Step);
+        };
+        load(v, 4 * tid);
+        for (int i0 = 4 * tid; i0 < a.n; i0 += 8 * Step) {
+            load(w, i0 + 4 * Step);
+            look(v, i0);
+            load(v, i0 + 8 * Step);
+            look(w, i0 + 4 * Step);
         }
     }
     __syncthreads();
