@@ -12,10 +12,9 @@
 // in 64 bits, always in the same order. (Weights in 32 bits would move the borders by about 2^-24 of the whole, and among 150000 flat
 // weights there is a border every 2^-17.)
 //
-// What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 72 us, 4.3 TB/s, the draws 117 us, of which
-// the second reading 57), for one row latencies, of one workgroup's steps one after the other (128256 logits, top_k 40: 5.5 and
-// 18 us). What is held of a row instead of reading it again, a byte for each logit, would be written and read for as much again as it saves
-// of the second reading's time.
+// What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 69 us, 4.5 TB/s, the draws 98 us, of which
+// the second reading 55), for one row latencies, of one workgroup's steps one after the other (128256 logits, top_k 40: 5.5 and
+// 18 us; a flat row of 151936 under top_p 0.8, of which all is read again by one CU, 25 us more).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -111,7 +110,7 @@ __device__ __forceinline__ double factorOf(const double* octaves, int b) {
 
 // ---------------------------------------------------------------------------------------------- bins of the pieces
 // 1024 threads hold a piece of 1024 R logits in registers: its maximum first, which gives ref, then the bins. (15 vector instructions a
-// token, 40 us of the 72 above: what need not be is not done for each token.)
+// token, 40 us of the 69 above: what need not be is not done for each token.)
 template <int R>
 __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) {
     __shared__ u64 bins[kBins];
@@ -432,42 +431,51 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     const int from[3] = {bU0, min(bP0, bM0), cutK ? bK : kBins};
     const int to[3] = {bU1, max(cutP ? bP1 : -1, cutM ? bM1 : -1), cutK ? bK : -1};
     const double offset = offsetOf(same(S.rowTop), slope, refOf(same(S.rowTop), slope));
-    float least[3], most[3];  // their logits, and what rounding may take off
+    // Their logits, and what rounding may take off: |l - mid| - half below 0 for one of them.
+    float mid[3], half[3], lowest = INFINITY;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        const float hiL = (float)(top - (from[k] - offset) / slope32), loL = (float)(top - (to[k] + 1 - offset) / slope32);
+        constexpr float kMost = 3.402823466e38f;  // (nothing here may be infinite: the difference of two is NaN, which is nobody's neighbour)
+        const float hiL = (float)fmax(fmin(top - (from[k] - offset) / slope32, (double)kMost), -(double)kMost);
+        const float loL = (float)fmax(fmin(top - (to[k] + 1 - offset) / slope32, (double)kMost), -(double)kMost);
         const float slack = 2.4e-7f * fmaxf((float)fabs(top), 1.2e-38f);
         const bool none = to[k] < from[k], all = slope == 0.0;  // (a slope of 0: all logits lie in one bin)
-        most[k] = same(none ? -INFINITY : all ? INFINITY : fmaf(fabsf(hiL), 2.4e-7f, hiL) + slack);
-        least[k] = same(none ? INFINITY : all ? -INFINITY : fminf(fmaf(fabsf(loL), -2.4e-7f, loL) - slack, 3.4e38f));
+        const float hi = fminf(fmaf(fabsf(hiL), 2.4e-7f, hiL) + slack, kMost), lo = fmaxf(fminf(fmaf(fabsf(loL), -2.4e-7f, loL) - slack, 3.4e38f), -kMost);
+        const float m = 0.5f * lo + 0.5f * hi;
+        mid[k] = same(none || all ? 0.0f : m);
+        half[k] = same(none ? -INFINITY : all ? INFINITY : fmaxf(hi - m, m - lo) * 1.000001f + 1.2e-38f);
+        lowest = fminf(lowest, same(none ? INFINITY : all ? -INFINITY : lo));
     }
-    auto near = [&](float l) {
-        return ((l >= least[0]) & (l <= most[0])) | ((l >= least[1]) & (l <= most[1])) | ((l >= least[2]) & (l <= most[2]));
+    auto near = [&](float l) {  // (its sign bit)
+        const float x0 = fabsf(l - mid[0]) - half[0], x1 = fabsf(l - mid[1]) - half[1], x2 = fabsf(l - mid[2]) - half[2];
+        return __builtin_bit_cast(unsigned, fminf(fminf(x0, x1), x2));
     };
     auto binAt = [&](float l, int at) {
         const int pc = at / a.piece;
         return min(binOf(distanceOf(l, S.top[pc], slope32, S.offset[pc])) + S.shift[pc], kFar);
     };
-    // Of the logits at at0 + step (i / 4) + i % 4 those whose bit i is set. (They are few, and read again: which register holds one is
-    // not known in advance.)
-    auto keep = [&](unsigned mask, int at0, int step) {
+    // Of 4 K values, at at0 + step k, those of the members. (They are few, and read again: which register holds one is not known in
+    // advance.)
+    const auto row = rowOf(x, a.n);
+    auto keep = [&](auto&& v, int at0, int step) {
+        constexpr int K = sizeof v / sizeof v[0];
+        unsigned mask = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mask = __builtin_amdgcn_alignbit(mask, near(v[k][e]), 31);  // (the first one's bit on top)
+        if (at0 + step * (K - 1) + 3 >= a.n)
+            for (int i = 0; i < 4 * K; ++i)
+                if (at0 + step * (i >> 2) + (i & 3) >= a.n) mask &= ~(1u << (4 * K - 1 - i));
         if (!mask) return;
         int pos = atomicAdd(&S.listed, __builtin_popcount(mask));
         for (; mask; mask &= mask - 1, ++pos) {
-            const int i = __builtin_ctz(mask), at = at0 + step * (i >> 2) + (i & 3);
+            const int i = 4 * K - 1 - __builtin_ctz(mask), at = at0 + step * (i >> 2) + (i & 3);
             if (pos < kList) S.list[pos] = codeOf(x[at], at);
         }
     };
-    const auto row = rowOf(x, a.n);
-    auto bitsOf = [&](const f32x4& v, int at) {
-        unsigned mask = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mask |= near(v[e]) && v[e] > -INFINITY ? 1u << e : 0u;
-        return at + 3 < a.n ? mask : mask & ((1u << max(a.n - at, 0)) - 1);
-    };
     // The groups whose largest logit is not below all of them: few where the borders are among a row's first tokens (one row of 128256
     // with top_k 40: 4.5 us, 14 for all logits). Of more than there is room for all logits are read.
-    const float lowest = fminf(fminf(least[0], least[1]), least[2]);
     for (int p0 = 0; p0 < a.pieces; p0 += 8) {
         float tops[8];
 #pragma unroll
@@ -487,16 +495,16 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     if (grouped <= kGroups) {
         const int per = a.piece / (4 * kThreads), lgPer = per == 8 ? 3 : 2;
         for (int c0 = tid; c0 < grouped << lgPer; c0 += 2 * NT) {
-            f32x4 v[2];
+            f32x4 v[2][1];
             int at[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int c = c0 + NT * k;
                 at[k] = c < grouped << lgPer ? (int)S.groups[c >> lgPer] + 4 * kThreads * (c & (per - 1)) : a.n;
-                v[k] = fourAt(row, at[k]);
+                v[k][0] = fourAt(row, at[k]);
             }
 #pragma unroll
-            for (int k = 0; k < 2; ++k) keep(bitsOf(v[k], at[k]), at[k], 0);
+            for (int k = 0; k < 2; ++k) keep(v[k], at[k], 0);
         }
     } else {
         // (the next ones are under way while these are looked at)
@@ -506,18 +514,12 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) z[k] = fourAt(row, i0 + Step * k);
         };
-        auto look = [&](const f32x4 (&z)[4], int i0) {
-            unsigned mask = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mask |= bitsOf(z[k], i0 + Step * k) << 4 * k;
-            keep(mask, i0, Step);
-        };
         load(v, 4 * tid);
         for (int i0 = 4 * tid; i0 < a.n; i0 += 8 * Step) {
             load(w, i0 + 4 * Step);
-            look(v, i0);
+            keep(v, i0, Step);
             load(v, i0 + 8 * Step);
-            look(w, i0 + 4 * Step);
+            keep(w, i0 + 4 * Step, Step);
         }
     }
     __syncthreads();
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
                 e = S.list[i];
             } else {
                 const float l = x[i];
-                if (!near(l) || l == -INFINITY) continue;
+                if (!(near(l) >> 31) || l == -INFINITY) continue;
                 e = codeOf(l, i) | (u64)binAt(l, i) << 52;
             }
             f(e & kCode, (int)(e >> 52));
@@ -561,8 +563,9 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     auto search = [&](int b, u64 want, bool byCount) {
         u64 lowest = 0, highest = kCode, before = 0;
         unsigned n = S.count[b] - countBefore(b), nBefore = 0;
-        while (n > 64) {
-            // the members' range, then the digits of ten bits from its top
+        // (nine bits of a code of 52 each time, which are all different: six times at most)
+        for (int round = 0; n > 64 && round < 6; ++round) {
+            // the members' range, then the digits from its top
             __syncthreads();
             if (tid == 0) {
                 S.found[0] = ~0ull;
@@ -592,6 +595,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             __syncthreads();
             lowest = S.found[0];
             highest = S.found[1];
+            if (lowest > highest) break;
             const int shift = max(0, 64 - __builtin_clzll((highest - lowest) | 1) - kDigitBits);
             overList([&](u64 code, int bb) {
                 if (bb == b && code >= lowest && code <= highest) {
