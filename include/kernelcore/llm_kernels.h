@@ -515,10 +515,11 @@ typedef struct kcRopeExtArgs {
  * [0, n_pages), from len[s] or from max_pages * page on is not seen. A token that sees none gets zeros; lse (may be null): [N][H], the
  * natural logarithm of the sum of exp(score), -infinity for such a token. Rows of tokens from start[seqs] (at most N) on are left as they
  * are. What a position holds that a token does not see (NaN and infinities too) does not reach that token; what it sees counts as in
- * flash_ext_f16. The same call gives the same bits; N and seqs take part in how the work is split, so the same tokens among others may
- * differ from themselves alone by roundings.
+ * flash_ext_f16. The same call gives the same bits; N, seqs and the table's size take part in how the work is split, so the same tokens
+ * among others, or with a longer table, may differ by roundings.
  * Rows, heads and base of K and V at multiples of 16 bytes; offsets are 64-bit, a page spans less than 2^31 bytes, the cache holds less
- * than 2^31 positions. part: kcFlashPagesPartBytes bytes of workspace, 16-byte aligned, which calls that may overlap must not share. */
+ * than 2^31 positions. part: kcFlashPagesPartBytes bytes of workspace, 16-byte aligned, which calls that may overlap must not share.
+ * out, lse and part overlap neither each other nor the inputs. */
 typedef struct kcFlashPagesDims {
     int H;
     int H_kv;
@@ -560,7 +561,7 @@ KC_API kcError_t kcFlashPagesPartBytes(const kcFlashPagesDims* dims, size_t* byt
  * for each row; null: 1, 0, 1 and 0. A logit of -infinity has weight 0. A row that holds NaN or +infinity, or -infinity alone, gives
  * token -1 and probability 0. Weights and sums are held in 64 bits, and results do not depend on the order of additions; a weight below
  * 2^-63 of the largest counts as 0. n_vocab at most 2^20; part: kcSampleRowsPartBytes bytes of workspace, 16-byte aligned, which calls
- * that may overlap must not share. */
+ * that may overlap must not share. tokens, probs and part overlap neither each other nor the inputs. */
 typedef struct kcSampleRowsArgs {
     const float* logits;
     const float* u;

@@ -8,6 +8,11 @@
 // sequence's length gives; all items' steps in a row are divided evenly among the workgroups. An item whose steps fall to several
 // workgroups is joined by a second kernel from their sums (in the order of the keys, so that results do not depend on
 // which workgroup was first).
+//
+// What bounds it: single tokens the cache's bytes (128 sequences of 4000 positions, 32 heads on 8 of 128: 368 us, 5.6 TB/s); wide trees products
+// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 228 us, 0.46 PFLOP/s
+// counted once, matrix units 47% and VALU 43% of the cycles); a small call the chain of shares, first loads, steps and join (one
+// token over 8191 positions: 10 + 4 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -663,20 +668,27 @@ __global__ __launch_bounds__(256) void flash_pages_join_kernel(FpParams a, int r
     }
 }
 
-// How a call is launched: the form by a sequence's rows on average, workgroups (as many as run at once), and the largest number of items.
+// How a call is launched: the form, workgroups (as many as run at once), rows of an item and the largest number of items.
 struct FpPlan {
     int form, rt, groups, items, each;
     size_t bytes;
 };
+// Few rows, or little work: 16 rows to a wavefront (form 0); up to 128 rows of a sequence on average: 32 (1); more: eight wavefronts over the rows
+// (2). The work is bounded by what the host knows, the tables' positions. us, 32 heads on 8, forms 0 / 1 / 2:
+//   D = 128: 32 sequences of 4000 positions, 8 rows 108 / 119 / 130, 24 rows 173 / 125 / 136, 128 rows 416 / 238 / 249, 256 rows 589 / 336 / 315;
+//   one of 2000, 128 rows 20 / 24 / 28; 4 of 2000, 64 rows 30 / 34 / 39; one of 32000, 64 rows 53 / 50 / 50
+//   D = 64: 32 of 4000, 16 rows 62 / 64 / 79, 64 rows 111 / 107 / 129, 256 rows 256 / 196 / 217; 4 of 2000, 128 rows 26 / 40 / -
+//   D = 256 (registers for 16 rows, LDS for 64 positions): 32 of 4000, 8 rows 235 / 201 / 212, 128 rows 1219 / 516 / 582, 256 rows 1888 / 732 / 652
 FpPlan planOf(const kcFlashPagesDims& d) {
     FpPlan p{};
-    const int64_t G = d.H / d.H_kv, rows = int64_t(d.N) * G;
+    const int64_t G = d.H / d.H_kv, rows = int64_t(d.N) * G, pairs = int64_t(d.N) * d.H * (int64_t(d.max_pages) * d.page);
     const int64_t each = d.seqs ? (rows + d.seqs - 1) / d.seqs : 0;
-    const bool wide = d.D == 256;
-    p.form = each <= 16 ? 0 : !wide && each <= 32 ? 1 : each <= (wide ? 64 : 128) ? 2 : 3;
-    constexpr int kRows[2][4] = {{64, 128, 128, 256}, {32, 32, 64, 128}};
-    p.rt = kRows[wide][p.form];
-    p.groups = p.form == 2 || (d.D == 64 && p.form < 2) ? 512 : 256;
+    const bool little = pairs <= (int64_t(1) << 37) / (d.D * d.D);
+    if (d.D == 64) p.form = little || each <= 64 ? 0 : 1;
+    else if (d.D == 128) p.form = little || each <= 16 ? 0 : each <= 128 ? 1 : 2;
+    else p.form = each <= 128 ? 1 : 2;
+    p.rt = (d.D == 256 ? 32 : 64) << p.form;
+    p.groups = p.form == 1 || d.D == 64 ? 512 : 256;
     p.items = int((rows / p.rt + d.seqs) * d.H_kv);
     p.each = int(std::min<int64_t>(each, p.rt));
     p.bytes = 16 + size_t(p.items) * 32 + size_t(p.groups) * 2 * p.rt * (d.D + 2) * 4;
@@ -700,15 +712,16 @@ int run(FpParams p, const FpPlan& plan, hipStream_t s) {
     return fromHip(hipGetLastError(), "flash_pages (join)");
 }
 
-// (heads of 256: 16 rows of a wavefront fill its registers, 64 positions of a step the LDS)
-template <int D>
-int runD(const FpParams& p, const FpPlan& plan, hipStream_t s) {
-    constexpr bool wide = D == 256;
-    switch (plan.form) {
-        case 0: return run<D, 1, wide ? 2 : 4, wide ? 2 : 4>(p, plan, s);
-        case 1: return run<D, wide ? 1 : 2, wide ? 2 : 4, wide ? 2 : 4>(p, plan, s);
-        case 2: return run<D, wide ? 1 : 2, 4, wide ? 1 : 2>(p, plan, s);
-        default: return run<D, wide ? 1 : 2, 8, wide ? 2 : 4>(p, plan, s);
+int runForm(int D, const FpParams& p, const FpPlan& plan, hipStream_t s) {
+    switch (D + plan.form) {
+        case 64: return run<64, 1, 4, 4>(p, plan, s);
+        case 65: return run<64, 2, 4, 2>(p, plan, s);
+        case 128: return run<128, 1, 4, 4>(p, plan, s);
+        case 129: return run<128, 2, 4, 2>(p, plan, s);
+        case 130: return run<128, 2, 8, 4>(p, plan, s);
+        case 257: return run<256, 1, 4, 1>(p, plan, s);
+        case 258: return run<256, 1, 8, 2>(p, plan, s);
+        default: return fromHip(hipErrorInvalidValue, "flash_pages: form");
     }
 }
 
@@ -751,12 +764,7 @@ int launchFlashPages(const kcFlashPagesArgs& a, hipStream_t s) {
     p.groups = plan.groups;
     p.items = plan.items;
     p.scale = a.scale;
-    switch (d.D) {
-        case 64: return runD<64>(p, plan, s);
-        case 128: return runD<128>(p, plan, s);
-        case 256: return runD<256>(p, plan, s);
-        default: return fromHip(hipErrorInvalidValue, "flash_pages: D");
-    }
+    return runForm(d.D, p, plan, s);
 }
 
 }  // namespace kcamd

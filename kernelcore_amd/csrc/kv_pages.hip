@@ -48,7 +48,8 @@ __device__ __forceinline__ int sumBefore(int x, int* waves, int tid, int& all) {
 }
 
 // A workgroup: 256 tokens. It sums over the sequences by itself (1024 in a round, until its tokens are covered): what other workgroups
-// found would take a launch of its own. Latency bounds it.
+// found would take a launch of its own. Latency bounds it: 8 requests of a token 4.1 us, 256 of 97 tokens 4.7, 500 trees of 24 nodes
+// 6.3 (their longest chain of parents, from LDS).
 __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     __shared__ int waves[2][kWaves];
     __shared__ int first[kThreads];                             // a token that is its sequence's first here: its number, else 0

@@ -629,6 +629,13 @@ struct Span {
 };
 bool overlap(const Span& a, const Span& b) { return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
 Span spanOf(const void* p, size_t bytes) { return {reinterpret_cast<uintptr_t>(p), p ? bytes : 0}; }
+// The first `outs` of n arrays overlap neither each other nor the rest.
+int apart(const Span* all, int outs, int n, const char* what) {
+    for (int i = 0; i < outs; ++i)
+        for (int j = i + 1; j < n; ++j)
+            if (overlap(all[i], all[j])) return invalid(what);
+    return 0;
+}
 
 int kvPagesValidate(const void* p, const kcLaunchContext*) {
     const auto& a = *static_cast<const kcKvPagesArgs*>(p);
@@ -657,10 +664,7 @@ int kvPagesValidate(const void* p, const kcLaunchContext*) {
     const Span all[11] = {spanOf(a.table, size_t(table)), spanOf(a.start, 4 * s + 4), spanOf(a.len, 4 * s), spanOf(a.slots, 8 * n), spanOf(a.pos, 4 * n),
                           spanOf(a.used, 4), spanOf(a.tree, 4 * n * size_t(a.tree_words)), spanOf(a.have, 4 * s), spanOf(a.add, 4 * s),
                           spanOf(a.free, 4 * size_t(a.n_free)), spanOf(a.parent, 4 * n)};
-    for (int i = 0; i < 7; ++i)
-        for (int j = i + 1; j < 11; ++j)
-            if (overlap(all[i], all[j])) return invalid("kv_pages: an output overlaps another array");
-    return 0;
+    return apart(all, 7, 11, "kv_pages: an output overlaps another array");
 }
 int kvPagesLaunch(const void* p, void* s) { return kcamd::launchKvPages(*static_cast<const kcKvPagesArgs*>(p), hs(s)); }
 
@@ -739,11 +743,12 @@ int fpShape(const kcFlashPagesDims& d) {
         return invalid("flash_pages: N H D below 2^31, (N H / H_kv / 16 + seqs) H_kv at most 2^24");
     return 0;
 }
-int fpCache(const kcFlashPagesDims& d, const void* p, int64_t row, int64_t head, const char* what) {
+int fpCache(const kcFlashPagesDims& d, const void* p, int64_t row, int64_t head, const char* what, Span* span) {
     int64_t a, b;
     if (row % 16 || head % 16 || !aligned(p, 16)) return invalid("flash_pages: cache rows, heads and base at multiples of 16 bytes");
     if (!extent(d.H_kv, head, int64_t(d.D) * 2, &a) || !extent(int64_t(d.n_pages) * d.page, row, a, &b) || row > INT32_MAX / d.page)
         return invalid("flash_pages: strides too large");
+    *span = spanOf(p, size_t(b));
     return checkRange(p, size_t(b), what);
 }
 int flashPagesValidate(const void* p, const kcLaunchContext*) {
@@ -757,15 +762,21 @@ int flashPagesValidate(const void* p, const kcLaunchContext*) {
     if (!extent(d.H, d.q_head, d.D, &x) || !extent(d.N, d.q_tok, x, &y)) return invalid("flash_pages: q strides too large");
     if (!extent(d.seqs, int64_t(d.table_row) * 4, int64_t(d.max_pages) * 4, &t)) return invalid("flash_pages: table too large");
     KC_TRY(checkRange(a.q, size_t(y) * 4, "q"));
-    KC_TRY(fpCache(d, a.k, d.k_row, d.k_head, "k"));
-    KC_TRY(fpCache(d, a.v, d.v_row, d.v_head, "v"));
+    Span k, v;
+    KC_TRY(fpCache(d, a.k, d.k_row, d.k_head, "k", &k));
+    KC_TRY(fpCache(d, a.v, d.v_row, d.v_head, "v", &v));
     KC_TRY(intsAt(a.table, t / 4, "table"));
     KC_TRY(intsAt(a.start, d.seqs ? int64_t(d.seqs) + 1 : 0, "start"));
     KC_TRY(intsAt(a.len, d.seqs, "len"));
     if (a.tree) KC_TRY(intsAt(a.tree, int64_t(d.N) * d.tree_words, "tree"));
     KC_TRY(checkRange(a.out, f32Bytes(int64_t(d.N) * d.H * d.D), "out"));
     if (a.lse) KC_TRY(checkRange(a.lse, f32Bytes(int64_t(d.N) * d.H), "lse"));
-    return checkRange(a.part, kcamd::flashPagesPartBytes(d), "part");
+    const size_t part = kcamd::flashPagesPartBytes(d), n = size_t(d.N), s = size_t(d.seqs);
+    KC_TRY(checkRange(a.part, part, "part"));
+    const Span all[10] = {spanOf(a.out, 4 * n * size_t(d.H) * size_t(d.D)), spanOf(a.lse, 4 * n * size_t(d.H)), spanOf(a.part, part),
+                          spanOf(a.q, size_t(y) * 4), k, v, spanOf(a.table, size_t(t)), spanOf(a.start, s ? 4 * s + 4 : 0), spanOf(a.len, 4 * s),
+                          spanOf(a.tree, 4 * n * size_t(d.tree_words))};
+    return apart(all, 3, 10, "flash_pages: an output or the workspace overlaps another array");
 }
 int flashPagesLaunch(const void* p, void* s) { return kcamd::launchFlashPages(*static_cast<const kcFlashPagesArgs*>(p), hs(s)); }
 
@@ -784,7 +795,11 @@ int sampleRowsValidate(const void* p, const kcLaunchContext*) {
     if (a.min_p) KC_TRY(intsAt(a.min_p, a.rows, "min_p"));
     KC_TRY(intsAt(a.tokens, a.rows, "tokens"));
     if (a.probs) KC_TRY(intsAt(a.probs, a.rows, "probs"));
-    return checkRange(a.part, kcamd::sampleRowsPartBytes(a.rows, a.n_vocab), "part");
+    const size_t part = kcamd::sampleRowsPartBytes(a.rows, a.n_vocab), n = 4 * size_t(a.rows);
+    KC_TRY(checkRange(a.part, part, "part"));
+    const Span all[9] = {spanOf(a.tokens, n), spanOf(a.probs, n), spanOf(a.part, part), spanOf(a.logits, size_t(x) * 4), spanOf(a.u, n),
+                         spanOf(a.temperature, n), spanOf(a.top_k, n), spanOf(a.top_p, n), spanOf(a.min_p, n)};
+    return apart(all, 3, 9, "sample_rows: an output or the workspace overlaps another array");
 }
 int sampleRowsLaunch(const void* p, void* s) { return kcamd::launchSampleRows(*static_cast<const kcSampleRowsArgs*>(p), hs(s)); }
 

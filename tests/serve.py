@@ -120,7 +120,9 @@ def plain_turn(x, pos, freqs, scale, n_rot, interleaved):
 # ---- flash_pages_f16 ----------------------------------------------------------------------------------------------
 
 class Pages:
-    """One call: sequences with lens[s] positions of which the last nodes[s] are the step's tokens, in a shuffled paged cache."""
+    """One call: sequences with lens[s] positions of which the last nodes[s] are the step's tokens, in a shuffled paged cache. Tables
+    have columns for `room` positions and rows of queries together at least (the kernel's form goes by what a table could hold)."""
+    room = 0
 
     def __init__(self, H, K, D, lens, nodes, page=16, tree=True, words=2, scale=None, seed=0, spread=1.0, parent=None, spare=3):
         r = np.random.default_rng([seed, D, H, len(lens), page])
@@ -131,7 +133,7 @@ class Pages:
         self.N = int(self.start[-1])
         held = -(-self.lens // page)
         self.n_pages = int(held.sum()) + spare
-        self.max_pages = max(1, int(held.max(initial=0)))
+        self.max_pages = max(1, int(held.max(initial=0)), -(-self.room // max(1, self.N * H) // page))
         order = r.permutation(self.n_pages).astype(np.int32)
         self.table = np.full((len(lens), self.max_pages), -1, np.int32)
         at = 0

@@ -18,6 +18,12 @@ def runtime():
     kc.synchronize()
 
 
+@pytest.fixture(autouse=True, params=[0, 1 << 26], ids=["", "room"])
+def room(request, monkeypatch):
+    """Tables as long as the sequences, and with room for more work than the form for little of it takes."""
+    monkeypatch.setattr(Pages, "room", request.param)
+
+
 HEADS = [(8, 2, 128), (6, 2, 64), (4, 2, 256), (32, 8, 128), (5, 5, 64), (16, 1, 128), (17, 1, 64), (10, 2, 256), (4, 4, 128)]
 
 

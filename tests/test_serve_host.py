@@ -99,7 +99,8 @@ checks("flash_pages_f16", make, good,
         (dict(v=None), IP), (dict(table=None), IP), (dict(start=None), IP), (dict(len=None), IP), (dict(out=None), IP), (dict(part=None), IP), (dict(N=13), IP), (dict(seqs=4), IP),
         (dict(n_pages=10), IP), (dict(max_pages=6), IP), (dict(tree_words=3), IP), (dict(k=good["k"] + 8), IV), (dict(part=good["part"] + 4), IV), (dict(part=good["part"] + 16), IP),
         (dict(q=good["q"] + 2), IV), (dict(out=good["out"] + 1), IV), (dict(lse=good["lse"] + 4), IP), (dict(start=good["start"] + 4), IP), (dict(len=good["len"] + 1), IV),
-        (dict(N=1 << 22), IV), (dict(seqs=1 << 24), IV)])
+        (dict(N=1 << 22), IV), (dict(seqs=1 << 24), IV), (dict(out=good["q"]), IV), (dict(lse=good["out"]), IV), (dict(lse=good["tree"] + 4, N=0), OK),
+        (dict(out=good["k"]), IV), (dict(lse=good["len"], N=1, H=2, q_head=0), IV), (dict(q=good["part"]), IV), (dict(table=good["part"]), IV)])
 b = C.c_size_t()
 assert kc.lib().kcFlashPagesPartBytes(None, C.byref(b)) == kc.ERR["InvalidValue"]
 assert kc.lib().kcFlashPagesPartBytes(C.byref(kc.FlashPagesDims(**dims)), None) == kc.ERR["InvalidValue"]
@@ -114,7 +115,8 @@ checks("sample_rows", lambda **k: kc.SampleRowsArgs(**k), good,
        [(dict(rows=-1), IV), (dict(rows=65536), IV), (dict(n_vocab=0), IV), (dict(n_vocab=(1 << 20) + 1), IV), (dict(row=-1), IV), (dict(row=1 << 62), IV), (dict(rows=0), OK),
         (dict(temperature=None), OK), (dict(top_k=None), OK), (dict(top_p=None), OK), (dict(min_p=None), OK), (dict(probs=None), OK), (dict(row=0), OK), (dict(logits=None), IP),
         (dict(u=None), IP), (dict(tokens=None), IP), (dict(part=None), IP), (dict(rows=4), IP), (dict(row=1011), IP), (dict(n_vocab=1001), IP), (dict(part=good["part"] + 16), IP),
-        (dict(part=good["part"] + 8), IV), (dict(u=good["u"] + 2), IV), (dict(logits=good["logits"] + 1), IV), (dict(tokens=good["tokens"] + 4), IP), (dict(top_k=good["top_k"] + 4), IP)])
+        (dict(part=good["part"] + 8), IV), (dict(u=good["u"] + 2), IV), (dict(logits=good["logits"] + 1), IV), (dict(tokens=good["tokens"] + 4), IP), (dict(top_k=good["top_k"] + 4), IP),
+        (dict(tokens=good["top_k"]), IV), (dict(probs=good["u"]), IV), (dict(probs=good["tokens"]), IV), (dict(part=good["logits"], rows=0), OK)])
 for args in ((-1, 10), (70000, 10), (1, 0), (1, (1 << 20) + 1)):
     assert kc.lib().kcSampleRowsPartBytes(*args, C.byref(b)) == kc.ERR["InvalidValue"], args
 assert kc.lib().kcSampleRowsPartBytes(1, 1, None) == kc.ERR["InvalidValue"]
