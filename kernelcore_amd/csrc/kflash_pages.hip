@@ -704,7 +704,10 @@ int run(FpParams p, const FpPlan& plan, hipStream_t s) {
     hipLaunchKernelGGL((flash_pages_kernel<D, NR, W, KM>), dim3(plan.groups), dim3(G::Threads), G::Lds, s, p);
     if (int e = fromHip(hipGetLastError(), "flash_pages")) return e;
     constexpr int Rows = 256 / (D / 4);
-    if (plan.items * 8 <= plan.groups) {  // many workgroups to an item
+    // Many workgroups to an item, and not so many rows that there is a join workgroup for each CU anyway: several threads to a value. (us, 32 heads
+    // on 8 of 128, with and without: one sequence of 20000 positions, 4 rows 27 / 31, 64 rows 44 / 52, 256 rows 77 / 75; 4 of 4000, 64 rows
+    // 40 / 45, 256 rows 70 / 64; 8 of 4000, 64 rows 56 / 53.)
+    if (plan.items * 8 <= plan.groups && plan.each <= 128) {
         hipLaunchKernelGGL((flash_pages_join_kernel<D, Rows>), dim3(plan.items, std::max(1, plan.each)), dim3(256), 0, s, p, G::RT);
     } else {
         hipLaunchKernelGGL((flash_pages_join_kernel<D, 1>), dim3(plan.items, (plan.each + Rows - 1) / Rows), dim3(256), 0, s, p, G::RT);

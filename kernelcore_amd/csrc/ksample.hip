@@ -220,7 +220,7 @@ struct Shared {
     };
     u64 list[kList];        // members of the wanted bins, the bin from bit 52 on
     u64 few[64];
-    double octaves[kOctave], top[kPieces], offset[kPieces];
+    double octaves[kOctave], top[kPieces], offset[kPieces];  // (64 pieces at most)
     int shift[kPieces];     // bins that a piece's lie further down
     u64 waves[kDraw / 64], waves2[kDraw / 64];
     u64 found[4], cut[4];
@@ -720,10 +720,12 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
 }
 
 int piecesOf(int rows, int n, int* piece) {
-    // pieces of 16384 logits until they fill the GPU twice, of 32768 beyond (a piece's bins are 16 KiB to write and read)
-    const int64_t small = ((int64_t)n + 16383) / 16384;
-    *piece = small * rows <= 512 ? 16384 : 32768;
-    return (int)(((int64_t)n + *piece - 1) / *piece);
+    // Pieces of 32768 logits, which are 16 KiB of bins each to write and read; of 16384 for few rows, which then have more workgroups, and for small
+    // vocabularies, which would be one piece or two. (us with pieces of 16384 / 32768: 128256 logits, 1 row 22.3 / 25.4; 151936 logits, 8 rows
+    // 26.1 / 26.0, 32 rows 36.8 / 33.2, 256 rows 66.3 / 62.8; 32000 logits, 1 row 21.5 / 22.7, 64 rows 24.2 / 26.7, 256 rows 32.7 / 33.9.)
+    const int small = (n + 16383) / 16384;
+    *piece = n <= 65536 || (int64_t)small * rows <= 64 ? 16384 : 32768;
+    return (n + *piece - 1) / *piece;
 }
 
 }  // namespace
