@@ -10,8 +10,8 @@
 // which workgroup was first).
 //
 // What bounds it: single tokens the cache's bytes (128 sequences of 4000 positions, 32 heads on 8 of 128: 368 us, 5.6 TB/s); wide trees products
-// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 228 us, 0.46 PFLOP/s
-// counted once, matrix units 47% and VALU 43% of the cycles); a small call the chain of shares, first loads, steps and join (one
+// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 221 us, 0.47 PFLOP/s
+// counted once, matrix units busy in 47% of the cycles, vector instructions in 43%); a small call the chain of shares, first loads, steps and join (one
 // token over 8191 positions: 10 + 4 us).
 #include <hip/hip_runtime.h>
 
