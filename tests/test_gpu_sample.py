@@ -63,6 +63,17 @@ def test_many_rows(V, rows):
         assert tokens[i] in want and abs(probs[i] - pr[want.index(tokens[i])]) < 1e-6
 
 
+@pytest.mark.parametrize("V", [65536, 65537, 1 << 20])
+@pytest.mark.parametrize("rows", [1, 2, 9])
+@pytest.mark.parametrize("kw", [dict(top_k=40), dict(top_p=0.8), {}], ids=str)
+def test_large_vocabulary(V, rows, kw):
+    """Few rows in small pieces and in large ones; borders among the first tokens, and where most logits are read again."""
+    print("sample_rows", V, rows, kw, flush=True)
+    r = np.random.default_rng([V, rows])
+    l = (r.standard_normal((rows, V)) * 1.5).astype(np.float32)
+    check(l, r.random(rows).astype(np.float32), **kw)
+
+
 @pytest.mark.parametrize("V", [1, 100, 5000, 40000, 128256])
 def test_ties(V):
     """Equal logits are ordered by their number, also where thousands are equal."""
