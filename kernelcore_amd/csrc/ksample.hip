@@ -12,9 +12,9 @@
 // in 64 bits, always in the same order. (Weights in 32 bits would move the borders by about 2^-24 of the whole, and among 150000 flat
 // weights there is a border every 2^-17.)
 //
-// What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 69 us, 4.5 TB/s, the draws 98 us, of which
+// What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 69 us, 4.5 TB/s, the draws 95 us, of which
 // the second reading 55), for one row latencies, of one workgroup's steps one after the other (128256 logits, top_k 40: 5.5 and
-// 18 us; a flat row of 151936 under top_p 0.8, of which all is read again by one CU, 25 us more).
+// 16 us; a flat row of 151936 under top_p 0.8, of which all is read again by one CU, 25 us more).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -259,6 +259,10 @@ __device__ __forceinline__ void scanTwo(X& x, Y& y, u64* wx, u64* wy, int tid) {
     y += yb;
 }
 
+// Lane i's value, i the same for all.
+__device__ __forceinline__ u64 laneOf(u64 x, int i) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, i);
+}
 __device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ float same(float x) { return __builtin_bit_cast(float, same(__builtin_bit_cast(int, x))); }
 __device__ __forceinline__ double same(double x) {
@@ -305,6 +309,11 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             S.listed = S.grouped = 0;
         }
     }
+    float ahead[8][kThreads / NT];  // (of the first pieces: on the way while the bins are looked at)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int h = 0; h < kThreads / NT; ++h) ahead[k][h] = pieces[min(k, a.pieces - 1)].tops[tid + NT * h];
     if (tid < 8) S.bins[tid] = kBins;
     if (wave == 1 && lane < kOctave) S.octaves[lane] = exp2(-(lane + 0.5) / kPerOctave);
     __syncthreads();
@@ -432,12 +441,13 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     const int to[3] = {bU1, max(cutP ? bP1 : -1, cutM ? bM1 : -1), cutK ? bK : -1};
     const double offset = offsetOf(same(S.rowTop), slope, refOf(same(S.rowTop), slope));
     // Their logits, and what rounding may take off: |l - mid| - half below 0 for one of them.
+    const double perBin = 1.0 / slope32;
     float mid[3], half[3], lowest = INFINITY;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         constexpr float kMost = 3.402823466e38f;  // (nothing here may be infinite: the difference of two is NaN, which is nobody's neighbour)
-        const float hiL = (float)fmax(fmin(top - (from[k] - offset) / slope32, (double)kMost), -(double)kMost);
-        const float loL = (float)fmax(fmin(top - (to[k] + 1 - offset) / slope32, (double)kMost), -(double)kMost);
+        const float hiL = (float)fmax(fmin(top - (from[k] - offset) * perBin, (double)kMost), -(double)kMost);
+        const float loL = (float)fmax(fmin(top - (to[k] + 1 - offset) * perBin, (double)kMost), -(double)kMost);
         const float slack = 2.4e-7f * fmaxf((float)fabs(top), 1.2e-38f);
         const bool none = to[k] < from[k], all = slope == 0.0;  // (a slope of 0: all logits lie in one bin)
         const float hi = fminf(fmaf(fabsf(hiL), 2.4e-7f, hiL) + slack, kMost), lo = fmaxf(fminf(fmaf(fabsf(loL), -2.4e-7f, loL) - slack, 3.4e38f), -kMost);
@@ -477,11 +487,11 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     // The groups whose largest logit is not below all of them: few where the borders are among a row's first tokens (one row of 128256
     // with top_k 40: 4.5 us, 14 for all logits). Of more than there is room for all logits are read.
     for (int p0 = 0; p0 < a.pieces; p0 += 8) {
-        float tops[8];
 #pragma unroll
         for (int h = 0; h < kThreads / NT; ++h) {
+            float tops[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) tops[k] = pieces[min(p0 + k, a.pieces - 1)].tops[tid + NT * h];
+            for (int k = 0; k < 8; ++k) tops[k] = p0 ? pieces[min(p0 + k, a.pieces - 1)].tops[tid + NT * h] : ahead[k][h];
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (p0 + k < a.pieces && tops[k] >= lowest) {
@@ -638,26 +648,20 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         });
         __syncthreads();
         if (wave == 0) {
-            const int m = min(S.nfew, 64);
+            const int m = min(same(S.nfew), 64);
             const u64 mine = lane < m ? S.few[lane] : ~0ull;
             const u64 w = lane < m ? unitOf(mine) : 0;
             u64 upTo = before;
-            unsigned rank = nBefore;
+            unsigned rank = 0;  // with itself
             for (int i = 0; i < m; ++i) {
-                const u64 other = S.few[i], ow = __shfl(w, i);
-                if (other <= mine) {
-                    upTo += ow;
-                    ++rank;
-                }
+                const u64 other = laneOf(mine, i), ow = laneOf(w, i);
+                upTo += other <= mine ? ow : 0;
+                rank += other <= mine;
             }
-            const bool reached = lane < m && (byCount ? rank >= want : upTo >= want);
-            u64 best = reached ? mine : ~0ull, last = lane < m ? mine : 0;
-#pragma unroll
-            for (int o = 32; o; o >>= 1) {
-                best = min(best, (u64)__shfl_xor(best, o));
-                last = max(last, (u64)__shfl_xor(last, o));
-            }
-            if (lane < m && mine == (best != ~0ull ? best : last)) {
+            // (the ones that do not reach it come first)
+            const bool reached = byCount ? nBefore + rank >= want : upTo >= want;
+            const int first = min(__builtin_popcountll(__ballot(lane < m && !reached)), m - 1);
+            if (lane < m && (int)rank == first + 1) {
                 S.found[0] = upTo;
                 S.found[1] = mine;
                 S.found[2] = w;
