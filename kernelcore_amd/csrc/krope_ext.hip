@@ -61,16 +61,18 @@ __device__ __forceinline__ Unit unitOf(int u, int n_rot, int D) {
     return x;
 }
 
+template <bool FULL>
 __device__ __forceinline__ f32x4 loadPart(const float* p, int n) {
-    if (n == 4) return *reinterpret_cast<const f4a4*>(p);
+    if (FULL || n == 4) return *reinterpret_cast<const f4a4*>(p);
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 3; ++e)
         if (e < n) x[e] = p[e];
     return x;
 }
+template <bool FULL>
 __device__ __forceinline__ void storePart(float* p, f32x4 x, int n) {
-    if (n == 4) {
+    if (FULL || n == 4) {
         *reinterpret_cast<f4a4*>(p) = x;
         return;
     }
@@ -78,8 +80,9 @@ __device__ __forceinline__ void storePart(float* p, f32x4 x, int n) {
     for (int e = 0; e < 3; ++e)
         if (e < n) p[e] = x[e];
 }
+template <bool FULL>
 __device__ __forceinline__ void storePart(_Float16* p, f32x4 x, int n) {
-    if (n == 4) {
+    if (FULL || n == 4) {
         *reinterpret_cast<h4a2*>(p) = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
         return;
     }
@@ -107,9 +110,11 @@ __device__ __forceinline__ void turn(f32x4& a, f32x4& b, const Unit& u, const fl
 
 // A workgroup takes all heads of q, or all of k and v, of q_tokens or kv_tokens tokens, eight values a thread at a time. The first kAhead
 // of a thread's are loaded before the angles are computed (once, into LDS) and repeated slots looked for: what bounds it is the
-// bytes, and for few tokens the latency of one load and the angles. 3333 tokens of 24 + 2 x 8 heads of 128, from memory: 28 us, 4.4 TB/s
+// bytes, and for few tokens the latency of one load and the angles. 3333 tokens of 24 + 2 x 8 heads of 128, from memory: 27 us, 4.5 TB/s
 // where a copy of as many bytes reaches 5.0 (35 us with loads after the angles and k and v last); one token 4 us.
-template <bool INTER>
+// FULL: every group has its four values (heads and rotated parts of whole eights), so that a load is one and none waits for another (the prompt
+// below 27 us, 28 without).
+template <bool INTER, bool FULL>
 __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
     __shared__ float2 cs[kPairs];
     __shared__ int later[16], rowOf[16];
@@ -144,12 +149,10 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
     auto load = [&](int x0) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            const int x = x0 + kThreads * k;
-            if (x < all) {
-                at[k] = placeOf(x);
-                lo[k] = loadPart(at[k].src + at[k].u.a, at[k].u.na);
-                hi[k] = loadPart(at[k].src + at[k].u.b, at[k].u.nb);
-            }
+            const int x = min(x0 + kThreads * k, all - 1);
+            at[k] = placeOf(x);
+            lo[k] = loadPart<FULL>(at[k].src + at[k].u.a, at[k].u.na);
+            hi[k] = loadPart<FULL>(at[k].src + at[k].u.b, at[k].u.nb);
         }
     };
     load(tid);
@@ -185,13 +188,13 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
             if (u.pa >= 0) turn<INTER>(lo[k], hi[k], u, cs + t * pairs, pairs);
             if (isQ) {
                 float* dst = a.q_out + (long long)(t0 + t) * a.out_tok + (long long)h * a.out_head;
-                storePart(dst + u.a, lo[k], u.na);
-                storePart(dst + u.b, hi[k], u.nb);
+                storePart<FULL>(dst + u.a, lo[k], u.na);
+                storePart<FULL>(dst + u.b, hi[k], u.nb);
             } else if (rowOf[t] >= 0 && !later[t]) {
                 char* to = at[k].isV ? a.v_cache + rowOf[t] * a.vc_row + h * a.vc_head : a.k_cache + rowOf[t] * a.kc_row + h * a.kc_head;
                 _Float16* dst = reinterpret_cast<_Float16*>(to);
-                storePart(dst + u.a, lo[k], u.na);
-                storePart(dst + u.b, hi[k], u.nb);
+                storePart<FULL>(dst + u.a, lo[k], u.na);
+                storePart<FULL>(dst + u.b, hi[k], u.nb);
             }
         }
     }
@@ -214,8 +217,11 @@ int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
     const int qBlocks = a.q ? (a.n_tokens + p.q_tokens - 1) / p.q_tokens : 0;
     p.kv_blocks = a.k ? (a.n_tokens + p.kv_tokens - 1) / p.kv_tokens : 0;
     const dim3 grid(p.kv_blocks + qBlocks);
-    if (a.interleaved) hipLaunchKernelGGL(rope_ext_kernel<true>, grid, dim3(kThreads), 0, s, p);
-    else hipLaunchKernelGGL(rope_ext_kernel<false>, grid, dim3(kThreads), 0, s, p);
+    const bool full = a.n_rot % 8 == 0 && a.D % 8 == 0;
+    if (a.interleaved && full) hipLaunchKernelGGL((rope_ext_kernel<true, true>), grid, dim3(kThreads), 0, s, p);
+    else if (a.interleaved) hipLaunchKernelGGL((rope_ext_kernel<true, false>), grid, dim3(kThreads), 0, s, p);
+    else if (full) hipLaunchKernelGGL((rope_ext_kernel<false, true>), grid, dim3(kThreads), 0, s, p);
+    else hipLaunchKernelGGL((rope_ext_kernel<false, false>), grid, dim3(kThreads), 0, s, p);
     return fromHip(hipGetLastError(), "rope_ext");
 }
 

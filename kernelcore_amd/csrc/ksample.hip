@@ -14,7 +14,7 @@
 //
 // What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 69 us, 4.5 TB/s, the draws 95 us, of which
 // the second reading 55), for one row latencies, of one workgroup's steps one after the other (128256 logits, top_k 40: 5.5 and
-// 16 us; a flat row of 151936 under top_p 0.8, of which all is read again by one CU, 25 us more).
+// 15 us; a flat row of 151936 under top_p 0.8, of which all is read again by one CU, 25 us more).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -66,9 +66,14 @@ __device__ __forceinline__ f32x4 fourAt(__amdgpu_buffer_rsrc_t x, int at) {
 }
 // (Rows that take the likeliest token count as temperature 1.)
 __device__ __forceinline__ bool greedy(float t) { return !(t > 0.0f); }
+// A row's value of an array that may be null. (The load is unconditional, of u's in its place: under a condition each would be waited for.)
+__device__ __forceinline__ float valueOf(const SampleArgs& a, const float* x, int r, float none) {
+    const float y = (x ? x : a.u)[r];
+    return x ? y : none;
+}
 // Octaves of weight per unit of logit.
 __device__ __forceinline__ double slopeOf(const SampleArgs& a, int r) {
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
+    const float t = valueOf(a, a.temperature, r, 1.0f);
     return greedy(t) ? 1.4426950408889634 : 1.4426950408889634 / (double)t;
 }
 // ref, and what the largest logit lies below it, in bins: within an octave, also where z is so large that integers are far apart.
@@ -281,16 +286,18 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     const Piece* pieces = reinterpret_cast<const Piece*>(a.part) + (size_t)r * a.pieces;
     const float* x = a.logits + (long long)r * a.row;
     const double slope = slopeOf(a, r), slope32 = kPerOctave * slope;
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
-    const float p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
-    const int tk = a.top_k ? a.top_k[r] : 0;
+    const float t = valueOf(a, a.temperature, r, 1.0f), p = valueOf(a, a.top_p, r, 1.0f), mp = valueOf(a, a.min_p, r, 0.0f);
+    const int tk = a.top_k ? __builtin_bit_cast(int, valueOf(a, reinterpret_cast<const float*>(a.top_k), r, 0.0f)) : 0;
     double u = a.u[r];
     unsigned finite = 0;
     if (wave == 0) {
         const bool in = lane < a.pieces;
-        const float mine = in ? pieces[lane].top : -INFINITY;
-        const bool wild = __any(in && pieces[lane].wild);
-        finite = in ? pieces[lane].finite : 0;
+        const Piece& piece = pieces[min(lane, a.pieces - 1)];
+        const float topHere = piece.top, mine = in ? topHere : -INFINITY;
+        const int wildHere = piece.wild;
+        const unsigned finiteHere = piece.finite;
+        const bool wild = __any(in && wildHere);
+        finite = in ? finiteHere : 0;
         float top = mine;
 #pragma unroll
         for (int o = 32; o; o >>= 1) {
