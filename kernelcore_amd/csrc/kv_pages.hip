@@ -48,8 +48,8 @@ __device__ __forceinline__ int sumBefore(int x, int* waves, int tid, int& all) {
 }
 
 // A workgroup: 256 tokens. It sums over the sequences by itself (1024 in a round, until its tokens are covered): what other workgroups
-// found would take a launch of its own. Latency bounds it: 8 requests of a token 4.1 us, 256 of 97 tokens 4.7, 500 trees of 24 nodes
-// 6.3 (their longest chain of parents, from LDS).
+// found would take a launch of its own. Latency bounds it: 8 requests of a token 4 us, 256 of 97 tokens 4.2, 500 trees of 24 nodes
+// 5.0 (their longest chain of parents, from LDS).
 __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     __shared__ int waves[2][kWaves];
     __shared__ int first[kThreads];                             // a token that is its sequence's first here: its number, else 0
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     a.slots[t] = page < 0 ? -1ll : ((long long)page << a.shift) + (p & (per - 1));
     int depth = node;
     if (a.parent && a.tree_words <= 2 && r.y >= t0 - kThreads) {
-        // up to 64 bits, all parents in LDS: the bits in registers (500 trees of 24 nodes: 5.5 us, 6.3 by the form below)
+        // up to 64 bits, all parents in LDS: the bits in registers (500 trees of 24 nodes: 5.0 us, 5.8 by the form below)
         const int* up = parents + (r.y - (t0 - kThreads));
         unsigned long long bits = 0;
         depth = -1;
