@@ -407,8 +407,8 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
             const char* kt = tiles + slot * G::Tile;
             const char* vt = kt + G::Tile / 2;
             float x[NR][8];
-            // (2 NR independent sums, and a wavefront in its products before one in its weights: 240 to 230 us for 64 nodes of 8 sequences
-            // of 100000 positions; two sums took the products' latency each time)
+            // (2 NR independent sums, and a wavefront in its products before one in its weights: 240 to 230 us for 64 nodes over 100000
+            // positions, 155 to 148 for trees of 32 sequences; two sums took the products' latency each time)
             f32x4 sc[2][NR];
 #pragma unroll
             for (int t = 0; t < 2; ++t)

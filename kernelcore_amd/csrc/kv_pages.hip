@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     a.slots[t] = page < 0 ? -1ll : ((long long)page << a.shift) + (p & (per - 1));
     int depth = node;
     if (a.parent && a.tree_words <= 2 && r.y >= t0 - kThreads) {
-        // up to 64 bits, all parents in LDS: the bits in registers (500 trees of 24 nodes: 5.0 us, 5.8 by the form below)
+        // up to 64 bits, all parents in LDS: the bits in registers (500 trees of 24 nodes: 0.8 us less than by the form below)
         const int* up = parents + (r.y - (t0 - kThreads));
         unsigned long long bits = 0;
         depth = -1;
