@@ -358,40 +358,39 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
             }
     }
     if (tid == NT - 1) cnt[BPT - 1] = words[BPT - 1] = 0;  // (the last bin)
-    {
-        double sums[BPT], sum = 0.0, own = 0.0;
-        unsigned n = 0;
+    double sumTo[BPT], own = 0.0;  // weights up to and with a bin, tokens likewise
+    unsigned countTo[BPT], n = 0;
 #pragma unroll
-        for (int e = 0; e < BPT; ++e) {
-            own += factorOf(S.octaves, BPT * tid + e) * (double)unitsOf(words[e], cnt[e]);
-            sums[e] = own;
-            n += cnt[e];
-        }
-        sum = own;
-        unsigned upTo = n;
-        scanTwo<NT / 64>(sum, upTo, S.waves, S.waves2, tid);
-        S.sum[BPT * tid + BPT - 1] = sum;
-        unsigned c = upTo - n;
+    for (int e = 0; e < BPT; ++e) {
+        own += factorOf(S.octaves, BPT * tid + e) * (double)unitsOf(words[e], cnt[e]);
+        sumTo[e] = own;
+        n += cnt[e];
+        countTo[e] = n;
+    }
+    double sum = own;
+    unsigned upTo = n;
+    scanTwo<NT / 64>(sum, upTo, S.waves, S.waves2, tid);
+    if (tid == NT - 1) {
+        cnt[BPT - 1] = finite - upTo;
+        countTo[BPT - 1] = finite - (upTo - n);
+    }
+    sumTo[BPT - 1] = S.sum[BPT * tid + BPT - 1] = sum;
 #pragma unroll
-        for (int e = 0; e < BPT; ++e) {
-            c += cnt[e];
-            S.count[BPT * tid + e] = c;
-        }
-        if (tid == NT - 1) S.count[kFar] = finite;
-        __syncthreads();
-        const double before = tid ? S.sum[BPT * tid - 1] : 0.0;
-#pragma unroll
-        for (int e = 0; e < BPT - 1; ++e) S.sum[BPT * tid + e] = before + sums[e];
-        if (tid == NT - 1) cnt[BPT - 1] = finite - S.count[kFar - 1];
+    for (int e = 0; e < BPT; ++e) {
+        countTo[e] += upTo - n;
+        S.count[BPT * tid + e] = countTo[e];
     }
     __syncthreads();
+    const double before = tid ? S.sum[BPT * tid - 1] : 0.0;
+#pragma unroll
+    for (int e = 0; e < BPT - 1; ++e) sumTo[e] = S.sum[BPT * tid + e] = before + sumTo[e];
     auto sumBefore = [&](int b) { return b ? S.sum[b - 1] : 0.0; };
     auto countBefore = [&](int b) { return b ? S.count[b - 1] : 0u; };
-    // the first bin with a token at which cond(bin) holds, kBins if none; to S.bins[slot]
+    // the first bin with a token at which cond(its number among the thread's) holds, kBins if none; to S.bins[slot]
     auto firstBin = [&](int slot, auto&& cond) {
         int first = kBins;
 #pragma unroll
-        for (int e = BPT - 1; e >= 0; --e) first = cnt[e] && cond(BPT * tid + e) ? BPT * tid + e : first;
+        for (int e = BPT - 1; e >= 0; --e) first = cnt[e] && cond(e) ? BPT * tid + e : first;
         const unsigned long long v = __ballot(first < kBins);
         if (v && lane == __builtin_ctzll(v)) atomicMin(S.bins + slot, first);
     };
@@ -402,7 +401,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     bool cutP = p < 1.0f && K > 1, cutM = mp > 0.0f && K > 1;
     u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
     firstBin(0, [&](int) { return true; });  // the largest token's
-    firstBin(1, [&](int b) { return S.count[b] >= K; });
+    firstBin(1, [&](int e) { return countTo[e] >= K; });
     __syncthreads();
     const int b0 = same(S.bins[0]), bK = same(S.bins[1]);
     // what top_k keeps: between kLo and kHi
@@ -410,8 +409,8 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     const double kHi = S.sum[bK], kLo = cutK ? sumBefore(bK) : kHi;
     int bP0 = kBins, bP1 = kBins;
     if (cutP) {
-        firstBin(2, [&](int b) { return S.sum[b] >= p * kLo; });
-        firstBin(3, [&](int b) { return S.sum[b] >= p * kHi; });
+        firstBin(2, [&](int e) { return sumTo[e] >= p * kLo; });
+        firstBin(3, [&](int e) { return sumTo[e] >= p * kHi; });
     }
     __syncthreads();
     if (cutP) {
@@ -438,8 +437,8 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     // the whole sum, and the draw's target: between these
     const int lo = min(min(bK, bP0), bM0), hi = min(min(bK, bP1), bM1);
     const double sLo = cutP || cutM ? sumBefore(lo) : kLo, sHi = cutP || cutM ? S.sum[hi] : kHi;
-    firstBin(4, [&](int b) { return S.sum[b] > u * sLo; });
-    firstBin(5, [&](int b) { return S.sum[b] > u * sHi; });
+    firstBin(4, [&](int e) { return sumTo[e] > u * sLo; });
+    firstBin(5, [&](int e) { return sumTo[e] > u * sHi; });
     __syncthreads();
     const int bU0 = min(same(S.bins[4]), hi), bU1 = min(same(S.bins[5]), hi);
 
