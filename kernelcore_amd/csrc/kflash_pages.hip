@@ -175,13 +175,19 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
     const int i = lane & 15, g = lane >> 4;
     const int wg = blockIdx.x;
 
-    // ---- this workgroup's share. A unit is what a step of 32 positions costs: a step over KG x 32 has KG (the cache's bytes bound it; two
-    // where eight wavefronts have rows of their own, whose products take as long as 64 positions take to load).
-    constexpr int lgW = W == 8 ? 3 : W == 4 ? 2 : 1, lgMin = W / KM == 4 ? 2 : W / KM == 2 ? 1 : 0, lgRows = NR == 2 ? 5 : 4;
+    // ---- this workgroup's share. Four units are what 32 positions of a KV head cost where the wavefronts stand side by side over the keys as
+    // much as they can (the cache's bytes bound that); positions of more rows cost more, and an item's first loads, its q and its join as much as
+    // Setup units, where it is not many workgroups that take an item. (us with one price for all positions, with these, with the items' own too,
+    // 32 heads on 8 of 128: trees of 8 to 24 nodes, 32 sequences of 4000 positions 150, 137, 134, 128 of 2000 307, 280, 275; trees of 20 to
+    // 64 nodes, where twice the price for more than 128 rows was too much, 279, 256, 249 and 533, 496, 473; one to seven tokens 129, 115,
+    // 113; single tokens of 128 sequences 196 and 189.)
+    constexpr int lgW = W == 8 ? 3 : 2, lgMin = W / KM == 4 ? 2 : W / KM == 2 ? 1 : 0, lgRows = NR == 2 ? 5 : 4;
+    constexpr int Setup = 24;
+    auto tileUnits = [](int lg) { return W == 8 ? (lg < lgW ? 4 : D == 256 ? 6 : 7) : 4 + 2 * (lg - lgMin); };
     static_assert(1 << lgW == W && KM << lgMin == W && 1 << lgRows == 16 * NR);
     struct Seq {
         int nodes, len, lg, blocks, steps, weight;  // tokens, positions, log2 RG, blocks of rows, steps, a step's units
-        long long units;                            // of all its items
+        long long units;                            // of all its items' steps
     };
     const int most = a.max_pages << a.shift;
     auto sequence = [&](int s) {
@@ -194,7 +200,7 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
         q.blocks = (waves + (1 << q.lg) - 1) >> q.lg;
         const int sh = 5 + lgW - q.lg;
         q.steps = max(1, (q.len >> sh) + ((q.len & ((1 << sh) - 1)) != 0));
-        q.weight = W == 8 && q.lg == lgW ? 2 : W >> q.lg;
+        q.weight = (W >> q.lg) * tileUnits(q.lg);
         q.units = (long long)q.blocks * a.H_kv * ((long long)q.steps * q.weight);
         return q;
     };
@@ -235,15 +241,21 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
     };
     for (int s0 = 0; s0 < a.seqs; s0 += NT) round(s0);
     if (wg == 0 && tid == 0) a.head[0] = (int)min(items, (long long)a.items);
-    // (a workgroup's units hold a step at least of each item that they touch: more than a step has, and a power of two of workgroups)
-    const long long share = max((long long)W, (total + a.groups - 1) >> (31 - __builtin_clz(a.groups)));
+    const int setup = items * 8 >= a.groups ? Setup : 0;
+    total += items * setup;
+    // (a workgroup's units hold a step at least of each item whose steps they touch: as many as a step has at most, and a power of two of
+    // workgroups)
+    // (few items: whole steps of most kinds, so that an item's last workgroup rather ends with it than begins the next)
+    long long share = max(4ll * W, (total + a.groups - 1) >> (31 - __builtin_clz(a.groups)));
+    if (!setup) share = (share + 7) & ~7ll;
     const long long u0 = wg * share, u1 = min(total, u0 + share);
     if (u0 >= u1) return;
     // the sequence of unit u0, the units and items before it
     auto find = [&](int s0) {
-        if (mine && u0 >= upTo - mine && u0 < upTo) {
+        const long long to = upTo + itemsTo * setup, from = to - mine - myItems * setup;
+        if (u0 >= from && u0 < to) {
             found[0] = s0 + tid;
-            found[1] = upTo - mine;
+            found[1] = from;
             found[2] = itemsTo - myItems;
         }
     };
@@ -271,8 +283,9 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
     for (long long u = u0; u < u1;) {
         // ---- the item of unit u
         Seq q = sequence(s);
-        while (u >= sBefore + q.units) {
-            sBefore += q.units;
+        const auto all = [&] { return q.units + (long long)q.blocks * a.H_kv * setup; };
+        while (u >= sBefore + all()) {
+            sBefore += all();
             sItems += q.blocks * a.H_kv;
             q = sequence(++s);
         }
@@ -286,22 +299,22 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
         it.base = a.len[s] - q.nodes;
         it.rows = q.nodes * a.G;
         it.table = a.table + (size_t)s * a.table_row;
-        const long long per = (long long)q.steps * q.weight;  // an item's units
+        const long long per = (long long)q.steps * q.weight + setup;  // an item's units
         const int at = over(u - sBefore, per);
         const long long i0 = sBefore + at * per;
         const int item = sItems + at;
         it.kvh = at / q.blocks;
         it.r0 = (at - it.kvh * q.blocks) * rt;
         // the steps whose first unit is in this workgroup's share
-        const int st0 = (int)(u - i0 + q.weight - 1) / q.weight;
-        const int st1 = (int)(min(u1 - i0, per) + q.weight - 1) / q.weight;
+        auto stepsBefore = [&](long long x) { return (int)(max(x - setup, 0ll) + q.weight - 1) / q.weight; };
+        const int st0 = stepsBefore(u - i0), st1 = stepsBefore(min(u1 - i0, per));
         const bool whole = st0 == 0 && st1 == q.steps;
         const int rows = min(rt, it.rows - it.r0);
         u = min(u1, i0 + per);
         if (item >= a.items) return;  // (more rows than N tokens have: sequences that overlap)
-        if (st0 >= st1) continue;     // (the item's last steps began in the share before)
+        if (st0 >= st1) continue;     // (the item's last steps began in the share before, or its first ones begin in the next)
         if (st0 == 0 && tid < 8) {
-            const int n = over(i0 + (long long)(q.steps - 1) * q.weight - u0, share) + 1;
+            const int n = over(i0 + setup + (long long)(q.steps - 1) * q.weight - u0, share) + 1;
             const int d[8] = {it.token0, it.r0, rows, it.kvh, wg, n, 0, 0};
             a.head[4 + 8 * item + tid] = d[tid];
         }
