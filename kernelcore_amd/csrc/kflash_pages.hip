@@ -9,8 +9,8 @@
 // workgroups is joined by a second kernel from their sums (in the order of the keys, so that results do not depend on
 // which workgroup was first).
 //
-// What bounds it: single tokens the cache's bytes (128 sequences of 4000 positions, 32 heads on 8 of 128: 368 us, 5.6 TB/s); wide trees products
-// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 221 us, 0.47 PFLOP/s
+// What bounds it: single tokens the cache's bytes (128 sequences of 4000 positions, 32 heads on 8 of 128: 363 us with the join, 5.7 TB/s); wide trees products
+// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 218 us, 0.48 PFLOP/s
 // counted once, matrix units busy in 47% of the cycles, vector instructions in 43%); a small call the chain of shares, first loads, steps and join (one
 // token over 8191 positions: 10 + 4 us).
 #include <hip/hip_runtime.h>
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
         it.kvh = at / q.blocks;
         it.r0 = (at - it.kvh * q.blocks) * rt;
         // the steps whose first unit is in this workgroup's share
-        auto stepsBefore = [&](long long x) { return (int)(max(x - setup, 0ll) + q.weight - 1) / q.weight; };
+        auto stepsBefore = [&](long long x) { return (int)((unsigned)(max(x - setup, 0ll) + q.weight - 1) / (unsigned)q.weight); };
         const int st0 = stepsBefore(u - i0), st1 = stepsBefore(min(u1 - i0, per));
         const bool whole = st0 == 0 && st1 == q.steps;
         const int rows = min(rt, it.rows - it.r0);
