@@ -67,8 +67,9 @@ __device__ __forceinline__ f32x4 fourAt(__amdgpu_buffer_rsrc_t x, int at) {
 // (Rows that take the likeliest token count as temperature 1.)
 __device__ __forceinline__ bool greedy(float t) { return !(t > 0.0f); }
 // A row's value of an array that may be null. (The load is unconditional, of u's in its place: under a condition each would be waited for.)
-__device__ __forceinline__ float valueOf(const SampleArgs& a, const float* x, int r, float none) {
-    const float y = (x ? x : a.u)[r];
+template <class T>
+__device__ __forceinline__ T valueOf(const SampleArgs& a, const T* x, int r, T none) {
+    const T y = (x ? x : reinterpret_cast<const T*>(a.u))[r];
     return x ? y : none;
 }
 // Octaves of weight per unit of logit.
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     const float* x = a.logits + (long long)r * a.row;
     const double slope = slopeOf(a, r), slope32 = kPerOctave * slope;
     const float t = valueOf(a, a.temperature, r, 1.0f), p = valueOf(a, a.top_p, r, 1.0f), mp = valueOf(a, a.min_p, r, 0.0f);
-    const int tk = a.top_k ? __builtin_bit_cast(int, valueOf(a, reinterpret_cast<const float*>(a.top_k), r, 0.0f)) : 0;
+    const int tk = valueOf(a, a.top_k, r, 0);
     double u = a.u[r];
     unsigned finite = 0;
     if (wave == 0) {
