@@ -368,23 +368,45 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         n += cnt[e];
         countTo[e] = n;
     }
-    double sum = own;
+    // Sums by halves: to those of a right half its left half's last one is added. So, roundings included, none is below the bin's before
+    // it and none differs from it where the bin has no token: what a comparison of sums finds is a bin with tokens, and u times a sum
+    // is reached below it. (Where each sum was added up in its own way, an empty bin's could lie a rounding above the last one with tokens,
+    // and a number of 1 or more draw from there.)
     unsigned upTo = n;
-    scanTwo<NT / 64>(sum, upTo, S.waves, S.waves2, tid);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const unsigned k = __shfl_up(upTo, o);
+        const double left = __shfl(sumTo[BPT - 1], (lane & -2 * o) + o - 1);
+        if (lane >= o) upTo += k;
+        if (lane & o) {
+#pragma unroll
+            for (int e = 0; e < BPT; ++e) sumTo[e] += left;
+        }
+    }
+    if (lane == 63) {
+        reinterpret_cast<double*>(S.waves)[wave] = sumTo[BPT - 1];
+        S.waves2[wave] = upTo;
+    }
+    __syncthreads();
+    {
+        double left = 0.0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+            left += w < wave ? reinterpret_cast<const double*>(S.waves)[w] : 0.0;
+            upTo += w < wave ? (unsigned)S.waves2[w] : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < BPT; ++e) S.sum[BPT * tid + e] = sumTo[e] = left + sumTo[e];
+    }
     if (tid == NT - 1) {
         cnt[BPT - 1] = finite - upTo;
         countTo[BPT - 1] = finite - (upTo - n);
     }
-    sumTo[BPT - 1] = S.sum[BPT * tid + BPT - 1] = sum;
 #pragma unroll
     for (int e = 0; e < BPT; ++e) {
         countTo[e] += upTo - n;
         S.count[BPT * tid + e] = countTo[e];
     }
-    __syncthreads();
-    const double before = tid ? S.sum[BPT * tid - 1] : 0.0;
-#pragma unroll
-    for (int e = 0; e < BPT - 1; ++e) sumTo[e] = S.sum[BPT * tid + e] = before + sumTo[e];
     auto sumBefore = [&](int b) { return b ? S.sum[b - 1] : 0.0; };
     auto countBefore = [&](int b) { return b ? S.count[b - 1] : 0u; };
     // the first bin with a token at which cond(its number among the thread's) holds, kBins if none; to S.bins[slot]
