@@ -707,6 +707,16 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
     auto unitsTo = [&](int b, double target) { return fmax(0.0, fmin((target - sumBefore(b)) / factorOf(S.octaves, b), 0x1p60)); };
 
     double kept = kLo;  // the weight of what is kept
+    // Where what is kept ends: its last bin, and what of that bin is kept. The draw's target is below the kept weight, but for roundings:
+    // it is looked for no further than here.
+    int lastBin = kBins;
+    u64 lastUnits = 0;
+    auto keepTo = [&](int b, u64 units) {
+        if (b < lastBin || (b == lastBin && units < lastUnits)) {
+            lastBin = b;
+            lastUnits = units;
+        }
+    };
     for (int stage = 0; stage < 3; ++stage) {  // the cuts by count and by weight, the draw
         int b = bK;
         u64 want;
@@ -732,10 +742,15 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s += factorOf(S.octaves, bM0 + k) * (double)S.cut[k];
                 kept = fmin(kept, s);
+                int k = 3;
+                while (k >= 0 && !S.cut[k]) --k;
+                if (k >= 0) keepTo(bM0 + k, S.cut[k]);
+                else keepTo(bM0 - 1, ~0ull);
             }
             const double target = u * kept;
-            b = walk(bU0, bU1, [&](int k) { return S.sum[k] > target; });
+            b = walk(bU0, min(bU1, lastBin), [&](int k) { return S.sum[k] > target; });
             want = (u64)unitsTo(b, target) + 1;
+            if (b == lastBin) want = min(want, lastUnits);
         }
         b = same(b);
         search(b, want, stage == 0);
@@ -747,6 +762,7 @@ __global__ __launch_bounds__(kDraw, 4) void sample_draw_kernel(SampleArgs a) {
         } else {
             const double s = sumBefore(b) + factorOf(S.octaves, b) * (double)S.found[0];
             kept = stage == 0 ? s : fmin(kept, s);
+            keepTo(b, S.found[0]);
             __syncthreads();
         }
     }

@@ -74,3 +74,16 @@ def test_no_cut(V, R, far):
     print("sample_rows", V, R, far, flush=True)
     l, t = rows_of(np.random.default_rng([V, far]), R, V, far)
     check(l, t)
+
+
+@pytest.mark.parametrize("V,R", [(7, 1500), (100, 1500), (399, 1500), (3000, 400), (40000, 60)])
+@pytest.mark.parametrize("cut", ["top_k", "top_p", "min_p", "all"])
+def test_cuts(V, R, cut):
+    """The last token that a cut keeps, whose bin holds tokens that it does not keep, and bins without tokens behind it."""
+    print("sample_rows", V, R, cut, flush=True)
+    r = np.random.default_rng([V, len(cut), cut[-1] == "k"])
+    l, t = rows_of(r, R, V, False)
+    k = r.integers(1, V + 1, R).astype(np.int32) if cut in ("top_k", "all") else None
+    p = r.uniform(0.05, 0.999, R).astype(np.float32) if cut in ("top_p", "all") else None
+    m = r.uniform(0.001, 0.4, R).astype(np.float32) if cut in ("min_p", "all") else None
+    check(l, t, k, p, m)
