@@ -482,7 +482,8 @@ typedef struct kcRopeScaling {
 KC_API kcError_t kcRopeFreqs(const kcRopeScaling* scaling, const float* ff, double* freqs, float* scale) KC_NOEXCEPT;
 /* rope_ext: q's and k's first n_rot values of each head turned by 2 pi pos[t] freqs[i] and multiplied by scale, the others as they are:
  * pairs (2 i, 2 i + 1) where interleaved is 1, (i, i + n_rot / 2) where it is 0; angles in 64 bits, so that far positions keep theirs.
- * q (with q_out) or k (with k_cache) may be null, v too. q_out may be q with the same strides (k may not be written to).
+ * q (with q_out) or k (with k_cache) may be null, v too. q_out may be q with the same strides; but for that, outputs share no value with
+ * each other or with an input. They may lie beside each other: q (in place), k and v of a token in one row, K and V in one cache row.
  * k, turned, and v, as it is, are rounded to fp16 and stored in rows slots[t] (int64) of the caches; slots outside [0, cache_rows) are
  * not stored, and of tokens with the same slot the last one is. Strides of q, k, v and q_out are in floats, of the
  * caches in bytes (multiples of 2; rows do not overlap). D even, at most 1024; n_rot even, at most D. */

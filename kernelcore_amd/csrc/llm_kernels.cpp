@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <numeric>
 
 #include "internal.hpp"
 #include "kflash_ext.hpp"
@@ -668,12 +669,36 @@ int kvPagesValidate(const void* p, const kcLaunchContext*) {
 }
 int kvPagesLaunch(const void* p, void* s) { return kcamd::launchKvPages(*static_cast<const kcKvPagesArgs*>(p), hs(s)); }
 
+// n rows of `heads` heads of `bytes` bytes each, strides in bytes (that of a single row or head is 0).
+struct HeadRows {
+    Span span;
+    int64_t row, head, rowBytes, headBytes, bytes;  // bytes from the first to the last of a row's heads, and of a head's rows
+};
+HeadRows headRowsOf(const void* p, int64_t n, int64_t row, int64_t heads, int64_t head, int64_t bytes) {  // (after extent: no overflow)
+    if (n <= 0 || heads <= 0) return {};
+    if (n == 1) row = 0;
+    if (heads == 1) head = 0;
+    const int64_t x = (heads - 1) * head + bytes, y = (n - 1) * row + bytes;
+    return {spanOf(p, p ? size_t(y + x - bytes) : 0), row, head, x, y, bytes};
+}
+// Whether two such arrays may share a value: not if one ends before the other begins, or if their rows, their heads or all of their values
+// repeat at a common distance and lie in different parts of it (q, k and v of a token side by side, K and V in one cache row).
+bool mayShare(const HeadRows& a, const HeadRows& b) {
+    if (!overlap(a.span, b.span)) return false;
+    const auto beside = [&](int64_t step, int64_t x, int64_t y) {
+        if (step == 0) return false;
+        const int64_t d = a.span.at <= b.span.at ? int64_t(b.span.at - a.span.at) % step : (step - int64_t(a.span.at - b.span.at) % step) % step;
+        return d >= x && y <= step - d;
+    };
+    const int64_t rows = std::gcd(a.row, b.row), heads = std::gcd(a.head, b.head);
+    return !beside(rows, a.rowBytes, b.rowBytes) && !beside(heads, a.headBytes, b.headBytes) && !beside(std::gcd(rows, heads), a.bytes, b.bytes);
+}
 // Rows of `heads` heads of D values, strides in units of `unit` bytes.
-int headRows(const void* p, int64_t n, int64_t row, int heads, int64_t head, int D, int unit, const char* what, Span* span) {
+int headRows(const void* p, int64_t n, int64_t row, int heads, int64_t head, int D, int unit, const char* what, HeadRows* rows) {
     int64_t x, y;
     if (row < 0 || head < 0 || !aligned(p, size_t(unit)) || !extent(heads, head, D, &x) || !extent(n, row, x, &y) || y > INT64_MAX / 8)
         return invalid("rope_ext: strides not negative, arrays aligned to their values");
-    *span = spanOf(p, size_t(y) * size_t(unit));
+    *rows = headRowsOf(p, n, row * unit, heads, head * unit, int64_t(D) * unit);
     return checkRange(p, size_t(y) * size_t(unit), what);
 }
 // Whether no two of n x heads rows share a value: heads within a row, or rows within a head. (After headRows or extent: no overflow.)
@@ -693,7 +718,7 @@ int ropeExtValidate(const void* p, const kcLaunchContext*) {
     if (!aligned(a.freqs, 8) || !aligned(a.slots, 8)) return invalid("rope_ext: freqs and slots 8-byte aligned");
     KC_TRY(intsAt(a.pos, a.n_tokens, "pos"));
     KC_TRY(checkRange(a.freqs, size_t(a.n_rot / 2) * 8, "freqs"));
-    Span in[3]{}, out[3]{};
+    HeadRows in[3]{}, out[3]{};
     if (a.q) {
         if (a.H <= 0 || a.H > 65536) return invalid("rope_ext: H from 1 to 65536");
         KC_TRY(headRows(a.q, a.n_tokens, a.q_tok, a.H, a.q_head, a.D, 4, "q", &in[0]));
@@ -714,14 +739,14 @@ int ropeExtValidate(const void* p, const kcLaunchContext*) {
                 return invalid("rope_ext: cache rows, heads and bases at multiples of 2 bytes");
             if (!rowsApart(a.cache_rows, row, a.H_kv, head, bytes)) return invalid("rope_ext: cache rows overlap");
             KC_TRY(checkRange(c, size_t(y), i ? "v_cache" : "k_cache"));
-            out[1 + i] = spanOf(c, size_t(y));
+            out[1 + i] = headRowsOf(c, a.cache_rows, row, a.H_kv, head, bytes);
         }
     }
     const Span small[3] = {spanOf(a.pos, size_t(a.n_tokens) * 4), spanOf(a.freqs, size_t(a.n_rot / 2) * 8), spanOf(a.k ? a.slots : nullptr, size_t(a.n_tokens) * 8)};
     const bool inPlace = a.q && a.q_out == a.q && a.out_tok == a.q_tok && a.out_head == a.q_head;
     for (int i = 0; i < 3; ++i)
         for (int j = 0; j < 3; ++j) {
-            if (overlap(out[i], small[j]) || (i < j && overlap(out[i], out[j])) || (overlap(out[i], in[j]) && !(i == 0 && j == 0 && inPlace)))
+            if (overlap(out[i].span, small[j]) || (i < j && mayShare(out[i], out[j])) || (mayShare(out[i], in[j]) && !(i == 0 && j == 0 && inPlace)))
                 return invalid("rope_ext: an output overlaps another array");
         }
     return 0;

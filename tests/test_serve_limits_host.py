@@ -1,0 +1,65 @@
+"""Which memory layouts and sizes the operators of a step over a paged cache accept, on the CPU (the library over tests/hip_stub, as in
+test_serve_host.py)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from tests.test_serve_host import CHILD, HERE
+
+PRELUDE = CHILD[:CHILD.index("# ---- kv_pages")]
+
+
+@pytest.fixture(scope="module")
+def stub(tmp_path_factory):
+    path = str(tmp_path_factory.mktemp("stub") / "hip_stub.so")
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", os.path.join(HERE, "hip_stub", "hip_stub.cpp"), "-o", path],
+                   check=True)
+    return path
+
+
+def run(stub, code):
+    r = subprocess.run([sys.executable, "-c", PRELUDE + code + '\nprint("done")\n', stub], capture_output=True, text=True, cwd=os.path.dirname(HERE), timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["done"], r.stdout + r.stderr
+
+
+def test_rope_layouts(stub):
+    """Arrays that lie beside each other are accepted wherever they share no value, and refused where they share one."""
+    run(stub, r"""
+import numpy as np
+r = np.random.default_rng(0)
+N, H, K, D, ROWS = 5, 4, 2, 64, 7
+T = (H + 2 * K) * D
+qkv, small, cache = buf(4 * N * T), dict(pos=buf(4 * N), freqs=buf(8 * 16), slots=buf(8 * N)), buf(2 * ROWS * 2 * K * D)
+make = lambda **k: kc.RopeExtArgs(**k)  # noqa: E731
+good = dict(small, q=qkv, k=qkv + 4 * H * D, v=qkv + 4 * (H + K) * D, q_out=qkv, k_cache=cache, v_cache=cache + 2 * K * D, n_tokens=N, H=H, H_kv=K, D=D, n_rot=32,
+            q_tok=T, q_head=D, k_tok=T, k_head=D, v_tok=T, v_head=D, out_tok=T, out_head=D, cache_rows=ROWS, kc_row=4 * K * D, kc_head=2 * D, vc_row=4 * K * D,
+            vc_head=2 * D, scale=1.0)
+checks("rope_ext", make, good,
+       [(dict(kc_head=4 * D, vc_head=4 * D, v_cache=cache + 2 * D), OK),  # K and V of a head side by side
+        (dict(kc_row=2 * D, vc_row=2 * D, kc_head=4 * D * ROWS, vc_head=4 * D * ROWS, v_cache=cache + 2 * D * ROWS), OK),  # heads outermost, K's rows then V's
+        (dict(kc_row=4 * D, vc_row=4 * D, kc_head=4 * D * ROWS, vc_head=4 * D * ROWS, v_cache=cache + 2 * D), OK),  # and side by side in each row
+        (dict(q_out=qkv + 4 * D * H, k=qkv, k_head=D), IV), (dict(k=qkv + 4 * (H * D - 1)), IV), (dict(v=qkv), IV), (dict(v_cache=cache + 2 * K * D - 2), IV),
+        (dict(v_cache=cache + 2 * D), IV), (dict(kc_head=4 * D, vc_head=4 * D, v_cache=cache + 2 * D - 2), IV), (dict(out_tok=T - D, n_tokens=4), IV)])
+# Layouts of two arrays at random: refused if they share a value, accepted if they do not and lie beside each other at a common distance.
+n, h, d, base = 3, 2, 2, buf(4096)
+seen = {OK: 0, IV: 0}
+for _ in range(8000):
+    step = lambda: int(r.choice([4, 6, 8, 12, 16, 24, 32, 48]))  # noqa: E731
+    k = (2 * int(r.integers(0, 60)), step(), step())  # offset, bytes between rows, between heads
+    v = (2 * int(r.integers(0, 60)), *(k[1:] if r.random() < 0.6 else (step(), step())))
+    if not all((head >= 2 * d and row >= head + 2 * d) or (row >= 2 * d and head >= 2 * row + 2 * d) for _, row, head in (k, v)):
+        continue  # rows and heads through each other are refused anyway
+    values = [{at + i * row + j * head + 2 * e for i in range(n) for j in range(h) for e in range(d)} for at, row, head in (k, v)]
+    got = status("rope_ext", make(**dict(small, k=qkv, v=qkv, k_cache=base + k[0], v_cache=base + v[0], n_tokens=2, H_kv=h, D=d, n_rot=2, k_tok=4, k_head=2, v_tok=4,
+                                         v_head=2, cache_rows=n, kc_row=k[1], kc_head=k[2], vc_row=v[1], vc_head=v[2], scale=1.0)))
+    seen[got] += 1
+    if values[0] & values[1]:
+        assert got == IV, (k, v)
+    elif k[1:] == v[1:]:
+        size = {k[1]: (h - 1) * k[2] + 2 * d, k[2]: (n - 1) * k[1] + 2 * d}
+        if any(size[x] <= (v[0] - k[0]) % x <= x - size[x] for x in size):
+            assert got == OK, (k, v)
+assert min(seen.values()) > 300, seen
+""")
