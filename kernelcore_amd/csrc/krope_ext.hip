@@ -20,6 +20,10 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef h4 h4a2 __attribute__((aligned(2)));
 
 constexpr int kThreads = 256, kAhead = 2, kPairs = 1024;  // pairs of a workgroup's tokens
+// Tokens of a launch: the search for repeated slots grows with their square. What a launch stores lies over what the one before it did, so
+// that no launch looks for later ones' slots. (24 + 2 x 8 heads of 128, 65536 tokens: 500 us, in launches of 16384 570, in one 770; 262144
+// tokens 2.0 ms and 7.9.)
+constexpr int kLaunch = 8192;
 
 struct RopeArgs {
     const float *q, *k, *v;
@@ -203,26 +207,31 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
 }  // namespace
 
 int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
-    if (a.n_tokens == 0) return 0;
-    RopeArgs p{a.q, a.k, a.v, a.pos, a.freqs, reinterpret_cast<const long long*>(a.slots), a.q_out, static_cast<char*>(a.k_cache),
-               static_cast<char*>(a.v_cache), a.n_tokens, a.H, a.H_kv, a.D, a.n_rot, a.q_tok, a.q_head, a.k_tok, a.k_head, a.v_tok, a.v_head,
-               a.out_tok, a.out_head, a.cache_rows, a.kc_row, a.kc_head, a.vc_row, a.vc_head, a.scale, 1, 1, 0};
-    // k and v: up to 16 tokens share the search for repeated slots, which reads all later tokens' slots, once there are four workgroups
-    // for each CU (3333 tokens with three to a workgroup 28 us, with six 31, with one 33)
-    const int most = std::max(1, std::min(16, kPairs / std::max(1, a.n_rot / 2)));
-    p.kv_tokens = std::max(1, std::min(most, a.n_tokens / 1024));
-    // q: what a workgroup loads ahead, likewise
-    const int units = a.n_rot / 8 + (a.D - a.n_rot + 7) / 8;
-    p.q_tokens = std::max(1, std::min({most, a.n_tokens / 512, kAhead * kThreads / std::max(1, a.H * units)}));
-    const int qBlocks = a.q ? (a.n_tokens + p.q_tokens - 1) / p.q_tokens : 0;
-    p.kv_blocks = a.k ? (a.n_tokens + p.kv_tokens - 1) / p.kv_tokens : 0;
-    const dim3 grid(p.kv_blocks + qBlocks);
-    const bool full = a.n_rot % 8 == 0 && a.D % 8 == 0;
-    if (a.interleaved && full) hipLaunchKernelGGL((rope_ext_kernel<true, true>), grid, dim3(kThreads), 0, s, p);
-    else if (a.interleaved) hipLaunchKernelGGL((rope_ext_kernel<true, false>), grid, dim3(kThreads), 0, s, p);
-    else if (full) hipLaunchKernelGGL((rope_ext_kernel<false, true>), grid, dim3(kThreads), 0, s, p);
-    else hipLaunchKernelGGL((rope_ext_kernel<false, false>), grid, dim3(kThreads), 0, s, p);
-    return fromHip(hipGetLastError(), "rope_ext");
+    for (int at = 0; at < a.n_tokens; at += kLaunch) {
+        const int n = std::min(kLaunch, a.n_tokens - at);
+        RopeArgs p{a.q ? a.q + (long long)at * a.q_tok : nullptr, a.k ? a.k + (long long)at * a.k_tok : nullptr, a.v ? a.v + (long long)at * a.v_tok : nullptr,
+                   a.pos + at, a.freqs, reinterpret_cast<const long long*>(a.slots) + (a.k ? at : 0), a.q ? a.q_out + (long long)at * a.out_tok : nullptr,
+                   static_cast<char*>(a.k_cache), static_cast<char*>(a.v_cache), n, a.H, a.H_kv, a.D, a.n_rot, a.q_tok, a.q_head, a.k_tok, a.k_head,
+                   a.v_tok, a.v_head, a.out_tok, a.out_head, a.cache_rows, a.kc_row, a.kc_head, a.vc_row, a.vc_head, a.scale, 1, 1, 0};
+        // k and v: up to 16 tokens share the search for repeated slots, which reads all later tokens' slots, once there are four workgroups
+        // for each CU (3333 tokens with three to a workgroup 28 us, with six 31, with one 33)
+        const int most = std::max(1, std::min(16, kPairs / std::max(1, a.n_rot / 2)));
+        p.kv_tokens = std::max(1, std::min(most, n / 1024));
+        // q: what a workgroup loads ahead, likewise
+        const int units = a.n_rot / 8 + (a.D - a.n_rot + 7) / 8;
+        p.q_tokens = std::max(1, std::min({most, n / 512, kAhead * kThreads / std::max(1, a.H * units)}));
+        const int qBlocks = a.q ? (n + p.q_tokens - 1) / p.q_tokens : 0;
+        p.kv_blocks = a.k ? (n + p.kv_tokens - 1) / p.kv_tokens : 0;
+        const dim3 grid(p.kv_blocks + qBlocks);
+        if (grid.x == 0) return 0;
+        const bool full = a.n_rot % 8 == 0 && a.D % 8 == 0;
+        if (a.interleaved && full) hipLaunchKernelGGL((rope_ext_kernel<true, true>), grid, dim3(kThreads), 0, s, p);
+        else if (a.interleaved) hipLaunchKernelGGL((rope_ext_kernel<true, false>), grid, dim3(kThreads), 0, s, p);
+        else if (full) hipLaunchKernelGGL((rope_ext_kernel<false, true>), grid, dim3(kThreads), 0, s, p);
+        else hipLaunchKernelGGL((rope_ext_kernel<false, false>), grid, dim3(kThreads), 0, s, p);
+        if (int e = fromHip(hipGetLastError(), "rope_ext")) return e;
+    }
+    return 0;
 }
 
 }  // namespace kcamd

@@ -5,6 +5,7 @@ import pytest
 
 import kernelcore_amd as kc
 from tests.serve import Out, Pages, up
+from tests.test_gpu_rope_ext import run
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +83,12 @@ def test_attention_of_a_shared_cache(D, by):
     assert np.array_equal(out.get().reshape(c.q.shape), want)
     for x in [kv, *b.values()]:
         x.free()
+
+
+@pytest.mark.parametrize("N", [8191, 8192, 8193, 16385, 30000])
+@pytest.mark.parametrize("rows", [50, 20000])
+def test_repeated_slots_of_many_tokens(N, rows):
+    """The last token with a slot is stored, wherever the others with it are."""
+    slots = np.random.default_rng(N).integers(-3, rows + 3, N)
+    run(N, 1, 2, 8, 8, False, rows=rows, slots=slots)
+    run(N, 2, 1, 6, 4, True, rows=rows, slots=slots, in_place=True, v=False)

@@ -63,3 +63,21 @@ for _ in range(8000):
             assert got == OK, (k, v)
 assert min(seen.values()) > 300, seen
 """)
+
+
+@pytest.mark.parametrize("N", [8192, 8193, 40000])
+def test_rope_launches(stub, N):
+    """A launch's search for repeated slots is bounded: many tokens take several launches, each with a part of them."""
+    run(stub, f"N = {N}" + r"""
+b = {n: buf(8 * N) for n in ("q", "k", "v", "pos", "freqs", "slots", "q_out", "k_cache", "v_cache")}
+args = dict(b, n_tokens=N, H=1, H_kv=1, D=2, n_rot=2, q_tok=2, q_head=2, k_tok=2, k_head=2, v_tok=2, v_head=2, out_tok=2, out_head=2, cache_rows=N, kc_row=4, kc_head=4,
+            vc_row=4, vc_head=4, scale=1.0)
+for change in ({}, dict(q=None, q_out=None), dict(k=None, k_cache=None, v=None, v_cache=None, slots=None)):
+    assert status("rope_ext", kc.RopeExtArgs(**dict(args, **change))) == OK
+    grids = [int(x.split()[-4]) for x in stub.stub_record().decode().splitlines()]
+    # (a workgroup has at most 16 tokens)
+    assert len(grids) == -(-N // 8192) and max(grids) <= 2 * 8192 and sum(grids) >= N // 16, grids
+stub.stub_clear()
+assert kc.launch_status("rope_ext", kc.RopeExtArgs(**dict(args, q=None, q_out=None, k=None, k_cache=None, v=None, v_cache=None, slots=None))) == OK
+assert stub.stub_record() == b""  # neither q nor k: nothing to do
+""")
