@@ -5,6 +5,7 @@
 // foot: every new page begins at a token of the step). So no token waits for what another workgroup writes.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 
@@ -15,6 +16,9 @@ namespace kcamd {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64, kPer = 4;  // sequences of a thread in a round
+// Tokens of a launch where there are trees: a token's walk up its tree ends with the launch's first one, and goes on from what the launch
+// before wrote. (A chain of 32768 nodes 4.3 ms, 130 ns a node; without this end the time of longer ones grew without bound.)
+constexpr int kLaunch = 32768;
 
 struct PagesArgs {
     const int *have, *add, *free, *parent;
@@ -23,6 +27,7 @@ struct PagesArgs {
     long long* slots;
     int *pos, *used, *tree;
     int seqs, n_tokens, n_free, shift, max_pages, table_row, tree_words;
+    int t0, end;  // the launch's tokens
 };
 
 // The sums of x over the threads before this one (all: over all of them).
@@ -49,14 +54,15 @@ __device__ __forceinline__ int sumBefore(int x, int* waves, int tid, int& all) {
 
 // A workgroup: 256 tokens. It sums over the sequences by itself (1024 in a round, until its tokens are covered): what other workgroups
 // found would take a launch of its own. Latency bounds it: 8 requests of a token 4 us, 256 of 97 tokens 4.2, 500 trees of 24 nodes
-// 5.0 (their longest chain of parents, from LDS).
+// 5.0 (their longest chain of parents, from LDS). Each token walks up its tree by itself, a load for each ancestor: a prompt of 2048 tokens that is
+// given as a chain among trees takes 360 us.
 __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     __shared__ int waves[2][kWaves];
     __shared__ int first[kThreads];                             // a token that is its sequence's first here: its number, else 0
     __shared__ int4 rec[kThreads];                              // its sequence: number, start, have, pages taken before it
     __shared__ int parents[2 * kThreads];
     __shared__ int last[kWaves];
-    const int tid = threadIdx.x, t0 = blockIdx.x * kThreads, t = t0 + tid;
+    const int tid = threadIdx.x, t0 = a.t0 + blockIdx.x * kThreads, t = t0 + tid;
     const int per = 1 << a.shift;
     int above[2] = {-1, -1};  // the parents of this token and of the one 256 before it, for LDS once the sums are done
     if (a.parent && a.n_tokens > 0) {
@@ -69,7 +75,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     first[tid] = 0;
     int tokens = 0, pages = 0;  // before the round's sequences
     for (int s0 = 0; s0 < a.seqs; s0 += kPer * kThreads) {
-        if (blockIdx.x && tokens >= t0 + kThreads) break;  // (workgroup 0 writes the sequences' numbers)
+        if (t0 && tokens >= t0 + kThreads) break;  // (the first workgroup writes the sequences' numbers)
         int have[kPer], add[kPer], need[kPer], sum = 0;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
@@ -126,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
                     first[x] = x + 1;
                     rec[x] = int4{s, at[e], have[e], pb};
                 }
-                if (blockIdx.x == 0) {
+                if (t0 == 0) {
                     a.start[s] = at[e];
                     a.len[s] = (int)min((long long)have[e] + add[e], (long long)INT_MAX);
                 }
@@ -136,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
     }
     parents[tid] = above[0];
     parents[tid + kThreads] = above[1];
-    if (blockIdx.x == 0 && tid == 0) {
+    if (t0 == 0 && tid == 0) {
         a.start[a.seqs] = tokens;
         a.used[0] = pages;
     }
@@ -154,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
         __syncthreads();
         for (int w = 0; w < wave; ++w) x = max(x, last[w]);
     }
-    if (t >= a.n_tokens) return;
+    if (t >= a.end) return;
     int* words = a.tree ? a.tree + (size_t)t * a.tree_words : nullptr;
     if (t >= tokens || x == 0) {  // (behind the last sequence; tokens is short only in workgroups that others' tokens end)
         a.slots[t] = -1;
@@ -198,6 +204,7 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
         int w = a.tree_words - 1;
         uint32_t bits = 0;
         int cur = node;
+        const unsigned least = max(a.t0 - r.y, 0);  // the sequence's first node of this launch
         while (true) {
             if (cur < 32 * a.tree_words) {
                 for (; w > cur >> 5; --w, bits = 0) words[w] = (int)bits;
@@ -205,9 +212,17 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
             }
             const int k = r.y + cur - (t0 - kThreads);
             const int up = k >= 0 ? parents[k] : a.parent[r.y + cur];
-            if (up < 0 || up >= cur) break;
+            if (up - least >= cur - least) break;
             cur = up;
             ++depth;
+        }
+        const int up = least ? a.parent[r.y + cur] : -1;
+        if (up >= 0 && up < cur) {
+            // (an ancestor of the launch before: its words and its position)
+            const int* others = a.tree + (size_t)(r.y + up) * a.tree_words;
+            for (; w >= 0; --w, bits = 0) words[w] = (int)bits | others[w];
+            if (a.pos) a.pos[t] = (int)min((long long)a.pos[r.y + up] + depth + 1, (long long)INT_MAX);
+            return;
         }
         for (; w >= 0; --w, bits = 0) words[w] = (int)bits;
     }
@@ -218,10 +233,15 @@ __global__ __launch_bounds__(kThreads) void kv_pages_kernel(PagesArgs a) {
 
 int launchKvPages(const kcKvPagesArgs& a, hipStream_t s) {
     PagesArgs p{a.have, a.add, a.free, a.parent, a.table, a.start, a.len, reinterpret_cast<long long*>(a.slots), a.pos, a.used,
-                a.tree, a.seqs, a.n_tokens, a.n_free, __builtin_ctz((unsigned)a.page), a.max_pages, a.table_row, a.tree ? a.tree_words : 0};
-    const int blocks = a.n_tokens > 0 ? (a.n_tokens - 1) / kThreads + 1 : 1;
-    hipLaunchKernelGGL(kv_pages_kernel, dim3(blocks), dim3(kThreads), 0, s, p);
-    return fromHip(hipGetLastError(), "kv_pages");
+                a.tree, a.seqs, a.n_tokens, a.n_free, __builtin_ctz((unsigned)a.page), a.max_pages, a.table_row, a.tree ? a.tree_words : 0, 0, 0};
+    do {
+        const int n = a.parent ? std::min(kLaunch, a.n_tokens - p.t0) : a.n_tokens;
+        p.end = p.t0 + n;
+        hipLaunchKernelGGL(kv_pages_kernel, dim3(n > 0 ? (n - 1) / kThreads + 1 : 1), dim3(kThreads), 0, s, p);
+        if (int e = fromHip(hipGetLastError(), "kv_pages")) return e;
+        p.t0 = p.end;
+    } while (p.t0 < a.n_tokens);
+    return 0;
 }
 
 }  // namespace kcamd

@@ -81,3 +81,16 @@ stub.stub_clear()
 assert kc.launch_status("rope_ext", kc.RopeExtArgs(**dict(args, q=None, q_out=None, k=None, k_cache=None, v=None, v_cache=None, slots=None))) == OK
 assert stub.stub_record() == b""  # neither q nor k: nothing to do
 """)
+
+
+@pytest.mark.parametrize("N", [0, 1, 32768, 32769, 100000])
+def test_tree_launches(stub, N):
+    """A launch's walks up the trees are bounded by its tokens; without trees there is one launch."""
+    run(stub, f"N = {N}" + r"""
+b = {n: buf(max(16, 8 * N)) for n in ("have", "add", "free", "table", "start", "len", "slots", "pos", "used", "parent", "tree")}
+for tree in (True, False):
+    a = dict(b) if tree else dict(b, parent=None, tree=None)
+    assert status("kv_pages", kc.KvPagesArgs(**a, seqs=2, n_tokens=N, n_free=1, page=16, max_pages=1, table_row=1, tree_words=2 if tree else 0)) == OK
+    grids = [int(x.split()[-4]) for x in stub.stub_record().decode().splitlines()]
+    assert sum(grids) == max(1, -(-N // 256)) and len(grids) == (max(1, -(-N // 32768)) if tree else 1), grids
+""")
