@@ -444,7 +444,8 @@ typedef struct kcKvGatherArgs {
  * parent[t] (may be null): a node's parent by its number in its sequence, -1 (or any other number that is not a smaller node's) for
  * a root; depth 0. tree[t] (given with it; tree_words 1 to 64 32-bit words): bit j of the words is set where node j of the
  * sequence, j < 32 tree_words, is node i itself or one of its ancestors.
- * Tokens from start[seqs] on get slot -1, pos 0 and no tree bit. Outputs overlap neither each other nor the inputs. */
+ * Tokens from start[seqs] on get slot -1, pos 0 and no tree bit. seqs and n_tokens at most 2^24. Outputs overlap neither each other nor
+ * the inputs. */
 typedef struct kcKvPagesArgs {
     const int* have;
     const int* add;

@@ -640,9 +640,10 @@ int apart(const Span* all, int outs, int n, const char* what) {
 
 int kvPagesValidate(const void* p, const kcLaunchContext*) {
     const auto& a = *static_cast<const kcKvPagesArgs*>(p);
-    if (a.seqs < 0 || a.seqs > INT32_MAX - 65536 || a.n_tokens < 0 || a.n_tokens > INT32_MAX - 65536 || a.n_free < 0 || !pageSize(a.page) || a.max_pages < 0 ||
+    // (each 256 tokens sum over the sequences before them: the limits bound a launch's time)
+    if (a.seqs < 0 || a.seqs > (1 << 24) || a.n_tokens < 0 || a.n_tokens > (1 << 24) || a.n_free < 0 || !pageSize(a.page) || a.max_pages < 0 ||
         a.table_row < a.max_pages)
-        return invalid("kv_pages: counts not negative, page a power of two from 16 to 65536, table_row at least max_pages");
+        return invalid("kv_pages: seqs and n_tokens from 0 to 2^24, n_free not negative, page a power of two from 16 to 65536, table_row at least max_pages");
     if ((a.parent != nullptr) != (a.tree != nullptr) || (a.tree ? a.tree_words < 1 || a.tree_words > 64 : a.tree_words != 0))
         return invalid("kv_pages: parent and tree are both given, with 1 to 64 tree_words, or both null, with none");
     if (!aligned(a.slots, 8)) return invalid("kv_pages: slots 8-byte aligned");

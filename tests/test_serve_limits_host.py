@@ -94,3 +94,13 @@ for tree in (True, False):
     grids = [int(x.split()[-4]) for x in stub.stub_record().decode().splitlines()]
     assert sum(grids) == max(1, -(-N // 256)) and len(grids) == (max(1, -(-N // 32768)) if tree else 1), grids
 """)
+
+
+def test_pages_sizes(stub):
+    """Each workgroup of tokens sums over the sequences before them: both are bounded."""
+    run(stub, r"""
+M = 1 << 24
+b = {n: buf(8 * M + 16) for n in ("have", "add", "free", "table", "start", "len", "slots", "pos", "used")}
+checks("kv_pages", lambda **k: kc.KvPagesArgs(**k), dict(b, seqs=M, n_tokens=M, n_free=1, page=16, max_pages=1, table_row=1),
+       [(dict(seqs=M + 1), IV), (dict(n_tokens=M + 1), IV), (dict(seqs=M + 1, n_tokens=0), IV), (dict(seqs=0, n_tokens=M + 1), IV), (dict(seqs=1), OK), (dict(n_tokens=1), OK)])
+""")
