@@ -520,7 +520,7 @@ typedef struct kcRopeExtArgs {
  * flash_ext_f16. The same call gives the same bits; N, seqs and the table's size take part in how the work is split, so the same tokens
  * among others, or with a longer table, may differ by roundings.
  * Rows, heads and base of K and V at multiples of 16 bytes; offsets are 64-bit, a page spans less than 2^31 bytes, the cache holds less
- * than 2^31 positions. part: kcFlashPagesPartBytes bytes of workspace, 16-byte aligned, which calls that may overlap must not share.
+ * than 2^31 positions. N H D is below 2^31, (N H / H_kv / 16 + seqs) H_kv below 2^24. part: kcFlashPagesPartBytes bytes of workspace, 16-byte aligned, which calls that may overlap must not share.
  * out, lse and part overlap neither each other nor the inputs. */
 typedef struct kcFlashPagesDims {
     int H;

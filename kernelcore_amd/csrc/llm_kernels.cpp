@@ -765,8 +765,8 @@ int fpShape(const kcFlashPagesDims& d) {
     if (d.tree_words < 0 || d.tree_words > 64) return invalid("flash_pages: tree_words from 0 to 64");
     if (d.q_tok < 0 || d.q_head < 0 || d.k_row < 0 || d.k_head < 0 || d.v_row < 0 || d.v_head < 0) return invalid("flash_pages: negative strides");
     const int64_t G = d.H / d.H_kv;
-    if (int64_t(d.N) * d.H * d.D > INT32_MAX || (int64_t(d.N) * G / 16 + d.seqs) * d.H_kv > (1 << 24))
-        return invalid("flash_pages: N H D below 2^31, (N H / H_kv / 16 + seqs) H_kv at most 2^24");
+    if (int64_t(d.N) * d.H * d.D > INT32_MAX || (int64_t(d.N) * G / 16 + d.seqs) * d.H_kv >= (1 << 24))  // (256 threads for each, below 2^32)
+        return invalid("flash_pages: N H D below 2^31, (N H / H_kv / 16 + seqs) H_kv below 2^24");
     return 0;
 }
 int fpCache(const kcFlashPagesDims& d, const void* p, int64_t row, int64_t head, const char* what, Span* span) {

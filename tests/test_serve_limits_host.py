@@ -104,3 +104,22 @@ b = {n: buf(8 * M + 16) for n in ("have", "add", "free", "table", "start", "len"
 checks("kv_pages", lambda **k: kc.KvPagesArgs(**k), dict(b, seqs=M, n_tokens=M, n_free=1, page=16, max_pages=1, table_row=1),
        [(dict(seqs=M + 1), IV), (dict(n_tokens=M + 1), IV), (dict(seqs=M + 1, n_tokens=0), IV), (dict(seqs=0, n_tokens=M + 1), IV), (dict(seqs=1), OK), (dict(n_tokens=1), OK)])
 """)
+
+
+def test_attention_sizes(stub):
+    """A launch has fewer than 2^32 threads."""
+    run(stub, r"""
+d = dict(H=2, H_kv=1, D=64, N=8, seqs=(1 << 24) - 2, page=16, max_pages=1, n_pages=1, tree_words=0, q_tok=128, q_head=64, table_row=1, k_row=128, k_head=128, v_row=128, v_head=128)
+b = C.c_size_t()
+size = lambda **k: kc.lib().kcFlashPagesPartBytes(C.byref(kc.FlashPagesDims(**dict(d, **k))), C.byref(b))  # noqa: E731
+assert size() == kc.ERR[OK] and size(N=7, seqs=d["seqs"] + 1) == kc.ERR[OK]
+assert size(N=16) == size(N=7, seqs=d["seqs"] + 2) == size(seqs=d["seqs"] + 1) == size(N=0, seqs=1 << 24) == kc.ERR[IV]
+size()
+n = 4 * d["seqs"] + 4
+a = {x: buf(n) for x in ("table", "start", "len")}
+args = dict(a, q=buf(4096 * 2), k=buf(4096), v=buf(4096), out=buf(4096 * 2), part=buf(b.value), scale=0.1)
+stub.stub_clear()
+assert kc.launch_status("flash_pages_f16", kc.FlashPagesArgs(d=kc.FlashPagesDims(**d), **args)) == OK, kc.lib().kcGetLastErrorDetail()
+for x in stub.stub_record().decode().splitlines():
+    assert int(x.split()[-4]) * int(x.split()[-1]) < 1 << 32, x
+""")
