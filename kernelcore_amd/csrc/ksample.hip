@@ -780,8 +780,10 @@ int piecesOf(int rows, int n, int* piece) {
 }  // namespace
 
 size_t sampleRowsPartBytes(int rows, int n_vocab) {
+    // (fewer rows may have more pieces: what is enough for some is enough for fewer)
     int piece;
-    return size_t(rows) * piecesOf(rows, n_vocab, &piece) * sizeof(Piece);
+    const int small = (n_vocab + 16383) / 16384, few = std::min(rows, 64 / small);
+    return std::max(size_t(rows) * piecesOf(rows, n_vocab, &piece), size_t(few) * piecesOf(few, n_vocab, &piece)) * sizeof(Piece);
 }
 
 int launchSampleRows(const kcSampleRowsArgs& a, hipStream_t s) {

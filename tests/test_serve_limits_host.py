@@ -123,3 +123,18 @@ assert kc.launch_status("flash_pages_f16", kc.FlashPagesArgs(d=kc.FlashPagesDims
 for x in stub.stub_record().decode().splitlines():
     assert int(x.split()[-4]) * int(x.split()[-1]) < 1 << 32, x
 """)
+
+
+def test_sample_workspace(stub):
+    """A workspace made for some rows is enough for fewer of them."""
+    run(stub, r"""
+for V in (1, 1000, 65536, 65537, 128256, 151936, 1 << 20):
+    need = [kc.sample_rows_part_bytes(R, V) for R in range(200)]
+    assert need == sorted(need) and need[0] == 0, V
+R, V = 40, 151936
+a = dict(logits=buf(4 * R * V), u=buf(4 * R), tokens=buf(4 * R), part=buf(kc.sample_rows_part_bytes(R, V)), row=V, n_vocab=V)
+for rows in range(R + 1):
+    assert status("sample_rows", kc.SampleRowsArgs(**a, rows=rows)) == OK, rows
+    for x in stub.stub_record().decode().splitlines()[:1]:
+        assert int(x.split()[-4]) * int(x.split()[-3]) * 20496 <= kc.sample_rows_part_bytes(rows, V)  # 2048 sums, 1024 maxima and three numbers a piece
+""")
