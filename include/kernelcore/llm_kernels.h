@@ -468,7 +468,7 @@ typedef struct kcKvPagesArgs {
 } kcKvPagesArgs;
 
 /* kcRopeFreqs (host): the revolutions per position of the n_rot / 2 pairs of a rotated part of n_rot values, and the factor of
- * cosine and sine: theta_i = base^(-2 i / n_rot), / ff[i] where ff (may be null) is given, / factor (a context stretched by it).
+ * cosine and sine: theta_i = base^(-2 i / n_rot), / ff[i] (positive) where ff (may be null) is given, / factor (a context stretched by it).
  * yarn_ctx > 0: YaRN (Peng et al., 2023) over the original context yarn_ctx: pairs that turn more than beta_fast times
  * within it keep their speed, those below beta_slow are slowed down by factor, those between are blended by their number; the
  * scale is then 1 + 0.1 ln(factor), else 1. (beta_fast and beta_slow: 32 and 1 where 0.) */
@@ -520,7 +520,8 @@ typedef struct kcRopeExtArgs {
  * flash_ext_f16. The same call gives the same bits; N, seqs and the table's size take part in how the work is split, so the same tokens
  * among others, or with a longer table, may differ by roundings.
  * Rows, heads and base of K and V at multiples of 16 bytes; offsets are 64-bit, a page spans less than 2^31 bytes, the cache holds less
- * than 2^31 positions. N H D is below 2^31, (N H / H_kv / 16 + seqs) H_kv below 2^24. part: kcFlashPagesPartBytes bytes of workspace, 16-byte aligned, which calls that may overlap must not share.
+ * than 2^31 positions. N H D is below 2^31, (N H / H_kv / 16 + seqs) H_kv below 2^24. part: kcFlashPagesPartBytes bytes of workspace,
+ * 16-byte aligned, which calls that may overlap must not share.
  * out, lse and part overlap neither each other nor the inputs. */
 typedef struct kcFlashPagesDims {
     int H;

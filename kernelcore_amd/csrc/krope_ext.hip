@@ -244,6 +244,11 @@ kcError_t kcRopeFreqs(const kcRopeScaling* r, const float* ff, double* freqs, fl
         return kc::Error::InvalidValue;
     }
     const int n = r->n_rot;
+    for (int i = 0; ff && i < n / 2; ++i)
+        if (!(ff[i] > 0.0f) || !std::isfinite(ff[i])) {
+            kcamd::setDetail("rope: frequency factors are positive and finite");
+            return kc::Error::InvalidValue;
+        }
     constexpr double kTwoPi = 6.283185307179586;
     // the pair that turns beta times within the original context
     const auto pairOf = [&](double beta) { return n * std::log(r->yarn_ctx / (beta * kTwoPi)) / (2 * std::log((double)r->base)); };

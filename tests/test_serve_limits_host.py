@@ -4,8 +4,10 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 
+import kernelcore_amd as kc
 from tests.test_serve_host import CHILD, HERE
 
 PRELUDE = CHILD[:CHILD.index("# ---- kv_pages")]
@@ -138,3 +140,14 @@ for rows in range(R + 1):
     for x in stub.stub_record().decode().splitlines()[:1]:
         assert int(x.split()[-4]) * int(x.split()[-3]) * 20496 <= kc.sample_rows_part_bytes(rows, V)  # 2048 sums, 1024 maxima and three numbers a piece
 """)
+
+
+@pytest.mark.parametrize("bad", [0.0, -0.0, -1.0, float("nan"), float("inf"), float("-inf")])
+def test_frequency_factors(bad):
+    """A factor that would make a frequency infinite, NaN, 0 or turn it round is refused."""
+    for at in (0, 5, 31):
+        ff = np.ones(32, np.float32)
+        assert np.isfinite(kc.rope_freqs(64, 1e4, ff=ff)[0]).all()
+        ff[at] = bad
+        with pytest.raises(kc.KcError, match="InvalidValue"):
+            kc.rope_freqs(64, 1e4, ff=ff)
