@@ -563,7 +563,7 @@ KC_API kcError_t kcFlashPagesPartBytes(const kcFlashPagesDims* dims, size_t* byt
  * A temperature of 0 or less, or NaN: the first token (u and the cuts do not matter). temperature, top_k, top_p and min_p hold a value
  * for each row; null: 1, 0, 1 and 0. A logit of -infinity has weight 0. A row that holds NaN or +infinity, or -infinity alone, gives
  * token -1 and probability 0. Weights and sums are held in 64 bits, and results do not depend on the order of additions; a weight below
- * 2^-63 of the largest counts as 0. n_vocab at most 2^20; part: kcSampleRowsPartBytes bytes of workspace (enough for fewer rows too),
+ * 2^-62 of the largest may count as 0. n_vocab at most 2^20; part: kcSampleRowsPartBytes bytes of workspace (enough for fewer rows too),
  * 16-byte aligned, which calls that may overlap must not share. tokens, probs and part overlap neither each other nor the inputs. */
 typedef struct kcSampleRowsArgs {
     const float* logits;

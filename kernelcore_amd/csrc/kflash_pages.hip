@@ -10,9 +10,9 @@
 // which workgroup was first).
 //
 // What bounds it: single tokens the cache's bytes (128 sequences of 4000 positions, 32 heads on 8 of 128: 363 us with the join, 5.7 TB/s); wide trees products
-// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 218 us, 0.48 PFLOP/s
-// counted once, matrix units busy in 47% of the cycles, vector instructions in 43%); a small call the chain of shares, first loads, steps and join (one
-// token over 8191 positions: 10 + 4 us).
+// of split operands and softmax, which a SIMD's two wavefronts hardly overlap (64 nodes over 100000 positions: 220 us, 0.48 PFLOP/s
+// counted once; in calls back to back 237; matrix units busy in 47% of the cycles, vector instructions in 43%); a small call the chain of
+// shares, first loads, steps and join (one token over 8191 positions: 12 + 4 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -185,6 +185,8 @@ __global__ __launch_bounds__(64 * W, W > KM ? 2 : 1) void flash_pages_kernel(FpP
     constexpr int Setup = 24;
     auto tileUnits = [](int lg) { return W == 8 ? (lg < lgW ? 4 : D == 256 ? 6 : 7) : 4 + 2 * (lg - lgMin); };
     static_assert(1 << lgW == W && KM << lgMin == W && 1 << lgRows == 16 * NR);
+    // A block of rows counts with all of its sequence's steps, also where its last row sees fewer (a prompt's chunk: 2048 tokens on none 158 us, 220
+    // TFLOP/s of the seen pairs, on 2048 278 and 370; 512 on none 31).
     struct Seq {
         int nodes, len, lg, blocks, steps, weight;  // tokens, positions, log2 RG, blocks of rows, steps, a step's units
         long long units;                            // of all its items' steps
@@ -687,11 +689,14 @@ struct FpPlan {
     size_t bytes;
 };
 // Few rows, or little work: 16 rows to a wavefront (form 0); up to 128 rows of a sequence on average: 32 (1); more: eight wavefronts over the rows
-// (2). The work is bounded by what the host knows, the tables' positions. us, 32 heads on 8, forms 0 / 1 / 2:
-//   D = 128: 32 sequences of 4000 positions, 8 rows 108 / 119 / 130, 24 rows 173 / 125 / 136, 128 rows 416 / 238 / 249, 256 rows 589 / 336 / 315;
-//   one of 2000, 128 rows 20 / 24 / 28; 4 of 2000, 64 rows 30 / 34 / 39; one of 32000, 64 rows 53 / 50 / 50
-//   D = 64: 32 of 4000, 16 rows 62 / 64 / 79, 64 rows 111 / 107 / 129, 256 rows 256 / 196 / 217; 4 of 2000, 128 rows 26 / 40 / -
-//   D = 256 (registers for 16 rows, LDS for 64 positions): 32 of 4000, 8 rows 235 / 201 / 212, 128 rows 1219 / 516 / 582, 256 rows 1888 / 732 / 652
+// (2). The work is bounded by what the host knows, the tables' positions: a table with room for more than there is takes the form for more (tree of
+// 24 nodes over 2050 positions: 19 us, with a table for 131072 25). us in calls back to back, 32 heads on 8, forms 0 / 1 / 2:
+//   D = 128: 32 sequences of 4000 positions, 8 rows 104 / 107 / 109, 24 rows 117 / 112 / 109, 64 rows 161 / 129 / 123, 128 rows 315 / 189 / 183,
+//   256 rows 612 / 308 / 302; the same, trees of 4 to 27 nodes on uneven lengths 229 / 154 / 178; one of 2000, 128 rows 20 / 23 / 28; 4 of 2000, 64
+//   rows 25 / 30 / 29; one of 32000, 64 rows 57 / 55 / 54
+//   D = 64, forms 0 / 1: 32 of 4000, 16 rows 62 / 60, 64 rows 89 / 75, 256 rows 288 / 222; one of 2000, 128 rows 18 / 21; 4 of 2000, 128 rows 23 / 31
+//   D = 256 (registers for 16 rows, LDS for 64 positions), forms 1 / 2: 32 of 4000, 8 rows 190 / 191, 128 rows 347 / 340, 256 rows 690 / 657; one of 2000,
+//   128 rows 25 / 34; 4 of 2000, 64 rows 44 / 37
 FpPlan planOf(const kcFlashPagesDims& d) {
     FpPlan p{};
     const int64_t G = d.H / d.H_kv, rows = int64_t(d.N) * G, pairs = int64_t(d.N) * d.H * (int64_t(d.max_pages) * d.page);

@@ -14,7 +14,9 @@
 //
 // What bounds it: for many rows the bytes, which are read twice (512 rows of 151936: the bins 69 us, 4.5 TB/s, the draws 95 us, of which
 // the second reading 55), for one row latencies, of one workgroup's steps one after the other (128256 logits, top_k 40: 5.5 and
-// 15 us; a flat row of 151936 under top_p 0.8, of which all is read again by one CU, 25 us more).
+// 15 us). A border among more members of its bins than the list holds costs readings of the row by one CU, two for each nine bits of
+// the order: a row of 151936 under top_p 0.8 and temperatures of 0.5 to 1.5 takes 40 us where its logits' deviation is 2.5, 330 where it is
+// 1, 780 where it is 0.3, 1570 where all are equal.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,7 +33,7 @@ typedef f32x4 f4a4 __attribute__((aligned(4)));
 typedef unsigned long long u64;
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
-// 64 octaves in bins; the last bin takes what is further (a millionth of millionths of millionths of the largest weight): counted, but of weight 0
+// 64 octaves below ref in bins; the last bin takes what is further, less than 2^-62 of the largest weight: counted, but of weight 0
 constexpr int kThreads = 1024, kWaves = 16, kDraw = 512, kBins = 2048, kFar = kBins - 1, kList = 5120, kGroups = 3 * kDraw, kPieces = 64;
 constexpr double kPerOctave = 32.0;
 constexpr int kUnitBits = 38;
