@@ -17,8 +17,9 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64, kPer = 4;  // sequences of a thread in a round
 // Tokens of a launch where there are trees: a token's walk up its tree ends with the launch's first one, and goes on from what the launch
-// before wrote. (A chain of 32768 nodes 4.3 ms, 130 ns a node; without this end the time of longer ones grew without bound.)
-constexpr int kLaunch = 32768;
+// before wrote. (130 ns a node, so that a launch takes 35 ms at most; without this end a longer chain's time grew without bound. Launches of 32768
+// would cost a step of many short trees more than they save: 20000 trees of 5 nodes 125 us for 40.)
+constexpr int kLaunch = 1 << 18;
 
 struct PagesArgs {
     const int *have, *add, *free, *parent;

@@ -39,24 +39,48 @@ def check(have, add, parent, words):
         assert np.array_equal(got[k], want[k]), (k, np.argwhere(got[k] != want[k])[:4].tolist())
 
 
-@pytest.mark.parametrize("words", [1, 2, 3, 64])
-@pytest.mark.parametrize("kind", ["chain", "near", "random", "wild"])
-@pytest.mark.parametrize("add", [[2048], [100, 33000, 300, 7], [32700, 64, 64, 64, 200], [40000], [32768, 32768, 1]], ids=str)
-def test_deep(words, kind, add):
-    print("kv_pages", add, kind, words, flush=True)
-    r = np.random.default_rng([words, len(add), add[0]])
+def trees(r, add, kind):
     parent = []
     for n in add:
         i = np.arange(n)
         parent.append(dict(chain=i - 1, near=i - 1 - np.minimum(r.integers(0, 4, n), i), random=(r.random(n) * i).astype(int) - (i == 0),
                            wild=np.where(r.random(n) < 0.02, r.choice([-1, -7, n, 2**31 - 1], n), i - 1 - r.integers(0, 40, n)))[kind])
-    check(r.integers(0, 100, len(add)), add, np.concatenate(parent), words)
+    return np.concatenate(parent)
+
+
+@pytest.mark.parametrize("words", [1, 2, 3, 64])
+@pytest.mark.parametrize("kind", ["chain", "near", "random", "wild"])
+@pytest.mark.parametrize("add", [[2048], [100, 20000, 300, 7]], ids=str)
+def test_deep(words, kind, add):
+    print("kv_pages", add, kind, words, flush=True)
+    r = np.random.default_rng([words, len(add), add[0]])
+    check(r.integers(0, 100, len(add)), add, trees(r, add, kind), words)
+
+
+LAUNCH = 1 << 18
+
+
+@pytest.mark.parametrize("words", [1, 3, 64])
+@pytest.mark.parametrize("kind", ["chain", "near", "wild"])
+@pytest.mark.parametrize("add", [[LAUNCH - 68, 64, 64, 64, 200], [30, LAUNCH + 500, 7]], ids=str)
+def test_several_launches(words, kind, add):
+    """A tree's nodes of a launch after the one that its root is in; one that begins with a launch."""
+    print("kv_pages", add, kind, words, flush=True)
+    r = np.random.default_rng([words, len(add), add[0]])
+    check(r.integers(0, 100, len(add)), add, trees(r, add, kind), words)
+
+
+@pytest.mark.parametrize("words", [1, 2])
+def test_short_trees(words):
+    """Trees of a few nodes on both sides of a launch's end."""
+    r = np.random.default_rng(words)
+    add = r.integers(1, 60, 10000)
+    check(r.integers(0, 100, len(add)), add, trees(r, add, "random"), words)
 
 
 def test_deep_far():
     """Positions past the largest number stay there, in every launch."""
-    have = 2**31 - 33000
-    page, n = 65536, 40000
-    parent = np.arange(n) - 1
-    got = run_pages([have], [n], np.zeros(1, np.int32), np.zeros((1, 1), np.int32), page, n, parent, 1)
+    n = LAUNCH + 7000
+    have, page = 2**31 - LAUNCH - 300, 65536
+    got = run_pages([have], [n], np.zeros(1, np.int32), np.zeros((1, 1), np.int32), page, n, np.arange(n) - 1, 1)
     assert np.array_equal(got["pos"], np.minimum(have + np.arange(n, dtype=np.int64), 2**31 - 1)) and (got["slots"] == -1).all() and got["len"] == 2**31 - 1

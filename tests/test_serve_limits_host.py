@@ -85,7 +85,7 @@ assert stub.stub_record() == b""  # neither q nor k: nothing to do
 """)
 
 
-@pytest.mark.parametrize("N", [0, 1, 32768, 32769, 100000])
+@pytest.mark.parametrize("N", [0, 1, 1 << 18, (1 << 18) + 1, 1000000])
 def test_tree_launches(stub, N):
     """A launch's walks up the trees are bounded by its tokens; without trees there is one launch."""
     run(stub, f"N = {N}" + r"""
@@ -94,7 +94,7 @@ for tree in (True, False):
     a = dict(b) if tree else dict(b, parent=None, tree=None)
     assert status("kv_pages", kc.KvPagesArgs(**a, seqs=2, n_tokens=N, n_free=1, page=16, max_pages=1, table_row=1, tree_words=2 if tree else 0)) == OK
     grids = [int(x.split()[-4]) for x in stub.stub_record().decode().splitlines()]
-    assert sum(grids) == max(1, -(-N // 256)) and len(grids) == (max(1, -(-N // 32768)) if tree else 1), grids
+    assert sum(grids) == max(1, -(-N // 256)) and len(grids) == (max(1, -(-N // (1 << 18))) if tree else 1), grids
 """)
 
 
