@@ -20,10 +20,11 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef h4 h4a2 __attribute__((aligned(2)));
 
 constexpr int kThreads = 256, kAhead = 2, kPairs = 1024;  // pairs of a workgroup's tokens
-// Tokens of a launch: the search for repeated slots grows with their square. What a launch stores lies over what the one before it did, so
-// that no launch looks for later ones' slots. (24 + 2 x 8 heads of 128, 65536 tokens: 500 us, in launches of 16384 570, in one 770; 262144
-// tokens 2.0 ms and 7.9.)
-constexpr int kLaunch = 8192;
+// Tokens of a launch that stores k and v, about: the search for repeated slots grows with their square. What a launch stores lies over what the
+// one before it did, so that no launch looks for later ones' slots. (24 + 2 x 8 heads of 128: 16384 tokens 119 us, in one launch 140; 65536
+// 500, in launches of 16384 570, in one 770; 262144 2.0 ms and 7.9. 8200 in two 51, in one 48; about 10000 alike.) Of q alone: what a launch's
+// threads allow.
+constexpr int kLaunch = 8192, kRest = 2048, kLaunchQ = 1 << 20;
 
 struct RopeArgs {
     const float *q, *k, *v;
@@ -207,8 +208,10 @@ __global__ __launch_bounds__(kThreads) void rope_ext_kernel(RopeArgs a) {
 }  // namespace
 
 int launchRopeExt(const kcRopeExtArgs& a, hipStream_t s) {
-    for (int at = 0; at < a.n_tokens; at += kLaunch) {
-        const int n = std::min(kLaunch, a.n_tokens - at);
+    const int launches = a.k ? std::max(1, (a.n_tokens - kRest + kLaunch - 1) / kLaunch) : 1;
+    const int each = std::min(kLaunchQ, (a.n_tokens + launches - 1) / launches);
+    for (int at = 0; at < a.n_tokens; at += each) {
+        const int n = std::min(each, a.n_tokens - at);
         RopeArgs p{a.q ? a.q + (long long)at * a.q_tok : nullptr, a.k ? a.k + (long long)at * a.k_tok : nullptr, a.v ? a.v + (long long)at * a.v_tok : nullptr,
                    a.pos + at, a.freqs, reinterpret_cast<const long long*>(a.slots) + (a.k ? at : 0), a.q ? a.q_out + (long long)at * a.out_tok : nullptr,
                    static_cast<char*>(a.k_cache), static_cast<char*>(a.v_cache), n, a.H, a.H_kv, a.D, a.n_rot, a.q_tok, a.q_head, a.k_tok, a.k_head,

@@ -85,7 +85,7 @@ def test_attention_of_a_shared_cache(D, by):
         x.free()
 
 
-@pytest.mark.parametrize("N", [8191, 8192, 8193, 16385, 30000])
+@pytest.mark.parametrize("N", [8192, 10240, 10241, 18433, 30000])
 @pytest.mark.parametrize("rows", [50, 20000])
 def test_repeated_slots_of_many_tokens(N, rows):
     """The last token with a slot is stored, wherever the others with it are."""

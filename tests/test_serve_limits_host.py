@@ -67,7 +67,7 @@ assert min(seen.values()) > 300, seen
 """)
 
 
-@pytest.mark.parametrize("N", [8192, 8193, 40000])
+@pytest.mark.parametrize("N", [1, 8192, 10240, 10241, 40000, (1 << 20) + 1])
 def test_rope_launches(stub, N):
     """A launch's search for repeated slots is bounded: many tokens take several launches, each with a part of them."""
     run(stub, f"N = {N}" + r"""
@@ -78,7 +78,9 @@ for change in ({}, dict(q=None, q_out=None), dict(k=None, k_cache=None, v=None, 
     assert status("rope_ext", kc.RopeExtArgs(**dict(args, **change))) == OK
     grids = [int(x.split()[-4]) for x in stub.stub_record().decode().splitlines()]
     # (a workgroup has at most 16 tokens)
-    assert len(grids) == -(-N // 8192) and max(grids) <= 2 * 8192 and sum(grids) >= N // 16, grids
+    stores = "k" not in change
+    assert len(grids) == (max(1, (N + 6143) // 8192) if stores else -(-N // (1 << 20))) and max(grids) <= (2 * 10240 if stores else 1 << 20), grids
+    assert sum(grids) >= N // 16
 stub.stub_clear()
 assert kc.launch_status("rope_ext", kc.RopeExtArgs(**dict(args, q=None, q_out=None, k=None, k_cache=None, v=None, v_cache=None, slots=None))) == OK
 assert stub.stub_record() == b""  # neither q nor k: nothing to do
